@@ -22,6 +22,8 @@ G4_APPEND_NORM_V = 2
 G4_APPEND_ROPE_K = 4
 G4_APPEND_NORM_Q = 8
 G4_APPEND_ROPE_Q = 16
+G4_PAGES_BF16 = 0
+G4_PAGES_E4M3 = 1
 G4_DECODE_SPLIT_KEYS = -1
 G4_DECODE_TWO_PASS = -2
 G4_LINEAR_PLAIN = 0
@@ -116,6 +118,40 @@ class G4LinearArgs(ctypes.Structure):
     ]
 
 
+class G4PagedCache(ctypes.Structure):
+    _fields_ = [
+        ("format", c_int32), ("num_pages", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+        ("page_size", c_int32), ("key", c_void_p), ("value", c_void_p), ("key_scale", c_void_p),
+        ("value_scale", c_void_p),
+    ]
+
+
+class G4PagedAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", G4PagedCache), ("batch", c_int32), ("seq", c_int32), ("group", c_int32), ("flags", c_int32),
+        ("eps", c_float), ("keep", c_int32), ("max_pages", c_int32), ("table_stride", c_int64),
+        ("page_table", c_void_p), ("write_pos", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q", c_void_p),
+        ("in_row_stride", c_int64), ("q_norm_weight", c_void_p), ("k_norm_weight", c_void_p),
+        ("rope_cos", c_void_p), ("rope_sin", c_void_p), ("q_out", c_void_p),
+    ]
+
+
+class G4PagedDecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", G4PagedCache), ("batch", c_int32), ("group", c_int32), ("window", c_int32),
+        ("max_pages", c_int32), ("table_stride", c_int64), ("page_table", c_void_p), ("lengths", c_void_p),
+        ("q", c_void_p), ("out", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class G4PagedReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", G4PagedCache), ("batch", c_int32), ("start", c_int32), ("count", c_int32),
+        ("max_pages", c_int32), ("table_stride", c_int64), ("page_table", c_void_p), ("lengths", c_void_p),
+        ("k_out", c_void_p), ("v_out", c_void_p),
+    ]
+
+
 class G4PrologueArgs(ctypes.Structure):
     _fields_ = [
         ("batch", c_int32), ("hidden", c_int32), ("vocab", c_int32), ("key_mask_stride", c_int32),
@@ -132,6 +168,10 @@ PROTOTYPES = {
     "g4_decode_attention": (c_int32, [POINTER(G4DecodeArgs), c_void_p]),
     "g4_decode_attention_noalloc": (c_int32, [POINTER(G4DecodeArgs), c_void_p]),
     "g4_prefill_attention": (c_int32, [POINTER(G4PrefillArgs), c_void_p]),
+    "g4_paged_append": (c_int32, [POINTER(G4PagedAppendArgs), c_void_p]),
+    "g4_paged_decode_workspace_size": (c_size_t, [POINTER(G4PagedDecodeArgs)]),
+    "g4_paged_decode_attention": (c_int32, [POINTER(G4PagedDecodeArgs), c_void_p]),
+    "g4_paged_read": (c_int32, [POINTER(G4PagedReadArgs), c_void_p]),
     "g4_kv_source_layers": (c_int32, [c_int32, c_int32, POINTER(c_int32), POINTER(c_int32)]),
     "g4_ring_slot_positions": (c_int32, [c_int32, c_int32, POINTER(c_int32)]),
     "g4_sample_tokens": (c_int32, [POINTER(G4SampleArgs), c_void_p]),
@@ -216,6 +256,7 @@ def ring_slot_positions(last_written: int, window_capacity: int) -> list[int]:
 
 
 __all__ = [
-    "G4AppendArgs", "G4DecodeArgs", "G4PrefillArgs", "G4LinearArgs", "G4PrologueArgs", "G4DecodePrep", "G4Error", "PROTOTYPES", "LIB_PATH", "lib", "check", "init_device",
+    "G4AppendArgs", "G4DecodeArgs", "G4PrefillArgs", "G4LinearArgs", "G4PrologueArgs", "G4DecodePrep", "G4PagedCache",
+    "G4PagedAppendArgs", "G4PagedDecodeArgs", "G4PagedReadArgs", "G4Error", "PROTOTYPES", "LIB_PATH", "lib", "check", "init_device",
     "kv_source_layers", "ring_slot_positions", "c_uint8",
 ]

@@ -28,6 +28,7 @@ int device_setup(int* device);
 int setup_decode_kernels(int device);
 int setup_prefill_kernels(int device);
 int setup_lm_head(int device);
+int setup_paged_kernels(int device);
 
 // Raises kernel `fn`'s dynamic-LDS limit to `bytes` on `device` (the current device; called from the
 // set-up steps only) and records whether that worked. lds_limit_raised(device, fn) reads the record

@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .kvcache import LayerKVCache, key_shape
+from .kvcache import LayerKVCache, PagedLayerCache, key_shape, paged_key_shape
 
 _DTYPES = {torch.float32: _lib.G4_DTYPE_F32, torch.bfloat16: _lib.G4_DTYPE_BF16}
 
@@ -322,6 +322,187 @@ def prefill_attention(
     )
     _lib.check(_lib.lib().g4_prefill_attention(ctypes.byref(a), _stream()), "g4_prefill_attention")
     return out
+
+
+# --- paged cache ------------------------------------------------------------------------------------------
+
+
+def _paged_cache(layer: PagedLayerCache) -> _lib.G4PagedCache:
+    """The checked C view of a layer's pages."""
+
+    value = layer.value
+    if value.dim() != 5 or value.shape[4] != 8:
+        raise ValueError(f"value pages: shape {tuple(value.shape)} is not [P, Hkv, page / 8, D, 8]")
+    P, H, groups, D, _ = value.shape
+    e4m3 = value.dtype == torch.float8_e4m3fn
+    if value.dtype != layer.key.dtype or not (e4m3 or value.dtype == torch.bfloat16):
+        raise TypeError(f"pages of {layer.key.dtype} / {value.dtype}; they hold bfloat16 or float8_e4m3fn")
+    if tuple(layer.key.shape) != paged_key_shape(P, H, groups * 8, D, e4m3):
+        raise ValueError(f"key pages {tuple(layer.key.shape)} do not match value pages {tuple(value.shape)}")
+    if not (layer.key.is_contiguous() and value.is_contiguous()):
+        raise ValueError("pages must be contiguous")
+    if e4m3:
+        for t in (layer.key_scale, layer.value_scale):
+            if (t is None or t.dtype != torch.float8_e8m0fnu or tuple(t.shape) != (P, H, groups * 8)
+                    or not t.is_contiguous() or t.device != value.device):
+                raise ValueError(f"e4m3 pages need contiguous float8_e8m0fnu scales of shape {(P, H, groups * 8)}")
+    elif layer.key_scale is not None or layer.value_scale is not None:
+        raise ValueError("bf16 pages have no scales")
+    if layer.key.device != value.device:
+        raise ValueError("key and value pages are on different devices")
+    return _lib.G4PagedCache(format=_lib.G4_PAGES_E4M3 if e4m3 else _lib.G4_PAGES_BF16, num_pages=P, kv_heads=H,
+                             head_dim=D, page_size=groups * 8, key=_ptr(layer.key), value=_ptr(value),
+                             key_scale=_ptr(layer.key_scale), value_scale=_ptr(layer.value_scale))
+
+
+def _on_device(layer: PagedLayerCache, *tensors: torch.Tensor | None) -> None:
+    """The operands are on the cache's device and it is the current one, whose stream the call goes to."""
+
+    dev = layer.value.device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"an operand is on {t.device}, the cache on {dev}")
+    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
+        raise ValueError(f"the cache is on {dev}, which is not the current device")
+
+
+def _page_rows(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> tuple[int, int, int]:
+    """(B, entries per row, stride) of a page table, ``rows`` being the int32 [B] tensor ``name``."""
+
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or 0 in page_table.shape:
+        raise ValueError("page_table must be a non-empty int32 [B, M] tensor")
+    B, M = page_table.shape
+    stride = page_table.stride(0) if B > 1 else M
+    if (M > 1 and page_table.stride(1) != 1) or stride < M:
+        raise ValueError("page_table rows must be contiguous and apart")
+    if rows.dtype != torch.int32 or tuple(rows.shape) != (B,) or not rows.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 [{B}] tensor")
+    return B, M, stride
+
+
+def paged_append(
+    layer: PagedLayerCache,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    page_table: torch.Tensor,
+    write_pos: torch.Tensor,
+    keep: int = 0,
+    flags: int = 0,
+    eps: float = 1e-6,
+    q: torch.Tensor | None = None,
+    q_out: torch.Tensor | None = None,
+    q_norm_weight: torch.Tensor | None = None,
+    k_norm_weight: torch.Tensor | None = None,
+    rope_cos: torch.Tensor | None = None,
+    rope_sin: torch.Tensor | None = None,
+) -> None:
+    """g4_paged_append: ``kv_append``'s work into pages, quantised where they hold e4m3. k / v ``[B, S, Hkv, D]``
+    (and q ``[B, S, Hkv, R, D]``) bf16 views of rows sharing one row stride; token s of row b is stored at position
+    ``write_pos[b] + s`` (int32 ``[B]``). Not stored: positions below 0 (the pads of a left-padded prompt that
+    starts at minus its pad count), beyond the table or without a page, and with ``keep`` > 0 all but the last
+    ``keep`` tokens. q / k / v are prepared by ``flags`` in f32 and rounded once, where they are stored."""
+
+    B, S, H, D = k.shape
+    rs = k.stride(1) if S > 1 else (k.stride(0) if B > 1 else H * D)
+    _check_rows(k, "k", B, S, H, D, rs)
+    _check_rows(v, "v", B, S, H, D, rs)
+    if k.dtype != torch.bfloat16 or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        raise TypeError("paged_append takes bfloat16 q / k / v")
+    rows, M, table_stride = _page_rows(page_table, "write_pos", write_pos)
+    if rows != B:
+        raise ValueError(f"page_table has {rows} rows for a batch of {B}")
+    if layer.kv_heads != H or layer.head_dim != D:
+        raise ValueError(f"pages of {layer.kv_heads} heads of {layer.head_dim} do not match k {tuple(k.shape)}")
+    if keep < 0:
+        raise ValueError(f"keep must not be negative, got {keep}")
+    R = 0
+    if q is not None:
+        R = q.shape[3] if q.dim() == 5 else 0
+        if tuple(q.shape) != (B, S, H, R, D) or q.stride(4) != 1 or q.stride(3) != D or (H > 1 and q.stride(2) != R * D):
+            raise ValueError(f"q: shape {tuple(q.shape)} / strides {q.stride()}")
+        if (S > 1 and q.stride(1) != rs) or (B > 1 and q.stride(0) != S * rs):
+            raise ValueError("q must share k's row stride")
+        if (q_out is None or q_out.dtype != q.dtype or tuple(q_out.shape) != (B, S, H, R, D)
+                or not q_out.is_contiguous()):
+            raise ValueError("q_out must be a contiguous bfloat16 [B, S, Hkv, R, D] tensor")
+    for name, t, on in (("q_norm_weight", q_norm_weight, q is not None and flags & _lib.G4_APPEND_NORM_Q),
+                        ("k_norm_weight", k_norm_weight, flags & _lib.G4_APPEND_NORM_K)):
+        if on and (t is None or t.dtype != k.dtype or tuple(t.shape) != (D,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous bfloat16 [{D}] tensor")
+    if flags & (_lib.G4_APPEND_ROPE_K | _lib.G4_APPEND_ROPE_Q):
+        for t in (rope_cos, rope_sin):
+            if t is None or t.dtype != torch.float32 or tuple(t.shape) != (B, S, D) or not t.is_contiguous():
+                raise ValueError("rope_cos/rope_sin must be contiguous float32 [B, S, D]")
+    _on_device(layer, k, v, q, q_out, page_table, write_pos, q_norm_weight, k_norm_weight, rope_cos, rope_sin)
+    a = _lib.G4PagedAppendArgs(
+        cache=_paged_cache(layer), batch=B, seq=S, group=R, flags=flags, eps=eps, keep=keep, max_pages=M,
+        table_stride=table_stride, page_table=_ptr(page_table), write_pos=_ptr(write_pos), k=_ptr(k), v=_ptr(v),
+        q=_ptr(q), in_row_stride=rs, q_norm_weight=_ptr(q_norm_weight), k_norm_weight=_ptr(k_norm_weight),
+        rope_cos=_ptr(rope_cos), rope_sin=_ptr(rope_sin), q_out=_ptr(q_out),
+    )
+    _lib.check(_lib.lib().g4_paged_append(ctypes.byref(a), _stream()), "g4_paged_append")
+
+
+def paged_decode_attention(
+    layer: PagedLayerCache,
+    q: torch.Tensor,
+    *,
+    page_table: torch.Tensor,
+    lengths: torch.Tensor,
+    window: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """g4_paged_decode_attention: q ``[B, Hkv, R, D]`` (bf16, at position ``lengths[b] - 1``) over the positions
+    below ``lengths[b]`` (int32 ``[B]``), the last ``window`` of them with ``window`` > 0; returns
+    ``[B, Hkv, R, D]`` bf16, zeros for a row without a position. The workspace comes from torch's caching
+    allocator."""
+
+    B, H, R, D = q.shape
+    if q.dtype != torch.bfloat16 or not q.is_contiguous():
+        raise ValueError("q must be a contiguous bfloat16 [B, Hkv, R, D] tensor")
+    rows, M, table_stride = _page_rows(page_table, "lengths", lengths)
+    if rows != B:
+        raise ValueError(f"page_table has {rows} rows for a batch of {B}")
+    if layer.kv_heads != H or layer.head_dim != D:
+        raise ValueError(f"pages of {layer.kv_heads} heads of {layer.head_dim} do not match q {tuple(q.shape)}")
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    if out is None:
+        out = torch.empty_like(q)
+    elif tuple(out.shape) != (B, H, R, D) or not out.is_contiguous() or out.dtype != q.dtype:
+        raise ValueError("out must be a contiguous [B, Hkv, R, D] tensor in q's dtype")
+    _on_device(layer, q, page_table, lengths, out)
+    a = _lib.G4PagedDecodeArgs(
+        cache=_paged_cache(layer), batch=B, group=R, window=window, max_pages=M, table_stride=table_stride,
+        page_table=_ptr(page_table), lengths=_ptr(lengths), q=_ptr(q), out=_ptr(out), workspace=None, workspace_bytes=0,
+    )
+    need = _lib.lib().g4_paged_decode_workspace_size(ctypes.byref(a))
+    ws = None
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    _lib.check(_lib.lib().g4_paged_decode_attention(ctypes.byref(a), _stream()), "g4_paged_decode_attention")
+    return out
+
+
+def paged_read(layer: PagedLayerCache, *, page_table: torch.Tensor, lengths: torch.Tensor, start: int,
+               count: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """g4_paged_read: the cache's ``(key, value)`` as ``[B, count, Hkv, D]`` bf16 rows of positions ``start ..
+    start + count - 1``; zeros at and beyond ``lengths[b]`` and where a row has no page."""
+
+    B, M, table_stride = _page_rows(page_table, "lengths", lengths)
+    if start < 0 or count <= 0:
+        raise ValueError(f"start {start} must not be negative and count {count} must be positive")
+    _on_device(layer, page_table, lengths)
+    cache = _paged_cache(layer)
+    shape = (B, count, layer.kv_heads, layer.head_dim)
+    k = torch.empty(shape, dtype=torch.bfloat16, device=layer.value.device)
+    v = torch.empty(shape, dtype=torch.bfloat16, device=layer.value.device)
+    a = _lib.G4PagedReadArgs(cache=cache, batch=B, start=start, count=count, max_pages=M, table_stride=table_stride,
+                             page_table=_ptr(page_table), lengths=_ptr(lengths), k_out=_ptr(k), v_out=_ptr(v))
+    _lib.check(_lib.lib().g4_paged_read(ctypes.byref(a), _stream()), "g4_paged_read")
+    return k, v
 
 
 # --- fused decoder-layer glue ------------------------------------------------------------------------

@@ -119,6 +119,70 @@ class LayerKVCache(NamedTuple):
         return k, v
 
 
+PAGE_SIZES = (32, 64, 128, 256, 512, 1024)
+
+
+def paged_key_shape(pages: int, heads: int, page_size: int, head_dim: int, e4m3: bool) -> tuple:
+    """Shape of a layer's key pages: ``[P, H, page / 32, D / KR, 2, 16, KR]``, the dense key layout per 32-slot
+    chunk with runs of KR = 32 (bf16) or 64 (e4m3) dims."""
+
+    kr = 64 if e4m3 else 32
+    return (pages, heads, page_size // 32, head_dim // kr, 2, 16, kr)
+
+
+class PagedLayerCache(NamedTuple):
+    """One layer's K/V in pages of ``page_size`` positions (g4_paged_append, g4_paged_decode_attention,
+    g4_paged_read), in bf16, or in e4m3 with one power-of-two scale per slot and head of each of K and V.
+    Which pages a row has, and in which order, is the caller's ``page_table [B, M]`` (int32): position p of
+    row b is slot ``p % page_size`` of page ``page_table[b, p // page_size]``, and an entry outside
+    ``[0, P)`` stands for no page. Rows may share pages."""
+
+    key: torch.Tensor  # paged_key_shape(...), bf16 or float8_e4m3fn
+    value: torch.Tensor  # [P, Hkv, page / 8, D, 8]
+    key_scale: torch.Tensor | None = None  # e4m3: [P, Hkv, page] float8_e8m0fnu
+    value_scale: torch.Tensor | None = None
+
+    @property
+    def num_pages(self) -> int:
+        return self.value.shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self.value.shape[1]
+
+    @property
+    def page_size(self) -> int:
+        return self.value.shape[2] * 8
+
+    @property
+    def head_dim(self) -> int:
+        return self.value.shape[3]
+
+    @property
+    def e4m3(self) -> bool:
+        return self.value.dtype == torch.float8_e4m3fn
+
+
+def new_paged_layer(num_pages: int, kv_heads: int, head_dim: int, page_size: int, *, e4m3: bool = False,
+                    device="cuda") -> PagedLayerCache:
+    """A zero-filled ``PagedLayerCache`` of ``num_pages`` pages, bf16 or e4m3."""
+
+    if num_pages <= 0 or kv_heads <= 0:
+        raise ValueError(f"num_pages and kv_heads must be positive, got {num_pages} and {kv_heads}")
+    if head_dim not in (64, 128, 256, 512):
+        raise ValueError(f"pages hold head dims 64, 128, 256 or 512, got {head_dim}")
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    key = paged_key_shape(num_pages, kv_heads, page_size, head_dim, e4m3)
+    value = (num_pages, kv_heads, page_size // 8, head_dim, 8)
+    if not e4m3:
+        return PagedLayerCache(*(torch.zeros(s, dtype=torch.bfloat16, device=device) for s in (key, value)))
+    key, value = (torch.zeros(s, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for s in (key, value))
+    scales = (torch.full((num_pages, kv_heads, page_size), 127, dtype=torch.uint8, device=device)
+              .view(torch.float8_e8m0fnu) for _ in range(2))
+    return PagedLayerCache(key, value, *scales)
+
+
 class KVCache(NamedTuple):
     layers: tuple  # LayerKVCache | None per layer
     key_mask: torch.Tensor  # [B, C] bool
@@ -149,5 +213,5 @@ def init_kv_cache(config: Gemma4TextConfig, batch_size: int, capacity: int, dtyp
     return KVCache(tuple(layers), key_mask, 0)
 
 
-__all__ = ["LayerKVCache", "KVCache", "init_kv_cache", "new_layer_cache", "slot_stride_for", "key_shape", "group_keys",
+__all__ = ["LayerKVCache", "KVCache", "PagedLayerCache", "PAGE_SIZES", "new_paged_layer", "paged_key_shape", "init_kv_cache", "new_layer_cache", "slot_stride_for", "key_shape", "group_keys",
            "ungroup_keys", "group_values", "ungroup_values", "FULL", "SLIDING"]

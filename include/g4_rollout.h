@@ -246,6 +246,125 @@ typedef struct G4PrefillArgs {
 int g4_prefill_attention(const G4PrefillArgs* args, void* stream);
 
 /*
+ * One layer's KV cache in pages, for rows that take memory as they grow and may share it (the
+ * completions of one prompt). No reference counterpart: its caches are one dense array per layer.
+ * A page holds page_size consecutive positions of a row, all kv heads:
+ *   key    [num_pages, Hkv, page_size/32, D/KR, 2, 16, KR]  the dense key layout above per 32-slot
+ *          chunk, KR = 32 (bf16) or 64 (e4m3) dims per run, so that one MFMA operand load reads 1 KiB
+ *   value  [num_pages, Hkv, page_size/8, D, 8]              the dense value layout above
+ * Formats: G4_PAGES_BF16; G4_PAGES_E4M3 stores one byte per element and, per (page, head, slot), one
+ * scale for the key and one for the value vector in key_scale / value_scale [num_pages, Hkv,
+ * page_size]: the byte e stands for 2^(e - 127) (27 <= e <= 247), and an element's value is its e4m3 value
+ * times that. A power of two scales exactly, and a floating format's relative error is the same
+ * under any scale, so nothing finer is stored.
+ * Position p of row b is slot p % page_size of page page_table[b * table_stride + p / page_size],
+ * 0 <= p < max_pages * page_size. A table entry outside [0, num_pages) means that the row has no such
+ * page: the position is not written, and reads as not there. Entries may repeat: a row whose table
+ * cycles through a few pages keeps a ring, and rows may share pages that neither writes.
+ */
+enum { G4_PAGES_BF16 = 0, G4_PAGES_E4M3 = 1 };
+
+typedef struct G4PagedCache {
+  int32_t format;      /* G4_PAGES_* */
+  int32_t num_pages;
+  int32_t kv_heads;
+  int32_t head_dim;    /* 64, 128, 256 or 512 */
+  int32_t page_size;   /* slots per page: a power of two, 32 .. 1024 */
+  void* key;           /* 16-byte aligned */
+  void* value;         /* 16-byte aligned */
+  uint8_t* key_scale;  /* G4_PAGES_E4M3 only; 8-byte aligned */
+  uint8_t* value_scale;
+} G4PagedCache;
+
+/*
+ * g4_kv_append's work into pages: the q / k norms and rotation, the v norm (flags as there, model.py:
+ * 463-482) and the write of k / v, quantised where the pages hold e4m3. Token s of row b stands at
+ * position p = write_pos[b] + s and is stored if p >= 0 (a negative start leaves out the pads of a
+ * left-padded prompt; -seq or less the whole row), p < max_pages * page_size, its page exists, and keep
+ * is 0 or s >= seq - keep (a sliding layer stores the last `keep` tokens; with a cyclic table keep is at
+ * most the cycle's positions less page_size - 1, or one call would write a slot twice). q_out is
+ * written for every token. bf16 inputs; f32 arithmetic with one rounding, at the store (g4_kv_append
+ * also rounds after the norm, as the reference does). e4m3: the scale is the least power of two
+ * 2^e >= max |x| / 448 over the vector's finite elements, e clamped to -100 .. 120; elements are
+ * rounded to nearest even, infinities and NaN become NaN. Rows that share a page write it in no
+ * defined order. No workspace.
+ */
+typedef struct G4PagedAppendArgs {
+  G4PagedCache cache;
+  int32_t batch;
+  int32_t seq;
+  int32_t group;              /* R (only read when q != NULL) */
+  int32_t flags;              /* G4_APPEND_* */
+  float eps;
+  int32_t keep;               /* 0 = every token */
+  int32_t max_pages;          /* entries of a table row */
+  int64_t table_stride;       /* elements between table rows, >= max_pages */
+  const int32_t* page_table;  /* device [B, max_pages] */
+  const int32_t* write_pos;   /* device [B] position of token 0 */
+  const void* k;              /* token (b,s): k + (b*S + s)*in_row_stride, heads [Hkv, D] */
+  const void* v;              /* may alias k */
+  const void* q;              /* optional, heads [Hkv, R, D] */
+  int64_t in_row_stride;
+  const void* q_norm_weight;  /* [D] (G4_APPEND_NORM_Q) */
+  const void* k_norm_weight;  /* [D] (G4_APPEND_NORM_K) */
+  const float* rope_cos;      /* [B, S, D] f32 (G4_APPEND_ROPE_*) */
+  const float* rope_sin;
+  void* q_out;                /* [B, S, Hkv, R, D] */
+} G4PagedAppendArgs;
+
+int g4_paged_append(const G4PagedAppendArgs* args, void* stream);
+
+/*
+ * One-token GQA attention over a paged cache: per row b and head, softmax(q . k) v over the positions
+ * max(0, lengths[b] - window) .. lengths[b] - 1 (window 0: from 0) whose page exists, scale 1.0
+ * (model.py:496-499 for S = 1; the query stands at position lengths[b] - 1, its own key already
+ * appended). Lengths beyond max_pages * page_size are read as that. A row with no position, or
+ * whose scores are all -inf, gives zeros. What the other slots hold, NaN included, does not matter.
+ * f32 scores, softmax and sums; the unnormalised probabilities (times the value's scale) are rounded
+ * to bf16 as the operand of the value product, the result once to bf16. The same call gives the
+ * same bits. Needs g4_paged_decode_workspace_size() bytes of scratch (16-byte aligned; no state is
+ * kept in it, so calls ordered on one stream may share it).
+ */
+typedef struct G4PagedDecodeArgs {
+  G4PagedCache cache;
+  int32_t batch;
+  int32_t group;              /* R, 1 .. 16 */
+  int32_t window;             /* 0 = all positions */
+  int32_t max_pages;
+  int64_t table_stride;
+  const int32_t* page_table;  /* device [B, max_pages] */
+  const int32_t* lengths;     /* device [B]; 0 or less: no position */
+  const void* q;              /* [B, Hkv, R, D] bf16, 16-byte aligned */
+  void* out;                  /* [B, Hkv, R, D] bf16, 16-byte aligned */
+  void* workspace;
+  size_t workspace_bytes;
+} G4PagedDecodeArgs;
+
+size_t g4_paged_decode_workspace_size(const G4PagedDecodeArgs* args);
+int g4_paged_decode_attention(const G4PagedDecodeArgs* args, void* stream);
+
+/*
+ * Reads a paged cache back: k_out / v_out [B, count, Hkv, D] bf16 (the reference's cache order,
+ * model.py:238-246) of positions start .. start + count - 1 of every row; positions at or beyond
+ * lengths[b], or without a page, read as zeros. Exact, but that values below bf16's least normal
+ * number 2^-126 may read as zero.
+ */
+typedef struct G4PagedReadArgs {
+  G4PagedCache cache;
+  int32_t batch;
+  int32_t start;
+  int32_t count;
+  int32_t max_pages;
+  int64_t table_stride;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  void* k_out;  /* 16-byte aligned */
+  void* v_out;
+} G4PagedReadArgs;
+
+int g4_paged_read(const G4PagedReadArgs* args, void* stream);
+
+/*
  * Host-side: KV-sharing map (model.py:153-168). layer_types[i] is 0 (sliding) or 1 (full);
  * out[i] = index of the layer whose K/V layer i uses (itself when not shared).
  */
