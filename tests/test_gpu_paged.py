@@ -192,6 +192,9 @@ ATTENDS = [  # D, H, R, page, lengths, window
     (512, 1, 8, 64, [1, 5001, 77], 0),
     (512, 2, 16, 32, [90, 333], 45),
     (512, 1, 2, 1024, [1030, 3], 0),
+    (512, 1, 16, 64, [4000], 0),
+    (64, 1, 4, 256, [20000], 0),
+    (128, 1, 2, 64, [9000, 3, 0, 9001, 0, 64], 5000),
 ]
 
 
@@ -214,6 +217,12 @@ def test_attention_many_rows(device, e4m3):
     lengths[150] = 900
     layer, table = _cache(device, e4m3, 1, 64, 32, lengths)
     _check(layer, table, lengths, _randn(9, len(lengths), 1, 5, 64, scale=0.25), 0, device)
+
+
+def test_attention_more_rows_than_one_launch(device):
+    lengths = [(7 * i) % 40 for i in range(4500)]
+    layer, table = _cache(device, True, 1, 64, 32, lengths)
+    _check(layer, table, lengths, _randn(9, len(lengths), 1, 1, 64, scale=0.25), 0, device)
 
 
 @pytest.mark.parametrize("e4m3", [False, True])
