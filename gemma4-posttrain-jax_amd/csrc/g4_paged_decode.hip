@@ -5,32 +5,34 @@
 // the value product, V^T as A. Neither scores nor probabilities leave the registers. One pass over
 // the keys: per wave a running maximum m and sum l in f32, o rescaled where m grows.
 //
-// The work is the rows' 32-slot chunks, row by row and head by head in one sequence, of which every
-// workgroup takes an equal range: ragged rows, few long rows and many short ones fill the chip alike. The
-// lengths stand on the device, so each workgroup sums up the chunks of the rows itself. A (row, head) that lies
-// in one range is finished there; the others leave (m, l, o) per range, which a second launch joins in the
-// ranges' order.
+// A (row, head) is one workgroup's work, or, where rows are long or few, pieces of at most `per` chunks of 32
+// slots: `per` follows from the sum of all rows' chunks, so that ragged rows, few long ones and many short
+// ones fill the chip alike. The lengths stand on the device, so each workgroup finds its piece from them
+// itself. A (row, head) of one piece is finished by it; the others leave (m, l, o) per piece, which a second
+// launch joins in the pieces' order.
 #include "g4_paged.h"
 
 namespace g4 {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * 64;
-constexpr int kMaxRows = 2048;  // rows of one launch: their chunk sums stand in LDS beside the largest o
-constexpr int kMinChunks = kWaves;  // chunks per workgroup at least: one per wave
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
+constexpr int kCus = 256, kXcds = 8;
 
-constexpr int kCus = 256;
-// workgroups that a CU holds at once (by registers)
-constexpr int groups_per_cu(int D) { return D == 512 ? 1 : (D == 256 ? 2 : (D == 128 ? 3 : 4)); }
+template <int D, bool SPLIT>
+struct Groups {
+  static constexpr int SIMD_WAVES = D == 512 ? 1 : (D == 256 ? 2 : 4);  // resident, by registers
+  static constexpr int WAVES = SPLIT || D == 512 ? 4 : 8;                // per workgroup
+  static constexpr int THREADS = 64 * WAVES;
+};
+// Workgroups of the split kernel that are resident at once (four waves: one on each SIMD).
+constexpr int resident(int D) { return kCus * (D == 512 ? 1 : (D == 256 ? 2 : 4)); }
 constexpr int q_stride(int D) { return D + 8; }  // elements between q rows in LDS: 16 lanes' reads fall on different banks
 
 struct Workspace {
-  float* o;      // [2 groups][R][D] o of a range's first and last (row, head) where those pass its ends
-  float* ml;     // [2 groups][R][2] their m and l
-  int2* ranges;  // [pairs] first range and number of ranges with a part of the (row, head), {0, 0}: none to join
+  float* o;      // [slots][R][D] o of each piece of a split (row, head)
+  float* ml;     // [slots][R][2] their m and l
+  int2* ranges;  // [pairs] first slot and number of slots of a (row, head), {0, 0}: not split
 };
 
 // The two MFMA A operands (keys: 8 dims each; values: 8 slots of a dim each) in 16 bytes of e4m3.
@@ -65,377 +67,452 @@ __device__ __forceinline__ RowKeys row_keys(const G4PagedDecodeArgs& a, int b) {
   return RowKeys{a.window > 0 && hi > a.window ? hi - a.window : 0, hi};
 }
 
-// sums[b] = chunks of the rows before b, b = 0 .. batch (every thread of the workgroup calls it).
-__device__ __forceinline__ void sum_chunks(const G4PagedDecodeArgs& a, int* sums, int* wave_sums) {
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int per = (a.batch + kThreads - 1) / kThreads;
-  const int b0 = tid * per, b1 = b0 + per < a.batch ? b0 + per : a.batch;
-  int own = 0;
-  for (int b = b0; b < b1; ++b) own += row_keys(a, b).chunks();
-  int incl = own;
+// Sums over the wave's lanes 0 .. own (every lane active), and over all lanes, by lane moves in the vector
+// pipeline: shifts within the rows of 16, then row ends broadcast to the rows after them.
+__device__ __forceinline__ int scan_incl(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int sum_lanes(int v) { return __builtin_amdgcn_readlane(scan_incl(v), 63); }
+
+constexpr int kTries = 5;
+
+// A workgroup's part of a (row, head): piece `index` of `count`.
+struct Piece {
+  int b, h, index, count, slot;  // slot: its place in the workspace (count > 1)
+  RowKeys keys;                  // of row b
+};
+
+// Piece blockIdx of a split call (false: none). Every wave finds it by itself: the rows' chunk counts are summed
+// over the wave, 64 rows at a time, then the pieces and the workspace slots before each row.
+// The host bounds the chunks of all (row, head) pairs by 2^30 and a row's by 2^22, which the f32 division needs.
+__device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room, int min_per, int lane, Piece& out) {
+  const int H = a.cache.kv_heads, B = a.batch;
+  int sum = 0;
+#pragma unroll 4
+  for (int b0 = 0; b0 < B; b0 += 64) sum += b0 + lane < B ? row_keys(a, b0 + lane).chunks() : 0;
+  const int total = sum_lanes(sum) * H;
+  // The least `per` of a few whose pieces are all resident at once: the rows' ends add at most one piece per
+  // (row, head) to total / per, so the last of them does where there are fewer of those than room. Where there are
+  // more, rows of up to twice the mean share of a workgroup stay whole.
+  const int pairs = B * H;
+  float share[kTries];  // 1 / per
+  int n_pieces[kTries];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int below = __shfl_up(incl, d, 64);
-    if (lane >= d) incl += below;
+  for (int i = 0; i < kTries; ++i) {
+    const int target = pairs < room ? room - (int)((int64_t)pairs * i / (kTries - 1)) : room / 2;
+    const int per = (int)((float)total / (float)target) + 1;
+    share[i] = 1.f / (float)(per > min_per ? per : min_per);
+    n_pieces[i] = 0;
   }
-  if (lane == 63) wave_sums[w] = incl;
-  __syncthreads();
-  int base = incl - own;
-  for (int i = 0; i < w; ++i) base += wave_sums[i];
-  if (tid == 0) sums[0] = 0;
-  for (int b = b0; b < b1; ++b) {
-    base += row_keys(a, b).chunks();
-    sums[b + 1] = base;
+  // ceil(n / per): floor((n - 1) / per) + 1, the quotient off a whole number by 1 / per at least where it is not one
+  auto pieces_of = [&](int n, float share) -> int { return n > 0 ? (int)((float)(n - 1) * share) + 1 : 1; };
+#pragma unroll 2
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    const int n = b0 + lane < B ? row_keys(a, b0 + lane).chunks() : 0;
+#pragma unroll
+    for (int i = 0; i < kTries; ++i) n_pieces[i] += b0 + lane < B ? pieces_of(n, share[i]) : 0;
   }
-  __syncthreads();
+  float cut = share[kTries - 1];
+  int count = 0;
+#pragma unroll
+  for (int i = kTries - 1; i >= 0; --i) {
+    n_pieces[i] = sum_lanes(n_pieces[i]) * H;
+    if (i == kTries - 1 || n_pieces[i] <= room) cut = share[i], count = n_pieces[i];
+  }
+  // consecutive pieces on one XCD (workgroup i runs on XCD i % 8): rows that share pages read them from its L2
+  const int xcd_share = (count + kXcds - 1) / kXcds;
+  const int y = blockIdx.x / kXcds, want = (int)(blockIdx.x % kXcds) * xcd_share + y;
+  if (y >= xcd_share || want >= count) return false;
+  int before = 0, slots = 0;  // pieces and slots of the rows before this 64
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    const bool on = b0 + lane < B;
+    const RowKeys keys = on ? row_keys(a, b0 + lane) : RowKeys{0, 0};
+    const int k = on ? pieces_of(keys.chunks(), cut) : 0, used = k > 1 ? k * H : 0;
+    const int incl = scan_incl(k * H), sincl = scan_incl(used);
+    const int end = before + __builtin_amdgcn_readlane(incl, 63);
+    if (want < end) {
+      const int at = __builtin_popcountll(__ballot(before + incl <= want));  // the row's lane
+      const int kk = __builtin_amdgcn_readlane(k, at);
+      const int local = want - before - (__builtin_amdgcn_readlane(incl, at) - kk * H);
+      out.b = b0 + at;
+      out.h = __builtin_amdgcn_readfirstlane(local / kk);
+      out.index = local - out.h * kk;
+      out.count = kk;
+      out.slot = slots + __builtin_amdgcn_readlane(sincl, at) - (kk > 1 ? kk * H : 0) + local;
+      out.keys = RowKeys{__builtin_amdgcn_readlane(keys.lo, at), __builtin_amdgcn_readlane(keys.hi, at)};
+      return true;
+    }
+    before = end;
+    slots += __builtin_amdgcn_readlane(sincl, 63);
+  }
+  return false;
 }
 
-template <int D, bool F8>
-__global__ __launch_bounds__(kThreads, groups_per_cu(D)) void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws) {
+template <int D, bool F8, bool SPLIT>
+__global__ __launch_bounds__((Groups<D, SPLIT>::THREADS)) __attribute__((amdgpu_waves_per_eu(Groups<D, SPLIT>::SIMD_WAVES)))
+void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
   using Sh = Shape<D, F8>;
-  // [kWaves][R][D] o | [R][q_stride(D)] q | [kWaves][16] m, l | chunk sums
+  constexpr int kWaves = Groups<D, SPLIT>::WAVES, kThreads = Groups<D, SPLIT>::THREADS;
+  // [kWaves][R][D] o | [R][q_stride(D)] q | [kWaves][16] m, l
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int R = a.group, H = a.cache.kv_heads, ps = a.cache.page_size;
   uint16_t* q_lds = reinterpret_cast<uint16_t*>(lds + kWaves * R * D);
   float* m_lds = reinterpret_cast<float*>(q_lds + R * q_stride(D));
   float* l_lds = m_lds + kWaves * 16;
-  int* wave_sums = reinterpret_cast<int*>(l_lds + kWaves * 16);
-  int* sums = wave_sums + kWaves;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int page_shift = __builtin_ctz(ps) - 5;  // chunks per page, log2
 
-  sum_chunks(a, sums, wave_sums);
-  const int64_t total = (int64_t)sums[a.batch] * H;
-  int64_t per = (total + gridDim.x - 1) / gridDim.x;
-  if (per < kMinChunks) per = kMinChunks;
-  int64_t f = blockIdx.x * per;
-  const int64_t f_end = f + per < total ? f + per : total;
-
-  // rows without a key
-  uint16_t* out_all = reinterpret_cast<uint16_t*>(a.out);
-  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-    if (sums[b + 1] != sums[b]) continue;
-    for (int i = tid; i < H * R * D; i += kThreads) out_all[(int64_t)b * H * R * D + i] = 0;
-    for (int h = tid; h < H; h += kThreads) ws.ranges[b * H + h] = make_int2(0, 0);
+  Piece piece{0, 0, 0, 1, 0, RowKeys{0, 0}};
+  if constexpr (SPLIT) {
+    if (!find_piece(a, room, kWaves, lane, piece)) return;
+  } else {
+    const int pairs = a.batch * H, share = (pairs + kXcds - 1) / kXcds;
+    const int y = blockIdx.x / kXcds, pair = (int)(blockIdx.x % kXcds) * share + y;
+    if (y >= share || pair >= pairs) return;
+    piece.b = pair / H;
+    piece.h = pair - piece.b * H;
+    piece.keys = row_keys(a, piece.b);
   }
-  if (f >= f_end) return;
+  const int b = piece.b, h = piece.h, pair = b * H + h;
+  const RowKeys keys = piece.keys;
+  const int n = keys.chunks();
+  // piece i of k: chunks [i n / k, (i + 1) n / k)
+  const int c_first = keys.first() + (SPLIT ? (int)((int64_t)n * piece.index / piece.count) : 0);
+  const int last = keys.first() + (SPLIT ? (int)((int64_t)n * (piece.index + 1) / piece.count) : n);
 
-  int b = 0;  // the row of chunk f: the last with sums[b] * H <= f
-  for (int lo = 0, hi = a.batch; hi - lo > 1;) {
-    const int mid = (lo + hi) >> 1;
-    if ((int64_t)sums[mid] * H <= f) lo = mid; else hi = mid;
-    b = lo;
-  }
-
-  while (f < f_end) {
-    while (sums[b + 1] == sums[b] || (int64_t)sums[b + 1] * H <= f) ++b;
-    b = __builtin_amdgcn_readfirstlane(b);
-    const RowKeys keys = row_keys(a, b);
-    const int n = keys.chunks();
-    const int64_t row_f = f - (int64_t)sums[b] * H;
-    const int h = __builtin_amdgcn_readfirstlane((int)(row_f / n));
-    const int pair = b * H + h;
-    const int64_t pair_f = (int64_t)sums[b] * H + (int64_t)h * n;  // the pair's first chunk
-    const int c0 = __builtin_amdgcn_readfirstlane((int)(f - pair_f));
-    const int64_t f_next = pair_f + n < f_end ? pair_f + n : f_end;
-    const int c1 = __builtin_amdgcn_readfirstlane((int)(f_next - pair_f));
-
-    float m = kNegInf, l = 0.f;
-    floatx4 o[D / 16];
+  // the q rows on their way to LDS, asked for before the keys: loads return in order
+  constexpr int kQLoads = 16 * D / 8 / kThreads > 0 ? 16 * D / 8 / kThreads : 1;
+  u32x4 qv[kQLoads];
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) o[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < kQLoads; ++j)
+    if (tid + j * kThreads < R * D / 8)
+      qv[j] = load16(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)pair * R * D + (tid + j * kThreads) * 8);
 
-    // One chunk ahead: the loads of a wave's next chunk are issued as the registers of this one's keys, then of
-    // its values, become free. A chunk without a page has a resource of no bytes: its loads give zeros.
-    u32x4 kv[2][Sh::KRUNS], vv[Sh::VLOADS];
-    uint2 kscale = make_uint2(0, 0), vscale = make_uint2(0, 0);
-    const int32_t* table = a.page_table + b * a.table_stride;
-    struct Place {
-      int64_t slot;  // slots before the chunk in the pool, of this head
-      bool there;
-    };
-    auto place_of = [&](int page, int c) -> Place {
-      const bool there = (uint32_t)page < (uint32_t)a.cache.num_pages;
-      return Place{((int64_t)(there ? page : 0) * H + h) * ps + (c * 32 & (ps - 1)), there};
-    };
-    auto page_of = [&](int c) -> int { return __builtin_amdgcn_readfirstlane(table[c >> page_shift]); };
-    auto load_keys = [&](const Place& at) {
-      const __amdgpu_buffer_rsrc_t r =
-          make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.key) + at.slot * (D * Sh::BYTES), at.there ? Sh::CHUNK : 0);
+  float m = kNegInf, l = 0.f;
+  floatx4 o[D / 16];
 #pragma unroll
-      for (int s = 0; s < Sh::KRUNS; ++s)
-#pragma unroll
-        for (int bb = 0; bb < 2; ++bb) kv[bb][s] = buffer_load16(r, col * 64 + grp * 16, (s * 2 + bb) * 1024);
-      if constexpr (F8) {
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.cache.key_scale + at.slot, at.there ? 32 : 0);
-        kscale = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * grp, 0, 0));
-      }
-    };
-    auto load_values = [&](const Place& at) {
-      const __amdgpu_buffer_rsrc_t r =
-          make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.value) + at.slot * (D * Sh::BYTES), at.there ? Sh::CHUNK : 0);
-#pragma unroll
-      for (int t = 0; t < Sh::VLOADS; ++t) vv[t] = buffer_load16(r, (grp * (Sh::VLOADS * 16) + col) * 16, t * 256);
-      if constexpr (F8) {
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.cache.value_scale + at.slot, at.there ? 32 : 0);
-        vscale = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * grp, 0, 0));
-      }
-    };
+  for (int t = 0; t < D / 16; ++t) o[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-    const int last = keys.first() + c1;
-    int c = keys.first() + c0 + w;
-    Place at{0, false};
-    int page_next = 0;
-    if (c < last) {
-      at = place_of(page_of(c), c);
-      load_keys(at);
-      load_values(at);
-      if (c + kWaves < last) page_next = page_of(c + kWaves);
+  // One chunk ahead: the loads of a wave's next chunk are issued as the registers of this one's keys, then of
+  // its values, become free. A chunk without a page has a resource of no bytes: its loads give zeros.
+  u32x4 kv[2][Sh::KRUNS], vv[Sh::VLOADS];
+  uint2 kscale = make_uint2(0, 0), vscale = make_uint2(0, 0);
+  const int32_t* table = a.page_table + b * a.table_stride;
+  struct Place {
+    int64_t slot;  // slots before the chunk in the pool, of this head
+    bool there;
+  };
+  auto place_of = [&](int page, int c) -> Place {
+    const bool there = (uint32_t)page < (uint32_t)a.cache.num_pages;
+    return Place{((int64_t)(there ? page : 0) * H + h) * ps + (c * 32 & (ps - 1)), there};
+  };
+  // the pages of this wave's next 64 chunks, one per lane
+  int pages = -1;
+  auto load_pages = [&](int c) {
+    const int mine = c + lane * kWaves;
+    pages = mine < last ? table[mine >> page_shift] : -1;
+  };
+  auto load_keys = [&](const Place& at) {
+    const __amdgpu_buffer_rsrc_t r =
+        make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.key) + at.slot * (D * Sh::BYTES), at.there ? Sh::CHUNK : 0);
+#pragma unroll
+    for (int s = 0; s < Sh::KRUNS; ++s)
+#pragma unroll
+      for (int bb = 0; bb < 2; ++bb) kv[bb][s] = buffer_load16(r, col * 64 + grp * 16, (s * 2 + bb) * 1024);
+    if constexpr (F8) {
+      const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.cache.key_scale + at.slot, at.there ? 32 : 0);
+      kscale = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * grp, 0, 0));
     }
-    // q rows in LDS; the columns beyond them compute on the last row and are dropped
-    for (int i = tid; i < R * D / 8; i += kThreads)
-      *reinterpret_cast<u32x4*>(q_lds + i / (D / 8) * q_stride(D) + i % (D / 8) * 8) =
-          load16(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)pair * R * D + i * 8);
-    __syncthreads();
-    const uint16_t* qrow = q_lds + (col < R ? col : R - 1) * q_stride(D) + (F8 ? 16 : 8) * grp;
-    // operand s: e4m3 keys come 16 consecutive dims a load, two operands
-    auto qop = [&](int s) -> bf16x8 { return as_bf16x8(load16(qrow + (F8 ? 64 * (s / 2) + 8 * (s % 2) : 32 * s))); };
-    for (; c < last; c += kWaves) {
-      const bool more = c + kWaves < last;
-      const Place next = place_of(more ? page_next : -1, c + kWaves);
-      if (c + 2 * kWaves < last) page_next = page_of(c + 2 * kWaves);
-      const int lo = at.there ? keys.lo : keys.hi, hi = keys.hi;  // this chunk's keys are those in [lo, hi)
-      floatx4 sc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+  };
+  auto load_values = [&](const Place& at) {
+    const __amdgpu_buffer_rsrc_t r =
+        make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.value) + at.slot * (D * Sh::BYTES), at.there ? Sh::CHUNK : 0);
 #pragma unroll
-      for (int s = 0; s < Sh::KRUNS; ++s)
-#pragma unroll
-        for (int bb = 0; bb < 2; ++bb) {
-          if constexpr (F8) {
-            sc[bb] = mfma16x16x32(e4m3_operand(kv[bb][s][0], kv[bb][s][1]), qop(2 * s), sc[bb]);
-            sc[bb] = mfma16x16x32(e4m3_operand(kv[bb][s][2], kv[bb][s][3]), qop(2 * s + 1), sc[bb]);
-          } else {
-            sc[bb] = mfma16x16x32(as_bf16x8(kv[bb][s]), qop(s), sc[bb]);
-          }
-        }
-      if constexpr (F8) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sc[j / 4][j % 4] *= exp2_byte((j < 4 ? kscale.x : kscale.y) >> (8 * (j % 4)) & 0xff);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (more) load_keys(next);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int t = 0; t < Sh::VLOADS; ++t) vv[t] = buffer_load16(r, (grp * (Sh::VLOADS * 16) + col) * 16, t * 256);
+    if constexpr (F8) {
+      const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.cache.value_scale + at.slot, at.there ? 32 : 0);
+      vscale = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * grp, 0, 0));
+    }
+  };
 
-      // keys 8 grp + j of the chunk
-      const bool inner = c * 32 >= lo && c * 32 + 32 <= hi;  // every slot is an attended key
-      float p[8], mx = m;
-      const int first = c * 32 + 8 * grp;
+  int c = c_first + w, turn = 0;  // the wave's chunk and its number among the wave's
+  // the first page by the scalar cache, the sooner
+  const int entry = (c < last ? c : (last > 0 ? last - 1 : 0)) >> page_shift;
+  const int page = __builtin_amdgcn_readfirstlane(table[entry]);
+  load_pages(c);
+  // every load below is issued by every wave, so that the waits for them can count: no branch but zero bytes
+  Place at = place_of(c < last ? page : -1, c);
+  load_keys(at);
+  load_values(at);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = inner || (first + j >= lo && first + j < hi) ? sc[j / 4][j % 4] : kNegInf;
-        mx = fmaxf(mx, p[j]);
+  for (int j = 0; j < kQLoads; ++j)
+    if (tid + j * kThreads < R * D / 8)
+      *reinterpret_cast<u32x4*>(q_lds + (tid + j * kThreads) / (D / 8) * q_stride(D) + tid % (D / 8) * 8) = qv[j];
+  __syncthreads();
+  // the columns beyond the R rows compute on the last row and are dropped
+  const uint16_t* qrow = q_lds + (col < R ? col : R - 1) * q_stride(D) + (F8 ? 16 : 8) * grp;
+  // operand s: e4m3 keys come 16 consecutive dims a load, two operands
+  auto qop = [&](int s) -> bf16x8 { return as_bf16x8(load16(qrow + (F8 ? 64 * (s / 2) + 8 * (s % 2) : 32 * s))); };
+  for (; c < last; c += kWaves) {
+    const bool more = c + kWaves < last;
+    ++turn;
+    if ((turn & 63) == 0) load_pages(c + kWaves);
+    const Place next = place_of(more ? __builtin_amdgcn_readlane(pages, turn & 63) : -1, c + kWaves);
+    const int lo = at.there ? keys.lo : keys.hi, hi = keys.hi;  // this chunk's keys are those in [lo, hi)
+    floatx4 sc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int s = 0; s < Sh::KRUNS; ++s)
+#pragma unroll
+      for (int bb = 0; bb < 2; ++bb) {
+        if constexpr (F8) {
+          sc[bb] = mfma16x16x32(e4m3_operand(kv[bb][s][0], kv[bb][s][1]), qop(2 * s), sc[bb]);
+          sc[bb] = mfma16x16x32(e4m3_operand(kv[bb][s][2], kv[bb][s][3]), qop(2 * s + 1), sc[bb]);
+        } else {
+          sc[bb] = mfma16x16x32(as_bf16x8(kv[bb][s]), qop(s), sc[bb]);
+        }
       }
-      mx = column_max(mx);
-      const float base = mx == kNegInf ? 0.f : mx;
+    if constexpr (F8) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sc[j / 4][j % 4] *= exp2_byte((j < 4 ? kscale.x : kscale.y) >> (8 * (j % 4)) & 0xff);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    load_keys(next);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // keys 8 grp + j of the chunk
+    const bool inner = c * 32 >= lo && c * 32 + 32 <= hi;  // every slot is an attended key
+    float p[8], mx = m;
+    const int first = c * 32 + 8 * grp;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      p[j] = inner || (first + j >= lo && first + j < hi) ? sc[j / 4][j % 4] : kNegInf;
+      mx = fmaxf(mx, p[j]);
+    }
+    mx = column_max(mx);
+    const float base = mx == kNegInf ? 0.f : mx;
+    if (__any(mx > m)) {
       const float alpha = __builtin_amdgcn_exp2f((m - base) * kLog2e);
       m = mx;
       l *= alpha;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) o[t] *= alpha;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = __builtin_amdgcn_exp2f((p[j] - base) * kLog2e);
-        l += p[j];
-        if constexpr (F8) {
-          const float v = p[j] * exp2_byte((j < 4 ? vscale.x : vscale.y) >> (8 * (j % 4)) & 0xff);
-          p[j] = inner || (first + j >= lo && first + j < hi) ? v : 0.f;
-        }
-      }
-      const bf16x8 pop = as_bf16x8(u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
-                                         pack_bf16x2(p[6], p[7])});
-      if (!inner) {  // the slots of no attended key may hold anything: 0 x NaN is no 0
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // e4m3: dword i is keys 4 (i % 2) .. + 3; bf16: keys 2 i, 2 i + 1
-          constexpr int KEYS = F8 ? 4 : 2;
-          uint32_t mask = 0;
-#pragma unroll
-          for (int j = 0; j < KEYS; ++j) {
-            const int key = first + KEYS * (i % (8 / KEYS)) + j;
-            if (key >= lo && key < hi) mask |= (F8 ? 0xffu : 0xffffu) << (32 / KEYS * j);
-          }
-#pragma unroll
-          for (int t = 0; t < Sh::VLOADS; ++t) vv[t][i] &= mask;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < Sh::VLOADS; ++t) {
-        if constexpr (F8) {
-          o[2 * t] = mfma16x16x32(e4m3_operand(vv[t][0], vv[t][1]), pop, o[2 * t]);
-          o[2 * t + 1] = mfma16x16x32(e4m3_operand(vv[t][2], vv[t][3]), pop, o[2 * t + 1]);
-        } else {
-          o[t] = mfma16x16x32(as_bf16x8(vv[t]), pop, o[t]);
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (more) load_values(next);
-      __builtin_amdgcn_sched_barrier(0);
-      at = next;
     }
-
-    // the waves' parts joined: o = sum_w exp(m_w - m) o_w, l likewise
-    l = column_sum(l);
-    if (grp == 0) m_lds[w * 16 + col] = m, l_lds[w * 16 + col] = l;
-    if (col < R) {
-      float* dst = lds + (w * R + col) * D;
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // row 4 grp + i of tile t is dim 16 t + 4 grp + i (bf16), or 32 (t / 2) + 2 (4 grp + i) + t % 2 (e4m3)
-          const int d = F8 ? 32 * (t / 2) + 2 * (4 * grp + i) + t % 2 : 16 * t + 4 * grp + i;
-          dst[d] = o[t][i];
-        }
-    }
-    __syncthreads();
-    const bool whole = c0 == 0 && c1 == n;
-    const int64_t part = 2 * (int64_t)blockIdx.x + (c0 == 0 ? 1 : 0);  // begun here: the range's last, else its first
-    uint16_t* out = out_all + (int64_t)pair * R * D;
-    for (int i = tid; i < R * D; i += kThreads) {
-      const int r = i / D;
-      float mm = kNegInf;
-#pragma unroll
-      for (int v = 0; v < kWaves; ++v) mm = fmaxf(mm, m_lds[v * 16 + r]);
-      const float base = mm == kNegInf ? 0.f : mm;
-      float num = 0.f, den = 0.f;
-#pragma unroll
-      for (int v = 0; v < kWaves; ++v) {
-        const float x = __builtin_amdgcn_exp2f((m_lds[v * 16 + r] - base) * kLog2e);
-        num += x * lds[v * R * D + i];
-        den += x * l_lds[v * 16 + r];
+    for (int j = 0; j < 8; ++j) {
+      p[j] = __builtin_amdgcn_exp2f((p[j] - base) * kLog2e);
+      l += p[j];
+      if constexpr (F8) {
+        const float v = p[j] * exp2_byte((j < 4 ? vscale.x : vscale.y) >> (8 * (j % 4)) & 0xff);
+        p[j] = inner || (first + j >= lo && first + j < hi) ? v : 0.f;
       }
-      if (whole) {
-        out[i] = (uint16_t)f32_to_bf16_bits(den == 0.f ? 0.f : num / den);
+    }
+    const bf16x8 pop = as_bf16x8(u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
+                                       pack_bf16x2(p[6], p[7])});
+    if (!inner) {  // the slots of no attended key may hold anything: 0 x NaN is no 0
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // e4m3: dword i is keys 4 (i % 2) .. + 3; bf16: keys 2 i, 2 i + 1
+        constexpr int KEYS = F8 ? 4 : 2;
+        uint32_t mask = 0;
+#pragma unroll
+        for (int j = 0; j < KEYS; ++j) {
+          const int key = first + KEYS * (i % (8 / KEYS)) + j;
+          if (key >= lo && key < hi) mask |= (F8 ? 0xffu : 0xffffu) << (32 / KEYS * j);
+        }
+#pragma unroll
+        for (int t = 0; t < Sh::VLOADS; ++t) vv[t][i] &= mask;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < Sh::VLOADS; ++t) {
+      if constexpr (F8) {
+        o[2 * t] = mfma16x16x32(e4m3_operand(vv[t][0], vv[t][1]), pop, o[2 * t]);
+        o[2 * t + 1] = mfma16x16x32(e4m3_operand(vv[t][2], vv[t][3]), pop, o[2 * t + 1]);
       } else {
-        ws.o[part * R * D + i] = num;
-        if (i % D == 0) ws.ml[(part * R + r) * 2] = mm, ws.ml[(part * R + r) * 2 + 1] = den;
+        o[t] = mfma16x16x32(as_bf16x8(vv[t]), pop, o[t]);
       }
     }
-    if (c0 == 0 && tid == 0) {
-      const int first_range = (int)(pair_f / per), last_range = (int)((pair_f + n - 1) / per);
-      ws.ranges[pair] = whole ? make_int2(0, 0) : make_int2(first_range, last_range - first_range + 1);
-    }
-    f = f_next;
-    if (f < f_end) __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(next);
+    __builtin_amdgcn_sched_barrier(0);
+    at = next;
   }
+
+  // the waves' parts joined: o = sum_w exp(m_w - m) o_w, l likewise
+  l = column_sum(l);
+  if (grp == 0) m_lds[w * 16 + col] = m, l_lds[w * 16 + col] = l;
+  if (col < R) {
+    float* dst = lds + (w * R + col) * D;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // row 4 grp + i of tile t is dim 16 t + 4 grp + i (bf16), or 32 (t / 2) + 2 (4 grp + i) + t % 2 (e4m3)
+        const int d = F8 ? 32 * (t / 2) + 2 * (4 * grp + i) + t % 2 : 16 * t + 4 * grp + i;
+        dst[d] = o[t][i];
+      }
+  }
+  __syncthreads();
+  const bool whole = !SPLIT || piece.count == 1;
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)pair * R * D;
+  for (int i = tid; i < R * D; i += kThreads) {
+    const int r = i / D;
+    float mm = kNegInf;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) mm = fmaxf(mm, m_lds[v * 16 + r]);
+    const float base = mm == kNegInf ? 0.f : mm;
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float x = __builtin_amdgcn_exp2f((m_lds[v * 16 + r] - base) * kLog2e);
+      num += x * lds[v * R * D + i];
+      den += x * l_lds[v * 16 + r];
+    }
+    if (whole) {
+      out[i] = (uint16_t)f32_to_bf16_bits(den == 0.f ? 0.f : num / den);
+    } else {
+      ws.o[(int64_t)piece.slot * R * D + i] = num;
+      if (i % D == 0) *reinterpret_cast<float2*>(ws.ml + ((int64_t)piece.slot * R + r) * 2) = make_float2(mm, den);
+    }
+  }
+  if (SPLIT && piece.index == 0 && tid == 0) ws.ranges[pair] = whole ? make_int2(0, 0) : make_int2(piece.slot, piece.count);
 }
 
 constexpr int kJoinDims = 64;  // elements of o per workgroup: 16 lanes of 4, 16 parts at a time
-constexpr int kJoinParts = kThreads / (kJoinDims / 4);
+constexpr int kJoinThreads = 256;
+constexpr int kJoinParts = kJoinThreads / (kJoinDims / 4);
 
-// The ranges' parts of a (row, head), joined in their order.
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(G4PagedDecodeArgs a, Workspace ws) {
+// The pieces of a (row, head), joined in their order; blockIdx.y of gridDim.y takes every so many stretches of
+// kJoinDims elements.
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(G4PagedDecodeArgs a, Workspace ws) {
   __shared__ float m_s[kJoinParts], l_s[kJoinParts];
   __shared__ __attribute__((aligned(16))) floatx4 o_s[kJoinParts][kJoinDims / 4];
   const int R = a.group, D = a.cache.head_dim;
-  const int pair = blockIdx.x, i0 = blockIdx.y * kJoinDims, r = i0 / D;
+  const int pair = blockIdx.x;
   const int2 range = ws.ranges[pair];
   if (range.y == 0) return;
   const int x = threadIdx.x % (kJoinDims / 4), y = threadIdx.x / (kJoinDims / 4);
-  // part j of the pair: the last of its first range, the first of the others
-  auto part = [&](int j) -> int64_t { return 2 * (int64_t)(range.x + j) + (j == 0 ? 1 : 0); };
-  float m = kNegInf;
-  for (int j = y; j < range.y; j += kJoinParts) m = fmaxf(m, ws.ml[(part(j) * R + r) * 2]);
-  if (x == 0) m_s[y] = m;
-  __syncthreads();
-  m = kNegInf;
-#pragma unroll
-  for (int j = 0; j < kJoinParts; ++j) m = fmaxf(m, m_s[j]);
-  const float base = m == kNegInf ? 0.f : m;
-  float l = 0.f;
-  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = blockIdx.y * kJoinDims; i0 < R * D; i0 += gridDim.y * kJoinDims) {
+    const int r = i0 / D;
+    // this lane's pieces y, y + 16, ..., each step's loads independent of the sums
+    float m = kNegInf, l = 0.f;
+    floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int j = y; j < range.y; j += kJoinParts) {
-    const int64_t at = part(j) * R + r;
-    const float f = __builtin_amdgcn_exp2f((ws.ml[at * 2] - base) * kLog2e);
-    l += f * ws.ml[at * 2 + 1];
-    o += f * *reinterpret_cast<const floatx4*>(ws.o + part(j) * R * D + i0 + 4 * x);
+    for (int j = y; j < range.y; j += kJoinParts) {
+      const int64_t at = (int64_t)(range.x + j) * R;
+      const float2 ml = *reinterpret_cast<const float2*>(ws.ml + (at + r) * 2);
+      const floatx4 part = *reinterpret_cast<const floatx4*>(ws.o + at * D + i0 + 4 * x);
+      const float mx = fmaxf(m, ml.x), base = mx == kNegInf ? 0.f : mx;
+      const float f = __builtin_amdgcn_exp2f((m - base) * kLog2e), g = __builtin_amdgcn_exp2f((ml.x - base) * kLog2e);
+      m = mx;
+      l = f * l + g * ml.y;
+      o = f * o + g * part;
+    }
+    if (x == 0) m_s[y] = m, l_s[y] = l;
+    o_s[y][x] = o;
+    __syncthreads();
+    if (y == 0) {
+      float mx = kNegInf;
+#pragma unroll
+      for (int j = 0; j < kJoinParts; ++j) mx = fmaxf(mx, m_s[j]);
+      const float base = mx == kNegInf ? 0.f : mx;
+      l = 0.f;
+      o = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < kJoinParts; ++j) {
+        const float f = __builtin_amdgcn_exp2f((m_s[j] - base) * kLog2e);
+        l += f * l_s[j];
+        o += f * o_s[j][x];
+      }
+      const float inv = 1.f / l;
+      if (l == 0.f) o = floatx4{0.f, 0.f, 0.f, 0.f};
+      else o *= inv;
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + (int64_t)pair * R * D + i0 + 4 * x) =
+          make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    }
+    __syncthreads();
   }
-  if (x == 0) l_s[y] = l;
-  o_s[y][x] = o;
-  __syncthreads();
-  if (y > 0) return;
-  for (int j = 1; j < kJoinParts; ++j) o += o_s[j][x], l += l_s[j];
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (l == 0.f) o = floatx4{0.f, 0.f, 0.f, 0.f};
-  uint2 w = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
-  *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + (int64_t)pair * R * D + i0 + 4 * x) = w;
 }
 
-size_t lds_bytes(int R, int D, int batch) {
-  return ((size_t)kWaves * R * D + (size_t)R * q_stride(D) / 2 + 2 * kWaves * 16 + kWaves + batch + 1) * sizeof(float);
+template <int D, bool SPLIT>
+size_t lds_bytes(int R) {
+  constexpr int W = Groups<D, SPLIT>::WAVES;
+  return ((size_t)W * R * D + (size_t)R * q_stride(D) / 2 + 2 * W * 16) * sizeof(float);
 }
 
-int groups(const G4PagedDecodeArgs& a) { return kCus * groups_per_cu(a.cache.head_dim); }
-
-// Rows of a launch: at most kMaxRows, and their chunks' sum fits 31 bits.
-int rows_per_launch(const G4PagedDecodeArgs& a) {
-  const int64_t chunks = (int64_t)a.max_pages * a.cache.page_size / 32;  // >= 1, < 2^26
-  const int64_t rows = 0x7fffffffLL / chunks;
-  return (int)(rows < kMaxRows ? (rows < a.batch ? rows : a.batch) : (kMaxRows < a.batch ? kMaxRows : a.batch));
+// Whether the rows are cut into pieces: where a row can have more chunks than its workgroup's waves take in
+// kWholeTurns turns.
+constexpr int kWholeTurns = 4;
+bool split(const G4PagedDecodeArgs& a) {
+  const int64_t cap = (int64_t)a.max_pages * a.cache.page_size;
+  const int64_t keys = a.window > 0 && a.window < cap ? a.window + 31 : cap;  // a window may begin inside a chunk
+  return (keys + 31) / 32 > (a.cache.head_dim == 512 ? 4 : 8) * kWholeTurns;
 }
+
+// A split (row, head) of n > per chunks has at most 2 n / per pieces, and per >= total / room but for the f32
+// division's rounding, for which there is room for a few more.
+constexpr int kSpare = 8;
+size_t slots(const G4PagedDecodeArgs& a) { return 2 * (size_t)resident(a.cache.head_dim) + kSpare; }
 
 size_t workspace_bytes(const G4PagedDecodeArgs& a) {
-  const size_t parts = 2 * (size_t)groups(a) * a.group;
-  return parts * a.cache.head_dim * 4 + parts * 8 + (size_t)rows_per_launch(a) * a.cache.kv_heads * 8;
+  if (!split(a)) return 0;
+  return slots(a) * a.group * ((size_t)a.cache.head_dim + 2) * 4 + (size_t)a.batch * a.cache.kv_heads * 8;
 }
 
-template <int D, bool F8>
-int launch(const G4PagedDecodeArgs& a, hipStream_t st) {
-  const size_t lds = lds_bytes(a.group, D, rows_per_launch(a));
+template <int D, bool F8, bool SPLIT>
+int launch_kernel(const G4PagedDecodeArgs& a, const Workspace& ws, int64_t groups, hipStream_t st) {
+  const size_t lds = lds_bytes<D, SPLIT>(a.group);
+  const void* fn = (const void*)paged_decode_kernel<D, F8, SPLIT>;
   if (lds > 64 * 1024) {
     int dev = 0;
     const int rc = device_setup(&dev);
     if (rc != G4_OK) return rc;
-    if (!lds_limit_raised(dev, (const void*)paged_decode_kernel<D, F8>))
+    if (!lds_limit_raised(dev, fn))
       return fail(G4_ERR_LAUNCH, "g4_paged_decode_attention: the kernel's LDS limit could not be raised");
   }
-  const int g = groups(a);
-  Workspace ws;
-  ws.o = reinterpret_cast<float*>(a.workspace);
-  ws.ml = ws.o + 2 * (size_t)g * a.group * D;
-  ws.ranges = reinterpret_cast<int2*>(ws.ml + 2 * (size_t)g * a.group * 2);
-  G4PagedDecodeArgs part = a;
-  for (int b = 0; b < a.batch; b += part.batch) {
-    part.batch = a.batch - b < rows_per_launch(a) ? a.batch - b : rows_per_launch(a);
-    const int64_t at = (int64_t)b * a.cache.kv_heads * a.group * D;
-    part.page_table = a.page_table + b * a.table_stride;
-    part.lengths = a.lengths + b;
-    part.q = reinterpret_cast<const uint16_t*>(a.q) + at;
-    part.out = reinterpret_cast<uint16_t*>(a.out) + at;
-    hipLaunchKernelGGL((paged_decode_kernel<D, F8>), dim3((unsigned)g), dim3(kThreads), lds, st, part, ws);
-    hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)(part.batch * a.cache.kv_heads), (unsigned)(a.group * D / kJoinDims)),
-                       dim3(kThreads), 0, st, part, ws);
-  }
+  const dim3 grid((unsigned)((groups + kXcds - 1) / kXcds * kXcds));
+  hipLaunchKernelGGL((paged_decode_kernel<D, F8, SPLIT>), grid, dim3(Groups<D, SPLIT>::THREADS), lds, st, a, ws, resident(D));
   return check_launch("g4_paged_decode_attention");
+}
+
+template <int D, bool F8>
+int launch(const G4PagedDecodeArgs& a, hipStream_t st) {
+  const int64_t pairs = (int64_t)a.batch * a.cache.kv_heads;
+  Workspace ws{};
+  if (!split(a)) return launch_kernel<D, F8, false>(a, ws, pairs, st);
+  ws.o = reinterpret_cast<float*>(a.workspace);
+  ws.ml = ws.o + slots(a) * a.group * D;
+  ws.ranges = reinterpret_cast<int2*>(ws.ml + slots(a) * a.group * 2);
+  const int rc = launch_kernel<D, F8, true>(a, ws, resident(D) + pairs + kSpare, st);
+  if (rc != G4_OK) return rc;
+  const int stretches = a.group * D / kJoinDims;
+  const dim3 grid((unsigned)pairs, (unsigned)(pairs * stretches <= 1024 ? stretches : 1));
+  hipLaunchKernelGGL(paged_join_kernel, grid, dim3(kJoinThreads), 0, st, a, ws);
+  return check_launch("g4_paged_decode_attention");
+}
+
+template <int D, bool F8, bool SPLIT>
+void setup(int device) {
+  const size_t most = lds_bytes<D, SPLIT>(16);
+  if (most > 64 * 1024) raise_lds_limit(device, (const void*)paged_decode_kernel<D, F8, SPLIT>, (int)most);
+}
+template <int D>
+void setup(int device) {
+  setup<D, false, false>(device), setup<D, false, true>(device);
+  setup<D, true, false>(device), setup<D, true, true>(device);
 }
 
 }  // namespace
 
 int setup_paged_kernels(int device) {
-  const struct {
-    const void* fn;
-    int dim;
-  } kernels[] = {
-      {(const void*)paged_decode_kernel<64, false>, 64},   {(const void*)paged_decode_kernel<64, true>, 64},
-      {(const void*)paged_decode_kernel<128, false>, 128}, {(const void*)paged_decode_kernel<128, true>, 128},
-      {(const void*)paged_decode_kernel<256, false>, 256}, {(const void*)paged_decode_kernel<256, true>, 256},
-      {(const void*)paged_decode_kernel<512, false>, 512}, {(const void*)paged_decode_kernel<512, true>, 512},
-  };
-  for (const auto& k : kernels) {
-    const size_t most = lds_bytes(16, k.dim, kMaxRows);
-    if (most > 64 * 1024) raise_lds_limit(device, k.fn, (int)most);
-  }
+  setup<64>(device), setup<128>(device), setup<256>(device), setup<512>(device);
   return G4_OK;
 }
 
@@ -449,6 +526,11 @@ int check_decode(const G4PagedDecodeArgs& a, const char* who) {
     return fail(G4_ERR_INVALID, "%s: batch %d group %d (1..16) window %d", who, a.batch, a.group, a.window);
   if ((int64_t)a.batch * a.cache.kv_heads > 0x7fffffLL)
     return fail(G4_ERR_UNSUPPORTED, "%s: batch %d x %d kv heads", who, a.batch, a.cache.kv_heads);
+  if ((int64_t)a.max_pages * a.cache.page_size > 1 << 27)
+    return fail(G4_ERR_UNSUPPORTED, "%s: %d pages of %d positions pass 2^27 positions", who, a.max_pages, a.cache.page_size);
+  if ((int64_t)a.batch * a.cache.kv_heads * ((int64_t)a.max_pages * a.cache.page_size / 32) > 0x3fffffffLL)
+    return fail(G4_ERR_UNSUPPORTED, "%s: batch %d x %d kv heads x %d pages pass 2^35 positions", who, a.batch,
+                a.cache.kv_heads, a.max_pages);
   if (!a.lengths || !a.q || !a.out) return fail(G4_ERR_INVALID, "%s: lengths / q / out is NULL", who);
   if (reinterpret_cast<uintptr_t>(a.q) % 16 || reinterpret_cast<uintptr_t>(a.out) % 16)
     return fail(G4_ERR_INVALID, "%s: q / out must be 16-byte aligned", who);
@@ -471,7 +553,7 @@ extern "C" int g4_paged_decode_attention(const G4PagedDecodeArgs* args, void* st
   const int rc = check_decode(a, who);
   if (rc != G4_OK) return rc;
   const size_t need = workspace_bytes(a);
-  if (!a.workspace || a.workspace_bytes < need || reinterpret_cast<uintptr_t>(a.workspace) % 16)
+  if (need && (!a.workspace || a.workspace_bytes < need || reinterpret_cast<uintptr_t>(a.workspace) % 16))
     return fail(G4_ERR_WORKSPACE, "%s needs %zu bytes of 16-byte aligned workspace", who, need);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool f8 = a.cache.format == G4_PAGES_E4M3;

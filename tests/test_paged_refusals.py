@@ -111,6 +111,7 @@ def test_abi_refuses_bad_tables(name, make, override, match):
     ("g4_paged_decode_attention", _decode, dict(group=17), "group"),
     ("g4_paged_decode_attention", _decode, dict(window=-1), "window"),
     ("g4_paged_decode_attention", _decode, dict(batch=1 << 24), "batch"),
+    ("g4_paged_decode_attention", _decode, dict(batch=1 << 16, max_pages=1 << 18, table_stride=1 << 18), "positions"),
     ("g4_paged_decode_attention", _decode, dict(lengths=None), "NULL"),
     ("g4_paged_decode_attention", _decode, dict(out=None), "NULL"),
     ("g4_paged_decode_attention", _decode, dict(q=(1 << 12) + 2), "aligned"),
@@ -129,6 +130,21 @@ def test_abi_refuses_null_args():
     for name, _ in CALLS:
         assert getattr(_lib.lib(), name)(None, None) == _lib.G4_ERR_INVALID
     assert _lib.lib().g4_paged_decode_workspace_size(None) == 0
+
+
+def test_abi_checks_the_attention_workspace():
+    """Rows that one workgroup takes need none; longer ones a fixed number of slots, whatever the lengths."""
+
+    L = _lib.lib()
+    assert L.g4_paged_decode_workspace_size(ctypes.byref(_decode())) == 0
+    long = dict(max_pages=1000, table_stride=1000)
+    need = L.g4_paged_decode_workspace_size(ctypes.byref(_decode(**long)))
+    assert 0 < need == L.g4_paged_decode_workspace_size(ctypes.byref(_decode(max_pages=5000, table_stride=5000)))
+    assert L.g4_paged_decode_workspace_size(ctypes.byref(_decode(**long, window=512))) == 0
+    for ws, size in ((None, need), (1 << 12, need - 1), ((1 << 12) + 4, need)):
+        a = _decode(**long, workspace=ws, workspace_bytes=size)
+        assert L.g4_paged_decode_attention(ctypes.byref(a), None) == _lib.G4_ERR_WORKSPACE
+        assert re.search("workspace", L.g4_last_error().decode())
 
 
 def test_new_paged_layer():
