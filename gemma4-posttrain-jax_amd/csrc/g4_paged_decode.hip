@@ -21,13 +21,25 @@ constexpr int kCus = 256, kXcds = 8;
 
 template <int D, bool SPLIT>
 struct Groups {
-  static constexpr int SIMD_WAVES = D == 512 ? 1 : (D == 256 ? 2 : 4);  // resident, by registers
-  static constexpr int WAVES = SPLIT || D == 512 ? 4 : 8;                // per workgroup
+  static constexpr int SIMD_WAVES = D >= 256 ? 2 : 4;          // resident, by registers
+  static constexpr int WAVES = SPLIT && D < 512 ? 4 : 8;        // per workgroup
+  static constexpr int PARTS = D == 512 ? 2 : 1;                // waves that share a chunk, a half of the dims each
+  static constexpr int KEYS = WAVES / PARTS;                    // chunks in work at a time
   static constexpr int THREADS = 64 * WAVES;
 };
-// Workgroups of the split kernel that are resident at once (four waves: one on each SIMD).
+// Workgroups of the split kernel that are resident at once.
 constexpr int resident(int D) { return kCus * (D == 512 ? 1 : (D == 256 ? 2 : 4)); }
-constexpr int q_stride(int D) { return D + 8; }  // elements between q rows in LDS: 16 lanes' reads fall on different banks
+// elements between q rows (bf16) and between o rows (f32) in LDS: 16 rows' accesses fall on different banks
+constexpr int q_stride(int D) { return D + 8; }
+constexpr int o_stride(int D) { return D + 4; }
+
+// Floats of LDS for the waves' o; with two parts the scores of two turns are exchanged there before.
+template <int D, bool SPLIT>
+__host__ __device__ constexpr int o_floats(int R) {
+  using G = Groups<D, SPLIT>;
+  const int o = G::KEYS * R * o_stride(D), scores = G::PARTS == 2 ? 2 * G::WAVES * 64 * 8 : 0;
+  return o > scores ? o : scores;
+}
 
 struct Workspace {
   float* o;      // [slots][R][D] o of each piece of a split (row, head)
@@ -46,12 +58,12 @@ __device__ __forceinline__ bf16x8 e4m3_operand(uint32_t w0, uint32_t w1) {
   return as_bf16x8(o);
 }
 
-template <int D, bool F8>
+// What one wave holds of a chunk: DW dims.
+template <int DW, bool F8>
 struct Shape {
-  static constexpr int KRUNS = F8 ? D / 64 : D / 32;  // 16-byte key loads per lane, chunk and half
-  static constexpr int VLOADS = F8 ? D / 32 : D / 16;  // 16-byte value loads per lane and chunk
+  static constexpr int KRUNS = F8 ? DW / 64 : DW / 32;  // 16-byte key loads per lane, chunk and half
+  static constexpr int VLOADS = F8 ? DW / 32 : DW / 16;  // 16-byte value loads per lane and chunk
   static constexpr int BYTES = F8 ? 1 : 2;
-  static constexpr int CHUNK = 32 * D * BYTES;  // bytes of a chunk's keys, and of its values
 };
 
 struct RowKeys {
@@ -60,10 +72,9 @@ struct RowKeys {
   __device__ __forceinline__ int chunks() const { return hi > lo ? ((hi + 31) >> 5) - (lo >> 5) : 0; }
 };
 
-__device__ __forceinline__ RowKeys row_keys(const G4PagedDecodeArgs& a, int b) {
+__device__ __forceinline__ RowKeys row_keys(const G4PagedDecodeArgs& a, int length) {
   const int cap = a.max_pages * a.cache.page_size;
-  int hi = a.lengths[b];
-  hi = hi < 0 ? 0 : (hi > cap ? cap : hi);
+  const int hi = length < 0 ? 0 : (length > cap ? cap : length);
   return RowKeys{a.window > 0 && hi > a.window ? hi - a.window : 0, hi};
 }
 
@@ -89,13 +100,30 @@ struct Piece {
 };
 
 // Piece blockIdx of a split call (false: none). Every wave finds it by itself: the rows' chunk counts are summed
-// over the wave, 64 rows at a time, then the pieces and the workspace slots before each row.
+// over the wave, kRows rows at a time (up to that many stay in registers), then the pieces and the workspace slots
+// before each row.
 // The host bounds the chunks of all (row, head) pairs by 2^30 and a row's by 2^22, which the f32 division needs.
+constexpr int kRowRegs = 4, kRows = 64 * kRowRegs;
+
 __device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room, int min_per, int lane, Piece& out) {
   const int H = a.cache.kv_heads, B = a.batch;
+  RowKeys rows[kRowRegs];  // of rows b0 + 64 i + lane; no positions behind the last row
+  auto load_rows = [&](int b0) {
+    int length[kRowRegs];
+#pragma unroll
+    for (int i = 0; i < kRowRegs; ++i) {
+      const int b = b0 + 64 * i + lane;
+      length[i] = a.lengths[b < B ? b : B - 1];
+    }
+#pragma unroll
+    for (int i = 0; i < kRowRegs; ++i) rows[i] = row_keys(a, b0 + 64 * i + lane < B ? length[i] : 0);
+  };
   int sum = 0;
-#pragma unroll 4
-  for (int b0 = 0; b0 < B; b0 += 64) sum += b0 + lane < B ? row_keys(a, b0 + lane).chunks() : 0;
+  for (int b0 = 0; b0 < B; b0 += kRows) {
+    load_rows(b0);
+#pragma unroll
+    for (int i = 0; i < kRowRegs; ++i) sum += rows[i].chunks();
+  }
   const int total = sum_lanes(sum) * H;
   // The least `per` of a few whose pieces are all resident at once: the rows' ends add at most one piece per
   // (row, head) to total / per, so the last of them does where there are fewer of those than room. Where there are
@@ -111,12 +139,13 @@ __device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room,
     n_pieces[i] = 0;
   }
   // ceil(n / per): floor((n - 1) / per) + 1, the quotient off a whole number by 1 / per at least where it is not one
-  auto pieces_of = [&](int n, float share) -> int { return n > 0 ? (int)((float)(n - 1) * share) + 1 : 1; };
-#pragma unroll 2
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const int n = b0 + lane < B ? row_keys(a, b0 + lane).chunks() : 0;
+  auto pieces_of = [&](int b, int n, float share) -> int { return b < B ? (n > 0 ? (int)((float)(n - 1) * share) : 0) + 1 : 0; };
+  for (int b0 = 0; b0 < B; b0 += kRows) {
+    if (B > kRows) load_rows(b0);
 #pragma unroll
-    for (int i = 0; i < kTries; ++i) n_pieces[i] += b0 + lane < B ? pieces_of(n, share[i]) : 0;
+    for (int j = 0; j < kRowRegs; ++j)
+#pragma unroll
+      for (int i = 0; i < kTries; ++i) n_pieces[i] += pieces_of(b0 + 64 * j + lane, rows[j].chunks(), share[i]);
   }
   float cut = share[kTries - 1];
   int count = 0;
@@ -129,27 +158,29 @@ __device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room,
   const int xcd_share = (count + kXcds - 1) / kXcds;
   const int y = blockIdx.x / kXcds, want = (int)(blockIdx.x % kXcds) * xcd_share + y;
   if (y >= xcd_share || want >= count) return false;
-  int before = 0, slots = 0;  // pieces and slots of the rows before this 64
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const bool on = b0 + lane < B;
-    const RowKeys keys = on ? row_keys(a, b0 + lane) : RowKeys{0, 0};
-    const int k = on ? pieces_of(keys.chunks(), cut) : 0, used = k > 1 ? k * H : 0;
-    const int incl = scan_incl(k * H), sincl = scan_incl(used);
-    const int end = before + __builtin_amdgcn_readlane(incl, 63);
-    if (want < end) {
-      const int at = __builtin_popcountll(__ballot(before + incl <= want));  // the row's lane
-      const int kk = __builtin_amdgcn_readlane(k, at);
-      const int local = want - before - (__builtin_amdgcn_readlane(incl, at) - kk * H);
-      out.b = b0 + at;
-      out.h = __builtin_amdgcn_readfirstlane(local / kk);
-      out.index = local - out.h * kk;
-      out.count = kk;
-      out.slot = slots + __builtin_amdgcn_readlane(sincl, at) - (kk > 1 ? kk * H : 0) + local;
-      out.keys = RowKeys{__builtin_amdgcn_readlane(keys.lo, at), __builtin_amdgcn_readlane(keys.hi, at)};
-      return true;
+  int before = 0, slots = 0;  // pieces and slots of the rows before these 64
+  for (int b0 = 0; b0 < B; b0 += kRows) {
+    if (B > kRows) load_rows(b0);
+#pragma unroll
+    for (int j = 0; j < kRowRegs; ++j) {
+      const int k = pieces_of(b0 + 64 * j + lane, rows[j].chunks(), cut), used = k > 1 ? k * H : 0;
+      const int incl = scan_incl(k * H), sincl = scan_incl(used);
+      const int end = before + __builtin_amdgcn_readlane(incl, 63);
+      if (want < end) {
+        const int at = __builtin_popcountll(__ballot(before + incl <= want));  // the row's lane
+        const int kk = __builtin_amdgcn_readlane(k, at);
+        const int local = want - before - (__builtin_amdgcn_readlane(incl, at) - kk * H);
+        out.b = b0 + 64 * j + at;
+        out.h = __builtin_amdgcn_readfirstlane(local / kk);
+        out.index = local - out.h * kk;
+        out.count = kk;
+        out.slot = slots + __builtin_amdgcn_readlane(sincl, at) - (kk > 1 ? kk * H : 0) + local;
+        out.keys = RowKeys{__builtin_amdgcn_readlane(rows[j].lo, at), __builtin_amdgcn_readlane(rows[j].hi, at)};
+        return true;
+      }
+      before = end;
+      slots += __builtin_amdgcn_readlane(sincl, 63);
     }
-    before = end;
-    slots += __builtin_amdgcn_readlane(sincl, 63);
   }
   return false;
 }
@@ -157,28 +188,31 @@ __device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room,
 template <int D, bool F8, bool SPLIT>
 __global__ __launch_bounds__((Groups<D, SPLIT>::THREADS)) __attribute__((amdgpu_waves_per_eu(Groups<D, SPLIT>::SIMD_WAVES)))
 void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
-  using Sh = Shape<D, F8>;
-  constexpr int kWaves = Groups<D, SPLIT>::WAVES, kThreads = Groups<D, SPLIT>::THREADS;
-  // [kWaves][R][D] o | [R][q_stride(D)] q | [kWaves][16] m, l
+  using G = Groups<D, SPLIT>;
+  constexpr int kThreads = G::THREADS, kKeys = G::KEYS, DW = D / G::PARTS;
+  using Sh = Shape<DW, F8>;
+  constexpr int kChunkBytes = 32 * D * Sh::BYTES;
+  // [kKeys][R][o_stride(D)] o, in its place before that the score exchange | [R][q_stride(D)] q | [kKeys][16] m, l
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int R = a.group, H = a.cache.kv_heads, ps = a.cache.page_size;
-  uint16_t* q_lds = reinterpret_cast<uint16_t*>(lds + kWaves * R * D);
+  uint16_t* q_lds = reinterpret_cast<uint16_t*>(lds + o_floats<D, SPLIT>(R));
   float* m_lds = reinterpret_cast<float*>(q_lds + R * q_stride(D));
-  float* l_lds = m_lds + kWaves * 16;
+  float* l_lds = m_lds + kKeys * 16;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int key_wave = w / G::PARTS, half = G::PARTS == 2 ? w & 1 : 0;
   const int page_shift = __builtin_ctz(ps) - 5;  // chunks per page, log2
 
   Piece piece{0, 0, 0, 1, 0, RowKeys{0, 0}};
   if constexpr (SPLIT) {
-    if (!find_piece(a, room, kWaves, lane, piece)) return;
+    if (!find_piece(a, room, kKeys, lane, piece)) return;
   } else {
     const int pairs = a.batch * H, share = (pairs + kXcds - 1) / kXcds;
     const int y = blockIdx.x / kXcds, pair = (int)(blockIdx.x % kXcds) * share + y;
     if (y >= share || pair >= pairs) return;
     piece.b = pair / H;
     piece.h = pair - piece.b * H;
-    piece.keys = row_keys(a, piece.b);
+    piece.keys = row_keys(a, a.lengths[piece.b]);
   }
   const int b = piece.b, h = piece.h, pair = b * H + h;
   const RowKeys keys = piece.keys;
@@ -196,9 +230,9 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
       qv[j] = load16(reinterpret_cast<const uint16_t*>(a.q) + (int64_t)pair * R * D + (tid + j * kThreads) * 8);
 
   float m = kNegInf, l = 0.f;
-  floatx4 o[D / 16];
+  floatx4 o[DW / 16];
 #pragma unroll
-  for (int t = 0; t < D / 16; ++t) o[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < DW / 16; ++t) o[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   // One chunk ahead: the loads of a wave's next chunk are issued as the registers of this one's keys, then of
   // its values, become free. A chunk without a page has a resource of no bytes: its loads give zeros.
@@ -216,16 +250,17 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
   // the pages of this wave's next 64 chunks, one per lane
   int pages = -1;
   auto load_pages = [&](int c) {
-    const int mine = c + lane * kWaves;
+    const int mine = c + lane * kKeys;
     pages = mine < last ? table[mine >> page_shift] : -1;
   };
+  auto wait_pages = [&]() { __asm__ volatile("" : "+v"(pages)); };  // here, not at every use behind a branch
   auto load_keys = [&](const Place& at) {
     const __amdgpu_buffer_rsrc_t r =
-        make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.key) + at.slot * (D * Sh::BYTES), at.there ? Sh::CHUNK : 0);
+        make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.key) + at.slot * (D * Sh::BYTES), at.there ? kChunkBytes : 0);
 #pragma unroll
     for (int s = 0; s < Sh::KRUNS; ++s)
 #pragma unroll
-      for (int bb = 0; bb < 2; ++bb) kv[bb][s] = buffer_load16(r, col * 64 + grp * 16, (s * 2 + bb) * 1024);
+      for (int bb = 0; bb < 2; ++bb) kv[bb][s] = buffer_load16(r, col * 64 + grp * 16, ((half * Sh::KRUNS + s) * 2 + bb) * 1024);
     if constexpr (F8) {
       const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.cache.key_scale + at.slot, at.there ? 32 : 0);
       kscale = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * grp, 0, 0));
@@ -233,16 +268,16 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
   };
   auto load_values = [&](const Place& at) {
     const __amdgpu_buffer_rsrc_t r =
-        make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.value) + at.slot * (D * Sh::BYTES), at.there ? Sh::CHUNK : 0);
+        make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.value) + at.slot * (D * Sh::BYTES), at.there ? kChunkBytes : 0);
 #pragma unroll
-    for (int t = 0; t < Sh::VLOADS; ++t) vv[t] = buffer_load16(r, (grp * (Sh::VLOADS * 16) + col) * 16, t * 256);
+    for (int t = 0; t < Sh::VLOADS; ++t) vv[t] = buffer_load16(r, (grp * (D * Sh::BYTES / 2) + col) * 16, (half * Sh::VLOADS + t) * 256);
     if constexpr (F8) {
       const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.cache.value_scale + at.slot, at.there ? 32 : 0);
       vscale = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * grp, 0, 0));
     }
   };
 
-  int c = c_first + w, turn = 0;  // the wave's chunk and its number among the wave's
+  int c = c_first + key_wave, turn = 0;  // the wave's chunk and its number among the wave's
   // the first page by the scalar cache, the sooner
   const int entry = (c < last ? c : (last > 0 ? last - 1 : 0)) >> page_shift;
   const int page = __builtin_amdgcn_readfirstlane(table[entry]);
@@ -251,20 +286,26 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
   Place at = place_of(c < last ? page : -1, c);
   load_keys(at);
   load_values(at);
+  wait_pages();
 #pragma unroll
   for (int j = 0; j < kQLoads; ++j)
     if (tid + j * kThreads < R * D / 8)
       *reinterpret_cast<u32x4*>(q_lds + (tid + j * kThreads) / (D / 8) * q_stride(D) + tid % (D / 8) * 8) = qv[j];
   __syncthreads();
   // the columns beyond the R rows compute on the last row and are dropped
-  const uint16_t* qrow = q_lds + (col < R ? col : R - 1) * q_stride(D) + (F8 ? 16 : 8) * grp;
+  const uint16_t* qrow = q_lds + (col < R ? col : R - 1) * q_stride(D) + half * DW + (F8 ? 16 : 8) * grp;
   // operand s: e4m3 keys come 16 consecutive dims a load, two operands
   auto qop = [&](int s) -> bf16x8 { return as_bf16x8(load16(qrow + (F8 ? 64 * (s / 2) + 8 * (s % 2) : 32 * s))); };
-  for (; c < last; c += kWaves) {
-    const bool more = c + kWaves < last;
+  // two parts meet at a barrier in every turn, so all waves take the turns of the first
+  const int turns = (last - (G::PARTS == 2 ? c_first : c) + kKeys - 1) / kKeys;
+  while (turn < turns) {
+    const bool more = c + kKeys < last;
     ++turn;
-    if ((turn & 63) == 0) load_pages(c + kWaves);
-    const Place next = place_of(more ? __builtin_amdgcn_readlane(pages, turn & 63) : -1, c + kWaves);
+    if ((turn & 63) == 0) {
+      load_pages(c + kKeys);
+      wait_pages();
+    }
+    const Place next = place_of(more ? __builtin_amdgcn_readlane(pages, turn & 63) : -1, c + kKeys);
     const int lo = at.there ? keys.lo : keys.hi, hi = keys.hi;  // this chunk's keys are those in [lo, hi)
     floatx4 sc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -278,6 +319,15 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
           sc[bb] = mfma16x16x32(as_bf16x8(kv[bb][s]), qop(s), sc[bb]);
         }
       }
+    if constexpr (G::PARTS == 2) {  // the sum of both halves' scores, the same in both waves
+      float* mine = lds + (((turn & 1) * G::WAVES + w) * 64 + lane) * 8;
+      const float* other = lds + (((turn & 1) * G::WAVES + (w ^ 1)) * 64 + lane) * 8;
+      *reinterpret_cast<floatx4*>(mine) = sc[0];
+      *reinterpret_cast<floatx4*>(mine + 4) = sc[1];
+      wg_barrier();
+      sc[0] += *reinterpret_cast<const floatx4*>(other);
+      sc[1] += *reinterpret_cast<const floatx4*>(other + 4);
+    }
     if constexpr (F8) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) sc[j / 4][j % 4] *= exp2_byte((j < 4 ? kscale.x : kscale.y) >> (8 * (j % 4)) & 0xff);
@@ -289,10 +339,12 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
     // keys 8 grp + j of the chunk
     const bool inner = c * 32 >= lo && c * 32 + 32 <= hi;  // every slot is an attended key
     float p[8], mx = m;
-    const int first = c * 32 + 8 * grp;
+    bool on[8];
+    const int j_lo = lo - (c * 32 + 8 * grp), j_hi = hi - (c * 32 + 8 * grp);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = inner || (first + j >= lo && first + j < hi) ? sc[j / 4][j % 4] : kNegInf;
+      on[j] = (j >= j_lo) & (j < j_hi);
+      p[j] = on[j] ? sc[j / 4][j % 4] : kNegInf;
       mx = fmaxf(mx, p[j]);
     }
     mx = column_max(mx);
@@ -302,7 +354,7 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
       m = mx;
       l *= alpha;
 #pragma unroll
-      for (int t = 0; t < D / 16; ++t) o[t] *= alpha;
+      for (int t = 0; t < DW / 16; ++t) o[t] *= alpha;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -310,7 +362,7 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
       l += p[j];
       if constexpr (F8) {
         const float v = p[j] * exp2_byte((j < 4 ? vscale.x : vscale.y) >> (8 * (j % 4)) & 0xff);
-        p[j] = inner || (first + j >= lo && first + j < hi) ? v : 0.f;
+        p[j] = on[j] ? v : 0.f;
       }
     }
     const bf16x8 pop = as_bf16x8(u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
@@ -322,10 +374,7 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
         constexpr int KEYS = F8 ? 4 : 2;
         uint32_t mask = 0;
 #pragma unroll
-        for (int j = 0; j < KEYS; ++j) {
-          const int key = first + KEYS * (i % (8 / KEYS)) + j;
-          if (key >= lo && key < hi) mask |= (F8 ? 0xffu : 0xffffu) << (32 / KEYS * j);
-        }
+        for (int j = 0; j < KEYS; ++j) mask |= on[KEYS * (i % (8 / KEYS)) + j] ? (F8 ? 0xffu : 0xffffu) << (32 / KEYS * j) : 0u;
 #pragma unroll
         for (int t = 0; t < Sh::VLOADS; ++t) vv[t][i] &= mask;
       }
@@ -343,42 +392,51 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
     load_values(next);
     __builtin_amdgcn_sched_barrier(0);
     at = next;
+    c += kKeys;
   }
 
   // the waves' parts joined: o = sum_w exp(m_w - m) o_w, l likewise
   l = column_sum(l);
-  if (grp == 0) m_lds[w * 16 + col] = m, l_lds[w * 16 + col] = l;
+  if constexpr (G::PARTS == 2) __syncthreads();  // o takes the place of the last turn's exchange
+  if (grp == 0 && half == 0) m_lds[key_wave * 16 + col] = m, l_lds[key_wave * 16 + col] = l;
   if (col < R) {
-    float* dst = lds + (w * R + col) * D;
+    float* dst = lds + (key_wave * R + col) * o_stride(D) + half * DW;
+    // row 4 grp + i of tile t is dim 16 t + 4 grp + i (bf16), or 32 (t / 2) + 2 (4 grp + i) + t % 2 (e4m3)
+    if constexpr (F8) {
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // row 4 grp + i of tile t is dim 16 t + 4 grp + i (bf16), or 32 (t / 2) + 2 (4 grp + i) + t % 2 (e4m3)
-        const int d = F8 ? 32 * (t / 2) + 2 * (4 * grp + i) + t % 2 : 16 * t + 4 * grp + i;
-        dst[d] = o[t][i];
+      for (int t = 0; t < DW / 32; ++t) {
+        const floatx4 x = o[2 * t], y = o[2 * t + 1];
+        *reinterpret_cast<floatx4*>(dst + 32 * t + 8 * grp) = floatx4{x[0], y[0], x[1], y[1]};
+        *reinterpret_cast<floatx4*>(dst + 32 * t + 8 * grp + 4) = floatx4{x[2], y[2], x[3], y[3]};
       }
+    } else {
+#pragma unroll
+      for (int t = 0; t < DW / 16; ++t) *reinterpret_cast<floatx4*>(dst + 16 * t + 4 * grp) = o[t];
+    }
   }
   __syncthreads();
   const bool whole = !SPLIT || piece.count == 1;
   uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)pair * R * D;
-  for (int i = tid; i < R * D; i += kThreads) {
+  for (int i = 4 * tid; i < R * D; i += 4 * kThreads) {
     const int r = i / D;
     float mm = kNegInf;
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) mm = fmaxf(mm, m_lds[v * 16 + r]);
+    for (int v = 0; v < kKeys; ++v) mm = fmaxf(mm, m_lds[v * 16 + r]);
     const float base = mm == kNegInf ? 0.f : mm;
-    float num = 0.f, den = 0.f;
+    floatx4 num = {0.f, 0.f, 0.f, 0.f};
+    float den = 0.f;
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
+    for (int v = 0; v < kKeys; ++v) {
       const float x = __builtin_amdgcn_exp2f((m_lds[v * 16 + r] - base) * kLog2e);
-      num += x * lds[v * R * D + i];
+      num += x * *reinterpret_cast<const floatx4*>(lds + (v * R + r) * o_stride(D) + i % D);
       den += x * l_lds[v * 16 + r];
     }
     if (whole) {
-      out[i] = (uint16_t)f32_to_bf16_bits(den == 0.f ? 0.f : num / den);
+      const float inv = 1.f / den;
+      num = den == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : num * inv;
+      *reinterpret_cast<uint2*>(out + i) = make_uint2(pack_bf16x2(num[0], num[1]), pack_bf16x2(num[2], num[3]));
     } else {
-      ws.o[(int64_t)piece.slot * R * D + i] = num;
+      *reinterpret_cast<floatx4*>(ws.o + (int64_t)piece.slot * R * D + i) = num;
       if (i % D == 0) *reinterpret_cast<float2*>(ws.ml + ((int64_t)piece.slot * R + r) * 2) = make_float2(mm, den);
     }
   }
@@ -387,6 +445,7 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
 
 constexpr int kJoinDims = 64;  // elements of o per workgroup: 16 lanes of 4, 16 parts at a time
 constexpr int kJoinThreads = 256;
+constexpr int kJoinGroups = 2048;  // workgroups of a join, about
 constexpr int kJoinParts = kJoinThreads / (kJoinDims / 4);
 
 // The pieces of a (row, head), joined in their order; blockIdx.y of gridDim.y takes every so many stretches of
@@ -443,8 +502,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(G4PagedDecodeA
 
 template <int D, bool SPLIT>
 size_t lds_bytes(int R) {
-  constexpr int W = Groups<D, SPLIT>::WAVES;
-  return ((size_t)W * R * D + (size_t)R * q_stride(D) / 2 + 2 * W * 16) * sizeof(float);
+  using G = Groups<D, SPLIT>;
+  return ((size_t)o_floats<D, SPLIT>(R) + (size_t)R * q_stride(D) / 2 + 2 * G::KEYS * 16) * sizeof(float);
 }
 
 // Whether the rows are cut into pieces: where a row can have more chunks than its workgroup's waves take in
@@ -453,7 +512,7 @@ constexpr int kWholeTurns = 4;
 bool split(const G4PagedDecodeArgs& a) {
   const int64_t cap = (int64_t)a.max_pages * a.cache.page_size;
   const int64_t keys = a.window > 0 && a.window < cap ? a.window + 31 : cap;  // a window may begin inside a chunk
-  return (keys + 31) / 32 > (a.cache.head_dim == 512 ? 4 : 8) * kWholeTurns;
+  return (keys + 31) / 32 > (a.cache.head_dim == 512 ? Groups<512, false>::KEYS : Groups<256, false>::KEYS) * kWholeTurns;
 }
 
 // A split (row, head) of n > per chunks has at most 2 n / per pieces, and per >= total / room but for the f32
@@ -493,7 +552,7 @@ int launch(const G4PagedDecodeArgs& a, hipStream_t st) {
   const int rc = launch_kernel<D, F8, true>(a, ws, resident(D) + pairs + kSpare, st);
   if (rc != G4_OK) return rc;
   const int stretches = a.group * D / kJoinDims;
-  const dim3 grid((unsigned)pairs, (unsigned)(pairs * stretches <= 1024 ? stretches : 1));
+  const dim3 grid((unsigned)pairs, (unsigned)(pairs * stretches <= kJoinGroups ? stretches : (pairs < kJoinGroups ? kJoinGroups / pairs : 1)));
   hipLaunchKernelGGL(paged_join_kernel, grid, dim3(kJoinThreads), 0, st, a, ws);
   return check_launch("g4_paged_decode_attention");
 }
