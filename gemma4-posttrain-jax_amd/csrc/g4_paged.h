@@ -32,15 +32,6 @@ __device__ __forceinline__ float exp2_byte(int byte) { return __uint_as_float((u
 
 __device__ __forceinline__ bool finite_f32(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// Two values (already divided by the scale: magnitudes <= 448) to packed e4m3, round to nearest even;
-// infinities and NaN become NaN (0x7f).
-__device__ __forceinline__ uint32_t pack_e4m3x2(float a, float b) {
-  uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
-  if (!finite_f32(a)) w = (w & 0xff00u) | 0x7fu;
-  if (!finite_f32(b)) w = (w & 0x00ffu) | 0x7f00u;
-  return w;
-}
-
 // 4 packed e4m3 bytes -> 4 bf16 (exact).
 __device__ __forceinline__ void unpack_e4m3(uint32_t w, uint32_t& lo, uint32_t& hi) {
   lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));

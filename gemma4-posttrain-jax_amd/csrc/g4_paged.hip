@@ -37,131 +37,390 @@ int check_page_table(const int32_t* table, int32_t max_pages, int64_t table_stri
 namespace {
 
 // --- append ------------------------------------------------------------------------------------------------
+//
+// A head vector of a token is one wave's: lane l holds elements [l PER, (l + 1) PER), PER = D / 64, so a rotation's
+// partner (d +- D / 2) is lane l ^ 32 in the same element. f32 throughout, rounded once where it is stored: with
+// i = (mean(x^2) + eps)^-1/2, c and s the rotary row and w the norm's weights,
+//   y_d = i (x_d (w_d c_d) + x_(d +- D/2) (-+ w_(d +- D/2) s_d)),
+// whose factors w c and w s are formed once per token for all its heads.
 
-// One head vector of a token per wave: lane l holds elements [l * PER, (l + 1) * PER), PER = D / 64, so a
-// rotation's partner (d +- D / 2) is lane l ^ 32. f32 throughout: y = x * (mean(x^2) + eps)^-1/2 * w, then
-// y cos + rotate_half(y) sin.
-template <int D>
-struct HeadVec {
-  static constexpr int PER = D / 64;
-  float x[PER];
-
-  __device__ __forceinline__ void load(const uint16_t* p, int lane, bool vec) {
-    if (PER == 1 || !vec) {
+// PER bf16 elements of a row, and the way back.
+template <int PER>
+__device__ __forceinline__ void load_row(const uint16_t* p, bool vec, float (&x)[PER]) {
+  if (PER == 1 || !vec) {
 #pragma unroll
-      for (int e = 0; e < PER; ++e) x[e] = bf16_bits_to_f32(p[lane * PER + e]);
-    } else {
-      uint32_t w[PER / 2 > 0 ? PER / 2 : 1];
-      __builtin_memcpy(w, __builtin_assume_aligned(p + lane * PER, PER * 2), PER * 2);
+    for (int e = 0; e < PER; ++e) x[e] = bf16_bits_to_f32(p[e]);
+  } else {
+    uint32_t w[PER / 2 > 0 ? PER / 2 : 1];
+    __builtin_memcpy(w, __builtin_assume_aligned(p, PER * 2), PER * 2);
 #pragma unroll
-      for (int i = 0; i < PER / 2; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < PER / 2; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
-
-  __device__ __forceinline__ void norm(const HeadVec* w, float eps) {
-    float ss = 0.f;
+}
+template <int PER>
+__device__ __forceinline__ void store_row(uint16_t* p, const float (&x)[PER]) {
+  if constexpr (PER == 1) {
+    *p = (uint16_t)f32_to_bf16_bits(x[0]);
+  } else {
+    uint32_t w[PER / 2];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) ss += x[e] * x[e];
-    ss = wave_sum(ss);
-    const float inv = 1.0f / __fsqrt_rn(ss * (1.0f / D) + eps);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) x[e] = w ? x[e] * inv * w->x[e] : x[e] * inv;
+    for (int i = 0; i < PER / 2; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    __builtin_memcpy(__builtin_assume_aligned(p, PER * 2), w, PER * 2);
   }
+}
 
-  __device__ __forceinline__ void rotate(const float* c, const float* s, int lane) {
+// The value of lane ^ 32, per element.
+__device__ __forceinline__ float other_half(float x, int lane) {
+  const uint32_t u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(lane < 32 ? r[1] : r[0]);
+}
+
+// What a token's q or k heads have in common.
+template <int PER>
+struct Prepare {
+  float own[PER], other[PER];  // factors of x_d and of its partner; other unused without rotation
+  bool norm, rope;
+  float eps;
+
+  // weight: [D] or NULL; c, s: this lane's elements of the token's rotary row
+  __device__ __forceinline__ void load(const uint16_t* weight, bool vec, const float (&c)[PER], const float (&s)[PER], int lane) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) own[e] = 1.f;
+    if (weight) load_row<PER>(weight + lane * PER, vec, own);
+    if (!rope) return;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const uint32_t u = __float_as_uint(x[e]);
-      const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // the low / high half's value
-      const float partner = lane < 32 ? -__uint_as_float(r[1]) : __uint_as_float(r[0]);
-      x[e] = x[e] * c[e] + partner * s[e];
+      const float partner = other_half(own[e], lane);
+      other[e] = (lane < 32 ? -partner : partner) * s[e];
+      own[e] *= c[e];
     }
   }
 
-  // The scale byte of the whole vector, and this lane's elements divided by it.
-  __device__ __forceinline__ int quantise() {
-    float a = 0.f;
+  __device__ __forceinline__ void apply(float (&x)[PER], int lane) const {
+    float inv = 1.f;
+    if (norm) {
+      float ss = 0.f;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) a = fmaxf(a, finite_f32(x[e]) ? fabsf(x[e]) : 0.f);
-    const int byte = scale_byte(wave_max(a));
-    const float inv = __uint_as_float((uint32_t)(2 * kScaleBias - byte) << 23);
+      for (int e = 0; e < PER; ++e) ss += x[e] * x[e];
+      inv = __builtin_amdgcn_rsqf(wave_sum(ss) * (1.0f / (64 * PER)) + eps);
+    }
 #pragma unroll
-    for (int e = 0; e < PER; ++e) x[e] *= inv;
-    return byte;
+    for (int e = 0; e < PER; ++e) {
+      float y = x[e] * own[e];
+      if (rope) y += other_half(x[e], lane) * other[e];
+      x[e] = norm ? y * inv : y;
+    }
   }
 };
 
-enum VecKind { kQ = 0, kK = 1, kV = 2 };
+// A vector's scale byte and its e4m3 bytes (this lane's in the low bytes of `w`).
+template <int PER>
+__device__ __forceinline__ int quantise(const float (&x)[PER], uint32_t (&w)[PER > 4 ? 2 : 1]) {
+  uint32_t top = 0;  // |x| orders as its bits do, infinities and NaN above the rest
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    const uint32_t u = __float_as_uint(x[e]) & 0x7fffffffu;
+    top = u > top ? u : top;
+  }
+  top = __float_as_uint(wave_max(__uint_as_float(top < 0x7f800000u ? top : 0u)));
+  const bool odd_ones = __any([&] {
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) bad |= !finite_f32(x[e]);
+    return bad;
+  }());
+  float a = __uint_as_float(top);
+  if (odd_ones) {  // the largest of the finite elements
+    float f = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) f = fmaxf(f, finite_f32(x[e]) ? fabsf(x[e]) : 0.f);
+    a = wave_max(f);
+  }
+  const int byte = scale_byte(a);
+  const float inv = __uint_as_float((uint32_t)(2 * kScaleBias - byte) << 23);
+#pragma unroll
+  for (int i = 0; i < (PER > 4 ? 2 : 1); ++i) {
+    constexpr int N = PER > 4 ? 4 : PER;
+    uint32_t v = 0;
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float lo = x[4 * i + e] * inv, hi = N > 1 ? x[4 * i + (N > 1 ? e + 1 : 0)] * inv : 0.f;
+      v = e < 2 ? (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)v, false)
+                : (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)v, true);
+    }
+    if (odd_ones) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (!finite_f32(x[4 * i + e])) v |= 0x7fu << (8 * e);  // NaN (either sign)
+    }
+    w[i] = v;
+  }
+  return byte;
+}
 
-// One workgroup per token, one wave per head vector (looping over more than 16).
+template <int PER>
+__device__ __forceinline__ void store_bytes(uint8_t* p, const uint32_t (&w)[PER > 4 ? 2 : 1]) {
+  __builtin_memcpy(__builtin_assume_aligned(p, PER), w, PER);
+}
+
+// The rotary rows and factors of one token.
+template <int D>
+struct Token {
+  static constexpr int PER = D / 64;
+  Prepare<PER> q, k;
+  bool norm_v;
+
+  __device__ __forceinline__ void load(const G4PagedAppendArgs& a, int64_t token, bool vec, bool with_k, int lane) {
+    float c[PER], s[PER];
+    const bool any_rope = a.flags & (G4_APPEND_ROPE_Q | G4_APPEND_ROPE_K);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) c[e] = s[e] = 0.f;
+    if (any_rope) {
+      __builtin_memcpy(c, a.rope_cos + token * D + lane * PER, PER * 4);
+      __builtin_memcpy(s, a.rope_sin + token * D + lane * PER, PER * 4);
+    }
+    q.norm = a.flags & G4_APPEND_NORM_Q, q.rope = a.flags & G4_APPEND_ROPE_Q, q.eps = a.eps;
+    k.norm = a.flags & G4_APPEND_NORM_K, k.rope = a.flags & G4_APPEND_ROPE_K, k.eps = a.eps;
+    norm_v = a.flags & G4_APPEND_NORM_V;
+    if (a.q) q.load(q.norm ? reinterpret_cast<const uint16_t*>(a.q_norm_weight) : nullptr, vec, c, s, lane);
+    if (with_k) k.load(k.norm ? reinterpret_cast<const uint16_t*>(a.k_norm_weight) : nullptr, vec, c, s, lane);
+  }
+
+  __device__ __forceinline__ void prepare_v(float (&x)[PER], float eps) const {
+    if (!norm_v) return;
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) ss += x[e] * x[e];
+    const float inv = __builtin_amdgcn_rsqf(wave_sum(ss) * (1.0f / D) + eps);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) x[e] *= inv;
+  }
+};
+
+// A prepared key or value vector into its slot: keys in the page's runs, values one element per 8-slot group.
+template <int D, bool F8, bool KEY>
+__device__ __forceinline__ void store_vector(const G4PagedCache& c, int64_t block, int slot, const float (&x)[D / 64], int lane) {
+  constexpr int PER = D / 64;
+  uint8_t* pages = reinterpret_cast<uint8_t*>(KEY ? c.key : c.value) + block * D * (F8 ? 1 : 2);
+  if constexpr (F8) {
+    uint32_t w[PER > 4 ? 2 : 1];
+    const int byte = quantise<PER>(x, w);
+    if (lane == 0) (KEY ? c.key_scale : c.value_scale)[block + slot] = (uint8_t)byte;
+    if constexpr (KEY) {
+      store_bytes<PER>(pages + paged_key_index<true>(slot, lane * PER, D), w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) pages[vt_index(slot, lane * PER + e, D)] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+    }
+  } else {
+    uint16_t* p = reinterpret_cast<uint16_t*>(pages);
+    if constexpr (KEY) {
+      store_row<PER>(p + paged_key_index<false>(slot, lane * PER, D), x);
+    } else {
+#pragma unroll
+      for (int e = 0; e < PER; ++e) p[vt_index(slot, lane * PER + e, D)] = (uint16_t)f32_to_bf16_bits(x[e]);
+    }
+  }
+}
+
+// The page of position `pos` of row b if token s is stored there, else -1.
+__device__ __forceinline__ int page_of(const G4PagedAppendArgs& a, int b, int64_t pos, int s) {
+  const int shift = __builtin_ctz(a.cache.page_size);
+  if (pos < 0 || (pos >> shift) >= a.max_pages || (a.keep > 0 && s < a.seq - a.keep)) return -1;
+  const int page = a.page_table[b * a.table_stride + (pos >> shift)];
+  return (uint32_t)page < (uint32_t)a.cache.num_pages ? page : -1;
+}
+
+// A step's tokens (and chunks of fewer than 8): one workgroup per token, one wave per head vector (looping over
+// more than 16). A wave's single vector is a chain of loads, so nothing is staged: 256 tokens of 2 x (4 + 2)
+// heads of 256 in 5.2 us, of which the launch takes most.
 template <int D, bool F8>
 __global__ __launch_bounds__(1024) void paged_append_kernel(G4PagedAppendArgs a, int vec) {
   constexpr int PER = D / 64;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nwaves = blockDim.x >> 6;
-  const int S = a.seq, H = a.cache.kv_heads, R = a.group, ps = a.cache.page_size;
+  const int S = a.seq, H = a.cache.kv_heads;
   const int token = blockIdx.x, b = token / S, s = token - b * S;
-  const int nq = a.q ? H * R : 0, nvec = nq + 2 * H;
-
+  const int nq = a.q ? H * a.group : 0, nvec = nq + 2 * H;
+  const int64_t in_base = (int64_t)token * a.in_row_stride + lane * PER;
   const int64_t pos = (int64_t)a.write_pos[b] + s;
-  int page = -1;
-  if (pos >= 0 && pos < (int64_t)a.max_pages * ps && (a.keep == 0 || s >= S - a.keep))
-    page = a.page_table[b * a.table_stride + pos / ps];
-  const bool stored = (uint32_t)page < (uint32_t)a.cache.num_pages;
-  const int slot = (int)(pos & (ps - 1));
-
-  const int64_t in_base = (int64_t)token * a.in_row_stride, rope_base = (int64_t)token * D + lane * PER;
+  const int page = page_of(a, b, pos, s);
+  const int slot = (int)(pos & (a.cache.page_size - 1));
+  Token<D> t;
+  t.load(a, token, vec, true, lane);
   for (int v = wave; v < nvec; v += nwaves) {
-    const int kind = v < nq ? kQ : (v < nq + H ? kK : kV);
-    const int head = kind == kQ ? v : (kind == kK ? v - nq : v - nq - H);  // q: its place among H * R
-    if (kind != kQ && !stored) continue;
-    const uint16_t* src = reinterpret_cast<const uint16_t*>(kind == kQ ? a.q : (kind == kK ? a.k : a.v));
-    HeadVec<D> x;
-    x.load(src + in_base + (int64_t)head * D, lane, vec);
-    const bool norm = a.flags & (kind == kQ ? G4_APPEND_NORM_Q : (kind == kK ? G4_APPEND_NORM_K : G4_APPEND_NORM_V));
-    if (norm) {
-      HeadVec<D> w;
-      if (kind != kV) w.load(reinterpret_cast<const uint16_t*>(kind == kQ ? a.q_norm_weight : a.k_norm_weight), lane, vec);
-      x.norm(kind != kV ? &w : nullptr, a.eps);
-    }
-    if (kind != kV && (a.flags & (kind == kQ ? G4_APPEND_ROPE_Q : G4_APPEND_ROPE_K))) {
-      float c[PER], sn[PER];
-#pragma unroll
-      for (int e = 0; e < PER; ++e) c[e] = a.rope_cos[rope_base + e], sn[e] = a.rope_sin[rope_base + e];
-      x.rotate(c, sn, lane);
-    }
-    if (kind == kQ) {
-      uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + ((int64_t)token * nq + head) * D + lane * PER;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) dst[e] = (uint16_t)f32_to_bf16_bits(x.x[e]);
+    float x[PER];
+    if (v < nq) {
+      load_row<PER>(reinterpret_cast<const uint16_t*>(a.q) + in_base + (int64_t)v * D, vec, x);
+      t.q.apply(x, lane);
+      store_row<PER>(reinterpret_cast<uint16_t*>(a.q_out) + ((int64_t)token * nq + v) * D + lane * PER, x);
       continue;
     }
-    const int64_t block = ((int64_t)page * H + head) * ps;
-    if constexpr (F8) {
-      const int byte = x.quantise();
-      if (lane == 0) (kind == kK ? a.cache.key_scale : a.cache.value_scale)[block + slot] = (uint8_t)byte;
-    }
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int d = lane * PER + e;
-      const int64_t at = block * D + (kind == kK ? paged_key_index<F8>(slot, d, D) : (int)vt_index(slot, d, D));
-      void* dst = kind == kK ? a.cache.key : a.cache.value;
-      if constexpr (F8)
-        reinterpret_cast<uint8_t*>(dst)[at] = (uint8_t)pack_e4m3x2(x.x[e], 0.f);
-      else
-        reinterpret_cast<uint16_t*>(dst)[at] = (uint16_t)f32_to_bf16_bits(x.x[e]);
+    if (page < 0) continue;
+    const bool key = v < nq + H;
+    const int head = v - nq - (key ? 0 : H);
+    const int64_t block = ((int64_t)page * H + head) * a.cache.page_size;
+    load_row<PER>(reinterpret_cast<const uint16_t*>(key ? a.k : a.v) + in_base + (int64_t)head * D, vec, x);
+    if (key) {
+      t.k.apply(x, lane);
+      store_vector<D, F8, true>(a.cache, block, slot, x, lane);
+    } else {
+      t.prepare_v(x, a.eps);
+      store_vector<D, F8, false>(a.cache, block, slot, x, lane);
     }
   }
 }
 
+// Chunks of 8 tokens and more: one workgroup per 8 positions p, p % 8 == 0, of a row, one token per wave, whose
+// head vectors are loaded kTileVecs at a time. The page holds 8 positions' values of a dim side by side, so the
+// value rows of a full group pass through LDS and are stored as whole 16-byte pieces; a group that the chunk, the
+// pads or `keep` cut stores its values one by one.
+constexpr int kTileTok = 8;
+constexpr int kTileThreads = 64 * kTileTok;
+constexpr int kTileVecs = 4;
+constexpr int kTileValueBytes = 32 * 1024;  // LDS for value rows; more heads than fit go in turns
+
+template <int D, bool F8>
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(D >= 512 ? 4 : 8))) void
+paged_append_tile_kernel(G4PagedAppendArgs a, int vec, int groups) {
+  constexpr int PER = D / 64, BYTES = F8 ? 1 : 2;
+  constexpr int kHeads = kTileValueBytes / (kTileTok * D * BYTES);
+  extern __shared__ __attribute__((aligned(16))) uint8_t v_lds[];  // [min(H, kHeads)][8 tokens][D]
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int S = a.seq, H = a.cache.kv_heads;
+  const int b = (int)blockIdx.x / groups;
+  const int64_t start = a.write_pos[b];
+  const int64_t p0 = (start & ~(int64_t)(kTileTok - 1)) + ((int)blockIdx.x - b * groups) * kTileTok;
+  const int64_t s0 = p0 - start;  // token of p0: -7 ..
+  if (s0 >= S) return;
+  const bool full = s0 >= 0 && s0 + kTileTok <= S && page_of(a, b, p0, (int)s0) >= 0;  // one page, the first token the earliest
+  const int64_t s64 = s0 + wave;
+  const bool on = s64 >= 0 && s64 < S;
+  const int s = on ? (int)s64 : 0;
+  const int page = on ? page_of(a, b, p0 + wave, s) : -1;
+  const int slot = (int)((p0 + wave) & (a.cache.page_size - 1));
+  const int64_t token = (int64_t)b * S + s, in_base = token * a.in_row_stride + lane * PER;
+  Token<D> t;
+  if (on) t.load(a, token, vec, page >= 0, lane);
+  if (on && a.q) {
+    const int nq = H * a.group;
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + in_base;
+    uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + token * nq * D + lane * PER;
+    for (int v0 = 0; v0 < nq; v0 += kTileVecs) {
+      float x[kTileVecs][PER];
+#pragma unroll
+      for (int i = 0; i < kTileVecs; ++i)
+        if (v0 + i < nq) load_row<PER>(src + (v0 + i) * D, vec, x[i]);
+#pragma unroll
+      for (int i = 0; i < kTileVecs; ++i)
+        if (v0 + i < nq) {
+          t.q.apply(x[i], lane);
+          store_row<PER>(dst + (v0 + i) * D, x[i]);
+        }
+    }
+  }
+  const int64_t page_block = (int64_t)page * H;
+  for (int h0 = 0; h0 < H; h0 += kHeads) {
+    const int h1 = h0 + kHeads < H ? h0 + kHeads : H;
+    if (page >= 0) {
+      const uint16_t* ksrc = reinterpret_cast<const uint16_t*>(a.k) + in_base;
+      const uint16_t* vsrc = reinterpret_cast<const uint16_t*>(a.v) + in_base;
+      for (int h = h0; h < h1; h += kTileVecs / 2) {
+        float x[kTileVecs][PER];
+#pragma unroll
+        for (int i = 0; i < kTileVecs / 2; ++i)
+          if (h + i < h1) {
+            load_row<PER>(ksrc + (int64_t)(h + i) * D, vec, x[2 * i]);
+            load_row<PER>(vsrc + (int64_t)(h + i) * D, vec, x[2 * i + 1]);
+          }
+#pragma unroll
+        for (int i = 0; i < kTileVecs / 2; ++i) {
+          if (h + i >= h1) break;
+          const int64_t block = (page_block + h + i) * a.cache.page_size;
+          t.k.apply(x[2 * i], lane);
+          store_vector<D, F8, true>(a.cache, block, slot, x[2 * i], lane);
+          t.prepare_v(x[2 * i + 1], a.eps);
+          if (!full) {
+            store_vector<D, F8, false>(a.cache, block, slot, x[2 * i + 1], lane);
+            continue;
+          }
+          uint8_t* row = v_lds + ((h + i - h0) * kTileTok + wave) * D * BYTES;
+          if constexpr (F8) {
+            uint32_t w[PER > 4 ? 2 : 1];
+            const int byte = quantise<PER>(x[2 * i + 1], w);
+            if (lane == 0) a.cache.value_scale[block + slot] = (uint8_t)byte;
+            store_bytes<PER>(row + lane * PER, w);
+          } else {
+            store_row<PER>(reinterpret_cast<uint16_t*>(row) + lane * PER, x[2 * i + 1]);
+          }
+        }
+      }
+    }
+    if (!full) continue;  // uniform over the workgroup
+    __syncthreads();
+    // 32 bytes per thread: 8 slots of 4 (e4m3) or 2 (bf16) dims, of which LDS holds a dword per slot
+    const int slot0 = (int)(p0 & (a.cache.page_size - 1));
+    constexpr int DWORDS = D * BYTES / 4;  // per row
+    for (int i = threadIdx.x; i < (h1 - h0) * DWORDS; i += kTileThreads) {
+      const int head = i / DWORDS, dw = i - head * DWORDS;
+      const uint32_t* col = reinterpret_cast<const uint32_t*>(v_lds) + head * kTileTok * DWORDS + dw;
+      uint32_t r[kTileTok];
+#pragma unroll
+      for (int j = 0; j < kTileTok; ++j) r[j] = col[j * DWORDS];
+      uint32_t out[8];
+      if constexpr (F8) {
+        // bytes of slots 4 g .. 4 g + 3: dim k's are byte k of each
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const uint32_t lo01 = __builtin_amdgcn_perm(r[4 * g + 1], r[4 * g], 0x05010400);  // d0: s0 s1, d1: s0 s1
+          const uint32_t hi01 = __builtin_amdgcn_perm(r[4 * g + 1], r[4 * g], 0x07030602);  // d2: s0 s1, d3: s0 s1
+          const uint32_t lo23 = __builtin_amdgcn_perm(r[4 * g + 3], r[4 * g + 2], 0x05010400);
+          const uint32_t hi23 = __builtin_amdgcn_perm(r[4 * g + 3], r[4 * g + 2], 0x07030602);
+          out[0 + g] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100);
+          out[2 + g] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302);
+          out[4 + g] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100);
+          out[6 + g] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          out[j] = __builtin_amdgcn_perm(r[2 * j + 1], r[2 * j], 0x05040100);
+          out[4 + j] = __builtin_amdgcn_perm(r[2 * j + 1], r[2 * j], 0x07060302);
+        }
+      }
+      const int64_t block = (page_block + h0 + head) * a.cache.page_size;  // full: every wave has the group's page
+      u32x4* dst = reinterpret_cast<u32x4*>(reinterpret_cast<uint8_t*>(a.cache.value) + (block + slot0) * D * BYTES + dw * 32);
+      dst[0] = u32x4{out[0], out[1], out[2], out[3]};
+      dst[1] = u32x4{out[4], out[5], out[6], out[7]};
+    }
+    if (h1 < H) __syncthreads();
+  }
+}
+
+template <int D, bool F8>
+void launch_append(const G4PagedAppendArgs& a, bool vec, hipStream_t st) {
+  const int H = a.cache.kv_heads;
+  // 8 consecutive positions from any start on lie in ceil((seq + 7) / 8) groups at most
+  const int64_t groups = ((int64_t)a.seq + 2 * kTileTok - 2) / kTileTok;
+  if (a.seq >= kTileTok && a.batch * groups <= 0x7fffffffLL) {
+    constexpr int kHeads = kTileValueBytes / (kTileTok * D * (F8 ? 1 : 2));
+    const size_t lds = (size_t)(H < kHeads ? H : kHeads) * kTileTok * D * (F8 ? 1 : 2);
+    hipLaunchKernelGGL((paged_append_tile_kernel<D, F8>), dim3((unsigned)(a.batch * groups)), dim3(kTileThreads), lds, st, a,
+                       (int)vec, (int)groups);
+    return;
+  }
+  const int nvec = (a.q ? H * a.group : 0) + 2 * H;
+  hipLaunchKernelGGL((paged_append_kernel<D, F8>), dim3((unsigned)((int64_t)a.batch * a.seq)),
+                     dim3((unsigned)(64 * (nvec > 16 ? 16 : nvec))), 0, st, a, (int)vec);
+}
 template <int D>
 void launch_append(const G4PagedAppendArgs& a, bool vec, hipStream_t st) {
-  const int nvec = (a.q ? a.cache.kv_heads * a.group : 0) + 2 * a.cache.kv_heads;
-  const dim3 grid((unsigned)((int64_t)a.batch * a.seq)), block((unsigned)(64 * (nvec > 16 ? 16 : nvec)));
   if (a.cache.format == G4_PAGES_E4M3)
-    hipLaunchKernelGGL((paged_append_kernel<D, true>), grid, block, 0, st, a, (int)vec);
+    launch_append<D, true>(a, vec, st);
   else
-    hipLaunchKernelGGL((paged_append_kernel<D, false>), grid, block, 0, st, a, (int)vec);
+    launch_append<D, false>(a, vec, st);
 }
 
 // --- read back ---------------------------------------------------------------------------------------------
