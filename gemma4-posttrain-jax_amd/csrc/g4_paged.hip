@@ -38,120 +38,136 @@ namespace {
 
 // --- append ------------------------------------------------------------------------------------------------
 //
-// A head vector of a token is one wave's: lane l holds elements [l PER, (l + 1) PER), PER = D / 64, so a rotation's
-// partner (d +- D / 2) is lane l ^ 32 in the same element. f32 throughout, rounded once where it is stored: with
-// i = (mean(x^2) + eps)^-1/2, c and s the rotary row and w the norm's weights,
+// A head vector is held by LANES = min(64, D / 4) lanes, so a wave has 64 / LANES of them at once; lane l of its
+// group holds elements [l PER, (l + 1) PER), and a rotation's partner (d +- D / 2) is the same element of lane
+// l ^ LANES / 2. f32 throughout, rounded once where it is stored: with i = (mean(x^2) + eps)^-1/2, c and s the
+// rotary row and w the norm's weights,
 //   y_d = i (x_d (w_d c_d) + x_(d +- D/2) (-+ w_(d +- D/2) s_d)),
 // whose factors w c and w s are formed once per token for all its heads.
+
+template <int D>
+struct Lanes {
+  static constexpr int LANES = D >= 256 ? 64 : D / 4;
+  static constexpr int PER = D / LANES;     // 4, 8 at D = 512
+  static constexpr int VECS = 64 / LANES;  // head vectors of a wave at once
+  int in, sub;  // lane in its vector, vector of the wave
+  __device__ __forceinline__ explicit Lanes(int lane) : in(lane % LANES), sub(lane / LANES) {}
+
+  // Over the lanes of one vector, the result in each (every lane of the wave active).
+  template <typename F>
+  __device__ static __forceinline__ float reduce(float v, F op) {
+    if constexpr (LANES >= 64) v = across32(v, op);
+    if constexpr (LANES >= 32) v = across16(v, op);
+    v = op(v, dpp<0x128>(v));    // row_ror:8
+    v = op(v, dpp<0x124>(v));    // row_ror:4
+    v = op(v, dpp<0x4e>(v));     // quad_perm:[2,3,0,1]
+    return op(v, dpp<0xb1>(v));  // quad_perm:[1,0,3,2]
+  }
+
+  // The value of the partner lane in the vector's other half.
+  __device__ __forceinline__ float partner(float x) const {
+    const uint32_t u = __float_as_uint(x);
+    if constexpr (LANES == 64) {
+      const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+      return __uint_as_float(low() ? r[1] : r[0]);
+    } else if constexpr (LANES == 32) {
+      const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+      return __uint_as_float(low() ? r[1] : r[0]);
+    } else {
+      return dpp<0x128>(x);  // row_ror:8
+    }
+  }
+  __device__ __forceinline__ bool low() const { return in < LANES / 2; }
+};
 
 // PER bf16 elements of a row, and the way back.
 template <int PER>
 __device__ __forceinline__ void load_row(const uint16_t* p, bool vec, float (&x)[PER]) {
-  if (PER == 1 || !vec) {
-#pragma unroll
-    for (int e = 0; e < PER; ++e) x[e] = bf16_bits_to_f32(p[e]);
-  } else {
-    uint32_t w[PER / 2 > 0 ? PER / 2 : 1];
+  uint32_t w[PER / 2];
+  if (vec) {
     __builtin_memcpy(w, __builtin_assume_aligned(p, PER * 2), PER * 2);
+  } else {
 #pragma unroll
-    for (int i = 0; i < PER / 2; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    for (int i = 0; i < PER / 2; ++i) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
   }
+#pragma unroll
+  for (int i = 0; i < PER / 2; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
 }
 template <int PER>
 __device__ __forceinline__ void store_row(uint16_t* p, const float (&x)[PER]) {
-  if constexpr (PER == 1) {
-    *p = (uint16_t)f32_to_bf16_bits(x[0]);
-  } else {
-    uint32_t w[PER / 2];
+  uint32_t w[PER / 2];
 #pragma unroll
-    for (int i = 0; i < PER / 2; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-    __builtin_memcpy(__builtin_assume_aligned(p, PER * 2), w, PER * 2);
-  }
-}
-
-// The value of lane ^ 32, per element.
-__device__ __forceinline__ float other_half(float x, int lane) {
-  const uint32_t u = __float_as_uint(x);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  return __uint_as_float(lane < 32 ? r[1] : r[0]);
+  for (int i = 0; i < PER / 2; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+  __builtin_memcpy(__builtin_assume_aligned(p, PER * 2), w, PER * 2);
 }
 
 // What a token's q or k heads have in common.
-template <int PER>
+template <int D>
 struct Prepare {
+  static constexpr int PER = Lanes<D>::PER;
   float own[PER], other[PER];  // factors of x_d and of its partner; other unused without rotation
   bool norm, rope;
   float eps;
 
   // weight: [D] or NULL; c, s: this lane's elements of the token's rotary row
-  __device__ __forceinline__ void load(const uint16_t* weight, bool vec, const float (&c)[PER], const float (&s)[PER], int lane) {
+  __device__ __forceinline__ void load(const uint16_t* weight, bool vec, const float (&c)[PER], const float (&s)[PER],
+                                       const Lanes<D>& ln) {
 #pragma unroll
     for (int e = 0; e < PER; ++e) own[e] = 1.f;
-    if (weight) load_row<PER>(weight + lane * PER, vec, own);
+    if (weight) load_row<PER>(weight + ln.in * PER, vec, own);
     if (!rope) return;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const float partner = other_half(own[e], lane);
-      other[e] = (lane < 32 ? -partner : partner) * s[e];
+      const float partner = ln.partner(own[e]);
+      other[e] = (ln.low() ? -partner : partner) * s[e];
       own[e] *= c[e];
     }
   }
 
-  __device__ __forceinline__ void apply(float (&x)[PER], int lane) const {
-    float inv = 1.f;
-    if (norm) {
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < PER; ++e) ss += x[e] * x[e];
-      inv = __builtin_amdgcn_rsqf(wave_sum(ss) * (1.0f / (64 * PER)) + eps);
-    }
+  __device__ __forceinline__ void apply(float (&x)[PER], const Lanes<D>& ln) const {
+    const float inv = norm ? inverse_rms(x, eps) : 1.f;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
       float y = x[e] * own[e];
-      if (rope) y += other_half(x[e], lane) * other[e];
+      if (rope) y += ln.partner(x[e]) * other[e];
       x[e] = norm ? y * inv : y;
     }
   }
+
+  __device__ static __forceinline__ float inverse_rms(const float (&x)[PER], float eps) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) ss += x[e] * x[e];
+    return __builtin_amdgcn_rsqf(Lanes<D>::reduce(ss, SumOp()) * (1.0f / D) + eps);
+  }
 };
 
-// A vector's scale byte and its e4m3 bytes (this lane's in the low bytes of `w`).
-template <int PER>
-__device__ __forceinline__ int quantise(const float (&x)[PER], uint32_t (&w)[PER > 4 ? 2 : 1]) {
-  uint32_t top = 0;  // |x| orders as its bits do, infinities and NaN above the rest
+// A vector's scale byte and its e4m3 bytes (this lane's in `w`).
+template <int D>
+__device__ __forceinline__ int quantise(const float (&x)[Lanes<D>::PER], uint32_t (&w)[Lanes<D>::PER / 4]) {
+  constexpr int PER = Lanes<D>::PER;
+  float a = 0.f;
+  bool odd_one = false;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
-    const uint32_t u = __float_as_uint(x[e]) & 0x7fffffffu;
-    top = u > top ? u : top;
+    a = fmaxf(a, fabsf(x[e]));  // of the numbers
+    odd_one |= !finite_f32(x[e]);
   }
-  top = __float_as_uint(wave_max(__uint_as_float(top < 0x7f800000u ? top : 0u)));
-  const bool odd_ones = __any([&] {
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) bad |= !finite_f32(x[e]);
-    return bad;
-  }());
-  float a = __uint_as_float(top);
+  const bool odd_ones = __any(odd_one);
   if (odd_ones) {  // the largest of the finite elements
-    float f = 0.f;
+    a = 0.f;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) f = fmaxf(f, finite_f32(x[e]) ? fabsf(x[e]) : 0.f);
-    a = wave_max(f);
+    for (int e = 0; e < PER; ++e) a = fmaxf(a, finite_f32(x[e]) ? fabsf(x[e]) : 0.f);
   }
-  const int byte = scale_byte(a);
+  const int byte = scale_byte(Lanes<D>::reduce(a, MaxOp()));
   const float inv = __uint_as_float((uint32_t)(2 * kScaleBias - byte) << 23);
 #pragma unroll
-  for (int i = 0; i < (PER > 4 ? 2 : 1); ++i) {
-    constexpr int N = PER > 4 ? 4 : PER;
-    uint32_t v = 0;
-#pragma unroll
-    for (int e = 0; e < N; e += 2) {
-      const float lo = x[4 * i + e] * inv, hi = N > 1 ? x[4 * i + (N > 1 ? e + 1 : 0)] * inv : 0.f;
-      v = e < 2 ? (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)v, false)
-                : (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(lo, hi, (int)v, true);
-    }
+  for (int i = 0; i < PER / 4; ++i) {
+    uint32_t v = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] * inv, x[4 * i + 1] * inv, 0, false);
+    v = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] * inv, x[4 * i + 3] * inv, (int)v, true);
     if (odd_ones) {
 #pragma unroll
-      for (int e = 0; e < N; ++e)
+      for (int e = 0; e < 4; ++e)
         if (!finite_f32(x[4 * i + e])) v |= 0x7fu << (8 * e);  // NaN (either sign)
     }
     w[i] = v;
@@ -160,66 +176,66 @@ __device__ __forceinline__ int quantise(const float (&x)[PER], uint32_t (&w)[PER
 }
 
 template <int PER>
-__device__ __forceinline__ void store_bytes(uint8_t* p, const uint32_t (&w)[PER > 4 ? 2 : 1]) {
+__device__ __forceinline__ void store_bytes(uint8_t* p, const uint32_t (&w)[PER / 4]) {
   __builtin_memcpy(__builtin_assume_aligned(p, PER), w, PER);
 }
 
 // The rotary rows and factors of one token.
 template <int D>
 struct Token {
-  static constexpr int PER = D / 64;
-  Prepare<PER> q, k;
+  static constexpr int PER = Lanes<D>::PER;
+  Prepare<D> q, k;
   bool norm_v;
 
-  __device__ __forceinline__ void load(const G4PagedAppendArgs& a, int64_t token, bool vec, bool with_k, int lane) {
+  __device__ __forceinline__ void load(const G4PagedAppendArgs& a, int64_t token, bool vec, bool with_k, const Lanes<D>& ln) {
     float c[PER], s[PER];
-    const bool any_rope = a.flags & (G4_APPEND_ROPE_Q | G4_APPEND_ROPE_K);
 #pragma unroll
     for (int e = 0; e < PER; ++e) c[e] = s[e] = 0.f;
-    if (any_rope) {
-      __builtin_memcpy(c, a.rope_cos + token * D + lane * PER, PER * 4);
-      __builtin_memcpy(s, a.rope_sin + token * D + lane * PER, PER * 4);
+    if (a.flags & (G4_APPEND_ROPE_Q | G4_APPEND_ROPE_K)) {
+      __builtin_memcpy(c, a.rope_cos + token * D + ln.in * PER, PER * 4);
+      __builtin_memcpy(s, a.rope_sin + token * D + ln.in * PER, PER * 4);
     }
     q.norm = a.flags & G4_APPEND_NORM_Q, q.rope = a.flags & G4_APPEND_ROPE_Q, q.eps = a.eps;
     k.norm = a.flags & G4_APPEND_NORM_K, k.rope = a.flags & G4_APPEND_ROPE_K, k.eps = a.eps;
     norm_v = a.flags & G4_APPEND_NORM_V;
-    if (a.q) q.load(q.norm ? reinterpret_cast<const uint16_t*>(a.q_norm_weight) : nullptr, vec, c, s, lane);
-    if (with_k) k.load(k.norm ? reinterpret_cast<const uint16_t*>(a.k_norm_weight) : nullptr, vec, c, s, lane);
+    if (a.q) q.load(q.norm ? reinterpret_cast<const uint16_t*>(a.q_norm_weight) : nullptr, vec, c, s, ln);
+    if (with_k) k.load(k.norm ? reinterpret_cast<const uint16_t*>(a.k_norm_weight) : nullptr, vec, c, s, ln);
   }
 
   __device__ __forceinline__ void prepare_v(float (&x)[PER], float eps) const {
     if (!norm_v) return;
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) ss += x[e] * x[e];
-    const float inv = __builtin_amdgcn_rsqf(wave_sum(ss) * (1.0f / D) + eps);
+    const float inv = Prepare<D>::inverse_rms(x, eps);
 #pragma unroll
     for (int e = 0; e < PER; ++e) x[e] *= inv;
   }
 };
 
-// A prepared key or value vector into its slot: keys in the page's runs, values one element per 8-slot group.
+// A prepared key or value vector into its slot (where `on`): keys in the page's runs, values one element per
+// 8-slot group.
 template <int D, bool F8, bool KEY>
-__device__ __forceinline__ void store_vector(const G4PagedCache& c, int64_t block, int slot, const float (&x)[D / 64], int lane) {
-  constexpr int PER = D / 64;
+__device__ __forceinline__ void store_vector(const G4PagedCache& c, int64_t block, int slot, const float (&x)[Lanes<D>::PER],
+                                             bool on, const Lanes<D>& ln) {
+  constexpr int PER = Lanes<D>::PER;
   uint8_t* pages = reinterpret_cast<uint8_t*>(KEY ? c.key : c.value) + block * D * (F8 ? 1 : 2);
   if constexpr (F8) {
-    uint32_t w[PER > 4 ? 2 : 1];
-    const int byte = quantise<PER>(x, w);
-    if (lane == 0) (KEY ? c.key_scale : c.value_scale)[block + slot] = (uint8_t)byte;
+    uint32_t w[PER / 4];
+    const int byte = quantise<D>(x, w);
+    if (!on) return;
+    if (ln.in == 0) (KEY ? c.key_scale : c.value_scale)[block + slot] = (uint8_t)byte;
     if constexpr (KEY) {
-      store_bytes<PER>(pages + paged_key_index<true>(slot, lane * PER, D), w);
+      store_bytes<PER>(pages + paged_key_index<true>(slot, ln.in * PER, D), w);
     } else {
 #pragma unroll
-      for (int e = 0; e < PER; ++e) pages[vt_index(slot, lane * PER + e, D)] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+      for (int e = 0; e < PER; ++e) pages[vt_index(slot, ln.in * PER + e, D)] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
     }
   } else {
+    if (!on) return;
     uint16_t* p = reinterpret_cast<uint16_t*>(pages);
     if constexpr (KEY) {
-      store_row<PER>(p + paged_key_index<false>(slot, lane * PER, D), x);
+      store_row<PER>(p + paged_key_index<false>(slot, ln.in * PER, D), x);
     } else {
 #pragma unroll
-      for (int e = 0; e < PER; ++e) p[vt_index(slot, lane * PER + e, D)] = (uint16_t)f32_to_bf16_bits(x[e]);
+      for (int e = 0; e < PER; ++e) p[vt_index(slot, ln.in * PER + e, D)] = (uint16_t)f32_to_bf16_bits(x[e]);
     }
   }
 }
@@ -232,42 +248,43 @@ __device__ __forceinline__ int page_of(const G4PagedAppendArgs& a, int b, int64_
   return (uint32_t)page < (uint32_t)a.cache.num_pages ? page : -1;
 }
 
-// A step's tokens (and chunks of fewer than 8): one workgroup per token, one wave per head vector (looping over
-// more than 16). A wave's single vector is a chain of loads, so nothing is staged: 256 tokens of 2 x (4 + 2)
-// heads of 256 in 5.2 us, of which the launch takes most.
+// A step's tokens (and chunks of fewer than 8): one workgroup per token, one wave per 64 / LANES head vectors of a
+// kind (looping over more than 16). A wave's vectors are a chain of loads, so nothing is staged: 256 tokens of
+// 2 x (4 + 2) heads of 256 in 4.4 us, of which the launch takes most.
 template <int D, bool F8>
 __global__ __launch_bounds__(1024) void paged_append_kernel(G4PagedAppendArgs a, int vec) {
-  constexpr int PER = D / 64;
-  const int lane = threadIdx.x & 63;
+  constexpr int PER = Lanes<D>::PER, VECS = Lanes<D>::VECS;
+  const Lanes<D> ln(threadIdx.x & 63);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nwaves = blockDim.x >> 6;
   const int S = a.seq, H = a.cache.kv_heads;
   const int token = blockIdx.x, b = token / S, s = token - b * S;
-  const int nq = a.q ? H * a.group : 0, nvec = nq + 2 * H;
-  const int64_t in_base = (int64_t)token * a.in_row_stride + lane * PER;
+  const int nq = a.q ? H * a.group : 0, q_waves = (nq + VECS - 1) / VECS, kv_waves = (H + VECS - 1) / VECS;
+  const int64_t in_base = (int64_t)token * a.in_row_stride + ln.in * PER;
   const int64_t pos = (int64_t)a.write_pos[b] + s;
   const int page = page_of(a, b, pos, s);
   const int slot = (int)(pos & (a.cache.page_size - 1));
   Token<D> t;
-  t.load(a, token, vec, true, lane);
-  for (int v = wave; v < nvec; v += nwaves) {
+  t.load(a, token, vec, true, ln);
+  for (int u = wave; u < q_waves + 2 * kv_waves; u += nwaves) {
     float x[PER];
-    if (v < nq) {
-      load_row<PER>(reinterpret_cast<const uint16_t*>(a.q) + in_base + (int64_t)v * D, vec, x);
-      t.q.apply(x, lane);
-      store_row<PER>(reinterpret_cast<uint16_t*>(a.q_out) + ((int64_t)token * nq + v) * D + lane * PER, x);
+    if (u < q_waves) {
+      const int v = u * VECS + ln.sub, at = v < nq ? v : nq - 1;
+      load_row<PER>(reinterpret_cast<const uint16_t*>(a.q) + in_base + (int64_t)at * D, vec, x);
+      t.q.apply(x, ln);
+      if (v < nq) store_row<PER>(reinterpret_cast<uint16_t*>(a.q_out) + ((int64_t)token * nq + v) * D + ln.in * PER, x);
       continue;
     }
     if (page < 0) continue;
-    const bool key = v < nq + H;
-    const int head = v - nq - (key ? 0 : H);
+    const bool key = u < q_waves + kv_waves;
+    const int v = (u - q_waves - (key ? 0 : kv_waves)) * VECS + ln.sub, head = v < H ? v : H - 1;
     const int64_t block = ((int64_t)page * H + head) * a.cache.page_size;
     load_row<PER>(reinterpret_cast<const uint16_t*>(key ? a.k : a.v) + in_base + (int64_t)head * D, vec, x);
     if (key) {
-      t.k.apply(x, lane);
-      store_vector<D, F8, true>(a.cache, block, slot, x, lane);
+      t.k.apply(x, ln);
+      store_vector<D, F8, true>(a.cache, block, slot, x, v < H, ln);
     } else {
       t.prepare_v(x, a.eps);
-      store_vector<D, F8, false>(a.cache, block, slot, x, lane);
+      store_vector<D, F8, false>(a.cache, block, slot, x, v < H, ln);
     }
   }
 }
@@ -284,10 +301,10 @@ constexpr int kTileValueBytes = 32 * 1024;  // LDS for value rows; more heads th
 template <int D, bool F8>
 __global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(D >= 512 ? 4 : 8))) void
 paged_append_tile_kernel(G4PagedAppendArgs a, int vec, int groups) {
-  constexpr int PER = D / 64, BYTES = F8 ? 1 : 2;
+  constexpr int PER = Lanes<D>::PER, VECS = Lanes<D>::VECS, BYTES = F8 ? 1 : 2;
   constexpr int kHeads = kTileValueBytes / (kTileTok * D * BYTES);
   extern __shared__ __attribute__((aligned(16))) uint8_t v_lds[];  // [min(H, kHeads)][8 tokens][D]
-  const int lane = threadIdx.x & 63;
+  const Lanes<D> ln(threadIdx.x & 63);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int S = a.seq, H = a.cache.kv_heads;
   const int b = (int)blockIdx.x / groups;
@@ -301,23 +318,26 @@ paged_append_tile_kernel(G4PagedAppendArgs a, int vec, int groups) {
   const int s = on ? (int)s64 : 0;
   const int page = on ? page_of(a, b, p0 + wave, s) : -1;
   const int slot = (int)((p0 + wave) & (a.cache.page_size - 1));
-  const int64_t token = (int64_t)b * S + s, in_base = token * a.in_row_stride + lane * PER;
+  const int64_t token = (int64_t)b * S + s, in_base = token * a.in_row_stride + ln.in * PER;
   Token<D> t;
-  if (on) t.load(a, token, vec, page >= 0, lane);
+  if (on) t.load(a, token, vec, page >= 0, ln);
   if (on && a.q) {
     const int nq = H * a.group;
     const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + in_base;
-    uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + token * nq * D + lane * PER;
-    for (int v0 = 0; v0 < nq; v0 += kTileVecs) {
+    uint16_t* dst = reinterpret_cast<uint16_t*>(a.q_out) + token * nq * D + ln.in * PER;
+    for (int v0 = 0; v0 < nq; v0 += kTileVecs * VECS) {
       float x[kTileVecs][PER];
 #pragma unroll
-      for (int i = 0; i < kTileVecs; ++i)
-        if (v0 + i < nq) load_row<PER>(src + (v0 + i) * D, vec, x[i]);
+      for (int i = 0; i < kTileVecs; ++i) {
+        const int v = v0 + i * VECS + ln.sub;
+        if (v0 + i * VECS < nq) load_row<PER>(src + (v < nq ? v : nq - 1) * D, vec, x[i]);
+      }
 #pragma unroll
       for (int i = 0; i < kTileVecs; ++i)
-        if (v0 + i < nq) {
-          t.q.apply(x[i], lane);
-          store_row<PER>(dst + (v0 + i) * D, x[i]);
+        if (v0 + i * VECS < nq) {
+          const int v = v0 + i * VECS + ln.sub;
+          t.q.apply(x[i], ln);
+          if (v < nq) store_row<PER>(dst + v * D, x[i]);
         }
     }
   }
@@ -327,33 +347,37 @@ paged_append_tile_kernel(G4PagedAppendArgs a, int vec, int groups) {
     if (page >= 0) {
       const uint16_t* ksrc = reinterpret_cast<const uint16_t*>(a.k) + in_base;
       const uint16_t* vsrc = reinterpret_cast<const uint16_t*>(a.v) + in_base;
-      for (int h = h0; h < h1; h += kTileVecs / 2) {
+      for (int h = h0; h < h1; h += kTileVecs / 2 * VECS) {
         float x[kTileVecs][PER];
 #pragma unroll
-        for (int i = 0; i < kTileVecs / 2; ++i)
-          if (h + i < h1) {
-            load_row<PER>(ksrc + (int64_t)(h + i) * D, vec, x[2 * i]);
-            load_row<PER>(vsrc + (int64_t)(h + i) * D, vec, x[2 * i + 1]);
+        for (int i = 0; i < kTileVecs / 2; ++i) {
+          const int v = h + i * VECS + ln.sub, head = v < h1 ? v : h1 - 1;
+          if (h + i * VECS < h1) {
+            load_row<PER>(ksrc + (int64_t)head * D, vec, x[2 * i]);
+            load_row<PER>(vsrc + (int64_t)head * D, vec, x[2 * i + 1]);
           }
+        }
 #pragma unroll
         for (int i = 0; i < kTileVecs / 2; ++i) {
-          if (h + i >= h1) break;
-          const int64_t block = (page_block + h + i) * a.cache.page_size;
-          t.k.apply(x[2 * i], lane);
-          store_vector<D, F8, true>(a.cache, block, slot, x[2 * i], lane);
+          if (h + i * VECS >= h1) break;
+          const int v = h + i * VECS + ln.sub, head = v < h1 ? v : h1 - 1;
+          const int64_t block = (page_block + head) * a.cache.page_size;
+          t.k.apply(x[2 * i], ln);
+          store_vector<D, F8, true>(a.cache, block, slot, x[2 * i], v < h1, ln);
           t.prepare_v(x[2 * i + 1], a.eps);
           if (!full) {
-            store_vector<D, F8, false>(a.cache, block, slot, x[2 * i + 1], lane);
+            store_vector<D, F8, false>(a.cache, block, slot, x[2 * i + 1], v < h1, ln);
             continue;
           }
-          uint8_t* row = v_lds + ((h + i - h0) * kTileTok + wave) * D * BYTES;
+          uint8_t* row = v_lds + ((head - h0) * kTileTok + wave) * D * BYTES;
           if constexpr (F8) {
-            uint32_t w[PER > 4 ? 2 : 1];
-            const int byte = quantise<PER>(x[2 * i + 1], w);
-            if (lane == 0) a.cache.value_scale[block + slot] = (uint8_t)byte;
-            store_bytes<PER>(row + lane * PER, w);
+            uint32_t w[PER / 4];
+            const int byte = quantise<D>(x[2 * i + 1], w);
+            if (v >= h1) continue;
+            if (ln.in == 0) a.cache.value_scale[block + slot] = (uint8_t)byte;
+            store_bytes<PER>(row + ln.in * PER, w);
           } else {
-            store_row<PER>(reinterpret_cast<uint16_t*>(row) + lane * PER, x[2 * i + 1]);
+            if (v < h1) store_row<PER>(reinterpret_cast<uint16_t*>(row) + ln.in * PER, x[2 * i + 1]);
           }
         }
       }
@@ -411,7 +435,8 @@ void launch_append(const G4PagedAppendArgs& a, bool vec, hipStream_t st) {
                        (int)vec, (int)groups);
     return;
   }
-  const int nvec = (a.q ? H * a.group : 0) + 2 * H;
+  constexpr int VECS = Lanes<D>::VECS;
+  const int nvec = ((a.q ? H * a.group : 0) + VECS - 1) / VECS + 2 * ((H + VECS - 1) / VECS);
   hipLaunchKernelGGL((paged_append_kernel<D, F8>), dim3((unsigned)((int64_t)a.batch * a.seq)),
                      dim3((unsigned)(64 * (nvec > 16 ? 16 : nvec))), 0, st, a, (int)vec);
 }
@@ -534,11 +559,12 @@ extern "C" int g4_paged_append(const G4PagedAppendArgs* args, void* stream) {
   if ((a.flags & G4_APPEND_NORM_K) && !a.k_norm_weight) return fail(G4_ERR_INVALID, "%s: NORM_K needs k_norm_weight", who);
   if ((a.flags & G4_APPEND_NORM_Q) && a.q && !a.q_norm_weight)
     return fail(G4_ERR_INVALID, "%s: NORM_Q needs q_norm_weight", who);
-  // each lane's D / 64 elements move in one access where every row is aligned to them
-  const uintptr_t al = (uintptr_t)(a.cache.head_dim / 64) * 2;
+  // each lane's 4 or 8 elements move in one access where every row is aligned to them
+  const uintptr_t al = a.cache.head_dim == 512 ? 16 : 8;
   bool vec = (a.in_row_stride * 2) % (int64_t)al == 0;
   for (const void* p : std::initializer_list<const void*>{a.k, a.v, a.q, a.k_norm_weight, a.q_norm_weight})
     vec = vec && reinterpret_cast<uintptr_t>(p) % al == 0;
+  if (reinterpret_cast<uintptr_t>(a.q_out) % al) return fail(G4_ERR_INVALID, "%s: q_out must be %d-byte aligned", who, (int)al);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (a.cache.head_dim) {
     case 64: launch_append<64>(a, vec, st); break;

@@ -103,6 +103,7 @@ def test_abi_refuses_bad_tables(name, make, override, match):
     ("g4_paged_append", _append, dict(write_pos=None), "NULL"),
     ("g4_paged_append", _append, dict(q=1 << 12), "q_out"),
     ("g4_paged_append", _append, dict(q=1 << 12, q_out=1 << 12, group=0), "group"),
+    ("g4_paged_append", _append, dict(q=1 << 12, q_out=(1 << 12) + 4), "q_out"),
     ("g4_paged_append", _append, dict(in_row_stride=500), "in_row_stride"),
     ("g4_paged_append", _append, dict(flags=_lib.G4_APPEND_ROPE_K), "RoPE"),
     ("g4_paged_append", _append, dict(flags=_lib.G4_APPEND_NORM_K), "k_norm_weight"),
