@@ -452,84 +452,90 @@ void launch_append(const G4PagedAppendArgs& a, bool vec, hipStream_t st) {
 
 constexpr int kReadThreads = 256;
 
-// One workgroup per (row, head, 32-slot chunk): a chunk's keys, then its values, are read in 16-byte
-// pieces in the page's order and turned into token-major rows in LDS.
+// One workgroup per (row, head, 32-slot chunk) and array: the chunk's 16-byte pieces are asked for at once, in the
+// page's order, and turned into token-major rows in LDS.
 template <int D, bool F8>
 __global__ __launch_bounds__(kReadThreads) void paged_read_kernel(G4PagedReadArgs a, int first_chunk, int n_chunks) {
-  constexpr int RS = D + 8;                        // LDS row stride, elements
-  constexpr int PIECES = 32 * D * (F8 ? 1 : 2) / 16;  // 16-byte pieces of a chunk
+  constexpr int RS = D + 8;                            // LDS row stride, elements
+  constexpr int PIECES = 32 * D * (F8 ? 1 : 2) / 16;   // 16-byte pieces of a chunk
+  constexpr int LOADS = (PIECES + kReadThreads - 1) / kReadThreads;
   __shared__ __attribute__((aligned(16))) uint16_t rows[32 * RS];
-  const int H = a.cache.kv_heads, ps = a.cache.page_size;
+  const bool values = blockIdx.y;
+  const int H = a.cache.kv_heads, ps = a.cache.page_size, tid = threadIdx.x;
   const int c = first_chunk + (int)(blockIdx.x % n_chunks);
   const int bh = blockIdx.x / n_chunks, b = bh / H, h = bh - b * H;
   const int p0 = c * 32;  // < 2^31: the host bounds start + count
   int len = a.lengths[b];
   if (len > a.max_pages * ps) len = a.max_pages * ps;
   int page = -1;
-  if (p0 < len) page = a.page_table[b * a.table_stride + p0 / ps];
+  if (p0 < len) page = a.page_table[b * a.table_stride + (p0 >> __builtin_ctz(ps))];
   const bool there = (uint32_t)page < (uint32_t)a.cache.num_pages;
-  const int64_t block = ((int64_t)page * H + h) * ps;
-  const int chunk = (p0 & (ps - 1)) >> 5;
-  for (int part = 0; part < 2; ++part) {
-    if (there) {
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(part ? a.cache.value : a.cache.key) +
-                           (block * D + (int64_t)chunk * 32 * D) * (F8 ? 1 : 2);
-      const uint8_t* scale = F8 ? (part ? a.cache.value_scale : a.cache.key_scale) + block + chunk * 32 : nullptr;
-      for (int i = threadIdx.x; i < PIECES; i += kReadThreads) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(src + i * 16);
-        if (part == 0) {
-          // a key piece: 16 (e4m3) or 8 (bf16) dims of one slot
-          const int col = i / 4 % 16, half = i / 64 % 2, run = i / 128;
-          const int slot = 8 * (col >> 2) + 4 * half + (col & 3);
-          if constexpr (F8) {
-            const float sc = exp2_byte(scale[slot]);
-            uint32_t o[8];
+  if (there) {
+    const int64_t block = ((int64_t)page * H + h) * ps + (p0 & (ps - 1));  // slots before the chunk
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(values ? a.cache.value : a.cache.key) + block * D * (F8 ? 1 : 2);
+    const uint8_t* scale = F8 ? (values ? a.cache.value_scale : a.cache.key_scale) + block : nullptr;
+    u32x4 w[LOADS];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              o[2 * j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j], sc, false));
-              o[2 * j + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j], sc, true));
-            }
-            u32x4* dst = reinterpret_cast<u32x4*>(rows + slot * RS + run * 64 + i % 4 * 16);
-            dst[0] = u32x4{o[0], o[1], o[2], o[3]};
-            dst[1] = u32x4{o[4], o[5], o[6], o[7]};
-          } else {
-            *reinterpret_cast<u32x4*>(rows + slot * RS + run * 32 + i % 4 * 8) = w;
+    for (int j = 0; j < LOADS; ++j)
+      if (PIECES % kReadThreads == 0 || tid + j * kReadThreads < PIECES)
+        w[j] = *reinterpret_cast<const u32x4*>(src + (tid + j * kReadThreads) * 16);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int i = tid + j * kReadThreads;
+      if (PIECES % kReadThreads != 0 && i >= PIECES) break;
+      if (!values) {
+        // a key piece: 16 (e4m3) or 8 (bf16) dims of one slot
+        const int col = i / 4 % 16, half = i / 64 % 2, run = i / 128;
+        const int slot = 8 * (col >> 2) + 4 * half + (col & 3);
+        if constexpr (F8) {
+          const float sc = exp2_byte(scale[slot]);
+          uint32_t o[8];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            o[2 * q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j][q], sc, false));
+            o[2 * q + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j][q], sc, true));
+          }
+          u32x4* dst = reinterpret_cast<u32x4*>(rows + slot * RS + run * 64 + i % 4 * 16);
+          dst[0] = u32x4{o[0], o[1], o[2], o[3]};
+          dst[1] = u32x4{o[4], o[5], o[6], o[7]};
+        } else {
+          *reinterpret_cast<u32x4*>(rows + slot * RS + run * 32 + i % 4 * 8) = w[j];
+        }
+      } else {
+        // a value piece: 8 slots of two dims (e4m3) or one dim (bf16)
+        const int d = F8 ? i * 2 % D : i % D, g = F8 ? i * 2 / D : i / D;
+        if constexpr (F8) {
+          const uint2 sc = *reinterpret_cast<const uint2*>(scale + 8 * g);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const uint32_t two = (w[j][q / 4] >> (8 * (q % 4)) & 0xffu) | ((w[j][2 + q / 4] >> (8 * (q % 4)) & 0xffu) << 8);
+            *reinterpret_cast<uint32_t*>(rows + (8 * g + q) * RS + d) = __builtin_bit_cast(
+                uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                              two, exp2_byte((q < 4 ? sc.x : sc.y) >> (8 * (q % 4)) & 0xff), false));
           }
         } else {
-          // a value piece: 8 slots of two dims (e4m3) or one dim (bf16)
-          const int d = F8 ? i * 2 % D : i % D, g = F8 ? i * 2 / D : i / D;
-          if constexpr (F8) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int slot = 8 * g + j;
-              const uint32_t two = (w[j / 4] >> (8 * (j % 4)) & 0xffu) | ((w[2 + j / 4] >> (8 * (j % 4)) & 0xffu) << 8);
-              *reinterpret_cast<uint32_t*>(rows + slot * RS + d) = __builtin_bit_cast(
-                  uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(two, exp2_byte(scale[slot]), false));
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) rows[(8 * g + j) * RS + d] = (uint16_t)(w[j / 2] >> (16 * (j % 2)));
-          }
+          for (int q = 0; q < 8; ++q) rows[(8 * g + q) * RS + d] = (uint16_t)(w[j][q / 2] >> (16 * (q % 2)));
         }
       }
     }
     __syncthreads();
-    uint16_t* out = reinterpret_cast<uint16_t*>(part ? a.v_out : a.k_out);
-    for (int i = threadIdx.x; i < 32 * D / 8; i += kReadThreads) {
-      const int slot = i / (D / 8), d = i % (D / 8) * 8;
-      const int p = p0 + slot;
-      if (p < a.start || p >= a.start + a.count) continue;
-      u32x4 w = {0u, 0u, 0u, 0u};
-      if (there && p < len) w = *reinterpret_cast<const u32x4*>(rows + slot * RS + d);
-      *reinterpret_cast<u32x4*>(out + (((int64_t)b * a.count + (p - a.start)) * H + h) * D + d) = w;
-    }
-    __syncthreads();
+  }
+  uint16_t* out = reinterpret_cast<uint16_t*>(values ? a.v_out : a.k_out);
+#pragma unroll 4
+  for (int i = tid; i < 32 * D / 8; i += kReadThreads) {
+    const int slot = i / (D / 8), d = i % (D / 8) * 8;
+    const int p = p0 + slot;
+    if (p < a.start || p >= a.start + a.count) continue;
+    u32x4 w = {0u, 0u, 0u, 0u};
+    if (there && p < len) w = *reinterpret_cast<const u32x4*>(rows + slot * RS + d);
+    *reinterpret_cast<u32x4*>(out + (((int64_t)b * a.count + (p - a.start)) * H + h) * D + d) = w;
   }
 }
 
 template <int D>
 void launch_read(const G4PagedReadArgs& a, int first, int n, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.batch * a.cache.kv_heads * n));
+  const dim3 grid((unsigned)((int64_t)a.batch * a.cache.kv_heads * n), 2);
   if (a.cache.format == G4_PAGES_E4M3)
     hipLaunchKernelGGL((paged_read_kernel<D, true>), grid, dim3(kReadThreads), 0, st, a, first, n);
   else
