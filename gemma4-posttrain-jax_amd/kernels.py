@@ -330,52 +330,56 @@ def prefill_attention(
 def _paged_cache(layer: PagedLayerCache) -> _lib.G4PagedCache:
     """The checked C view of a layer's pages."""
 
-    value = layer.value
+    key, value, key_scale, value_scale = layer
     if value.dim() != 5 or value.shape[4] != 8:
         raise ValueError(f"value pages: shape {tuple(value.shape)} is not [P, Hkv, page / 8, D, 8]")
     P, H, groups, D, _ = value.shape
-    e4m3 = value.dtype == torch.float8_e4m3fn
-    if value.dtype != layer.key.dtype or not (e4m3 or value.dtype == torch.bfloat16):
-        raise TypeError(f"pages of {layer.key.dtype} / {value.dtype}; they hold bfloat16 or float8_e4m3fn")
-    if tuple(layer.key.shape) != paged_key_shape(P, H, groups * 8, D, e4m3):
-        raise ValueError(f"key pages {tuple(layer.key.shape)} do not match value pages {tuple(value.shape)}")
-    if not (layer.key.is_contiguous() and value.is_contiguous()):
+    dtype = value.dtype
+    e4m3 = dtype == torch.float8_e4m3fn
+    if key.dtype != dtype or not (e4m3 or dtype == torch.bfloat16):
+        raise TypeError(f"pages of {key.dtype} / {dtype}; they hold bfloat16 or float8_e4m3fn")
+    if key.shape != paged_key_shape(P, H, groups * 8, D, e4m3):
+        raise ValueError(f"key pages {tuple(key.shape)} do not match value pages {tuple(value.shape)}")
+    if not (key.is_contiguous() and value.is_contiguous()):
         raise ValueError("pages must be contiguous")
     if e4m3:
-        for t in (layer.key_scale, layer.value_scale):
-            if (t is None or t.dtype != torch.float8_e8m0fnu or tuple(t.shape) != (P, H, groups * 8)
-                    or not t.is_contiguous() or t.device != value.device):
+        for t in (key_scale, value_scale):
+            if (t is None or t.dtype != torch.float8_e8m0fnu or t.shape != (P, H, groups * 8) or not t.is_contiguous()):
                 raise ValueError(f"e4m3 pages need contiguous float8_e8m0fnu scales of shape {(P, H, groups * 8)}")
-    elif layer.key_scale is not None or layer.value_scale is not None:
+        return _lib.G4PagedCache(_lib.G4_PAGES_E4M3, P, H, D, groups * 8, key.data_ptr(), value.data_ptr(),
+                                 key_scale.data_ptr(), value_scale.data_ptr())
+    if key_scale is not None or value_scale is not None:
         raise ValueError("bf16 pages have no scales")
-    if layer.key.device != value.device:
-        raise ValueError("key and value pages are on different devices")
-    return _lib.G4PagedCache(format=_lib.G4_PAGES_E4M3 if e4m3 else _lib.G4_PAGES_BF16, num_pages=P, kv_heads=H,
-                             head_dim=D, page_size=groups * 8, key=_ptr(layer.key), value=_ptr(value),
-                             key_scale=_ptr(layer.key_scale), value_scale=_ptr(layer.value_scale))
+    return _lib.G4PagedCache(_lib.G4_PAGES_BF16, P, H, D, groups * 8, key.data_ptr(), value.data_ptr(), None, None)
 
 
-def _on_device(layer: PagedLayerCache, *tensors: torch.Tensor | None) -> None:
-    """The operands are on the cache's device and it is the current one, whose stream the call goes to."""
+def _device_of(layer: PagedLayerCache, *tensors: torch.Tensor | None) -> int:
+    """The index of the device that all operands are on, which has to be the current one: the call goes to its
+    stream. (``get_device`` is -1 on the host.)"""
 
-    dev = layer.value.device
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"an operand is on {t.device}, the cache on {dev}")
-    if dev.type == "cuda" and dev.index != torch.cuda.current_device():
-        raise ValueError(f"the cache is on {dev}, which is not the current device")
+    dev = layer.value.get_device()
+    if dev < 0:
+        raise ValueError("kernel operands must be device tensors")
+    for t in (*layer, *tensors):
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"an operand is on {t.device}, the cache on {layer.value.device}")
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError(f"the cache is on {layer.value.device}, which is not the current device")
+    return dev
 
 
 def _page_rows(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> tuple[int, int, int]:
     """(B, entries per row, stride) of a page table, ``rows`` being the int32 [B] tensor ``name``."""
 
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or 0 in page_table.shape:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.numel() == 0:
         raise ValueError("page_table must be a non-empty int32 [B, M] tensor")
     B, M = page_table.shape
-    stride = page_table.stride(0) if B > 1 else M
-    if (M > 1 and page_table.stride(1) != 1) or stride < M:
+    stride, inner = page_table.stride()
+    if B == 1:
+        stride = M
+    if (M > 1 and inner != 1) or stride < M:
         raise ValueError("page_table rows must be contiguous and apart")
-    if rows.dtype != torch.int32 or tuple(rows.shape) != (B,) or not rows.is_contiguous():
+    if rows.dtype != torch.int32 or rows.shape != (B,) or not rows.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 [{B}] tensor")
     return B, M, stride
 
@@ -404,44 +408,48 @@ def paged_append(
     ``keep`` tokens. q / k / v are prepared by ``flags`` in f32 and rounded once, where they are stored."""
 
     B, S, H, D = k.shape
-    rs = k.stride(1) if S > 1 else (k.stride(0) if B > 1 else H * D)
-    _check_rows(k, "k", B, S, H, D, rs)
-    _check_rows(v, "v", B, S, H, D, rs)
-    if k.dtype != torch.bfloat16 or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+    strides = k.stride()
+    rs = strides[1] if S > 1 else (strides[0] if B > 1 else H * D)
+    if strides != (S * rs, rs, D, 1):
+        _check_rows(k, "k", B, S, H, D, rs)
+    if v.stride() != strides or v.shape != k.shape:
+        _check_rows(v, "v", B, S, H, D, rs)
+    bf16 = torch.bfloat16
+    if k.dtype != bf16 or v.dtype != bf16 or (q is not None and q.dtype != bf16):
         raise TypeError("paged_append takes bfloat16 q / k / v")
     rows, M, table_stride = _page_rows(page_table, "write_pos", write_pos)
     if rows != B:
         raise ValueError(f"page_table has {rows} rows for a batch of {B}")
-    if layer.kv_heads != H or layer.head_dim != D:
-        raise ValueError(f"pages of {layer.kv_heads} heads of {layer.head_dim} do not match k {tuple(k.shape)}")
+    cache = _paged_cache(layer)
+    if cache.kv_heads != H or cache.head_dim != D:
+        raise ValueError(f"pages of {cache.kv_heads} heads of {cache.head_dim} do not match k {tuple(k.shape)}")
     if keep < 0:
         raise ValueError(f"keep must not be negative, got {keep}")
     R = 0
     if q is not None:
         R = q.shape[3] if q.dim() == 5 else 0
-        if tuple(q.shape) != (B, S, H, R, D) or q.stride(4) != 1 or q.stride(3) != D or (H > 1 and q.stride(2) != R * D):
-            raise ValueError(f"q: shape {tuple(q.shape)} / strides {q.stride()}")
-        if (S > 1 and q.stride(1) != rs) or (B > 1 and q.stride(0) != S * rs):
+        if q.shape != (B, S, H, R, D):
+            raise ValueError(f"q: shape {tuple(q.shape)} is not [{B}, {S}, {H}, R, {D}]")
+        qs = q.stride()
+        if qs[4] != 1 or (R > 1 and qs[3] != D) or (H > 1 and qs[2] != R * D):
+            raise ValueError(f"q: strides {qs} of [Hkv, R, D] rows")
+        if (S > 1 and qs[1] != rs) or (B > 1 and qs[0] != S * rs):
             raise ValueError("q must share k's row stride")
-        if (q_out is None or q_out.dtype != q.dtype or tuple(q_out.shape) != (B, S, H, R, D)
-                or not q_out.is_contiguous()):
+        if q_out is None or q_out.dtype != bf16 or q_out.shape != q.shape or not q_out.is_contiguous():
             raise ValueError("q_out must be a contiguous bfloat16 [B, S, Hkv, R, D] tensor")
     for name, t, on in (("q_norm_weight", q_norm_weight, q is not None and flags & _lib.G4_APPEND_NORM_Q),
                         ("k_norm_weight", k_norm_weight, flags & _lib.G4_APPEND_NORM_K)):
-        if on and (t is None or t.dtype != k.dtype or tuple(t.shape) != (D,) or not t.is_contiguous()):
+        if on and (t is None or t.dtype != bf16 or t.shape != (D,) or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous bfloat16 [{D}] tensor")
     if flags & (_lib.G4_APPEND_ROPE_K | _lib.G4_APPEND_ROPE_Q):
         for t in (rope_cos, rope_sin):
-            if t is None or t.dtype != torch.float32 or tuple(t.shape) != (B, S, D) or not t.is_contiguous():
+            if t is None or t.dtype != torch.float32 or t.shape != (B, S, D) or not t.is_contiguous():
                 raise ValueError("rope_cos/rope_sin must be contiguous float32 [B, S, D]")
-    _on_device(layer, k, v, q, q_out, page_table, write_pos, q_norm_weight, k_norm_weight, rope_cos, rope_sin)
-    a = _lib.G4PagedAppendArgs(
-        cache=_paged_cache(layer), batch=B, seq=S, group=R, flags=flags, eps=eps, keep=keep, max_pages=M,
-        table_stride=table_stride, page_table=_ptr(page_table), write_pos=_ptr(write_pos), k=_ptr(k), v=_ptr(v),
-        q=_ptr(q), in_row_stride=rs, q_norm_weight=_ptr(q_norm_weight), k_norm_weight=_ptr(k_norm_weight),
-        rope_cos=_ptr(rope_cos), rope_sin=_ptr(rope_sin), q_out=_ptr(q_out),
-    )
-    _lib.check(_lib.lib().g4_paged_append(ctypes.byref(a), _stream()), "g4_paged_append")
+    dev = _device_of(layer, k, v, q, q_out, page_table, write_pos, q_norm_weight, k_norm_weight, rope_cos, rope_sin)
+    ptrs = [None if t is None else t.data_ptr() for t in (q, q_norm_weight, k_norm_weight, rope_cos, rope_sin, q_out)]
+    a = _lib.G4PagedAppendArgs(cache, B, S, R, flags, eps, keep, M, table_stride, page_table.data_ptr(),
+                               write_pos.data_ptr(), k.data_ptr(), v.data_ptr(), ptrs[0], rs, *ptrs[1:])
+    _lib.check(_lib.lib().g4_paged_append(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_append")
 
 
 def paged_decode_attention(
@@ -464,25 +472,25 @@ def paged_decode_attention(
     rows, M, table_stride = _page_rows(page_table, "lengths", lengths)
     if rows != B:
         raise ValueError(f"page_table has {rows} rows for a batch of {B}")
-    if layer.kv_heads != H or layer.head_dim != D:
-        raise ValueError(f"pages of {layer.kv_heads} heads of {layer.head_dim} do not match q {tuple(q.shape)}")
+    cache = _paged_cache(layer)
+    if cache.kv_heads != H or cache.head_dim != D:
+        raise ValueError(f"pages of {cache.kv_heads} heads of {cache.head_dim} do not match q {tuple(q.shape)}")
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
+    if out is not None and (out.shape != q.shape or not out.is_contiguous() or out.dtype != q.dtype):
+        raise ValueError("out must be a contiguous [B, Hkv, R, D] tensor in q's dtype")
+    dev = _device_of(layer, q, page_table, lengths, out)
     if out is None:
         out = torch.empty_like(q)
-    elif tuple(out.shape) != (B, H, R, D) or not out.is_contiguous() or out.dtype != q.dtype:
-        raise ValueError("out must be a contiguous [B, Hkv, R, D] tensor in q's dtype")
-    _on_device(layer, q, page_table, lengths, out)
-    a = _lib.G4PagedDecodeArgs(
-        cache=_paged_cache(layer), batch=B, group=R, window=window, max_pages=M, table_stride=table_stride,
-        page_table=_ptr(page_table), lengths=_ptr(lengths), q=_ptr(q), out=_ptr(out), workspace=None, workspace_bytes=0,
-    )
-    need = _lib.lib().g4_paged_decode_workspace_size(ctypes.byref(a))
-    ws = None
+    a = _lib.G4PagedDecodeArgs(cache, B, R, window, M, table_stride, page_table.data_ptr(), lengths.data_ptr(),
+                               q.data_ptr(), out.data_ptr(), None, 0)
+    ref = ctypes.byref(a)
+    need = _lib.lib().g4_paged_decode_workspace_size(ref)
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    _lib.check(_lib.lib().g4_paged_decode_attention(ctypes.byref(a), _stream()), "g4_paged_decode_attention")
+    _lib.check(_lib.lib().g4_paged_decode_attention(ref, torch._C._cuda_getCurrentRawStream(dev)),
+               "g4_paged_decode_attention")
     return out
 
 
@@ -494,14 +502,13 @@ def paged_read(layer: PagedLayerCache, *, page_table: torch.Tensor, lengths: tor
     B, M, table_stride = _page_rows(page_table, "lengths", lengths)
     if start < 0 or count <= 0:
         raise ValueError(f"start {start} must not be negative and count {count} must be positive")
-    _on_device(layer, page_table, lengths)
     cache = _paged_cache(layer)
-    shape = (B, count, layer.kv_heads, layer.head_dim)
-    k = torch.empty(shape, dtype=torch.bfloat16, device=layer.value.device)
-    v = torch.empty(shape, dtype=torch.bfloat16, device=layer.value.device)
-    a = _lib.G4PagedReadArgs(cache=cache, batch=B, start=start, count=count, max_pages=M, table_stride=table_stride,
-                             page_table=_ptr(page_table), lengths=_ptr(lengths), k_out=_ptr(k), v_out=_ptr(v))
-    _lib.check(_lib.lib().g4_paged_read(ctypes.byref(a), _stream()), "g4_paged_read")
+    dev = _device_of(layer, page_table, lengths)
+    k = torch.empty((B, count, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=layer.value.device)
+    v = torch.empty_like(k)
+    a = _lib.G4PagedReadArgs(cache, B, start, count, M, table_stride, page_table.data_ptr(), lengths.data_ptr(),
+                             k.data_ptr(), v.data_ptr())
+    _lib.check(_lib.lib().g4_paged_read(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_read")
     return k, v
 
 
