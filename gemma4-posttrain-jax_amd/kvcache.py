@@ -189,6 +189,65 @@ class KVCache(NamedTuple):
     length: int
 
 
+class PagedSpec(NamedTuple):
+    """How ``init_paged_kv_cache`` lays out a cache: positions per page, and whether pages hold e4m3 (one byte
+    per element and one scale per vector) instead of bf16."""
+
+    page_size: int = 64
+    e4m3: bool = False
+
+
+class PagedKVCache(NamedTuple):
+    """A model's cache in pages. Rows hold their real tokens only: position p of a row is its logical (RoPE)
+    position, so left pads take no slot and a finished row's masked steps append nothing. Sliding layers
+    share ``window_table``, whose rows cycle through the few pages that a window touches; global layers
+    ``page_table``. ``length`` counts the physical positions processed, pads included, as ``KVCache.length``."""
+
+    layers: tuple  # PagedLayerCache | None per layer
+    page_table: torch.Tensor  # [B, M] int32, of the global layers
+    window_table: torch.Tensor  # [B, M] int32, of the sliding layers
+    length: int
+
+    @property
+    def batch(self) -> int:
+        return self.page_table.shape[0]
+
+    @property
+    def device(self) -> torch.device:
+        return self.page_table.device
+
+    @property
+    def capacity(self) -> int:
+        """Positions that a row can hold."""
+
+        return self.page_table.shape[1] * next(x for x in self.layers if x is not None).page_size
+
+
+def init_paged_kv_cache(config: Gemma4TextConfig, batch_size: int, capacity: int, spec: PagedSpec = PagedSpec(),
+                        device="cuda") -> PagedKVCache:
+    """``init_kv_cache`` in pages: every row gets the pages of ``capacity`` positions on global layers and those
+    that a window can touch on sliding ones, ``None`` on kv-shared layers; zero-filled."""
+
+    if batch_size <= 0 or capacity <= 0:
+        raise ValueError(f"batch_size and capacity must be positive, got {batch_size} and {capacity}")
+    ps = spec.page_size
+    if ps not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {ps}")
+    width = (capacity + ps - 1) // ps
+    cycle = min(width, (config.sliding_window + ps - 2) // ps + 1)  # pages that a window touches at most
+    layers = []
+    for i in range(config.num_hidden_layers):
+        if is_kv_shared(config, i):
+            layers.append(None)
+            continue
+        pages = batch_size * (cycle if config.layer_types[i] == SLIDING else width)
+        layers.append(new_paged_layer(pages, layer_kv_heads(config, i), layer_head_dim(config, i), ps, e4m3=spec.e4m3,
+                                      device=device))
+    rows = torch.arange(batch_size, dtype=torch.int32, device=device)[:, None]
+    entry = torch.arange(width, dtype=torch.int32, device=device)[None, :]
+    return PagedKVCache(tuple(layers), rows * width + entry, rows * cycle + entry % cycle, 0)
+
+
 def new_layer_cache(batch: int, kv_heads: int, head_dim: int, capacity: int, ring: bool, dtype, device) -> LayerKVCache:
     ss = slot_stride_for(capacity)
     key = torch.zeros(key_shape(batch, kv_heads, ss, head_dim), dtype=dtype, device=device)
@@ -213,5 +272,5 @@ def init_kv_cache(config: Gemma4TextConfig, batch_size: int, capacity: int, dtyp
     return KVCache(tuple(layers), key_mask, 0)
 
 
-__all__ = ["LayerKVCache", "KVCache", "PagedLayerCache", "PAGE_SIZES", "new_paged_layer", "paged_key_shape", "init_kv_cache", "new_layer_cache", "slot_stride_for", "key_shape", "group_keys",
+__all__ = ["LayerKVCache", "KVCache", "PagedLayerCache", "PagedKVCache", "PagedSpec", "PAGE_SIZES", "new_paged_layer", "paged_key_shape", "init_kv_cache", "init_paged_kv_cache", "new_layer_cache", "slot_stride_for", "key_shape", "group_keys",
            "ungroup_keys", "group_values", "ungroup_values", "FULL", "SLIDING"]

@@ -37,7 +37,15 @@ from .config import (
     layer_intermediate_size,
     layer_kv_heads,
 )
-from .kvcache import KVCache, LayerKVCache, init_kv_cache, key_shape, slot_stride_for
+from .kvcache import (
+    KVCache,
+    LayerKVCache,
+    PagedKVCache,
+    init_kv_cache,
+    key_shape,
+    new_layer_cache,
+    slot_stride_for,
+)
 
 # --- parameter pytree (model.py:193-235) -----------------------------------------------------------
 
@@ -383,13 +391,13 @@ def forward_gemma4_text(
     *,
     config: Gemma4TextConfig,
     attention_mask: torch.Tensor | None = None,
-    kv_cache: KVCache | None = None,
+    kv_cache: KVCache | PagedKVCache | None = None,
     cache_mode: Literal["prefill", "append"] = "prefill",
     layer_outputs: list | None = None,
     remat_layers: bool = False,
     lora=None,
     write_pos: torch.Tensor | None = None,
-) -> tuple[torch.Tensor, KVCache | None]:
+) -> tuple[torch.Tensor, KVCache | PagedKVCache | None]:
     """model.py:571-673: hidden after the final norm and the updated cache.
 
     Without a cache the forward runs in prefill form over a scratch cache (the reference's
@@ -415,7 +423,13 @@ def forward_gemma4_text(
     ``write_pos`` (append mode only): int32 ``[B]`` device tensor holding the physical slot of
     this step (``kv_cache.length``) for every row. The kernels then read the slot on the device
     and the key mask is updated in place, so the step has no host-side value baked in and can be
-    captured in a HIP graph and replayed."""
+    captured in a HIP graph and replayed.
+
+    With a ``PagedKVCache`` (bf16 models) a token's place follows from ``position_ids`` and
+    ``attention_mask`` alone: each row holds its real tokens at their logical positions. A prefill
+    takes an empty cache and left-padded rows (a mask of zeros, then ones); a masked token of an
+    append is not stored and its row attends to nothing. ``write_pos`` then only asks for a step
+    without host-side values, whose token ids and positions are int32 on the device."""
 
     if lora is not None:
         raise NotImplementedError("LoRA adapters are not supported by the native rollout path")
@@ -427,6 +441,12 @@ def forward_gemma4_text(
         attention_mask = torch.ones((B, S), dtype=torch.bool, device=dev)
     attention_mask = attention_mask.to(torch.bool)
 
+    paged = isinstance(kv_cache, PagedKVCache)
+    if paged and params.embed_tokens.dtype != torch.bfloat16:
+        raise ValueError(f"a paged cache needs a bfloat16 model, got {params.embed_tokens.dtype}")
+    if paged and cache_mode == "prefill" and kv_cache.length != 0:
+        raise ValueError(f"a paged prefill needs an empty cache, this one holds {kv_cache.length} positions")
+
     # graphed decode step: the embedding, key-mask update and rotary tables in one native launch
     fused_prologue = (write_pos is not None and cache_mode == "append" and kv_cache is not None and S == 1
                       and params.embed_tokens.dtype == torch.bfloat16 and not config.hidden_size_per_layer_input
@@ -434,8 +454,9 @@ def forward_gemma4_text(
     if fused_prologue:
         tabs = (SLIDING, FULL)
         x, tables = kernels.decode_prologue(
-            params.embed_tokens, input_ids[:, 0], position_ids[:, 0], attention_mask[:, 0], write_pos,
-            kv_cache.key_mask, embed_scale=pw.embed_scale_f, inv_freq=[pw.inv_freq[t] for t in tabs])
+            params.embed_tokens, input_ids[:, 0], position_ids[:, 0], attention_mask[:, 0],
+            # a paged cache has no key mask: the step's own mask gets the values that it holds
+            position_ids[:, 0] if paged else write_pos, attention_mask if paged else kv_cache.key_mask, embed_scale=pw.embed_scale_f, inv_freq=[pw.inv_freq[t] for t in tabs])
         x = x.view(B, 1, -1)
         rot = {t: (c.view(B, 1, -1), sn.view(B, 1, -1)) for t, (c, sn) in zip(tabs, tables)}
         pli = None
@@ -451,12 +472,20 @@ def forward_gemma4_text(
     if cache_mode == "append" and S != 1:
         raise ValueError(f'cache_mode="append" requires one token, got {S}')
     length = int(kv_cache.length)
-    capacity = kv_cache.key_mask.shape[1]
+    capacity = kv_cache.capacity if paged else kv_cache.key_mask.shape[1]
     if S > capacity:
         raise ValueError(f"{S} tokens do not fit a cache of {capacity} positions")
-    if write_pos is not None:
-        if cache_mode != "append":
-            raise ValueError("write_pos is only used in append mode")
+    if write_pos is not None and cache_mode != "append":
+        raise ValueError("write_pos is only used in append mode")
+    if paged:
+        tables = {SLIDING: kv_cache.window_table, FULL: kv_cache.page_table}
+        if cache_mode == "prefill":  # token s of a row with n real tokens stands at position s - (S - n)
+            slot = attention_mask.sum(dim=-1, dtype=torch.int32) - S
+        else:
+            pos = position_ids[:, 0].to(torch.int32)
+            slot = torch.where(attention_mask[:, 0], pos, -1)
+            lengths = torch.where(attention_mask[:, 0], pos + 1, 0)
+    elif write_pos is not None:
         key_mask = kv_cache.key_mask
         if not fused_prologue:
             key_mask.scatter_(1, write_pos[:, None].long(), attention_mask)
@@ -466,7 +495,7 @@ def forward_gemma4_text(
         mask_start = min(max(length, 0), capacity - S)  # lax.dynamic_update_slice's clamp (model.py:602)
         key_mask[:, mask_start:mask_start + S] = attention_mask
         slot = length
-    chunk_prefill = cache_mode == "prefill" and length != 0  # model.py:615-617: the chunk attends to itself
+    chunk_prefill = cache_mode == "prefill" and length != 0 and not paged  # model.py:615-617: the chunk attends to itself
     if not fused_prologue:
         exact = x.dtype == torch.float32
         rot = {t: rotary_tables(pw.inv_freq[t], position_ids, exact) for t in (SLIDING, FULL)}
@@ -488,8 +517,35 @@ def forward_gemma4_text(
         layer_cache = kv_cache.layers[i]
         shared = is_kv_shared(config, i)
         qk_norms = [n if n is None else n.weight for n in (lp.attention.q_norm, lp.attention.k_norm)]
-        if write_pos is not None and _fused_decode_prep(x, B * H, D, new_layers[sources[i]] if shared else layer_cache,
-                                                        qk_norms):
+        if paged:
+            q_out = torch.empty((B, S, H, R, D), dtype=x.dtype, device=dev)
+            prep_q = dict(q_norm_weight=qk_norms[0], eps=eps, rope_cos=cos, rope_sin=sin)
+            src = sources[i] if shared else i
+            new_layers.append(layer_cache)
+            if shared:
+                kernels.prepare_q(q, q_out, flags=flags_q, **prep_q)
+            else:
+                k = qkv[..., H * R * D: (H * R + H) * D].view(B, S, H, D)
+                v = qkv[..., (H * R + H) * D:].view(B, S, H, D) if pk.has_v else k
+                flags = flags_kv
+                if cache_mode == "prefill":  # the chunk attends to itself, in bf16; the pages keep what later steps read
+                    chunk = new_layer_cache(B, H, D, S, False, x.dtype, dev)
+                    kernels.kv_append(chunk, k, v, write_pos=0, flags=flags_q | flags_kv, q=q, q_out=q_out,
+                                      k_norm_weight=qk_norms[1], **prep_q)
+                    prompt_kv[i] = (chunk.key, chunk.value_t)
+                else:
+                    flags |= flags_q
+                kernels.paged_append(layer_cache, k, v, page_table=tables[lt], write_pos=slot, keep=window, flags=flags,
+                                     k_norm_weight=qk_norms[1], q=q if flags & flags_q else None, q_out=q_out, **prep_q)
+            if cache_mode == "prefill":
+                attn = kernels.prefill_attention(q_out, *prompt_kv[src], attention_mask.contiguous(), window=window)
+                if src not in sources[i + 1:]:
+                    del prompt_kv[src]
+            else:
+                attn = kernels.paged_decode_attention(kv_cache.layers[src], q_out.view(B, H, R, D), page_table=tables[lt],
+                                                      lengths=lengths, window=window).view(B, 1, H, R, D)
+        elif write_pos is not None and _fused_decode_prep(
+                x, B * H, D, new_layers[sources[i]] if shared else layer_cache, qk_norms):
             # graphed decode step: g4_kv_append's work runs inside the
             # two-launch attention (G4DecodePrep) on the raw projection rows
             if shared:
@@ -579,6 +635,8 @@ def forward_gemma4_text(
     hidden = h
     if scratch_cache:
         return hidden, None
+    if paged:
+        return hidden, kv_cache._replace(length=length + S)
     return hidden, KVCache(tuple(new_layers), key_mask, length + S)
 
 
@@ -625,7 +683,7 @@ def forward_gemma4_lm(
     *,
     config: Gemma4TextConfig,
     attention_mask: torch.Tensor | None = None,
-    kv_cache: KVCache | None = None,
+    kv_cache: KVCache | PagedKVCache | None = None,
     cache_mode: Literal["prefill", "append"] = "prefill",
     logits_to_keep: int = 0,
     lora=None,

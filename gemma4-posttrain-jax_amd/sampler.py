@@ -19,7 +19,7 @@ import torch
 
 from . import _lib, kernels
 from .config import Gemma4TextConfig
-from .kvcache import KVCache, init_kv_cache
+from .kvcache import KVCache, PagedKVCache, PagedSpec, init_kv_cache, init_paged_kv_cache
 from .model import Gemma4Output, Gemma4TextParams, _proj, checked_softcap, forward_gemma4_lm, forward_gemma4_text
 
 
@@ -74,8 +74,10 @@ def prefill(
     cache_dtype: Any | None = None,
     mesh=None,
     lora=None,
+    paged: PagedSpec | None = None,
 ) -> Gemma4Output:
-    """sampler.py:70-106: encode a left-padded prompt and populate the caches."""
+    """sampler.py:70-106: encode a left-padded prompt and populate the caches. With ``paged`` (bf16 models) the
+    cache is a ``PagedKVCache`` of that layout: each row keeps its real tokens only, in bf16 or e4m3."""
 
     _no_mesh(mesh)
     if prompt_ids.dim() != 2 or tuple(prompt_mask.shape) != tuple(prompt_ids.shape):
@@ -85,6 +87,15 @@ def prefill(
         raise ValueError(f"max_new_tokens must be non-negative, got {max_new_tokens}")
     B, P = prompt_ids.shape
     dtype = params.embed_tokens.dtype if cache_dtype is None else cache_dtype
+    if paged is not None:
+        if cache_dtype is not None:
+            raise ValueError("a paged cache's format is its spec's: leave cache_dtype out")
+        real = prompt_mask.to(torch.bool)
+        if bool((real[:, :-1] & ~real[:, 1:]).any()):
+            raise ValueError("a paged prefill takes left-padded prompts: a mask of zeros, then ones")
+        pages = init_paged_kv_cache(config, B, P + max_new_tokens, paged, prompt_ids.device)
+        return forward_gemma4_lm(params, prompt_ids, _position_ids(prompt_mask), config=config, attention_mask=real,
+                                 kv_cache=pages, cache_mode="prefill", logits_to_keep=1, lora=lora)
     cache = init_kv_cache(config, B, P + max_new_tokens, dtype, prompt_ids.device)
     return forward_gemma4_lm(params, prompt_ids, _position_ids(prompt_mask), config=config,
                              attention_mask=prompt_mask.to(torch.bool), kv_cache=cache, cache_mode="prefill",
@@ -96,7 +107,7 @@ def decode_step(
     config: Gemma4TextConfig,
     token_ids: torch.Tensor,
     position_ids: torch.Tensor,
-    kv_cache: KVCache,
+    kv_cache: KVCache | PagedKVCache,
     *,
     attention_mask: torch.Tensor | None = None,
     mesh=None,
@@ -133,19 +144,23 @@ class GraphedDecodeStep:
     logits.
 
     Capture runs the step once eagerly first (library handles, packed weights); that warm-up
-    writes the cache slot ``cache.length``, which the first replay then overwrites.
+    writes the cache slot ``cache.length``, which the first replay then overwrites (nothing in a paged
+    cache).
     """
 
-    def __init__(self, params: Gemma4TextParams, config: Gemma4TextConfig, cache: KVCache, *,
+    def __init__(self, params: Gemma4TextParams, config: Gemma4TextConfig, cache: KVCache | PagedKVCache, *,
                  temperature: float | None = None, key: torch.Tensor | None = None, top_k: int = 0,
                  top_p: float = 1.0) -> None:
-        dev = cache.key_mask.device
-        B = cache.key_mask.shape[0]
+        if isinstance(cache, PagedKVCache):
+            dev, B = cache.device, cache.batch
+        else:
+            dev, B = cache.key_mask.device, cache.key_mask.shape[0]
         self.params, self.config, self.cache = params, config, cache
         self.length = int(cache.length)
         self.tok = torch.zeros(B, dtype=torch.int32, device=dev)
         self.pos = torch.zeros(B, dtype=torch.int32, device=dev)
-        self.active = torch.ones(B, dtype=torch.bool, device=dev)
+        # the warm-up's place is its positions' (0) in pages, a real token's: with the rows inactive it stores nothing
+        self.active = torch.full((B,), not isinstance(cache, PagedKVCache), dtype=torch.bool, device=dev)
         self.slot = torch.full((B,), self.length, dtype=torch.int32, device=dev)
         if temperature is not None and temperature > 0 and key is None:
             raise ValueError("sampling in the graph needs the device key")
@@ -245,7 +260,7 @@ class GraphedDecodeStep:
         return self.logits
 
     @property
-    def kv_cache(self) -> KVCache:
+    def kv_cache(self) -> KVCache | PagedKVCache:
         return self.cache._replace(length=self.length)
 
 
@@ -343,10 +358,11 @@ def generate(
     key=None,
     mesh=None,
     lora=None,
+    paged: PagedSpec | None = None,
 ) -> RolloutBatch:
     """sampler.py:204-322: prefill, then up to ``max_new_tokens`` sample + append steps, stopping
     once every row has emitted an EOS id. Inactive rows emit pad with logp 0; the decode on the
-    final step is skipped, so the cache never overflows."""
+    final step is skipped, so the cache never overflows. ``paged``: the cache in pages (``prefill``)."""
 
     _no_mesh(mesh)
     sc = sampler_config
@@ -363,7 +379,8 @@ def generate(
     checked_softcap(config.final_logit_softcapping)
 
     prompt_mask = prompt_mask.to(torch.bool)
-    out = prefill(params, config, prompt_ids, prompt_mask, max_new_tokens=sc.max_new_tokens, mesh=mesh, lora=lora)
+    out = prefill(params, config, prompt_ids, prompt_mask, max_new_tokens=sc.max_new_tokens, mesh=mesh, lora=lora,
+                  paged=paged)
     dev = prompt_ids.device
     B, N = prompt_ids.shape[0], sc.max_new_tokens
     key_state = key_tensor(key, dev, sc.seed)  # the loop's key, split once per step on the device
@@ -442,8 +459,9 @@ class NativeRollout:
     """sampler.py:325-352 (``PureJaxRollout``): host-side parameter holder around ``generate``."""
 
     def __init__(self, params: Gemma4TextParams, model_config: Gemma4TextConfig, sampler_config: SamplerConfig,
-                 mesh=None) -> None:
+                 mesh=None, paged: PagedSpec | None = None) -> None:
         _no_mesh(mesh)
+        self.paged = paged
         self.params = params
         self.model_config = model_config
         self.sampler_config = sampler_config
@@ -454,7 +472,7 @@ class NativeRollout:
 
     def generate(self, prompt_ids: torch.Tensor, prompt_mask: torch.Tensor, *, key=None) -> RolloutBatch:
         return generate(self.params, self.model_config, prompt_ids, prompt_mask, sampler_config=self.sampler_config,
-                        key=key, mesh=self.mesh)
+                        key=key, mesh=self.mesh, paged=self.paged)
 
 
 PureJaxRollout = NativeRollout  # the reference's class name, for drop-in callers

@@ -231,3 +231,27 @@ def test_front_end_refuses_bad_operands():
         read(start=-1)
     with pytest.raises(ValueError, match="count"):
         read(count=0)
+
+
+def test_init_paged_kv_cache():
+    import hf_util as H
+    from gemma4_posttrain_jax_amd import config as C
+    from gemma4_posttrain_jax_amd.kvcache import PagedSpec, init_paged_kv_cache
+
+    cfg = C.config_from_hf(dict(H.CFG1, sliding_window=40))
+    cache = init_paged_kv_cache(cfg, 3, 200, PagedSpec(32), device="cpu")
+    assert cache.batch == 3 and cache.capacity == 224 and cache.length == 0
+    assert tuple(cache.page_table.shape) == tuple(cache.window_table.shape) == (3, 7)
+    cycle = 3  # 40 positions touch 2 or 3 pages of 32
+    for i, layer in enumerate(cache.layers):
+        sliding = cfg.layer_types[i] == C.SLIDING
+        table = cache.window_table if sliding else cache.page_table
+        assert layer.num_pages == 3 * (cycle if sliding else 7)
+        assert int(table.min()) == 0 and int(table.max()) == layer.num_pages - 1
+        for b in range(3):
+            assert len(set(table[b].tolist())) == (cycle if sliding else 7)
+            for j in range(7 - cycle):  # no page twice within a window
+                assert len(set(table[b, j: j + cycle].tolist())) == cycle
+    for bad in (dict(batch_size=0), dict(capacity=0), dict(spec=PagedSpec(40))):
+        with pytest.raises(ValueError):
+            init_paged_kv_cache(cfg, **{**dict(batch_size=1, capacity=10, device="cpu"), **bad})
