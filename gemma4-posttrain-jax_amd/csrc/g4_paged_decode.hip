@@ -10,6 +10,8 @@
 // ones fill the chip alike. The lengths stand on the device, so each workgroup finds its piece from them
 // itself. A (row, head) of one piece is finished by it; the others leave (m, l, o) per piece, which a second
 // launch joins in the pieces' order.
+#include <type_traits>
+
 #include "g4_paged.h"
 
 namespace g4 {
@@ -19,14 +21,24 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr int kCus = 256, kXcds = 8;
 
-template <int D, bool SPLIT>
+// 16 bytes by the caches' usual way, or past them.
+template <bool NT>
+__device__ __forceinline__ u32x4 load_piece(std::bool_constant<NT>, __amdgpu_buffer_rsrc_t r, uint32_t voffset, uint32_t soffset) {
+  if constexpr (NT)
+    return buffer_load16_nt(r, voffset, soffset);
+  else
+    return buffer_load16(r, voffset, soffset);
+}
+
+template <int D, int WAVES_>
 struct Groups {
-  static constexpr int SIMD_WAVES = D >= 256 ? 2 : 4;          // resident, by registers
-  static constexpr int WAVES = SPLIT && D < 512 ? 4 : 8;        // per workgroup
-  static constexpr int PARTS = D == 512 ? 2 : 1;                // waves that share a chunk, a half of the dims each
-  static constexpr int KEYS = WAVES / PARTS;                    // chunks in work at a time
+  static constexpr int WAVES = WAVES_;                  // per workgroup
+  static constexpr int SIMD_WAVES = D >= 256 ? 2 : 4;   // resident, by registers
+  static constexpr int PARTS = D == 512 ? 2 : 1;        // waves that share a chunk, a half of the dims each
+  static constexpr int KEYS = WAVES / PARTS;            // chunks in work at a time
   static constexpr int THREADS = 64 * WAVES;
 };
+constexpr int split_waves(int D) { return D == 512 ? 8 : 4; }
 // Workgroups of the split kernel that are resident at once.
 constexpr int resident(int D) { return kCus * (D == 512 ? 1 : (D == 256 ? 2 : 4)); }
 // elements between q rows (bf16) and between o rows (f32) in LDS: 16 rows' accesses fall on different banks
@@ -34,9 +46,9 @@ constexpr int q_stride(int D) { return D + 8; }
 constexpr int o_stride(int D) { return D + 4; }
 
 // Floats of LDS for the waves' o; with two parts the scores of two turns are exchanged there before.
-template <int D, bool SPLIT>
+template <int D, int WAVES>
 __host__ __device__ constexpr int o_floats(int R) {
-  using G = Groups<D, SPLIT>;
+  using G = Groups<D, WAVES>;
   const int o = G::KEYS * R * o_stride(D), scores = G::PARTS == 2 ? 2 * G::WAVES * 64 * 8 : 0;
   return o > scores ? o : scores;
 }
@@ -134,8 +146,8 @@ __device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room,
 #pragma unroll
   for (int i = 0; i < kTries; ++i) {
     const int target = pairs < room ? room - (int)((int64_t)pairs * i / (kTries - 1)) : room / 2;
-    const int per = (int)((float)total / (float)target) + 1;
-    share[i] = 1.f / (float)(per > min_per ? per : min_per);
+    const int per = (int)((float)total * __builtin_amdgcn_rcpf((float)target)) + 1;
+    share[i] = __builtin_amdgcn_rcpf((float)(per > min_per ? per : min_per));
     n_pieces[i] = 0;
   }
   // ceil(n / per): floor((n - 1) / per) + 1, the quotient off a whole number by 1 / per at least where it is not one
@@ -143,9 +155,11 @@ __device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room,
   for (int b0 = 0; b0 < B; b0 += kRows) {
     if (B > kRows) load_rows(b0);
 #pragma unroll
-    for (int j = 0; j < kRowRegs; ++j)
+    for (int j = 0; j < kRowRegs; ++j) {
+      if (b0 + 64 * j >= B) break;
 #pragma unroll
       for (int i = 0; i < kTries; ++i) n_pieces[i] += pieces_of(b0 + 64 * j + lane, rows[j].chunks(), share[i]);
+    }
   }
   float cut = share[kTries - 1];
   int count = 0;
@@ -163,6 +177,7 @@ __device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room,
     if (B > kRows) load_rows(b0);
 #pragma unroll
     for (int j = 0; j < kRowRegs; ++j) {
+      if (b0 + 64 * j >= B) break;
       const int k = pieces_of(b0 + 64 * j + lane, rows[j].chunks(), cut), used = k > 1 ? k * H : 0;
       const int incl = scan_incl(k * H), sincl = scan_incl(used);
       const int end = before + __builtin_amdgcn_readlane(incl, 63);
@@ -185,17 +200,17 @@ __device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room,
   return false;
 }
 
-template <int D, bool F8, bool SPLIT>
-__global__ __launch_bounds__((Groups<D, SPLIT>::THREADS)) __attribute__((amdgpu_waves_per_eu(Groups<D, SPLIT>::SIMD_WAVES)))
-void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
-  using G = Groups<D, SPLIT>;
+template <int D, bool F8, int WAVES, bool SPLIT>
+__global__ __launch_bounds__((Groups<D, WAVES>::THREADS)) __attribute__((amdgpu_waves_per_eu(Groups<D, WAVES>::SIMD_WAVES)))
+void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room, int large) {
+  using G = Groups<D, WAVES>;
   constexpr int kThreads = G::THREADS, kKeys = G::KEYS, DW = D / G::PARTS;
   using Sh = Shape<DW, F8>;
   constexpr int kChunkBytes = 32 * D * Sh::BYTES;
   // [kKeys][R][o_stride(D)] o, in its place before that the score exchange | [R][q_stride(D)] q | [kKeys][16] m, l
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int R = a.group, H = a.cache.kv_heads, ps = a.cache.page_size;
-  uint16_t* q_lds = reinterpret_cast<uint16_t*>(lds + o_floats<D, SPLIT>(R));
+  uint16_t* q_lds = reinterpret_cast<uint16_t*>(lds + o_floats<D, WAVES>(R));
   float* m_lds = reinterpret_cast<float*>(q_lds + R * q_stride(D));
   float* l_lds = m_lds + kKeys * 16;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, grp = lane >> 4;
@@ -254,146 +269,156 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room) {
     pages = mine < last ? table[mine >> page_shift] : -1;
   };
   auto wait_pages = [&]() { __asm__ volatile("" : "+v"(pages)); };  // here, not at every use behind a branch
-  auto load_keys = [&](const Place& at) {
+  int c = c_first + key_wave, turn = 0;  // the wave's chunk and its number among the wave's
+  // the first page by the scalar cache, the sooner
+  const int entry = (c < last ? c : (last > 0 ? last - 1 : 0)) >> page_shift;
+  const int page = __builtin_amdgcn_readfirstlane(table[entry]);
+  // Keys and values that this call reads once pass the caches by (non-temporal loads), unless a row beside this one
+  // has the same page here, or the call is so small that its latency counts (kStreamBytes).
+  const int before = table[entry - (b > 0 ? a.table_stride : 0)], after = table[entry + (b + 1 < a.batch ? a.table_stride : 0)];
+  const bool stream = large && !(b > 0 && before == page) && !(b + 1 < a.batch && after == page);
+  auto load_keys = [&](const Place& at, auto nt) {
     const __amdgpu_buffer_rsrc_t r =
         make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.key) + at.slot * (D * Sh::BYTES), at.there ? kChunkBytes : 0);
+    const int lane_at = col * 64 + grp * 16;
 #pragma unroll
-    for (int s = 0; s < Sh::KRUNS; ++s)
-#pragma unroll
-      for (int bb = 0; bb < 2; ++bb) kv[bb][s] = buffer_load16(r, col * 64 + grp * 16, ((half * Sh::KRUNS + s) * 2 + bb) * 1024);
+    for (int i = 0; i < 2 * Sh::KRUNS; ++i) kv[i % 2][i / 2] = load_piece(nt, r, lane_at, (2 * half * Sh::KRUNS + i) * 1024);
     if constexpr (F8) {
       const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.cache.key_scale + at.slot, at.there ? 32 : 0);
       kscale = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * grp, 0, 0));
     }
   };
-  auto load_values = [&](const Place& at) {
+  auto load_values = [&](const Place& at, auto nt) {
     const __amdgpu_buffer_rsrc_t r =
         make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.value) + at.slot * (D * Sh::BYTES), at.there ? kChunkBytes : 0);
+    const int lane_at = (grp * (D * Sh::BYTES / 2) + col) * 16;
 #pragma unroll
-    for (int t = 0; t < Sh::VLOADS; ++t) vv[t] = buffer_load16(r, (grp * (D * Sh::BYTES / 2) + col) * 16, (half * Sh::VLOADS + t) * 256);
+    for (int t = 0; t < Sh::VLOADS; ++t) vv[t] = load_piece(nt, r, lane_at, (half * Sh::VLOADS + t) * 256);
     if constexpr (F8) {
       const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.cache.value_scale + at.slot, at.there ? 32 : 0);
       vscale = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * grp, 0, 0));
     }
   };
 
-  int c = c_first + key_wave, turn = 0;  // the wave's chunk and its number among the wave's
-  // the first page by the scalar cache, the sooner
-  const int entry = (c < last ? c : (last > 0 ? last - 1 : 0)) >> page_shift;
-  const int page = __builtin_amdgcn_readfirstlane(table[entry]);
   load_pages(c);
-  // every load below is issued by every wave, so that the waits for them can count: no branch but zero bytes
-  Place at = place_of(c < last ? page : -1, c);
-  load_keys(at);
-  load_values(at);
-  wait_pages();
+  auto attend = [&](auto nt) {
+    // every load below is issued by every wave, so that the waits for them can count: no branch but zero bytes
+    Place at = place_of(c < last ? page : -1, c);
+    load_keys(at, nt);
+    load_values(at, nt);
+    wait_pages();
 #pragma unroll
-  for (int j = 0; j < kQLoads; ++j)
-    if (tid + j * kThreads < R * D / 8)
-      *reinterpret_cast<u32x4*>(q_lds + (tid + j * kThreads) / (D / 8) * q_stride(D) + tid % (D / 8) * 8) = qv[j];
-  __syncthreads();
-  // the columns beyond the R rows compute on the last row and are dropped
-  const uint16_t* qrow = q_lds + (col < R ? col : R - 1) * q_stride(D) + half * DW + (F8 ? 16 : 8) * grp;
-  // operand s: e4m3 keys come 16 consecutive dims a load, two operands
-  auto qop = [&](int s) -> bf16x8 { return as_bf16x8(load16(qrow + (F8 ? 64 * (s / 2) + 8 * (s % 2) : 32 * s))); };
-  // two parts meet at a barrier in every turn, so all waves take the turns of the first
-  const int turns = (last - (G::PARTS == 2 ? c_first : c) + kKeys - 1) / kKeys;
-  while (turn < turns) {
-    const bool more = c + kKeys < last;
-    ++turn;
-    if ((turn & 63) == 0) {
-      load_pages(c + kKeys);
-      wait_pages();
-    }
-    const Place next = place_of(more ? __builtin_amdgcn_readlane(pages, turn & 63) : -1, c + kKeys);
-    const int lo = at.there ? keys.lo : keys.hi, hi = keys.hi;  // this chunk's keys are those in [lo, hi)
-    floatx4 sc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
+    for (int j = 0; j < kQLoads; ++j)
+      if (tid + j * kThreads < R * D / 8)
+        *reinterpret_cast<u32x4*>(q_lds + (tid + j * kThreads) / (D / 8) * q_stride(D) + tid % (D / 8) * 8) = qv[j];
+    __syncthreads();
+    // the columns beyond the R rows compute on the last row and are dropped
+    const uint16_t* qrow = q_lds + (col < R ? col : R - 1) * q_stride(D) + half * DW + (F8 ? 16 : 8) * grp;
+    // operand s: e4m3 keys come 16 consecutive dims a load, two operands
+    auto qop = [&](int s) -> bf16x8 { return as_bf16x8(load16(qrow + (F8 ? 64 * (s / 2) + 8 * (s % 2) : 32 * s))); };
+    // two parts meet at a barrier in every turn, so all waves take the turns of the first
+    const int turns = (last - (G::PARTS == 2 ? c_first : c) + kKeys - 1) / kKeys;
+    while (turn < turns) {
+      const bool more = c + kKeys < last;
+      ++turn;
+      if ((turn & 63) == 0) {
+        load_pages(c + kKeys);
+        wait_pages();
+      }
+      const Place next = place_of(more ? __builtin_amdgcn_readlane(pages, turn & 63) : -1, c + kKeys);
+      const int lo = at.there ? keys.lo : keys.hi, hi = keys.hi;  // this chunk's keys are those in [lo, hi)
+      floatx4 sc[2] = {floatx4{0.f, 0.f, 0.f, 0.f}, floatx4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int s = 0; s < Sh::KRUNS; ++s)
+      for (int s = 0; s < Sh::KRUNS; ++s)
 #pragma unroll
-      for (int bb = 0; bb < 2; ++bb) {
+        for (int bb = 0; bb < 2; ++bb) {
+          if constexpr (F8) {
+            sc[bb] = mfma16x16x32(e4m3_operand(kv[bb][s][0], kv[bb][s][1]), qop(2 * s), sc[bb]);
+            sc[bb] = mfma16x16x32(e4m3_operand(kv[bb][s][2], kv[bb][s][3]), qop(2 * s + 1), sc[bb]);
+          } else {
+            sc[bb] = mfma16x16x32(as_bf16x8(kv[bb][s]), qop(s), sc[bb]);
+          }
+        }
+      if constexpr (G::PARTS == 2) {  // the sum of both halves' scores, the same in both waves
+        float* mine = lds + (((turn & 1) * G::WAVES + w) * 64 + lane) * 8;
+        const float* other = lds + (((turn & 1) * G::WAVES + (w ^ 1)) * 64 + lane) * 8;
+        *reinterpret_cast<floatx4*>(mine) = sc[0];
+        *reinterpret_cast<floatx4*>(mine + 4) = sc[1];
+        wg_barrier();
+        sc[0] += *reinterpret_cast<const floatx4*>(other);
+        sc[1] += *reinterpret_cast<const floatx4*>(other + 4);
+      }
+      if constexpr (F8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j / 4][j % 4] *= exp2_byte((j < 4 ? kscale.x : kscale.y) >> (8 * (j % 4)) & 0xff);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_keys(next, nt);
+      __builtin_amdgcn_sched_barrier(0);
+
+      // keys 8 grp + j of the chunk
+      const bool inner = c * 32 >= lo && c * 32 + 32 <= hi;  // every slot is an attended key
+      float p[8], mx = m;
+      bool on[8];
+      const int j_lo = lo - (c * 32 + 8 * grp), j_hi = hi - (c * 32 + 8 * grp);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        on[j] = (j >= j_lo) & (j < j_hi);
+        p[j] = on[j] ? sc[j / 4][j % 4] : kNegInf;
+        mx = fmaxf(mx, p[j]);
+      }
+      mx = column_max(mx);
+      const float base = mx == kNegInf ? 0.f : mx;
+      if (__any(mx > m)) {
+        const float alpha = __builtin_amdgcn_exp2f((m - base) * kLog2e);
+        m = mx;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < DW / 16; ++t) o[t] *= alpha;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f((p[j] - base) * kLog2e);
+        l += p[j];
         if constexpr (F8) {
-          sc[bb] = mfma16x16x32(e4m3_operand(kv[bb][s][0], kv[bb][s][1]), qop(2 * s), sc[bb]);
-          sc[bb] = mfma16x16x32(e4m3_operand(kv[bb][s][2], kv[bb][s][3]), qop(2 * s + 1), sc[bb]);
-        } else {
-          sc[bb] = mfma16x16x32(as_bf16x8(kv[bb][s]), qop(s), sc[bb]);
+          const float v = p[j] * exp2_byte((j < 4 ? vscale.x : vscale.y) >> (8 * (j % 4)) & 0xff);
+          p[j] = on[j] ? v : 0.f;
         }
       }
-    if constexpr (G::PARTS == 2) {  // the sum of both halves' scores, the same in both waves
-      float* mine = lds + (((turn & 1) * G::WAVES + w) * 64 + lane) * 8;
-      const float* other = lds + (((turn & 1) * G::WAVES + (w ^ 1)) * 64 + lane) * 8;
-      *reinterpret_cast<floatx4*>(mine) = sc[0];
-      *reinterpret_cast<floatx4*>(mine + 4) = sc[1];
-      wg_barrier();
-      sc[0] += *reinterpret_cast<const floatx4*>(other);
-      sc[1] += *reinterpret_cast<const floatx4*>(other + 4);
-    }
-    if constexpr (F8) {
+      const bf16x8 pop = as_bf16x8(u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
+                                         pack_bf16x2(p[6], p[7])});
+      if (!inner) {  // the slots of no attended key may hold anything: 0 x NaN is no 0
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sc[j / 4][j % 4] *= exp2_byte((j < 4 ? kscale.x : kscale.y) >> (8 * (j % 4)) & 0xff);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    load_keys(next);
-    __builtin_amdgcn_sched_barrier(0);
-
-    // keys 8 grp + j of the chunk
-    const bool inner = c * 32 >= lo && c * 32 + 32 <= hi;  // every slot is an attended key
-    float p[8], mx = m;
-    bool on[8];
-    const int j_lo = lo - (c * 32 + 8 * grp), j_hi = hi - (c * 32 + 8 * grp);
+        for (int i = 0; i < 4; ++i) {
+          // e4m3: dword i is keys 4 (i % 2) .. + 3; bf16: keys 2 i, 2 i + 1
+          constexpr int KEYS = F8 ? 4 : 2;
+          uint32_t mask = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      on[j] = (j >= j_lo) & (j < j_hi);
-      p[j] = on[j] ? sc[j / 4][j % 4] : kNegInf;
-      mx = fmaxf(mx, p[j]);
-    }
-    mx = column_max(mx);
-    const float base = mx == kNegInf ? 0.f : mx;
-    if (__any(mx > m)) {
-      const float alpha = __builtin_amdgcn_exp2f((m - base) * kLog2e);
-      m = mx;
-      l *= alpha;
+          for (int j = 0; j < KEYS; ++j) mask |= on[KEYS * (i % (8 / KEYS)) + j] ? (F8 ? 0xffu : 0xffffu) << (32 / KEYS * j) : 0u;
 #pragma unroll
-      for (int t = 0; t < DW / 16; ++t) o[t] *= alpha;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      p[j] = __builtin_amdgcn_exp2f((p[j] - base) * kLog2e);
-      l += p[j];
-      if constexpr (F8) {
-        const float v = p[j] * exp2_byte((j < 4 ? vscale.x : vscale.y) >> (8 * (j % 4)) & 0xff);
-        p[j] = on[j] ? v : 0.f;
+          for (int t = 0; t < Sh::VLOADS; ++t) vv[t][i] &= mask;
+        }
       }
-    }
-    const bf16x8 pop = as_bf16x8(u32x4{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]),
-                                       pack_bf16x2(p[6], p[7])});
-    if (!inner) {  // the slots of no attended key may hold anything: 0 x NaN is no 0
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // e4m3: dword i is keys 4 (i % 2) .. + 3; bf16: keys 2 i, 2 i + 1
-        constexpr int KEYS = F8 ? 4 : 2;
-        uint32_t mask = 0;
-#pragma unroll
-        for (int j = 0; j < KEYS; ++j) mask |= on[KEYS * (i % (8 / KEYS)) + j] ? (F8 ? 0xffu : 0xffffu) << (32 / KEYS * j) : 0u;
-#pragma unroll
-        for (int t = 0; t < Sh::VLOADS; ++t) vv[t][i] &= mask;
+      for (int t = 0; t < Sh::VLOADS; ++t) {
+        if constexpr (F8) {
+          o[2 * t] = mfma16x16x32(e4m3_operand(vv[t][0], vv[t][1]), pop, o[2 * t]);
+          o[2 * t + 1] = mfma16x16x32(e4m3_operand(vv[t][2], vv[t][3]), pop, o[2 * t + 1]);
+        } else {
+          o[t] = mfma16x16x32(as_bf16x8(vv[t]), pop, o[t]);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
+      load_values(next, nt);
+      __builtin_amdgcn_sched_barrier(0);
+      at = next;
+      c += kKeys;
     }
-#pragma unroll
-    for (int t = 0; t < Sh::VLOADS; ++t) {
-      if constexpr (F8) {
-        o[2 * t] = mfma16x16x32(e4m3_operand(vv[t][0], vv[t][1]), pop, o[2 * t]);
-        o[2 * t + 1] = mfma16x16x32(e4m3_operand(vv[t][2], vv[t][3]), pop, o[2 * t + 1]);
-      } else {
-        o[t] = mfma16x16x32(as_bf16x8(vv[t]), pop, o[t]);
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    load_values(next);
-    __builtin_amdgcn_sched_barrier(0);
-    at = next;
-    c += kKeys;
-  }
+  };
+  if (stream)
+    attend(std::true_type{});
+  else
+    attend(std::false_type{});
 
   // the waves' parts joined: o = sum_w exp(m_w - m) o_w, l likewise
   l = column_sum(l);
@@ -500,19 +525,33 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(G4PagedDecodeA
   }
 }
 
-template <int D, bool SPLIT>
+template <int D, int WAVES>
 size_t lds_bytes(int R) {
-  using G = Groups<D, SPLIT>;
-  return ((size_t)o_floats<D, SPLIT>(R) + (size_t)R * q_stride(D) / 2 + 2 * G::KEYS * 16) * sizeof(float);
+  return ((size_t)o_floats<D, WAVES>(R) + (size_t)R * q_stride(D) / 2 + 2 * Groups<D, WAVES>::KEYS * 16) * sizeof(float);
 }
 
-// Whether the rows are cut into pieces: where a row can have more chunks than its workgroup's waves take in
-// kWholeTurns turns.
-constexpr int kWholeTurns = 4;
+// Whether the rows are cut into pieces: where a row can have more chunks than one workgroup is as fast with. Finding
+// the pieces and joining them takes about 4 us; a workgroup takes 1 us for 100 keys of 256 dims in bf16, 130 in e4m3 (us
+// per call, whole / split: 2 pairs of 512 keys 8.7 / 9.7, of 1024 13.8 / 9.7, 16 pairs of 1024 15.6 / 11.8, but 64 pairs of
+// 1024 16.3 / 18.6, 128 pairs 28 / 32, 512 pairs 94 / 99, where the whole rows fill the chip).
+constexpr int kSplitPairs = 32, kWholeChunksFew = 20, kWholeChunks = 32;
 bool split(const G4PagedDecodeArgs& a) {
   const int64_t cap = (int64_t)a.max_pages * a.cache.page_size;
   const int64_t keys = a.window > 0 && a.window < cap ? a.window + 31 : cap;  // a window may begin inside a chunk
-  return (keys + 31) / 32 > (a.cache.head_dim == 512 ? Groups<512, false>::KEYS : Groups<256, false>::KEYS) * kWholeTurns;
+  const bool few = (int64_t)a.batch * a.cache.kv_heads <= kSplitPairs;
+  return (keys + 31) / 32 > (few ? kWholeChunksFew : kWholeChunks);
+}
+
+// Whether the call's keys and values are many enough to pass the caches by. From caches in turn that together pass
+// the last-level cache (us per call, plain / non-temporal): 512 pairs of 200 - 767 keys in bf16, 256 MB, 54.4 / 48.2, 16 x 2
+// rows of up to 32768 keys 102 / 90 (e4m3 58.4 / 51.3), 128 pairs of 512 keys in e4m3 13.2 / 12.1, but 2 pairs of 512 keys
+// 10.6 / 12.1. Rows that share pages read them from their XCD's cache: 64 rows, 8 of each with the same 4096 positions,
+// 28.2 / 35.5.
+constexpr int64_t kStreamBytes = 8 << 20;
+bool large(const G4PagedDecodeArgs& a) {
+  const int64_t cap = (int64_t)a.max_pages * a.cache.page_size;
+  const int64_t keys = a.window > 0 && a.window < cap ? a.window : cap;
+  return keys * a.batch * a.cache.kv_heads * a.cache.head_dim * (a.cache.format == G4_PAGES_E4M3 ? 2 : 4) >= kStreamBytes;
 }
 
 // A split (row, head) of n > per chunks has at most 2 n / per pieces, and per >= total / room but for the f32
@@ -525,10 +564,10 @@ size_t workspace_bytes(const G4PagedDecodeArgs& a) {
   return slots(a) * a.group * ((size_t)a.cache.head_dim + 2) * 4 + (size_t)a.batch * a.cache.kv_heads * 8;
 }
 
-template <int D, bool F8, bool SPLIT>
+template <int D, bool F8, int WAVES, bool SPLIT>
 int launch_kernel(const G4PagedDecodeArgs& a, const Workspace& ws, int64_t groups, hipStream_t st) {
-  const size_t lds = lds_bytes<D, SPLIT>(a.group);
-  const void* fn = (const void*)paged_decode_kernel<D, F8, SPLIT>;
+  const size_t lds = lds_bytes<D, WAVES>(a.group);
+  const void* fn = (const void*)paged_decode_kernel<D, F8, WAVES, SPLIT>;
   if (lds > 64 * 1024) {
     int dev = 0;
     const int rc = device_setup(&dev);
@@ -537,19 +576,35 @@ int launch_kernel(const G4PagedDecodeArgs& a, const Workspace& ws, int64_t group
       return fail(G4_ERR_LAUNCH, "g4_paged_decode_attention: the kernel's LDS limit could not be raised");
   }
   const dim3 grid((unsigned)((groups + kXcds - 1) / kXcds * kXcds));
-  hipLaunchKernelGGL((paged_decode_kernel<D, F8, SPLIT>), grid, dim3(Groups<D, SPLIT>::THREADS), lds, st, a, ws, resident(D));
+  hipLaunchKernelGGL((paged_decode_kernel<D, F8, WAVES, SPLIT>), grid, dim3(Groups<D, WAVES>::THREADS), lds, st, a, ws,
+                     resident(D), (int)large(a));
   return check_launch("g4_paged_decode_attention");
 }
+
+// Waves of a whole row's workgroup. A CU's vector cache gives 64 bytes a clock, which four waves of bf16 loads take
+// up, so more of them only add to the join at the end (512 keys of 256 dims, us per call, 8 / 4 waves: 2 pairs 9.6 /
+// 8.7, 64 pairs 11.5 / 10.5, 512 pairs 50.1 / 48.6). e4m3 halves the bytes and adds the conversions, which eight waves
+// share better while CUs are to spare (2 pairs 7.9 / 8.7, 64 pairs 9.2 / 9.9, 256 pairs 14.2 / 13.6, 512 pairs 30.4 /
+// 27.3).
+constexpr int kFewPairs = 256;
 
 template <int D, bool F8>
 int launch(const G4PagedDecodeArgs& a, hipStream_t st) {
   const int64_t pairs = (int64_t)a.batch * a.cache.kv_heads;
   Workspace ws{};
-  if (!split(a)) return launch_kernel<D, F8, false>(a, ws, pairs, st);
+  if (!split(a)) {
+    if constexpr (D == 512) {
+      return launch_kernel<D, F8, 8, false>(a, ws, pairs, st);
+    } else {
+      if constexpr (F8)
+        if (pairs < kFewPairs) return launch_kernel<D, F8, 8, false>(a, ws, pairs, st);
+      return launch_kernel<D, F8, 4, false>(a, ws, pairs, st);
+    }
+  }
   ws.o = reinterpret_cast<float*>(a.workspace);
   ws.ml = ws.o + slots(a) * a.group * D;
   ws.ranges = reinterpret_cast<int2*>(ws.ml + slots(a) * a.group * 2);
-  const int rc = launch_kernel<D, F8, true>(a, ws, resident(D) + pairs + kSpare, st);
+  const int rc = launch_kernel<D, F8, split_waves(D), true>(a, ws, resident(D) + pairs + kSpare, st);
   if (rc != G4_OK) return rc;
   const int stretches = a.group * D / kJoinDims;
   const dim3 grid((unsigned)pairs, (unsigned)(pairs * stretches <= kJoinGroups ? stretches : (pairs < kJoinGroups ? kJoinGroups / pairs : 1)));
@@ -557,15 +612,20 @@ int launch(const G4PagedDecodeArgs& a, hipStream_t st) {
   return check_launch("g4_paged_decode_attention");
 }
 
-template <int D, bool F8, bool SPLIT>
+template <int D, bool F8, int WAVES, bool SPLIT>
 void setup(int device) {
-  const size_t most = lds_bytes<D, SPLIT>(16);
-  if (most > 64 * 1024) raise_lds_limit(device, (const void*)paged_decode_kernel<D, F8, SPLIT>, (int)most);
+  const size_t most = lds_bytes<D, WAVES>(16);
+  if (most > 64 * 1024) raise_lds_limit(device, (const void*)paged_decode_kernel<D, F8, WAVES, SPLIT>, (int)most);
+}
+template <int D, bool F8>
+void setup(int device) {
+  if constexpr (F8 || D == 512) setup<D, F8, 8, false>(device);
+  if constexpr (D < 512) setup<D, F8, 4, false>(device);
+  setup<D, F8, split_waves(D), true>(device);
 }
 template <int D>
 void setup(int device) {
-  setup<D, false, false>(device), setup<D, false, true>(device);
-  setup<D, true, false>(device), setup<D, true, true>(device);
+  setup<D, false>(device), setup<D, true>(device);
 }
 
 }  // namespace
