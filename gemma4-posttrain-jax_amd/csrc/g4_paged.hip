@@ -558,7 +558,9 @@ extern "C" int g4_paged_append(const G4PagedAppendArgs* args, void* stream) {
   if ((int64_t)a.batch * a.seq > 0x7fffffffLL) return fail(G4_ERR_UNSUPPORTED, "%s: too many tokens", who);
   if (!a.k || !a.v || !a.write_pos) return fail(G4_ERR_INVALID, "%s: k / v / write_pos is NULL", who);
   if (a.q && (a.group <= 0 || !a.q_out)) return fail(G4_ERR_INVALID, "%s: q needs group > 0 and q_out", who);
-  if (a.in_row_stride < (int64_t)a.cache.kv_heads * a.cache.head_dim)
+  const int64_t heads = (int64_t)a.cache.kv_heads * (a.q ? a.group : 1);
+  if (heads > 0xffff) return fail(G4_ERR_UNSUPPORTED, "%s: %lld heads", who, (long long)heads);
+  if ((int64_t)a.batch * a.seq > 1 && a.in_row_stride < heads * a.cache.head_dim)
     return fail(G4_ERR_INVALID, "%s: in_row_stride %lld too small", who, (long long)a.in_row_stride);
   if ((a.flags & (G4_APPEND_ROPE_K | G4_APPEND_ROPE_Q)) && (!a.rope_cos || !a.rope_sin))
     return fail(G4_ERR_INVALID, "%s: RoPE flags need rope_cos / rope_sin", who);

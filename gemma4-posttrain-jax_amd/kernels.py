@@ -487,7 +487,7 @@ def paged_decode_attention(
     ref = ctypes.byref(a)
     need = _lib.lib().g4_paged_decode_workspace_size(ref)
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(need, dtype=torch.uint8)
         a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _lib.check(_lib.lib().g4_paged_decode_attention(ref, torch._C._cuda_getCurrentRawStream(dev)),
                "g4_paged_decode_attention")

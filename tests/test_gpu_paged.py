@@ -10,6 +10,7 @@ import torch
 
 import paged_util as P
 from gemma4_posttrain_jax_amd import kernels
+from gemma4_posttrain_jax_amd._lib import G4Error
 from gemma4_posttrain_jax_amd.kvcache import new_paged_layer
 
 pytestmark = pytest.mark.gpu
@@ -87,6 +88,39 @@ def test_append_moves_and_quantises_exactly(device, e4m3, D, H, ps, S, write_pos
     got_k, got_v = P.slots_of(layer)
     _same(got_k, want_k)
     _same(got_v, want_v)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("D,S", [(64, 1), (128, 9), (256, 17), (512, 3), (512, 8)])
+def test_append_of_rows_at_any_offset(device, e4m3, D, S):
+    """Rows, weights and table rows that start anywhere: an odd row stride, an odd first element, a table cut out of a
+    wider one; the same bits as aligned copies."""
+
+    H, R, B, ps = 3, 2, 2, 32
+    wide = _randn(2, B, S, (R + 2) * H * D + 5).to(device)[..., 1:-2]
+    wide = wide.as_strided((B, S, (R + 2) * H * D), wide.stride(), wide.storage_offset())
+    weights = _randn(3, 2 * D + 3).to(device)
+    angle = torch.rand((B, S, D), generator=torch.Generator().manual_seed(4)).to(device)
+    tables = torch.arange(2 * 8, dtype=torch.int32, device=device).view(2, 8)
+
+    def run(rows, qw, kw, table):
+        layer = new_paged_layer(16, H, D, ps, e4m3=e4m3, device=device)
+        q_out = torch.empty((B, S, H, R, D), dtype=BF16, device=device)
+        kernels.paged_append(layer, rows[..., H * R * D: H * (R + 1) * D].unflatten(-1, (H, D)),
+                             rows[..., H * (R + 1) * D: H * (R + 2) * D].unflatten(-1, (H, D)), page_table=table,
+                             write_pos=_i32([3, 30], device), flags=P.ALL_FLAGS,
+                             q=rows[..., : H * R * D].unflatten(-1, (H, R, D)), q_out=q_out, q_norm_weight=qw,
+                             k_norm_weight=kw, rope_cos=angle.cos(), rope_sin=angle.sin())
+        return [q_out] + [x.view(torch.uint8) for x in layer if x is not None]
+
+    got = run(wide, weights[1: D + 1], weights[D + 3:], tables[:, 2:5])
+    want = run(wide.contiguous(), weights[1: D + 1].clone(), weights[D + 3:].clone(), tables[:, 2:5].contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    n = _i32([3 + S, 30 + S], device)
+    layer = new_paged_layer(16, H, D, ps, e4m3=e4m3, device=device)
+    with pytest.raises(G4Error, match="aligned"):
+        q = torch.empty(B * H * R * D + 1, dtype=BF16, device=device)[1:].view(B, H, R, D)
+        kernels.paged_decode_attention(layer, q, page_table=tables[:, 2:5], lengths=n)
 
 
 def test_append_quantises_every_bf16_value(device):
@@ -219,7 +253,28 @@ def test_attention_many_rows(device, e4m3):
     _check(layer, table, lengths, _randn(9, len(lengths), 1, 5, 64, scale=0.25), 0, device)
 
 
-def test_attention_more_rows_than_one_launch(device):
+@pytest.mark.parametrize("e4m3,D,H,R,B,M,window", [
+    (True, 64, 1, 2, 700, 40, 0), (False, 64, 1, 1, 257, 64, 0), (True, 128, 3, 3, 300, 36, 1100),
+    (False, 256, 1, 4, 90, 50, 0), (True, 256, 2, 1, 40, 300, 0), (True, 512, 2, 2, 200, 34, 0),
+    (False, 512, 1, 16, 3, 200, 0), (True, 64, 2, 4, 1100, 33, 0),
+])
+def test_attention_of_cut_rows(device, e4m3, D, H, R, B, M, window):
+    """Tables so long that rows are cut into pieces: more rows than a wave looks at once, more (row, head)s than
+    workgroups are resident, long rows among empty and one-token ones. The tables' pages are drawn at random, so rows
+    share them."""
+
+    g = torch.Generator().manual_seed(B)
+    ps, pages = 32, 64
+    table = torch.randint(-1, pages, (B, M), generator=g).to(torch.int32)
+    lengths = torch.randint(0, 70, (B,), generator=g)
+    lengths[torch.randperm(B, generator=g)[: max(2, B // 40)]] = torch.randint(M * ps // 2, M * ps + 50, (max(2, B // 40),), generator=g)
+    lengths[0], lengths[B - 1] = 0, M * ps
+    layer = P.filled(pages, H, D, ps, e4m3, _randn(1, pages, H, ps, D), _randn(2, pages, H, ps, D), device)
+    got = _check(layer, table, lengths.tolist(), _randn(9, B, H, R, D, scale=2.0 / math.sqrt(D)), window, device)
+    assert (got[0] == 0).all()
+
+
+def test_attention_more_rows_than_fit_a_workgroup_row(device):
     lengths = [(7 * i) % 40 for i in range(4500)]
     layer, table = _cache(device, True, 1, 64, 32, lengths)
     _check(layer, table, lengths, _randn(9, len(lengths), 1, 1, 64, scale=0.25), 0, device)

@@ -247,6 +247,23 @@ def test_graphed_steps_equal_eager_ones(device, e4m3):
         assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
+def test_one_row_steps(device):
+    """A single sequence: one token's rows have no stride to follow."""
+
+    cfg = C.config_from_hf(CFG)
+    params = _params(cfg, device)
+    ids, mask = _prompts(cfg, [3], 20, device)
+    out = SMP.prefill(params, cfg, ids, mask, max_new_tokens=6, paged=PagedSpec(32, True))
+    step = SMP.GraphedDecodeStep(params, cfg, out.kv_cache)
+    eager = SMP.prefill(params, cfg, ids, mask, max_new_tokens=6, paged=PagedSpec(32, True)).kv_cache
+    for i in range(6):
+        tok, pos = torch.tensor([7 + i], dtype=torch.int32, device=device), torch.tensor([17 + i], dtype=torch.int32, device=device)
+        got = step.step(tok, pos, torch.ones(1, dtype=torch.bool, device=device)).clone()
+        ref = SMP.decode_step(params, cfg, tok, pos, eager)
+        eager = ref.kv_cache
+        assert torch.equal(got, ref.logits[:, -1].float())
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_captured_operators_replay_like_eager(device, e4m3):
     """Append, split attention (its workspace the graph's own) and read in one graph, replayed with new inputs and

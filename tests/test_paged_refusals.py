@@ -45,7 +45,7 @@ def _cache(**kw):
 def _append(cache=None, **kw):
     base = dict(cache=_cache(**(cache or {})), batch=2, seq=3, group=4, flags=0, eps=1e-6, keep=0, max_pages=4,
                 table_stride=4, page_table=1 << 12, write_pos=1 << 12, k=1 << 12, v=1 << 12, q=None,
-                in_row_stride=1024, q_norm_weight=None, k_norm_weight=None, rope_cos=None, rope_sin=None, q_out=None)
+                in_row_stride=2048, q_norm_weight=None, k_norm_weight=None, rope_cos=None, rope_sin=None, q_out=None)
     base.update(kw)
     return _lib.G4PagedAppendArgs(**base)
 
@@ -105,6 +105,8 @@ def test_abi_refuses_bad_tables(name, make, override, match):
     ("g4_paged_append", _append, dict(q=1 << 12, q_out=1 << 12, group=0), "group"),
     ("g4_paged_append", _append, dict(q=1 << 12, q_out=(1 << 12) + 4), "q_out"),
     ("g4_paged_append", _append, dict(in_row_stride=500), "in_row_stride"),
+    ("g4_paged_append", _append, dict(q=1 << 12, q_out=1 << 12, in_row_stride=2047), "in_row_stride"),
+    ("g4_paged_append", _append, dict(q=1 << 12, q_out=1 << 12, group=1 << 20, in_row_stride=1 << 40), "heads"),
     ("g4_paged_append", _append, dict(flags=_lib.G4_APPEND_ROPE_K), "RoPE"),
     ("g4_paged_append", _append, dict(flags=_lib.G4_APPEND_NORM_K), "k_norm_weight"),
     ("g4_paged_append", _append, dict(q=1 << 12, q_out=1 << 12, flags=_lib.G4_APPEND_NORM_Q), "q_norm_weight"),
