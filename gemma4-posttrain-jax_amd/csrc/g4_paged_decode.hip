@@ -305,13 +305,13 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room, int large)
     // every load below is issued by every wave, so that the waits for them can count: no branch but zero bytes
     Place at = place_of(c < last ? page : -1, c);
     load_keys(at, nt);
-    load_values(at, nt);
     wait_pages();
 #pragma unroll
     for (int j = 0; j < kQLoads; ++j)
       if (tid + j * kThreads < R * D / 8)
         *reinterpret_cast<u32x4*>(q_lds + (tid + j * kThreads) / (D / 8) * q_stride(D) + tid % (D / 8) * 8) = qv[j];
     __syncthreads();
+    load_values(at, nt);  // behind the barrier: a CU issues the loads of its waves one after the other, the keys' first
     // the columns beyond the R rows compute on the last row and are dropped
     const uint16_t* qrow = q_lds + (col < R ? col : R - 1) * q_stride(D) + half * DW + (F8 ? 16 : 8) * grp;
     // operand s: e4m3 keys come 16 consecutive dims a load, two operands
