@@ -531,10 +531,17 @@ size_t lds_bytes(int R) {
 }
 
 // Whether the rows are cut into pieces: where a row can have more chunks than one workgroup is as fast with. Finding
-// the pieces and joining them takes about 4 us; a workgroup takes 1 us for 100 keys of 256 dims in bf16, 130 in e4m3 (us
-// per call, whole / split: 2 pairs of 512 keys 8.7 / 9.7, of 1024 13.8 / 9.7, 16 pairs of 1024 15.6 / 11.8, but 64 pairs of
-// 1024 16.3 / 18.6, 128 pairs 28 / 32, 512 pairs 94 / 99, where the whole rows fill the chip).
-constexpr int kSplitPairs = 32, kWholeChunksFew = 20, kWholeChunks = 32;
+// the pieces and joining them takes about 4 us. us per call at 256 dims from twelve caches in turn, whole / split, bf16
+// and e4m3:
+//     pairs   512 keys               1024 keys               2048 keys
+//       2     9.7/9.2   7.8/8.9      15.2/9.4   11.4/8.9     26.2/10.7  17.8/9.5
+//      16     12.8/10.6 8.7/10.1     21.9/11.2  14.1/9.6     39.9/13.6  23.3/11.1
+//      64     14.5/13.4 10.2/11.1    23.6/19.5  15.4/14.7    45.0/29.5  26.1/19.5
+//     128     16.2/20.0 11.3/14.8    28.0/29.5  17.6/19.6    51.4/49.7  29.6/29.5
+//     512     43.7/47.3 24.7/28.1    84.0/87.5  45.0/48.0    164/168    85.6/88.8
+// Up to 64 pairs the border is set at 640 keys, where both formats come out even and a single call has one launch less;
+// beyond, at 1024, although equal rows stay faster whole: a long row among short ones would hold its one CU alone.
+constexpr int kSplitPairs = 64, kWholeChunksFew = 20, kWholeChunks = 32;
 bool split(const G4PagedDecodeArgs& a) {
   const int64_t cap = (int64_t)a.max_pages * a.cache.page_size;
   const int64_t keys = a.window > 0 && a.window < cap ? a.window + 31 : cap;  // a window may begin inside a chunk
