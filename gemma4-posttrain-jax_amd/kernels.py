@@ -327,59 +327,64 @@ def prefill_attention(
 # --- paged cache ------------------------------------------------------------------------------------------
 
 
+_BF16, _E4M3, _E8M0, _I32, _F32 = (torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.int32,
+                                   torch.float32)  # a module's name is the cheaper one to look up
+
+
 def _paged_cache(layer: PagedLayerCache) -> _lib.G4PagedCache:
     """The checked C view of a layer's pages."""
 
     key, value, key_scale, value_scale = layer
-    if value.dim() != 5 or value.shape[4] != 8:
-        raise ValueError(f"value pages: shape {tuple(value.shape)} is not [P, Hkv, page / 8, D, 8]")
-    P, H, groups, D, _ = value.shape
-    dtype = value.dtype
-    e4m3 = dtype == torch.float8_e4m3fn
-    if key.dtype != dtype or not (e4m3 or dtype == torch.bfloat16):
+    shape, dtype = value.shape, value.dtype
+    if len(shape) != 5 or shape[4] != 8:
+        raise ValueError(f"value pages: shape {tuple(shape)} is not [P, Hkv, page / 8, D, 8]")
+    P, H, groups, D, _ = shape
+    page = 8 * groups
+    e4m3 = dtype == _E4M3
+    if key.dtype != dtype or not (e4m3 or dtype == _BF16):
         raise TypeError(f"pages of {key.dtype} / {dtype}; they hold bfloat16 or float8_e4m3fn")
-    if key.shape != paged_key_shape(P, H, groups * 8, D, e4m3):
-        raise ValueError(f"key pages {tuple(key.shape)} do not match value pages {tuple(value.shape)}")
+    if key.shape != paged_key_shape(P, H, page, D, e4m3):
+        raise ValueError(f"key pages {tuple(key.shape)} do not match value pages {tuple(shape)}")
     if not (key.is_contiguous() and value.is_contiguous()):
         raise ValueError("pages must be contiguous")
-    if e4m3:
-        for t in (key_scale, value_scale):
-            if (t is None or t.dtype != torch.float8_e8m0fnu or t.shape != (P, H, groups * 8) or not t.is_contiguous()):
-                raise ValueError(f"e4m3 pages need contiguous float8_e8m0fnu scales of shape {(P, H, groups * 8)}")
-        return _lib.G4PagedCache(_lib.G4_PAGES_E4M3, P, H, D, groups * 8, key.data_ptr(), value.data_ptr(),
-                                 key_scale.data_ptr(), value_scale.data_ptr())
-    if key_scale is not None or value_scale is not None:
-        raise ValueError("bf16 pages have no scales")
-    return _lib.G4PagedCache(_lib.G4_PAGES_BF16, P, H, D, groups * 8, key.data_ptr(), value.data_ptr(), None, None)
+    if not e4m3:
+        if key_scale is not None or value_scale is not None:
+            raise ValueError("bf16 pages have no scales")
+        return _lib.G4PagedCache(0, P, H, D, page, key.data_ptr(), value.data_ptr(), None, None)
+    for t in (key_scale, value_scale):
+        if t is None or t.dtype != _E8M0 or t.shape != (P, H, page) or not t.is_contiguous():
+            raise ValueError(f"e4m3 pages need contiguous float8_e8m0fnu scales of shape {(P, H, page)}")
+    return _lib.G4PagedCache(1, P, H, D, page, key.data_ptr(), value.data_ptr(), key_scale.data_ptr(),
+                             value_scale.data_ptr())
 
 
-def _device_of(layer: PagedLayerCache, *tensors: torch.Tensor | None) -> int:
+def _device_of(tensors) -> int:
     """The index of the device that all operands are on, which has to be the current one: the call goes to its
     stream. (``get_device`` is -1 on the host.)"""
 
-    dev = layer.value.get_device()
+    dev = torch._C._cuda_getDevice() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"an operand is on {t.device}, where the cache's {tensors[0].device} has to be the current "
+                             f"device and hold them all")
     if dev < 0:
         raise ValueError("kernel operands must be device tensors")
-    for t in (*layer, *tensors):
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"an operand is on {t.device}, the cache on {layer.value.device}")
-    if dev != torch._C._cuda_getDevice():
-        raise ValueError(f"the cache is on {layer.value.device}, which is not the current device")
     return dev
 
 
 def _page_rows(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> tuple[int, int, int]:
     """(B, entries per row, stride) of a page table, ``rows`` being the int32 [B] tensor ``name``."""
 
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.numel() == 0:
+    shape = page_table.shape
+    if page_table.dtype != _I32 or len(shape) != 2 or 0 in shape:
         raise ValueError("page_table must be a non-empty int32 [B, M] tensor")
-    B, M = page_table.shape
+    B, M = shape
     stride, inner = page_table.stride()
     if B == 1:
         stride = M
     if (M > 1 and inner != 1) or stride < M:
         raise ValueError("page_table rows must be contiguous and apart")
-    if rows.dtype != torch.int32 or rows.shape != (B,) or not rows.is_contiguous():
+    if rows.dtype != _I32 or rows.shape != (B,) or not rows.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 [{B}] tensor")
     return B, M, stride
 
@@ -414,8 +419,7 @@ def paged_append(
         _check_rows(k, "k", B, S, H, D, rs)
     if v.stride() != strides or v.shape != k.shape:
         _check_rows(v, "v", B, S, H, D, rs)
-    bf16 = torch.bfloat16
-    if k.dtype != bf16 or v.dtype != bf16 or (q is not None and q.dtype != bf16):
+    if k.dtype != _BF16 or v.dtype != _BF16 or (q is not None and q.dtype != _BF16):
         raise TypeError("paged_append takes bfloat16 q / k / v")
     rows, M, table_stride = _page_rows(page_table, "write_pos", write_pos)
     if rows != B:
@@ -435,21 +439,27 @@ def paged_append(
             raise ValueError(f"q: strides {qs} of [Hkv, R, D] rows")
         if (S > 1 and qs[1] != rs) or (B > 1 and qs[0] != S * rs):
             raise ValueError("q must share k's row stride")
-        if q_out is None or q_out.dtype != bf16 or q_out.shape != q.shape or not q_out.is_contiguous():
+        if q_out is None or q_out.dtype != _BF16 or q_out.shape != q.shape or not q_out.is_contiguous():
             raise ValueError("q_out must be a contiguous bfloat16 [B, S, Hkv, R, D] tensor")
-    for name, t, on in (("q_norm_weight", q_norm_weight, q is not None and flags & _lib.G4_APPEND_NORM_Q),
-                        ("k_norm_weight", k_norm_weight, flags & _lib.G4_APPEND_NORM_K)):
-        if on and (t is None or t.dtype != bf16 or t.shape != (D,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous bfloat16 [{D}] tensor")
+        if flags & _lib.G4_APPEND_NORM_Q:
+            _norm_weight(q_norm_weight, "q_norm_weight", D)
+    if flags & _lib.G4_APPEND_NORM_K:
+        _norm_weight(k_norm_weight, "k_norm_weight", D)
     if flags & (_lib.G4_APPEND_ROPE_K | _lib.G4_APPEND_ROPE_Q):
         for t in (rope_cos, rope_sin):
-            if t is None or t.dtype != torch.float32 or t.shape != (B, S, D) or not t.is_contiguous():
+            if t is None or t.dtype != _F32 or t.shape != (B, S, D) or not t.is_contiguous():
                 raise ValueError("rope_cos/rope_sin must be contiguous float32 [B, S, D]")
-    dev = _device_of(layer, k, v, q, q_out, page_table, write_pos, q_norm_weight, k_norm_weight, rope_cos, rope_sin)
-    ptrs = [None if t is None else t.data_ptr() for t in (q, q_norm_weight, k_norm_weight, rope_cos, rope_sin, q_out)]
+    optional = (q, q_norm_weight, k_norm_weight, rope_cos, rope_sin, q_out)
+    dev = _device_of((*layer, k, v, page_table, write_pos, *optional))
+    q_p, qw_p, kw_p, cos_p, sin_p, out_p = [None if t is None else t.data_ptr() for t in optional]
     a = _lib.G4PagedAppendArgs(cache, B, S, R, flags, eps, keep, M, table_stride, page_table.data_ptr(),
-                               write_pos.data_ptr(), k.data_ptr(), v.data_ptr(), ptrs[0], rs, *ptrs[1:])
+                               write_pos.data_ptr(), k.data_ptr(), v.data_ptr(), q_p, rs, qw_p, kw_p, cos_p, sin_p, out_p)
     _lib.check(_lib.lib().g4_paged_append(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_append")
+
+
+def _norm_weight(t: torch.Tensor | None, name: str, D: int) -> None:
+    if t is None or t.dtype != _BF16 or t.shape != (D,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous bfloat16 [{D}] tensor")
 
 
 def paged_decode_attention(
@@ -467,7 +477,7 @@ def paged_decode_attention(
     allocator."""
 
     B, H, R, D = q.shape
-    if q.dtype != torch.bfloat16 or not q.is_contiguous():
+    if q.dtype != _BF16 or not q.is_contiguous():
         raise ValueError("q must be a contiguous bfloat16 [B, Hkv, R, D] tensor")
     rows, M, table_stride = _page_rows(page_table, "lengths", lengths)
     if rows != B:
@@ -479,7 +489,7 @@ def paged_decode_attention(
         raise ValueError(f"window must not be negative, got {window}")
     if out is not None and (out.shape != q.shape or not out.is_contiguous() or out.dtype != q.dtype):
         raise ValueError("out must be a contiguous [B, Hkv, R, D] tensor in q's dtype")
-    dev = _device_of(layer, q, page_table, lengths, out)
+    dev = _device_of((*layer, q, page_table, lengths, out))
     if out is None:
         out = torch.empty_like(q)
     a = _lib.G4PagedDecodeArgs(cache, B, R, window, M, table_stride, page_table.data_ptr(), lengths.data_ptr(),
@@ -503,8 +513,8 @@ def paged_read(layer: PagedLayerCache, *, page_table: torch.Tensor, lengths: tor
     if start < 0 or count <= 0:
         raise ValueError(f"start {start} must not be negative and count {count} must be positive")
     cache = _paged_cache(layer)
-    dev = _device_of(layer, page_table, lengths)
-    k = torch.empty((B, count, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=layer.value.device)
+    dev = _device_of((*layer, page_table, lengths))
+    k = torch.empty((B, count, cache.kv_heads, cache.head_dim), dtype=_BF16, device=layer.value.device)
     v = torch.empty_like(k)
     a = _lib.G4PagedReadArgs(cache, B, start, count, M, table_stride, page_table.data_ptr(), lengths.data_ptr(),
                              k.data_ptr(), v.data_ptr())
