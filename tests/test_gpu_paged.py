@@ -349,6 +349,31 @@ def test_attention_of_infinite_scores(device):
     assert got[2].isnan().all() and got[3].isnan().all()
 
 
+@pytest.mark.parametrize("D", [64, 512])
+def test_e4m3_pages_of_infinities_and_nan(device, D):
+    """An element that is no number is NaN in e4m3 and takes nothing from its neighbours: a key's makes the row's
+    result NaN where it is attended, a value's its own dim only; reading gives NaN for the element alone."""
+
+    ps, n = 32, 9
+    k, v = _randn(1, 3, n, 1, D), _randn(2, 3, n, 1, D)
+    k[0, 3, 0, 5] = math.inf
+    v[1, 2, 0, 7], v[1, 4, 0, 60] = -math.inf, math.nan
+    layer = new_paged_layer(3, 1, D, ps, e4m3=True, device=device)
+    table = _i32([[0], [1], [2]], device)
+    kernels.paged_append(layer, k.to(device), v.to(device), page_table=table, write_pos=_i32([0, 0, 0], device))
+    q = _randn(3, 3, 1, 2, D, scale=0.1).to(device)
+    call = lambda lengths: kernels.paged_decode_attention(layer, q, page_table=table, lengths=_i32(lengths, device)).cpu()  # noqa: E731
+    out = call([n, n, n])
+    assert out[0].isnan().all() and out[2].isfinite().all()
+    bad = torch.zeros(D, dtype=torch.bool)
+    bad[[7, 60]] = True
+    assert out[1][..., bad].isnan().all() and out[1][..., ~bad].isfinite().all()
+    assert call([3, 2, n])[:2].isfinite().all()  # none of them attended
+    rk, rv = kernels.paged_read(layer, page_table=table, lengths=_i32([n] * 3, device), start=0, count=n)
+    for got, x in ((rk, k), (rv, v)):
+        _same(got, P.dequantised(x))
+
+
 def test_attention_beyond_32_bit_offsets(device):
     """Pages whose places in the pool pass 2^32 bytes and elements."""
 
