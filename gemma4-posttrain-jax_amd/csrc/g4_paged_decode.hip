@@ -274,9 +274,11 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room, int large)
   const int entry = (c < last ? c : (last > 0 ? last - 1 : 0)) >> page_shift;
   const int page = __builtin_amdgcn_readfirstlane(table[entry]);
   // Keys and values that this call reads once pass the caches by (non-temporal loads), unless a row beside this one
-  // has the same page here, or the call is so small that its latency counts (kStreamBytes).
-  const int before = table[entry - (b > 0 ? a.table_stride : 0)], after = table[entry + (b + 1 < a.batch ? a.table_stride : 0)];
-  const bool stream = large && !(b > 0 && before == page) && !(b + 1 < a.batch && after == page);
+  // has the same page where this piece begins, or the call is so small that its latency counts (kStreamBytes). One
+  // answer for the workgroup, whose waves meet at barriers in what follows.
+  const int32_t* mine = table + (c_first >> page_shift);
+  const int own = mine[0], above = mine[b > 0 ? -a.table_stride : 0], below = mine[b + 1 < a.batch ? a.table_stride : 0];
+  const bool stream = large && !(b > 0 && above == own) && !(b + 1 < a.batch && below == own);
   auto load_keys = [&](const Place& at, auto nt) {
     const __amdgpu_buffer_rsrc_t r =
         make_rsrc(reinterpret_cast<const uint8_t*>(a.cache.key) + at.slot * (D * Sh::BYTES), at.there ? kChunkBytes : 0);

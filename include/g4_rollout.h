@@ -48,11 +48,11 @@ enum {
 };
 
 /*
- * One-time set-up of the current HIP device: raises the dynamic-LDS limit of the decode and
- * prefill kernels that launch with more than the 64 KiB default (hipFuncSetAttribute). The first
+ * One-time set-up of the current HIP device: raises the dynamic-LDS limit of the decode, prefill
+ * and paged attention kernels that launch with more than the 64 KiB default (hipFuncSetAttribute). The first
  * call on a device does the work (std::call_once: concurrent first calls wait for it), later calls
- * return its recorded result. g4_decode_attention and g4_prefill_attention call it themselves
- * before their first launch on a device; a caller that captures those calls into a HIP graph calls
+ * return its recorded result. g4_decode_attention, g4_prefill_attention and
+ * g4_paged_decode_attention call it themselves before their first launch on a device that needs it; a caller that captures those calls into a HIP graph calls
  * g4_init once per device beforehand, so that no set-up call falls inside the capture. No
  * reference counterpart: XLA sets kernel attributes when it compiles the module.
  */
@@ -322,8 +322,10 @@ int g4_paged_append(const G4PagedAppendArgs* args, void* stream);
  * whose scores are all -inf, gives zeros. What the other slots hold, NaN included, does not matter.
  * f32 scores, softmax and sums; the unnormalised probabilities (times the value's scale) are rounded
  * to bf16 as the operand of the value product, the result once to bf16. The same call gives the
- * same bits. Needs g4_paged_decode_workspace_size() bytes of scratch (16-byte aligned; no state is
- * kept in it, so calls ordered on one stream may share it).
+ * same bits. Rows of more than 640 or 1024 positions (by the number of (row, head) pairs) are cut into
+ * pieces that a second launch joins: those calls need g4_paged_decode_workspace_size() bytes of scratch
+ * (16-byte aligned; no state is kept in it, so calls ordered on one stream may share it; calls at the
+ * same time may not). At most 2^27 positions per row, 2^35 over all (row, head) pairs of a call.
  */
 typedef struct G4PagedDecodeArgs {
   G4PagedCache cache;
