@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .kvcache import LayerKVCache, PagedLayerCache, key_shape, paged_key_shape
+from .kvcache import LayerKVCache, PagedLayerCache, key_shape
 
 _DTYPES = {torch.float32: _lib.G4_DTYPE_F32, torch.bfloat16: _lib.G4_DTYPE_BF16}
 
@@ -340,21 +340,24 @@ def _paged_cache(layer: PagedLayerCache) -> _lib.G4PagedCache:
         raise ValueError(f"value pages: shape {tuple(shape)} is not [P, Hkv, page / 8, D, 8]")
     P, H, groups, D, _ = shape
     page = 8 * groups
-    e4m3 = dtype == _E4M3
-    if key.dtype != dtype or not (e4m3 or dtype == _BF16):
+    e4m3 = dtype is _E4M3
+    if key.dtype is not dtype or not (e4m3 or dtype is _BF16):
         raise TypeError(f"pages of {key.dtype} / {dtype}; they hold bfloat16 or float8_e4m3fn")
-    if key.shape != paged_key_shape(P, H, page, D, e4m3):
+    run = 64 if e4m3 else 32
+    if key.shape != (P, H, groups // 4, D // run, 2, 16, run):  # paged_key_shape
         raise ValueError(f"key pages {tuple(key.shape)} do not match value pages {tuple(shape)}")
     if not (key.is_contiguous() and value.is_contiguous()):
         raise ValueError("pages must be contiguous")
     if not e4m3:
         if key_scale is not None or value_scale is not None:
             raise ValueError("bf16 pages have no scales")
-        return _lib.G4PagedCache(0, P, H, D, page, key.data_ptr(), value.data_ptr(), None, None)
-    for t in (key_scale, value_scale):
-        if t is None or t.dtype != _E8M0 or t.shape != (P, H, page) or not t.is_contiguous():
-            raise ValueError(f"e4m3 pages need contiguous float8_e8m0fnu scales of shape {(P, H, page)}")
-    return _lib.G4PagedCache(1, P, H, D, page, key.data_ptr(), value.data_ptr(), key_scale.data_ptr(),
+        return _lib.G4PagedCache(_lib.G4_PAGES_BF16, P, H, D, page, key.data_ptr(), value.data_ptr())
+    scales = (P, H, page)
+    if (key_scale is None or value_scale is None or key_scale.dtype is not _E8M0 or value_scale.dtype is not _E8M0
+            or key_scale.shape != scales or value_scale.shape != scales
+            or not (key_scale.is_contiguous() and value_scale.is_contiguous())):
+        raise ValueError(f"e4m3 pages need contiguous float8_e8m0fnu scales of shape {scales}")
+    return _lib.G4PagedCache(_lib.G4_PAGES_E4M3, P, H, D, page, key.data_ptr(), value.data_ptr(), key_scale.data_ptr(),
                              value_scale.data_ptr())
 
 
@@ -376,7 +379,7 @@ def _page_rows(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> tuple
     """(B, entries per row, stride) of a page table, ``rows`` being the int32 [B] tensor ``name``."""
 
     shape = page_table.shape
-    if page_table.dtype != _I32 or len(shape) != 2 or 0 in shape:
+    if page_table.dtype is not _I32 or len(shape) != 2 or 0 in shape:
         raise ValueError("page_table must be a non-empty int32 [B, M] tensor")
     B, M = shape
     stride, inner = page_table.stride()
@@ -384,7 +387,7 @@ def _page_rows(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> tuple
         stride = M
     if (M > 1 and inner != 1) or stride < M:
         raise ValueError("page_table rows must be contiguous and apart")
-    if rows.dtype != _I32 or rows.shape != (B,) or not rows.is_contiguous():
+    if rows.dtype is not _I32 or rows.shape != (B,) or not rows.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 [{B}] tensor")
     return B, M, stride
 
@@ -412,14 +415,14 @@ def paged_append(
     starts at minus its pad count), beyond the table or without a page, and with ``keep`` > 0 all but the last
     ``keep`` tokens. q / k / v are prepared by ``flags`` in f32 and rounded once, where they are stored."""
 
-    B, S, H, D = k.shape
-    strides = k.stride()
+    shape, strides = k.shape, k.stride()
+    B, S, H, D = shape
     rs = strides[1] if S > 1 else (strides[0] if B > 1 else H * D)
-    if strides != (S * rs, rs, D, 1):
+    if strides != (S * rs, rs, D, 1):  # or of dims that have one element only
         _check_rows(k, "k", B, S, H, D, rs)
-    if v.stride() != strides or v.shape != k.shape:
+    if v.stride() != strides or v.shape != shape:
         _check_rows(v, "v", B, S, H, D, rs)
-    if k.dtype != _BF16 or v.dtype != _BF16 or (q is not None and q.dtype != _BF16):
+    if k.dtype is not _BF16 or v.dtype is not _BF16 or (q is not None and q.dtype is not _BF16):
         raise TypeError("paged_append takes bfloat16 q / k / v")
     rows, M, table_stride = _page_rows(page_table, "write_pos", write_pos)
     if rows != B:
@@ -431,15 +434,16 @@ def paged_append(
         raise ValueError(f"keep must not be negative, got {keep}")
     R = 0
     if q is not None:
-        R = q.shape[3] if q.dim() == 5 else 0
-        if q.shape != (B, S, H, R, D):
-            raise ValueError(f"q: shape {tuple(q.shape)} is not [{B}, {S}, {H}, R, {D}]")
-        qs = q.stride()
-        if qs[4] != 1 or (R > 1 and qs[3] != D) or (H > 1 and qs[2] != R * D):
-            raise ValueError(f"q: strides {qs} of [Hkv, R, D] rows")
-        if (S > 1 and qs[1] != rs) or (B > 1 and qs[0] != S * rs):
-            raise ValueError("q must share k's row stride")
-        if q_out is None or q_out.dtype != _BF16 or q_out.shape != q.shape or not q_out.is_contiguous():
+        q_shape, qs = q.shape, q.stride()
+        if len(q_shape) != 5 or q_shape[:3] != shape[:3] or q_shape[4] != D:
+            raise ValueError(f"q: shape {tuple(q_shape)} is not [{B}, {S}, {H}, R, {D}]")
+        R = q_shape[3]
+        if qs != (S * rs, rs, R * D, D, 1):
+            if qs[4] != 1 or (R > 1 and qs[3] != D) or (H > 1 and qs[2] != R * D):
+                raise ValueError(f"q: strides {qs} of [Hkv, R, D] rows")
+            if (S > 1 and qs[1] != rs) or (B > 1 and qs[0] != S * rs):
+                raise ValueError("q must share k's row stride")
+        if q_out is None or q_out.dtype is not _BF16 or q_out.shape != q_shape or not q_out.is_contiguous():
             raise ValueError("q_out must be a contiguous bfloat16 [B, S, Hkv, R, D] tensor")
         if flags & _lib.G4_APPEND_NORM_Q:
             _norm_weight(q_norm_weight, "q_norm_weight", D)
@@ -447,7 +451,7 @@ def paged_append(
         _norm_weight(k_norm_weight, "k_norm_weight", D)
     if flags & (_lib.G4_APPEND_ROPE_K | _lib.G4_APPEND_ROPE_Q):
         for t in (rope_cos, rope_sin):
-            if t is None or t.dtype != _F32 or t.shape != (B, S, D) or not t.is_contiguous():
+            if t is None or t.dtype is not _F32 or t.shape != (B, S, D) or not t.is_contiguous():
                 raise ValueError("rope_cos/rope_sin must be contiguous float32 [B, S, D]")
     optional = (q, q_norm_weight, k_norm_weight, rope_cos, rope_sin, q_out)
     dev = _device_of((*layer, k, v, page_table, write_pos, *optional))
@@ -458,7 +462,7 @@ def paged_append(
 
 
 def _norm_weight(t: torch.Tensor | None, name: str, D: int) -> None:
-    if t is None or t.dtype != _BF16 or t.shape != (D,) or not t.is_contiguous():
+    if t is None or t.dtype is not _BF16 or t.shape != (D,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous bfloat16 [{D}] tensor")
 
 
@@ -477,7 +481,7 @@ def paged_decode_attention(
     allocator."""
 
     B, H, R, D = q.shape
-    if q.dtype != _BF16 or not q.is_contiguous():
+    if q.dtype is not _BF16 or not q.is_contiguous():
         raise ValueError("q must be a contiguous bfloat16 [B, Hkv, R, D] tensor")
     rows, M, table_stride = _page_rows(page_table, "lengths", lengths)
     if rows != B:
@@ -514,8 +518,8 @@ def paged_read(layer: PagedLayerCache, *, page_table: torch.Tensor, lengths: tor
         raise ValueError(f"start {start} must not be negative and count {count} must be positive")
     cache = _paged_cache(layer)
     dev = _device_of((*layer, page_table, lengths))
-    k = torch.empty((B, count, cache.kv_heads, cache.head_dim), dtype=_BF16, device=layer.value.device)
-    v = torch.empty_like(k)
+    shape = (B, count, cache.kv_heads, cache.head_dim)
+    k, v = layer.value.new_empty(shape, dtype=_BF16), layer.value.new_empty(shape, dtype=_BF16)
     a = _lib.G4PagedReadArgs(cache, B, start, count, M, table_stride, page_table.data_ptr(), lengths.data_ptr(),
                              k.data_ptr(), v.data_ptr())
     _lib.check(_lib.lib().g4_paged_read(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_read")
