@@ -274,6 +274,79 @@ def test_attention_of_cut_rows(device, e4m3, D, H, R, B, M, window):
     assert (got[0] == 0).all()
 
 
+SHARED = [  # D, H, R, page, rows, common pages, pages of a row, window
+    (256, 2, 4, 64, 8, 12, 16, 0),
+    (256, 1, 4, 32, 7, 25, 40, 0),
+    (256, 2, 2, 128, 9, 6, 7, 500),
+    (128, 2, 1, 32, 19, 30, 41, 0),
+    (128, 1, 3, 64, 5, 40, 40, 0),  # all pages
+    (64, 3, 8, 32, 4, 21, 90, 0),
+    (64, 1, 5, 1024, 6, 2, 4, 1100),
+    (64, 2, 4, 32, 130, 20, 25, 0),  # more rows than a wave looks at once
+    (512, 1, 4, 64, 4, 12, 20, 0),
+    (128, 1, 16, 64, 4, 12, 20, 0),
+]
+
+
+def _shared_table(D, B, common, M):
+    """Rows that begin with the same pages and go on with pages of their own; one page of the pool is in no row."""
+
+    pages = common + B * (M - common) + 1
+    table = torch.empty(B, M, dtype=torch.int32)
+    g = torch.Generator().manual_seed(D)
+    ids = torch.randperm(pages, generator=g).to(torch.int32)
+    for b in range(B):
+        table[b, :common] = ids[:common]
+        table[b, common:] = ids[common + b * (M - common): common + (b + 1) * (M - common)]
+    return table, pages, ids
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("spoil", ["none", "page", "hole", "first", "short", "empty"])
+@pytest.mark.parametrize("D,H,R,ps,B,common,M,window", SHARED)
+def test_attention_of_rows_that_share_pages(device, e4m3, spoil, D, H, R, ps, B, common, M, window):
+    """Rows with the same pages at their beginning and ragged ends; then with one row of them that has another page or
+    none in the middle of it or at its start, ends in it, or is empty."""
+
+    table, pages, ids = _shared_table(D, B, common, M)
+    lengths = [common * ps + (37 * b * b + 5 * b) % ((M - common) * ps + 1) - (b % 3 == 2) * (ps // 2) for b in range(B)]
+    odd = 2 if B > 2 else 1
+    if spoil == "page":
+        table[odd, common // 2] = ids[-1]
+    elif spoil == "hole":
+        table[odd, common // 2] = -1
+        table[0, common - 1] = 2 ** 31 - 1
+    elif spoil == "first":
+        table[odd, 0] = ids[-1]
+        table[B - 1, common - 1] = -5
+    elif spoil == "short":
+        lengths[odd] = common // 2 * ps + 7
+    elif spoil == "empty":
+        lengths[odd] = 0
+    layer = P.filled(pages, H, D, ps, e4m3, _randn(1, pages, H, ps, D), _randn(2, pages, H, ps, D), device)
+    _check(layer, table, lengths, _randn(9, B, H, R, D, scale=2.0 / math.sqrt(D)), window, device)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_nan_of_one_row_stays_there(device, e4m3):
+    """Rows that share pages: a NaN in one row's own page, or in its query, reaches no other row."""
+
+    D, ps, B, common, M = 128, 64, 4, 12, 14
+    table, pages, _ = _shared_table(D, B, common, M)
+    lengths = [common * ps + 70, common * ps + 3, common * ps, common * ps + 128]
+    k, v, q = _randn(1, pages, 1, ps, D), _randn(2, pages, 1, ps, D), _randn(9, B, 1, 4, D, scale=0.2)
+    layer = P.filled(pages, 1, D, ps, e4m3, k, v, device)
+    want = _check(layer, table, lengths, q, 0, device)
+    k[int(table[1, common]), 0, 1, 5] = math.nan
+    v[int(table[3, common]), 0, 9, 5] = math.nan
+    q[2, 0, 1, 3] = math.nan
+    layer = P.filled(pages, 1, D, ps, e4m3, k, v, device)
+    got = kernels.paged_decode_attention(layer, q.to(device), page_table=table.to(device), lengths=_i32(lengths, device))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2, 0, [0, 2, 3]], want[2, 0, [0, 2, 3]])
+    assert got[1].isnan().all() and got[2, 0, 1].isnan().all() and got[3, :, :, 5].isnan().all()
+    assert torch.equal(got[3, :, :, 6:], want[3, :, :, 6:]) or e4m3  # an e4m3 vector's NaN may change its scale
+
+
 def test_attention_more_rows_than_fit_a_workgroup_row(device):
     lengths = [(7 * i) % 40 for i in range(4500)]
     layer, table = _cache(device, True, 1, 64, 32, lengths)
