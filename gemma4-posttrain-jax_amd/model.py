@@ -453,10 +453,16 @@ def forward_gemma4_text(
                       and params.embed_tokens.shape[1] % 8 == 0)
     if fused_prologue:
         tabs = (SLIDING, FULL)
+        if paged:
+            # a paged cache has no key mask: rows of one column (whatever view the mask is of), which get what they hold
+            # where the slot is 0 and nothing elsewhere
+            own_mask = attention_mask.contiguous()
+            slot, key_mask = position_ids[:, 0], own_mask.as_strided((B, 1), (1, 1))
+        else:
+            slot, key_mask = write_pos, kv_cache.key_mask
         x, tables = kernels.decode_prologue(
-            params.embed_tokens, input_ids[:, 0], position_ids[:, 0], attention_mask[:, 0],
-            # a paged cache has no key mask: the step's own mask gets the values that it holds
-            position_ids[:, 0] if paged else write_pos, attention_mask if paged else kv_cache.key_mask, embed_scale=pw.embed_scale_f, inv_freq=[pw.inv_freq[t] for t in tabs])
+            params.embed_tokens, input_ids[:, 0], position_ids[:, 0], attention_mask[:, 0], slot, key_mask,
+            embed_scale=pw.embed_scale_f, inv_freq=[pw.inv_freq[t] for t in tabs])
         x = x.view(B, 1, -1)
         rot = {t: (c.view(B, 1, -1), sn.view(B, 1, -1)) for t, (c, sn) in zip(tabs, tables)}
         pli = None

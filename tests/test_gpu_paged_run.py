@@ -405,3 +405,25 @@ def test_paged_model_refusals(device):
     with pytest.raises(ValueError, match="bfloat16 model"):
         M.forward_gemma4_text(f32, ids, ids, config=cfg, attention_mask=mask,
                               kv_cache=init_paged_kv_cache(cfg, 2, 20, PagedSpec(), device))
+
+
+@pytest.mark.parametrize("B", [1, 3])
+def test_a_step_leaves_the_callers_mask(device, B):
+    """A step without host-side values whose mask is a column of a wider tensor: that tensor stays, and the result
+    is that of a mask of its own."""
+
+    cfg = C.config_from_hf(CFG)
+    params = _params(cfg, device)
+    ids, mask = _prompts(cfg, [3, 0, 9][:B], 20, device)
+    tok = torch.tensor([5, 6, 7][:B], dtype=torch.int32, device=device)[:, None]
+    pos = mask.sum(-1, keepdim=True).to(torch.int32)
+    wide = torch.zeros((B + 1, 64), dtype=torch.bool, device=device)  # a row behind the last
+    wide[:B, 40] = torch.tensor([True, False, True][:B], device=device)
+    before = wide.clone()
+    outs = []
+    for m in (wide[:B, 40:41], wide[:B, 40:41].clone(memory_format=torch.contiguous_format)):
+        cache = SMP.prefill(params, cfg, ids, mask, max_new_tokens=4, paged=PagedSpec(32)).kv_cache
+        outs.append(M.forward_gemma4_lm(params, tok, pos, config=cfg, attention_mask=m, kv_cache=cache, cache_mode="append",
+                                      write_pos=pos[:, 0].clone()).logits)
+        assert torch.equal(wide, before)
+    assert torch.equal(*outs)
