@@ -39,6 +39,7 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t w, uint32_t& lo, uint32_t& 
 }
 
 // Host-side checks of one layer's pages and table; G4_OK or the error (text under `who`).
+constexpr int64_t kMaxThreads = 0xffffffff;  // of a grid's dimension
 int check_paged_cache(const G4PagedCache& c, const char* who);
 int check_page_table(const int32_t* table, int32_t max_pages, int64_t table_stride, int32_t page_size, const char* who);
 

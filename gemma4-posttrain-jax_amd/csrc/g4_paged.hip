@@ -426,28 +426,30 @@ paged_append_tile_kernel(G4PagedAppendArgs a, int vec, int groups) {
 }
 
 template <int D, bool F8>
-void launch_append(const G4PagedAppendArgs& a, bool vec, hipStream_t st) {
+int launch_append(const G4PagedAppendArgs& a, bool vec, hipStream_t st) {
   const int H = a.cache.kv_heads;
-  // 8 consecutive positions from any start on lie in ceil((seq + 7) / 8) groups at most
-  const int64_t groups = ((int64_t)a.seq + 2 * kTileTok - 2) / kTileTok;
-  if (a.seq >= kTileTok && a.batch * groups <= 0x7fffffffLL) {
+  if (a.seq >= kTileTok) {
+    // 8 consecutive positions from any start on lie in ceil((seq + 7) / 8) groups at most
+    const int64_t groups = ((int64_t)a.seq + 2 * kTileTok - 2) / kTileTok;
+    if (a.batch * groups * kTileThreads > kMaxThreads)
+      return fail(G4_ERR_UNSUPPORTED, "g4_paged_append: too many tokens (%d rows of %d)", a.batch, a.seq);
     constexpr int kHeads = kTileValueBytes / (kTileTok * D * (F8 ? 1 : 2));
     const size_t lds = (size_t)(H < kHeads ? H : kHeads) * kTileTok * D * (F8 ? 1 : 2);
     hipLaunchKernelGGL((paged_append_tile_kernel<D, F8>), dim3((unsigned)(a.batch * groups)), dim3(kTileThreads), lds, st, a,
                        (int)vec, (int)groups);
-    return;
+  } else {
+    constexpr int VECS = Lanes<D>::VECS;
+    const int nvec = ((a.q ? H * a.group : 0) + VECS - 1) / VECS + 2 * ((H + VECS - 1) / VECS);
+    const int64_t tokens = (int64_t)a.batch * a.seq, threads = 64 * (nvec > 16 ? 16 : nvec);
+    if (tokens * threads > kMaxThreads)
+      return fail(G4_ERR_UNSUPPORTED, "g4_paged_append: too many tokens (%d rows of %d)", a.batch, a.seq);
+    hipLaunchKernelGGL((paged_append_kernel<D, F8>), dim3((unsigned)tokens), dim3((unsigned)threads), 0, st, a, (int)vec);
   }
-  constexpr int VECS = Lanes<D>::VECS;
-  const int nvec = ((a.q ? H * a.group : 0) + VECS - 1) / VECS + 2 * ((H + VECS - 1) / VECS);
-  hipLaunchKernelGGL((paged_append_kernel<D, F8>), dim3((unsigned)((int64_t)a.batch * a.seq)),
-                     dim3((unsigned)(64 * (nvec > 16 ? 16 : nvec))), 0, st, a, (int)vec);
+  return check_launch("g4_paged_append");
 }
 template <int D>
-void launch_append(const G4PagedAppendArgs& a, bool vec, hipStream_t st) {
-  if (a.cache.format == G4_PAGES_E4M3)
-    launch_append<D, true>(a, vec, st);
-  else
-    launch_append<D, false>(a, vec, st);
+int launch_append(const G4PagedAppendArgs& a, bool vec, hipStream_t st) {
+  return a.cache.format == G4_PAGES_E4M3 ? launch_append<D, true>(a, vec, st) : launch_append<D, false>(a, vec, st);
 }
 
 // --- read back ---------------------------------------------------------------------------------------------
@@ -579,12 +581,11 @@ extern "C" int g4_paged_append(const G4PagedAppendArgs* args, void* stream) {
   if (reinterpret_cast<uintptr_t>(a.q_out) % al) return fail(G4_ERR_INVALID, "%s: q_out must be %d-byte aligned", who, (int)al);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (a.cache.head_dim) {
-    case 64: launch_append<64>(a, vec, st); break;
-    case 128: launch_append<128>(a, vec, st); break;
-    case 256: launch_append<256>(a, vec, st); break;
-    default: launch_append<512>(a, vec, st); break;
+    case 64: return launch_append<64>(a, vec, st);
+    case 128: return launch_append<128>(a, vec, st);
+    case 256: return launch_append<256>(a, vec, st);
+    default: return launch_append<512>(a, vec, st);
   }
-  return check_launch(who);
 }
 
 extern "C" int g4_paged_read(const G4PagedReadArgs* args, void* stream) {
@@ -601,7 +602,7 @@ extern "C" int g4_paged_read(const G4PagedReadArgs* args, void* stream) {
   if (reinterpret_cast<uintptr_t>(a.k_out) % 16 || reinterpret_cast<uintptr_t>(a.v_out) % 16)
     return fail(G4_ERR_INVALID, "%s: k_out / v_out must be 16-byte aligned", who);
   const int first = a.start / 32, n = (a.start + a.count - 1) / 32 - first + 1;
-  if ((int64_t)a.batch * a.cache.kv_heads * n > 0x7fffffffLL) return fail(G4_ERR_UNSUPPORTED, "%s: too many positions", who);
+  if ((int64_t)a.batch * a.cache.kv_heads * n > kMaxThreads / kReadThreads) return fail(G4_ERR_UNSUPPORTED, "%s: too many positions", who);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (a.cache.head_dim) {
     case 64: launch_read<64>(a, first, n, st); break;

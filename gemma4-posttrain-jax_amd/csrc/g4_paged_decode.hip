@@ -650,13 +650,17 @@ int setup_paged_kernels(int device) {
 
 namespace {
 
+// A grid of as many workgroups of up to 512 threads, the pieces' and XCDs' spare ones included, has its threads counted
+// in 32 bits.
+constexpr int64_t kMaxPairs = kMaxThreads / 512 - resident(64) - kSpare - kXcds;
+
 int check_decode(const G4PagedDecodeArgs& a, const char* who) {
   int rc = check_paged_cache(a.cache, who);
   if (rc == G4_OK) rc = check_page_table(a.page_table, a.max_pages, a.table_stride, a.cache.page_size, who);
   if (rc != G4_OK) return rc;
   if (a.batch <= 0 || a.group <= 0 || a.group > 16 || a.window < 0)
     return fail(G4_ERR_INVALID, "%s: batch %d group %d (1..16) window %d", who, a.batch, a.group, a.window);
-  if ((int64_t)a.batch * a.cache.kv_heads > 0x7fffffLL)
+  if ((int64_t)a.batch * a.cache.kv_heads > kMaxPairs)
     return fail(G4_ERR_UNSUPPORTED, "%s: batch %d x %d kv heads", who, a.batch, a.cache.kv_heads);
   if ((int64_t)a.max_pages * a.cache.page_size > 1 << 27)
     return fail(G4_ERR_UNSUPPORTED, "%s: %d pages of %d positions pass 2^27 positions", who, a.max_pages, a.cache.page_size);

@@ -272,5 +272,6 @@ def init_kv_cache(config: Gemma4TextConfig, batch_size: int, capacity: int, dtyp
     return KVCache(tuple(layers), key_mask, 0)
 
 
-__all__ = ["LayerKVCache", "KVCache", "PagedLayerCache", "PagedKVCache", "PagedSpec", "PAGE_SIZES", "new_paged_layer", "paged_key_shape", "init_kv_cache", "init_paged_kv_cache", "new_layer_cache", "slot_stride_for", "key_shape", "group_keys",
-           "ungroup_keys", "group_values", "ungroup_values", "FULL", "SLIDING"]
+__all__ = ["LayerKVCache", "KVCache", "PagedLayerCache", "PagedKVCache", "PagedSpec", "PAGE_SIZES", "new_paged_layer",
+           "paged_key_shape", "init_kv_cache", "init_paged_kv_cache", "new_layer_cache", "slot_stride_for", "key_shape",
+           "group_keys", "ungroup_keys", "group_values", "ungroup_values", "FULL", "SLIDING"]

@@ -49,12 +49,13 @@ enum {
 
 /*
  * One-time set-up of the current HIP device: raises the dynamic-LDS limit of the decode, prefill
- * and paged attention kernels that launch with more than the 64 KiB default (hipFuncSetAttribute). The first
- * call on a device does the work (std::call_once: concurrent first calls wait for it), later calls
- * return its recorded result. g4_decode_attention, g4_prefill_attention and
- * g4_paged_decode_attention call it themselves before their first launch on a device that needs it; a caller that captures those calls into a HIP graph calls
- * g4_init once per device beforehand, so that no set-up call falls inside the capture. No
- * reference counterpart: XLA sets kernel attributes when it compiles the module.
+ * and paged attention kernels that launch with more than the 64 KiB default (hipFuncSetAttribute).
+ * The first call on a device does the work (std::call_once: concurrent first calls wait for it),
+ * later calls return its recorded result. g4_decode_attention, g4_prefill_attention and
+ * g4_paged_decode_attention call it themselves before their first launch on a device that needs it;
+ * a caller that captures those calls into a HIP graph calls g4_init once per device beforehand, so
+ * that no set-up call falls inside the capture. No reference counterpart: XLA sets kernel attributes
+ * when it compiles the module.
  */
 int g4_init(void);
 
@@ -287,7 +288,8 @@ typedef struct G4PagedCache {
  * also rounds after the norm, as the reference does). e4m3: the scale is the least power of two
  * 2^e >= max |x| / 448 over the vector's finite elements, e clamped to -100 .. 120; elements are
  * rounded to nearest even, infinities and NaN become NaN. Rows that share a page write it in no
- * defined order. No workspace.
+ * defined order. No workspace. A call's grid has less than 2^32 threads (some 2^26 tokens, fewer in rows of less than
+ * 8); more are refused.
  */
 typedef struct G4PagedAppendArgs {
   G4PagedCache cache;
@@ -325,7 +327,8 @@ int g4_paged_append(const G4PagedAppendArgs* args, void* stream);
  * same bits. Rows of more than 640 or 1024 positions (by the number of (row, head) pairs) are cut into
  * pieces that a second launch joins: those calls need g4_paged_decode_workspace_size() bytes of scratch
  * (16-byte aligned; no state is kept in it, so calls ordered on one stream may share it; calls at the
- * same time may not). At most 2^27 positions per row, 2^35 over all (row, head) pairs of a call.
+ * same time may not). At most 2^27 positions per row, 2^35 over all (row, head) pairs of a call, and just under 2^23
+ * such pairs.
  */
 typedef struct G4PagedDecodeArgs {
   G4PagedCache cache;

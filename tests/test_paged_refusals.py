@@ -99,6 +99,8 @@ def test_abi_refuses_bad_tables(name, make, override, match):
     ("g4_paged_append", _append, dict(seq=0), "seq"),
     ("g4_paged_append", _append, dict(keep=-1), "keep"),
     ("g4_paged_append", _append, dict(batch=1 << 20, seq=1 << 20), "tokens"),
+    ("g4_paged_append", _append, dict(batch=1 << 20, seq=1 << 10), "tokens"),  # a grid of 2^32 threads or more
+    ("g4_paged_append", _append, dict(batch=1 << 24, seq=1, in_row_stride=512), "tokens"),
     ("g4_paged_append", _append, dict(k=None), "NULL"),
     ("g4_paged_append", _append, dict(write_pos=None), "NULL"),
     ("g4_paged_append", _append, dict(q=1 << 12), "q_out"),
@@ -122,6 +124,8 @@ def test_abi_refuses_bad_tables(name, make, override, match):
     ("g4_paged_read", _read, dict(count=0), "count"),
     ("g4_paged_read", _read, dict(start=2**31 - 1000, count=100), "count"),
     ("g4_paged_read", _read, dict(batch=1 << 20, count=1 << 20), "positions"),
+    ("g4_paged_read", _read, dict(batch=1 << 18, count=1 << 12), "positions"),
+    ("g4_paged_decode_attention", _decode, dict(batch=0x3fffff), "batch"),
     ("g4_paged_read", _read, dict(k_out=None), "NULL"),
     ("g4_paged_read", _read, dict(v_out=(1 << 12) + 8), "aligned"),
 ])
