@@ -198,15 +198,21 @@ class PagedSpec(NamedTuple):
 
 
 class PagedKVCache(NamedTuple):
-    """A model's cache in pages. Rows hold their real tokens only: position p of a row is its logical (RoPE)
-    position, so left pads take no slot and a finished row's masked steps append nothing. Sliding layers
-    share ``window_table``, whose rows cycle through the few pages that a window touches; global layers
-    ``page_table``. ``length`` counts the physical positions processed, pads included, as ``KVCache.length``."""
+    """A model's cache in pages. Rows hold their real tokens only, in the order in which they came: left pads and
+    the masked steps of a finished row take no slot, and a sliding layer's window is over what the row holds.
+    Sliding layers share ``window_table``, whose rows cycle through the few pages that a window touches; global
+    layers ``page_table``. ``length`` counts the physical positions processed, pads included, as
+    ``KVCache.length``.
+
+    ``held`` are the rows' token counts, so the place of their next tokens. A prefill sets it. ``None`` (an empty
+    cache, or one whose pages the caller fills by ``kernels.paged_append``) leaves the places to the caller: a
+    step's token goes to ``position_ids``, and every place below it has to be filled."""
 
     layers: tuple  # PagedLayerCache | None per layer
     page_table: torch.Tensor  # [B, M] int32, of the global layers
     window_table: torch.Tensor  # [B, M] int32, of the sliding layers
     length: int
+    held: torch.Tensor | None = None  # [B] int32
 
     @property
     def batch(self) -> int:

@@ -425,11 +425,13 @@ def forward_gemma4_text(
     and the key mask is updated in place, so the step has no host-side value baked in and can be
     captured in a HIP graph and replayed.
 
-    With a ``PagedKVCache`` (bf16 models) a token's place follows from ``position_ids`` and
-    ``attention_mask`` alone: each row holds its real tokens at their logical positions. A prefill
-    takes an empty cache and left-padded rows (a mask of zeros, then ones); a masked token of an
-    append is not stored and its row attends to nothing. ``write_pos`` then only asks for a step
-    without host-side values, whose token ids and positions are int32 on the device."""
+    With a ``PagedKVCache`` (bf16 models) each row holds its real tokens one after the other, whatever
+    their ``position_ids``, which only turn the rotary embedding. A prefill takes an empty cache and
+    left-padded rows (a mask of zeros, then ones); a masked token of an append is not stored and
+    its row attends to nothing. Sliding layers count their window in tokens that the row holds.
+    ``write_pos`` then only asks for a step without host-side values, whose token ids and positions
+    are int32 on the device; such a step adds to the input cache's ``held`` in place. In a cache
+    without ``held`` an append's place is its ``position_ids``."""
 
     if lora is not None:
         raise NotImplementedError("LoRA adapters are not supported by the native rollout path")
@@ -486,11 +488,18 @@ def forward_gemma4_text(
     if paged:
         tables = {SLIDING: kv_cache.window_table, FULL: kv_cache.page_table}
         if cache_mode == "prefill":  # token s of a row with n real tokens stands at position s - (S - n)
-            slot = attention_mask.sum(dim=-1, dtype=torch.int32) - S
+            held = attention_mask.sum(dim=-1, dtype=torch.int32)
+            slot = held - S
         else:
-            pos = position_ids[:, 0].to(torch.int32)
-            slot = torch.where(attention_mask[:, 0], pos, -1)
-            lengths = torch.where(attention_mask[:, 0], pos + 1, 0)
+            real, held = attention_mask[:, 0], kv_cache.held
+            if held is None:
+                end = position_ids[:, 0].to(torch.int32) + 1
+            elif write_pos is not None:
+                end = held.add_(real)
+            else:
+                end = held = held + real
+            lengths = end * real
+            slot = lengths - 1
     elif write_pos is not None:
         key_mask = kv_cache.key_mask
         if not fused_prologue:
@@ -642,7 +651,7 @@ def forward_gemma4_text(
     if scratch_cache:
         return hidden, None
     if paged:
-        return hidden, kv_cache._replace(length=length + S)
+        return hidden, kv_cache._replace(length=length + S, held=held)
     return hidden, KVCache(tuple(new_layers), key_mask, length + S)
 
 

@@ -153,13 +153,15 @@ class GraphedDecodeStep:
                  top_p: float = 1.0) -> None:
         if isinstance(cache, PagedKVCache):
             dev, B = cache.device, cache.batch
+            if cache.held is not None:  # advanced by every replay: the caller's stays
+                cache = cache._replace(held=cache.held.clone())
         else:
             dev, B = cache.key_mask.device, cache.key_mask.shape[0]
         self.params, self.config, self.cache = params, config, cache
         self.length = int(cache.length)
         self.tok = torch.zeros(B, dtype=torch.int32, device=dev)
         self.pos = torch.zeros(B, dtype=torch.int32, device=dev)
-        # the warm-up's place is its positions' (0) in pages, a real token's: with the rows inactive it stores nothing
+        # in pages the warm-up would take a place, or without `held` a real token's (0): with the rows inactive none
         self.active = torch.full((B,), not isinstance(cache, PagedKVCache), dtype=torch.bool, device=dev)
         self.slot = torch.full((B,), self.length, dtype=torch.int32, device=dev)
         if temperature is not None and temperature > 0 and key is None:
@@ -261,7 +263,10 @@ class GraphedDecodeStep:
 
     @property
     def kv_cache(self) -> KVCache | PagedKVCache:
-        return self.cache._replace(length=self.length)
+        cache = self.cache._replace(length=self.length)
+        if isinstance(cache, PagedKVCache) and cache.held is not None:  # as of now: later replays go on
+            cache = cache._replace(held=cache.held.clone())
+        return cache
 
 
 # Steps the generation loop may run ahead of the device's any-active flag when EOS ids are set.
