@@ -384,6 +384,16 @@ def _per_layer_inputs(params: Gemma4TextParams, config: Gemma4TextConfig, ids: t
     return ((ctx.float() + token.float()).to(dt).float() * (2.0 ** -0.5)).to(dt)
 
 
+def _check_left_padded(mask: torch.Tensor) -> None:
+    """Refuses a mask that is not zeros, then ones, in every row. The answer is waited for, which a capture cannot:
+    there the mask is the caller's to get right."""
+
+    if mask.is_cuda and torch.cuda.is_current_stream_capturing():
+        return
+    if bool((mask[:, :-1] & ~mask[:, 1:]).any()):
+        raise ValueError("a paged prefill takes left-padded prompts: a mask of zeros, then ones")
+
+
 def forward_gemma4_text(
     params: Gemma4TextParams,
     input_ids: torch.Tensor,
@@ -427,8 +437,8 @@ def forward_gemma4_text(
 
     With a ``PagedKVCache`` (bf16 models) each row holds its real tokens one after the other, whatever
     their ``position_ids``, which only turn the rotary embedding. A prefill takes an empty cache and
-    left-padded rows (a mask of zeros, then ones); a masked token of an append is not stored and
-    its row attends to nothing. Sliding layers count their window in tokens that the row holds.
+    left-padded rows (a mask of zeros, then ones; others are refused, but under capture, where the
+    host cannot look); a masked token of an append is not stored and its row attends to nothing. Sliding layers count their window in tokens that the row holds.
     ``write_pos`` then only asks for a step without host-side values, whose token ids and positions
     are int32 on the device; such a step adds to the input cache's ``held`` in place. In a cache
     without ``held`` an append's place is its ``position_ids``."""
@@ -446,8 +456,14 @@ def forward_gemma4_text(
     paged = isinstance(kv_cache, PagedKVCache)
     if paged and params.embed_tokens.dtype != torch.bfloat16:
         raise ValueError(f"a paged cache needs a bfloat16 model, got {params.embed_tokens.dtype}")
-    if paged and cache_mode == "prefill" and kv_cache.length != 0:
-        raise ValueError(f"a paged prefill needs an empty cache, this one holds {kv_cache.length} positions")
+    if paged:
+        if attention_mask.dim() != 2 or any(m not in (1, n) for m, n in zip(attention_mask.shape, (B, S))):
+            raise ValueError(f"attention_mask {tuple(attention_mask.shape)} does not match [{B}, {S}] tokens")
+        attention_mask = attention_mask.expand(B, S)
+        if cache_mode == "prefill":
+            if kv_cache.length != 0:
+                raise ValueError(f"a paged prefill needs an empty cache, this one holds {kv_cache.length} positions")
+            _check_left_padded(attention_mask)
 
     # graphed decode step: the embedding, key-mask update and rotary tables in one native launch
     fused_prologue = (write_pos is not None and cache_mode == "append" and kv_cache is not None and S == 1

@@ -90,12 +90,10 @@ def prefill(
     if paged is not None:
         if cache_dtype is not None:
             raise ValueError("a paged cache's format is its spec's: leave cache_dtype out")
-        real = prompt_mask.to(torch.bool)
-        if bool((real[:, :-1] & ~real[:, 1:]).any()):
-            raise ValueError("a paged prefill takes left-padded prompts: a mask of zeros, then ones")
         pages = init_paged_kv_cache(config, B, P + max_new_tokens, paged, prompt_ids.device)
-        return forward_gemma4_lm(params, prompt_ids, _position_ids(prompt_mask), config=config, attention_mask=real,
-                                 kv_cache=pages, cache_mode="prefill", logits_to_keep=1, lora=lora)
+        return forward_gemma4_lm(params, prompt_ids, _position_ids(prompt_mask), config=config,
+                                 attention_mask=prompt_mask.to(torch.bool), kv_cache=pages, cache_mode="prefill",
+                                 logits_to_keep=1, lora=lora)
     cache = init_kv_cache(config, B, P + max_new_tokens, dtype, prompt_ids.device)
     return forward_gemma4_lm(params, prompt_ids, _position_ids(prompt_mask), config=config,
                              attention_mask=prompt_mask.to(torch.bool), kv_cache=cache, cache_mode="prefill",
