@@ -206,13 +206,16 @@ class PagedKVCache(NamedTuple):
 
     ``held`` are the rows' token counts, so the place of their next tokens. A prefill sets it. ``None`` (an empty
     cache, or one whose pages the caller fills by ``kernels.paged_append``) leaves the places to the caller: a
-    step's token goes to ``position_ids``, and every place below it has to be filled."""
+    step's token goes to ``position_ids``, and every place below it has to be filled. ``pad`` are the pads that
+    all rows of the prefill began with: the longest row holds at most ``length - pad`` tokens, and a step is
+    refused where that is ``capacity``."""
 
     layers: tuple  # PagedLayerCache | None per layer
     page_table: torch.Tensor  # [B, M] int32, of the global layers
     window_table: torch.Tensor  # [B, M] int32, of the sliding layers
     length: int
     held: torch.Tensor | None = None  # [B] int32
+    pad: int = 0
 
     @property
     def batch(self) -> int:
@@ -227,6 +230,13 @@ class PagedKVCache(NamedTuple):
         """Positions that a row can hold."""
 
         return self.page_table.shape[1] * next(x for x in self.layers if x is not None).page_size
+
+    def check_room(self, length: int) -> None:
+        """ValueError if a row may be full after ``length`` physical positions: another token would have no page."""
+
+        if length - self.pad >= self.capacity:
+            raise ValueError(f"no place for another token: the cache holds {self.capacity} positions, and "
+                             f"{length - self.pad} were processed")
 
 
 def init_paged_kv_cache(config: Gemma4TextConfig, batch_size: int, capacity: int, spec: PagedSpec = PagedSpec(),

@@ -384,14 +384,16 @@ def _per_layer_inputs(params: Gemma4TextParams, config: Gemma4TextConfig, ids: t
     return ((ctx.float() + token.float()).to(dt).float() * (2.0 ** -0.5)).to(dt)
 
 
-def _check_left_padded(mask: torch.Tensor) -> None:
-    """Refuses a mask that is not zeros, then ones, in every row. The answer is waited for, which a capture cannot:
-    there the mask is the caller's to get right."""
+def _common_pads(mask: torch.Tensor) -> int:
+    """The pads that all rows of a left-padded mask begin with; a mask that is not zeros, then ones, in every row is
+    refused. The answer is waited for, which a capture cannot: there the mask is the caller's to get right."""
 
     if mask.is_cuda and torch.cuda.is_current_stream_capturing():
-        return
-    if bool((mask[:, :-1] & ~mask[:, 1:]).any()):
+        return 0
+    gaps, longest = torch.stack([(mask[:, :-1] & ~mask[:, 1:]).sum(), mask.sum(dim=-1).max()]).tolist()
+    if gaps:
         raise ValueError("a paged prefill takes left-padded prompts: a mask of zeros, then ones")
+    return mask.shape[1] - longest
 
 
 def forward_gemma4_text(
@@ -463,7 +465,10 @@ def forward_gemma4_text(
         if cache_mode == "prefill":
             if kv_cache.length != 0:
                 raise ValueError(f"a paged prefill needs an empty cache, this one holds {kv_cache.length} positions")
-            _check_left_padded(attention_mask)
+            pad = _common_pads(attention_mask)
+        else:
+            pad = kv_cache.pad
+            kv_cache.check_room(int(kv_cache.length))
 
     # graphed decode step: the embedding, key-mask update and rotary tables in one native launch
     fused_prologue = (write_pos is not None and cache_mode == "append" and kv_cache is not None and S == 1
@@ -667,7 +672,7 @@ def forward_gemma4_text(
     if scratch_cache:
         return hidden, None
     if paged:
-        return hidden, kv_cache._replace(length=length + S, held=held)
+        return hidden, kv_cache._replace(length=length + S, held=held, pad=pad)
     return hidden, KVCache(tuple(new_layers), key_mask, length + S)
 
 

@@ -218,6 +218,11 @@ class GraphedDecodeStep:
         self.tok.copy_(token_ids)
         self.pos.copy_(position_ids)
         self.active.copy_(active)
+        self._launch()
+
+    def _launch(self) -> None:
+        if isinstance(self.cache, PagedKVCache):
+            self.cache.check_room(self.length)
         self.graph.replay()
         self.length += 1
 
@@ -246,8 +251,7 @@ class GraphedDecodeStep:
 
         if self.temperature is None:
             raise RuntimeError("this step was captured without sampling: use replay_logits")
-        self.graph.replay()
-        self.length += 1
+        self._launch()
         return self.token_out, self.logp_out
 
     def replay_logits(self) -> torch.Tensor:
@@ -255,8 +259,7 @@ class GraphedDecodeStep:
 
         if self.temperature is not None:
             raise RuntimeError("this step was captured with fused sampling: use replay_sample")
-        self.graph.replay()
-        self.length += 1
+        self._launch()
         return self.logits
 
     @property

@@ -128,3 +128,52 @@ def test_places_of_a_cache_without_counts_are_the_positions(device, graphed):
                 cache = out.kv_cache
         assert (cache.held is None) == (not counted) and cache.length == 33
     assert all(torch.equal(a, b) for a, b in zip(*logits))
+
+
+@pytest.mark.parametrize("graphed", [False, True])
+def test_steps_up_to_a_full_cache(device, graphed):
+    """Rows may fill their last page, pads that all of them have not counted; the step behind it is refused. Up to
+    there the logits are those of a wider table."""
+
+    cfg = C.config_from_hf(CFG)
+    params = _params(cfg, device)
+    ids, mask = _prompts(cfg, [4, 9], 24, device)
+    n = mask.sum(-1).to(torch.int32)
+    tok, on = torch.tensor([5, 90], dtype=torch.int32, device=device), torch.ones(2, dtype=torch.bool, device=device)
+    logits = []
+    for more in (8, 40):  # one page or two
+        cache = SMP.prefill(params, cfg, ids, mask, max_new_tokens=more, paged=PagedSpec(32)).kv_cache
+        assert cache.capacity == (32 if more == 8 else 64) and cache.pad == 4
+        gs = SMP.GraphedDecodeStep(params, cfg, cache) if graphed else None
+        logits.append([])
+        for i in range(12):  # the longest row holds 20 tokens of the prompt
+            if graphed:
+                logits[-1].append(gs.step(tok + i, n + i, on).clone())
+            else:
+                out = SMP.decode_step(params, cfg, tok + i, n + i, cache)
+                logits[-1].append(out.logits.clone())
+                cache = out.kv_cache
+        if more == 8:
+            with pytest.raises(ValueError, match="no place"):
+                gs.step(tok, n + 12, on) if graphed else SMP.decode_step(params, cfg, tok, n + 12, cache)
+            if graphed:
+                with pytest.raises(ValueError, match="no place"):
+                    gs.replay_logits()
+                assert gs.length == 36 and gs.kv_cache.held.tolist() == [32, 27]
+    assert all(torch.equal(a, b) for a, b in zip(*logits))
+
+
+def test_a_drawing_step_refuses_a_full_cache(device):
+    cfg = C.config_from_hf(CFG)
+    params = _params(cfg, device)
+    ids, mask = _prompts(cfg, [0, 9], 31, device)
+    cache = SMP.prefill(params, cfg, ids, mask, max_new_tokens=1, paged=PagedSpec(32)).kv_cache
+    gs = SMP.GraphedDecodeStep(params, cfg, cache, temperature=0.0)
+    n, on = mask.sum(-1).to(torch.int32), torch.ones(2, dtype=torch.bool, device=device)
+    gs.step_sample(n, n, on)
+    with pytest.raises(ValueError, match="no place"):
+        gs.step_sample(n, n + 1, on)
+    with pytest.raises(ValueError, match="no place"):
+        gs.replay_sample()
+    with pytest.raises(ValueError, match="no place"):
+        SMP.GraphedDecodeStep(params, cfg, gs.kv_cache)

@@ -76,3 +76,20 @@ def test_step_refuses_a_mask_of_more_columns(run, graphed):
         forward(ids[:, :1], mask, cache, "append", **kw)
     with pytest.raises(ValueError, match="attention_mask"):
         forward(ids, mask[:, 1:], _cache(cfg))
+
+
+@pytest.mark.parametrize("graphed", [False, True])
+@pytest.mark.parametrize("held", [None, [20, 17]])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_step_refuses_a_full_cache(run, graphed, held, pad):
+    """A token behind the last page would be dropped, and its row's attention would go on without it."""
+
+    cfg, _, ids, mask, forward = run
+    kw = dict(write_pos=torch.tensor([63, 63], dtype=torch.int32)) if graphed else {}
+    cache = _cache(cfg)._replace(held=None if held is None else torch.tensor(held, dtype=torch.int32), pad=pad)
+    assert cache.capacity == 64
+    with pytest.raises(Launched):
+        forward(ids[:, :1], mask[:, -1:], cache._replace(length=63 + pad), "append", **kw)
+    for length in (64, 65, 1000):
+        with pytest.raises(ValueError, match="no place"):
+            forward(ids[:, :1], mask[:, -1:], cache._replace(length=length + pad), "append", **kw)
