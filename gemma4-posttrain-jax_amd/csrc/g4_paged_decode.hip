@@ -61,6 +61,7 @@ struct Workspace {
   float* o;      // [slots][R][D] o of each piece of a split (row, head)
   float* ml;     // [slots][R][2] their m and l
   int2* ranges;  // [pairs] first slot and number of slots of a (row, head), {0, 0}: not split
+  int2* plan;    // [batch + 1] pieces and slots before each row; NULL up to kRows rows
 };
 
 // The two MFMA A operands (keys: 8 dims each; values: 8 slots of a dim each) in 16 bytes of e4m3.
@@ -107,101 +108,192 @@ __device__ __forceinline__ int scan_incl(int v) {
 }
 __device__ __forceinline__ int sum_lanes(int v) { return __builtin_amdgcn_readlane(scan_incl(v), 63); }
 
-constexpr int kTries = 5;
-
 // A workgroup's part of a (row, head): piece `index` of `count`.
 struct Piece {
   int b, h, index, count, slot;  // slot: its place in the workspace (count > 1)
   RowKeys keys;                  // of row b
 };
 
-// Piece blockIdx of a split call (false: none). Every wave finds it by itself: the rows' chunk counts are summed
-// over the wave, kRows rows at a time (up to that many stay in registers), then the pieces and the workspace slots
-// before each row.
+// How long the pieces are: the least of kTries lengths `per` whose pieces are all resident at once. The rows' ends add
+// at most one piece per (row, head) to total / per, so the last of them does where there are fewer of those than room.
+// Where there are more, rows of up to twice the mean share of a workgroup stay whole.
 // The host bounds the chunks of all (row, head) pairs by 2^30 and a row's by 2^22, which the f32 division needs.
-constexpr int kRowRegs = 4, kRows = 64 * kRowRegs;
+constexpr int kTries = 5;
+__device__ __forceinline__ float try_share(int i, int total, int pairs, int room, int min_per) {  // 1 / per
+  const int target = pairs < room ? room - (int)((int64_t)pairs * i / (kTries - 1)) : room / 2;
+  const int per = (int)((float)total * __builtin_amdgcn_rcpf((float)target)) + 1;
+  return __builtin_amdgcn_rcpf((float)(per > min_per ? per : min_per));
+}
+// ceil(n / per), 1 of a row without chunks: floor((n - 1) / per) + 1, the quotient off a whole number by 1 / per at
+// least where it is not one
+__device__ __forceinline__ int pieces_of(int n, float share) { return (n > 0 ? (int)((float)(n - 1) * share) : 0) + 1; }
+
+// Consecutive pieces on one XCD (workgroup i runs on XCD i % 8): rows that share pages read them from its L2. False:
+// none for this workgroup.
+__device__ __forceinline__ bool my_piece(int count, int& want) {
+  const int xcd_share = (count + kXcds - 1) / kXcds, y = blockIdx.x / kXcds;
+  want = (int)(blockIdx.x % kXcds) * xcd_share + y;
+  return y < xcd_share && want < count;
+}
+
+// Piece blockIdx of a cut call of up to kRows rows. Every wave finds it by itself: the rows' chunk counts are summed over the
+// wave, then the pieces and the workspace slots before each row.
+constexpr int kRowRegs = 8, kRows = 64 * kRowRegs;
 
 __device__ __forceinline__ bool find_piece(const G4PagedDecodeArgs& a, int room, int min_per, int lane, Piece& out) {
   const int H = a.cache.kv_heads, B = a.batch;
-  RowKeys rows[kRowRegs];  // of rows b0 + 64 i + lane; no positions behind the last row
-  auto load_rows = [&](int b0) {
-    int length[kRowRegs];
+  RowKeys rows[kRowRegs] = {};  // of rows 64 i + lane; no positions behind the last row
+  int length[kRowRegs];
+  const bool upper = B > kRows / 2;  // one branch for the upper half: the loads are on their way together
 #pragma unroll
-    for (int i = 0; i < kRowRegs; ++i) {
-      const int b = b0 + 64 * i + lane;
-      length[i] = a.lengths[b < B ? b : B - 1];
-    }
-#pragma unroll
-    for (int i = 0; i < kRowRegs; ++i) rows[i] = row_keys(a, b0 + 64 * i + lane < B ? length[i] : 0);
-  };
+  for (int i = 0; i < kRowRegs; ++i) {
+    if (i == kRowRegs / 2 && !upper) break;
+    const int b = 64 * i + lane;
+    length[i] = a.lengths[b < B ? b : B - 1];
+  }
   int sum = 0;
-  for (int b0 = 0; b0 < B; b0 += kRows) {
-    load_rows(b0);
 #pragma unroll
-    for (int i = 0; i < kRowRegs; ++i) sum += rows[i].chunks();
+  for (int i = 0; i < kRowRegs; ++i) {
+    if (i == kRowRegs / 2 && !upper) break;
+    rows[i] = row_keys(a, 64 * i + lane < B ? length[i] : 0);
+    sum += rows[i].chunks();
   }
   const int total = sum_lanes(sum) * H;
-  // The least `per` of a few whose pieces are all resident at once: the rows' ends add at most one piece per
-  // (row, head) to total / per, so the last of them does where there are fewer of those than room. Where there are
-  // more, rows of up to twice the mean share of a workgroup stay whole.
-  const int pairs = B * H;
-  float share[kTries];  // 1 / per
+  float share[kTries];
   int n_pieces[kTries];
 #pragma unroll
   for (int i = 0; i < kTries; ++i) {
-    const int target = pairs < room ? room - (int)((int64_t)pairs * i / (kTries - 1)) : room / 2;
-    const int per = (int)((float)total * __builtin_amdgcn_rcpf((float)target)) + 1;
-    share[i] = __builtin_amdgcn_rcpf((float)(per > min_per ? per : min_per));
+    share[i] = try_share(i, total, B * H, room, min_per);
     n_pieces[i] = 0;
   }
-  // ceil(n / per): floor((n - 1) / per) + 1, the quotient off a whole number by 1 / per at least where it is not one
-  auto pieces_of = [&](int b, int n, float share) -> int { return b < B ? (n > 0 ? (int)((float)(n - 1) * share) : 0) + 1 : 0; };
-  for (int b0 = 0; b0 < B; b0 += kRows) {
-    if (B > kRows) load_rows(b0);
 #pragma unroll
-    for (int j = 0; j < kRowRegs; ++j) {
-      if (b0 + 64 * j >= B) break;
+  for (int j = 0; j < kRowRegs; ++j) {
+    if (64 * j >= B) break;
 #pragma unroll
-      for (int i = 0; i < kTries; ++i) n_pieces[i] += pieces_of(b0 + 64 * j + lane, rows[j].chunks(), share[i]);
-    }
+    for (int i = 0; i < kTries; ++i) n_pieces[i] += 64 * j + lane < B ? pieces_of(rows[j].chunks(), share[i]) : 0;
   }
   float cut = share[kTries - 1];
-  int count = 0;
+  int count = 0, want;
 #pragma unroll
   for (int i = kTries - 1; i >= 0; --i) {
     n_pieces[i] = sum_lanes(n_pieces[i]) * H;
     if (i == kTries - 1 || n_pieces[i] <= room) cut = share[i], count = n_pieces[i];
   }
-  // consecutive pieces on one XCD (workgroup i runs on XCD i % 8): rows that share pages read them from its L2
-  const int xcd_share = (count + kXcds - 1) / kXcds;
-  const int y = blockIdx.x / kXcds, want = (int)(blockIdx.x % kXcds) * xcd_share + y;
-  if (y >= xcd_share || want >= count) return false;
+  if (!my_piece(count, want)) return false;
   int before = 0, slots = 0;  // pieces and slots of the rows before these 64
-  for (int b0 = 0; b0 < B; b0 += kRows) {
-    if (B > kRows) load_rows(b0);
 #pragma unroll
-    for (int j = 0; j < kRowRegs; ++j) {
-      if (b0 + 64 * j >= B) break;
-      const int k = pieces_of(b0 + 64 * j + lane, rows[j].chunks(), cut), used = k > 1 ? k * H : 0;
-      const int incl = scan_incl(k * H), sincl = scan_incl(used);
-      const int end = before + __builtin_amdgcn_readlane(incl, 63);
-      if (want < end) {
-        const int at = __builtin_popcountll(__ballot(before + incl <= want));  // the row's lane
-        const int kk = __builtin_amdgcn_readlane(k, at);
-        const int local = want - before - (__builtin_amdgcn_readlane(incl, at) - kk * H);
-        out.b = b0 + 64 * j + at;
-        out.h = __builtin_amdgcn_readfirstlane(local / kk);
-        out.index = local - out.h * kk;
-        out.count = kk;
-        out.slot = slots + __builtin_amdgcn_readlane(sincl, at) - (kk > 1 ? kk * H : 0) + local;
-        out.keys = RowKeys{__builtin_amdgcn_readlane(rows[j].lo, at), __builtin_amdgcn_readlane(rows[j].hi, at)};
-        return true;
-      }
-      before = end;
-      slots += __builtin_amdgcn_readlane(sincl, 63);
+  for (int j = 0; j < kRowRegs; ++j) {
+    if (64 * j >= B) break;
+    const int k = 64 * j + lane < B ? pieces_of(rows[j].chunks(), cut) : 0, used = k > 1 ? k * H : 0;
+    const int incl = scan_incl(k * H), sincl = scan_incl(used);
+    const int end = before + __builtin_amdgcn_readlane(incl, 63);
+    if (want < end) {
+      const int at = __builtin_popcountll(__ballot(before + incl <= want));  // the row's lane
+      const int kk = __builtin_amdgcn_readlane(k, at);
+      const int local = want - before - (__builtin_amdgcn_readlane(incl, at) - kk * H);
+      out.b = 64 * j + at;
+      out.h = __builtin_amdgcn_readfirstlane(local / kk);
+      out.index = local - out.h * kk;
+      out.count = kk;
+      out.slot = slots + __builtin_amdgcn_readlane(sincl, at) - (kk > 1 ? kk * H : 0) + local;
+      out.keys = RowKeys{__builtin_amdgcn_readlane(rows[j].lo, at), __builtin_amdgcn_readlane(rows[j].hi, at)};
+      return true;
     }
+    before = end;
+    slots += __builtin_amdgcn_readlane(sincl, 63);
   }
   return false;
+}
+
+// Of more rows a launch of one workgroup writes the pieces and slots before each row and before their end, [batch + 1],
+// and a wave looks its piece up: reading all lengths in every workgroup of a grid that grows with the rows would take
+// time with their square. us per call of rows of 20 - 199 keys in a table of 4096, e4m3, found by each wave (1024 rows and
+// more: in turns of 256) / planned:
+//     rows                     257        384        512        1024       4096
+//     2 heads of 256 dims   16.4/19.5  21.0/23.1  25.8/25.2  64.0/39.9   541/134
+//     1 head of 64 dims     11.7/15.0  13.3/15.5  15.4/16.3  26.7/16.1   206/33
+// Beyond 512 rows their lengths would take more registers than the loop leaves.
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+
+// Over the workgroup: the sum of v, and of the threads before this one.
+__device__ __forceinline__ int scan_workgroup(int v, int& before, int (&waves)[kPlanWaves]) {
+  const int incl = scan_incl(v), wave = threadIdx.x >> 6;
+  __syncthreads();  // what was read from `waves` before
+  if ((threadIdx.x & 63) == 63) waves[wave] = incl;
+  __syncthreads();
+  int total = 0;
+  before = incl - v;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    before += w < wave ? waves[w] : 0;
+    total += waves[w];
+  }
+  return total;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(G4PagedDecodeArgs a, int2* plan, int room, int min_per) {
+  __shared__ int waves[kPlanWaves];
+  const int H = a.cache.kv_heads, B = a.batch;
+  // this thread's rows
+  const int b0 = (int)((int64_t)B * threadIdx.x / kPlanThreads), b1 = (int)((int64_t)B * (threadIdx.x + 1) / kPlanThreads);
+  auto chunks_of = [&](int b) { return row_keys(a, a.lengths[b]).chunks(); };
+  int sum = 0, before, slots;
+  for (int b = b0; b < b1; ++b) sum += chunks_of(b);
+  const int total = scan_workgroup(sum, before, waves) * H;
+  float share[kTries], cut = 0.f;
+  int n_pieces[kTries];
+#pragma unroll
+  for (int i = 0; i < kTries; ++i) {
+    share[i] = try_share(i, total, B * H, room, min_per);
+    n_pieces[i] = 0;
+  }
+  for (int b = b0; b < b1; ++b) {
+    const int n = chunks_of(b);
+#pragma unroll
+    for (int i = 0; i < kTries; ++i) n_pieces[i] += pieces_of(n, share[i]);
+  }
+#pragma unroll
+  for (int i = kTries - 1; i >= 0; --i) {
+    const int count = scan_workgroup(n_pieces[i], before, waves) * H;
+    if (i == kTries - 1 || count <= room) cut = share[i];
+  }
+  int pieces = 0, used = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int k = pieces_of(chunks_of(b), cut) * H;
+    pieces += k;
+    used += k > H ? k : 0;
+  }
+  const int count = scan_workgroup(pieces, before, waves), all_slots = scan_workgroup(used, slots, waves);
+  for (int b = b0; b < b1; ++b) {
+    const int k = pieces_of(chunks_of(b), cut) * H;
+    plan[b] = make_int2(before, slots);
+    before += k;
+    slots += k > H ? k : 0;
+  }
+  if (threadIdx.x == 0) plan[B] = make_int2(count, all_slots);
+}
+
+__device__ __forceinline__ bool find_planned(const G4PagedDecodeArgs& a, const int2* plan, int lane, Piece& out) {
+  const int H = a.cache.kv_heads, B = a.batch;
+  int want;
+  if (!my_piece(plan[B].x, want)) return false;
+  int b = 0, n = B;  // the row is one of b .. b + n - 1
+  while (n > 1) {
+    const int step = (n + 63) / 64, at = lane * step;
+    const int before = at < n ? plan[b + at].x : 0x7fffffff;
+    const int skip = (__builtin_popcountll(__ballot(before <= want)) - 1) * step;
+    b += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  const int2 first = plan[b];
+  const int kk = __builtin_amdgcn_readfirstlane((plan[b + 1].x - first.x) / H), local = want - first.x;
+  out.b = b;
+  out.h = __builtin_amdgcn_readfirstlane(local / kk);
+  out.index = local - out.h * kk;
+  out.count = kk;
+  out.slot = first.y + local;
+  out.keys = row_keys(a, a.lengths[b]);
+  return true;
 }
 
 template <int D, bool F8, int WAVES, bool SPLIT>
@@ -224,7 +316,7 @@ void paged_decode_kernel(G4PagedDecodeArgs a, Workspace ws, int room, int large)
 
   Piece piece{0, 0, 0, 1, 0, RowKeys{0, 0}};
   if constexpr (SPLIT) {
-    if (!find_piece(a, room, kKeys, lane, piece)) return;
+    if (!(ws.plan ? find_planned(a, ws.plan, lane, piece) : find_piece(a, room, kKeys, lane, piece))) return;
   } else {
     const int pairs = a.batch * H, share = (pairs + kXcds - 1) / kXcds;
     const int y = blockIdx.x / kXcds, pair = (int)(blockIdx.x % kXcds) * share + y;
@@ -537,7 +629,7 @@ size_t lds_bytes(int R) {
 }
 
 // Whether the rows are cut into pieces: where a row can have more chunks than one workgroup is as fast with. Finding
-// the pieces and joining them takes about 4 us. us per call at 256 dims from twelve caches in turn, whole / split, bf16
+// the pieces and joining them takes about 4 us up to 512 rows, their plan beyond 2 - 4 us more. us per call at 256 dims from twelve caches in turn, whole / split, bf16
 // and e4m3:
 //     pairs   512 keys               1024 keys               2048 keys
 //       2     9.7/9.2   7.8/8.9      15.2/9.4   11.4/8.9     26.2/10.7  17.8/9.5
@@ -574,7 +666,8 @@ size_t slots(const G4PagedDecodeArgs& a) { return 2 * (size_t)resident(a.cache.h
 
 size_t workspace_bytes(const G4PagedDecodeArgs& a) {
   if (!split(a)) return 0;
-  return slots(a) * a.group * ((size_t)a.cache.head_dim + 2) * 4 + (size_t)a.batch * a.cache.kv_heads * 8;
+  const size_t plan = a.batch > kRows ? (size_t)a.batch + 1 : 0;
+  return slots(a) * a.group * ((size_t)a.cache.head_dim + 2) * 4 + ((size_t)a.batch * a.cache.kv_heads + plan) * 8;
 }
 
 template <int D, bool F8, int WAVES, bool SPLIT>
@@ -617,6 +710,13 @@ int launch(const G4PagedDecodeArgs& a, hipStream_t st) {
   ws.o = reinterpret_cast<float*>(a.workspace);
   ws.ml = ws.o + slots(a) * a.group * D;
   ws.ranges = reinterpret_cast<int2*>(ws.ml + slots(a) * a.group * 2);
+  if (a.batch > kRows) {
+    ws.plan = ws.ranges + pairs;
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a, ws.plan, resident(D),
+                       (int)Groups<D, split_waves(D)>::KEYS);
+    const int rc = check_launch("g4_paged_decode_attention");
+    if (rc != G4_OK) return rc;
+  }
   const int rc = launch_kernel<D, F8, split_waves(D), true>(a, ws, resident(D) + pairs + kSpare, st);
   if (rc != G4_OK) return rc;
   const int stretches = a.group * D / kJoinDims;
