@@ -637,12 +637,20 @@ size_t lds_bytes(int R) {
 //      64     14.5/13.4 10.2/11.1    23.6/19.5  15.4/14.7    45.0/29.5  26.1/19.5
 //     128     16.2/20.0 11.3/14.8    28.0/29.5  17.6/19.6    51.4/49.7  29.6/29.5
 //     512     43.7/47.3 24.7/28.1    84.0/87.5  45.0/48.0    164/168    85.6/88.8
-// Up to 64 pairs the border is set at 640 keys, where both formats come out even and a single call has one launch less;
-// beyond, at 1024, although equal rows stay faster whole: a long row among short ones would hold its one CU alone.
+// Up to 64 pairs the border is set at 20 chunks, beyond at 32, although equal rows stay faster whole: a long row among
+// short ones would hold its one CU alone. One border for all head dims and formats, although a row's work goes with its
+// bytes. Just behind it, at windows of 640 (up to 64 pairs) and 1024, whole / cut:
+//                       2 pairs    16         80         128        256        512
+//     64 dims, e4m3     6.1/8.0    6.2/8.1    7.3/10.5   7.4/12.3   9.7/14.3   13.5/19.4
+//     128 dims, bf16    7.2/8.3    7.4/8.5    12.8/14.8  16.0/19.7  23.3/30.8  45/56
+//     256 dims, e4m3    9.4/9.3    9.5/9.6    14.1/14.6  17.1/18.5  23.3/30.4  45/48
+//     256 dims, bf16    11.2/9.6   11.4/9.8   25.7/20.8  28.6/29.2  44.0/51.3  86/89
+// and at 512 dims in e4m3 (1, 8, 32, 40, 64, 128, 256 pairs) 17.4/11.8, 17.8/12.2, 18.3/14.2, 18.9/19.1, 24.1/24.0,
+// 34.7/37.0, 48/52. A window may begin inside a chunk, so it counts 31 positions more.
 constexpr int kSplitPairs = 64, kWholeChunksFew = 20, kWholeChunks = 32;
 bool split(const G4PagedDecodeArgs& a) {
   const int64_t cap = (int64_t)a.max_pages * a.cache.page_size;
-  const int64_t keys = a.window > 0 && a.window < cap ? a.window + 31 : cap;  // a window may begin inside a chunk
+  const int64_t keys = a.window > 0 && a.window < cap ? a.window + 31 : cap;
   const bool few = (int64_t)a.batch * a.cache.kv_heads <= kSplitPairs;
   return (keys + 31) / 32 > (few ? kWholeChunksFew : kWholeChunks);
 }
