@@ -250,7 +250,7 @@ __device__ __forceinline__ int page_of(const G4PagedAppendArgs& a, int b, int64_
 
 // A step's tokens (and chunks of fewer than 8): one workgroup per token, one wave per 64 / LANES head vectors of a
 // kind (looping over more than 16). A wave's vectors are a chain of loads, so nothing is staged: 256 tokens of
-// 2 x (4 + 2) heads of 256 in 4.4 us, of which the launch takes most.
+// 2 x (4 + 2) heads of 256 in 4.4 us, of which an empty launch takes 1.7.
 template <int D, bool F8>
 __global__ __launch_bounds__(1024) void paged_append_kernel(G4PagedAppendArgs a, int vec) {
   constexpr int PER = Lanes<D>::PER, VECS = Lanes<D>::VECS;
@@ -293,8 +293,8 @@ __global__ __launch_bounds__(1024) void paged_append_kernel(G4PagedAppendArgs a,
 // head vectors are loaded kTileVecs at a time. The page holds 8 positions' values of a dim side by side, so the
 // value rows of a full group pass through LDS and are stored as whole 16-byte pieces; a group that the chunk, the
 // pads or `keep` cut stores its values one by one. Bound by HBM: 256 x 256 tokens of 2 x (4 + 2) heads of 256 into e4m3
-// pages, 797 MB, in 159 us (5.0 TB/s; a copy reaches 4.85); with one workgroup per token and every value byte stored
-// alone 524 us.
+// pages, 797 MB, in 159 us (5.0 TB/s; a plain copy of that size reaches 5.7, or 6.4 non-temporally); with one workgroup
+// per token and every value byte stored alone 524 us.
 constexpr int kTileTok = 8;
 constexpr int kTileThreads = 64 * kTileTok;
 constexpr int kTileVecs = 4;
@@ -458,8 +458,8 @@ constexpr int kReadThreads = 256;
 
 // One workgroup per (row, head, 32-slot chunk) and array: the chunk's 16-byte pieces are asked for at once, in the
 // page's order, and turned into token-major rows in LDS. Bound by HBM: 16 rows of up to 8191 positions of 2 heads of 256
-// out of e4m3 pages, 353 MB, in 70 us (5.0 TB/s); 500 positions of 512 dims in 4.1 us, 6.3 with both arrays in one
-// workgroup.
+// out of e4m3 pages, 353 MB, in 70 us (5.0 TB/s; a plain copy 5.7); 500 positions of 512 dims in 4.1 us, 6.3 with both
+// arrays in one workgroup.
 template <int D, bool F8>
 __global__ __launch_bounds__(kReadThreads) void paged_read_kernel(G4PagedReadArgs a, int first_chunk, int n_chunks) {
   constexpr int RS = D + 8;                            // LDS row stride, elements

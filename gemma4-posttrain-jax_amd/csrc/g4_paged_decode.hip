@@ -12,8 +12,8 @@
 // launch joins in the pieces' order.
 //
 // Bound by HBM where there is enough to read: 16 rows x 2 heads of 1024 .. 32768 keys of 256 dims, 553 MB in bf16 in
-// 87.8 us (6.3 TB/s; a plain read reaches 6.0), 277 MB in e4m3 in 45.6 us (6.1), and 3 - 4 us more for the join; 256 rows
-// of 200 .. 767 keys, 256 MB, in 47 us (5.4). By latency where there is little: 2 (row, head)s of 512 keys 9.6 us.
+// 87.8 us (6.3 TB/s; a plain non-temporal read reaches 7.1), 277 MB in e4m3 in 45.6 us (6.1), and 3 - 4 us more for the
+// join; 256 rows of 200 .. 767 keys, 256 MB, in 47 us (5.4). By latency where there is little: 2 (row, head)s of 512 keys 9.6 us.
 #include <type_traits>
 
 #include "g4_paged.h"
@@ -629,8 +629,8 @@ size_t lds_bytes(int R) {
 }
 
 // Whether the rows are cut into pieces: where a row can have more chunks than one workgroup is as fast with. Finding
-// the pieces and joining them takes about 4 us up to 512 rows, their plan beyond 2 - 4 us more. us per call at 256 dims from twelve caches in turn, whole / split, bf16
-// and e4m3:
+// the pieces and joining them takes about 4 us up to 512 rows, their plan beyond 2 - 4 us more. us per call at 256 dims
+// from twelve caches in turn, whole / split, bf16 and e4m3:
 //     pairs   512 keys               1024 keys               2048 keys
 //       2     9.7/9.2   7.8/8.9      15.2/9.4   11.4/8.9     26.2/10.7  17.8/9.5
 //      16     12.8/10.6 8.7/10.1     21.9/11.2  14.1/9.6     39.9/13.6  23.3/11.1

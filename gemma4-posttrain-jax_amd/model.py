@@ -558,7 +558,7 @@ def forward_gemma4_text(
             prep_q = dict(q_norm_weight=qk_norms[0], eps=eps, rope_cos=cos, rope_sin=sin)
             src = sources[i] if shared else i
             new_layers.append(layer_cache)
-            if shared:
+            if shared:  # nothing to append: the dense path's preparation, which also rounds after the norm
                 kernels.prepare_q(q, q_out, flags=flags_q, **prep_q)
             else:
                 k = qkv[..., H * R * D: (H * R + H) * D].view(B, S, H, D)

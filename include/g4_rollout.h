@@ -353,7 +353,8 @@ int g4_paged_decode_attention(const G4PagedDecodeArgs* args, void* stream);
  * Reads a paged cache back: k_out / v_out [B, count, Hkv, D] bf16 (the reference's cache order,
  * model.py:238-246) of positions start .. start + count - 1 of every row; positions at or beyond
  * lengths[b], or without a page, read as zeros. Exact, but that values below bf16's least normal
- * number 2^-126 may read as zero.
+ * number 2^-126 may read as zero, and that an e4m3 element stored as 256 * 2^120 (a magnitude of
+ * 248 * 2^120 and more) is 2^128 and reads as infinity.
  */
 typedef struct G4PagedReadArgs {
   G4PagedCache cache;
