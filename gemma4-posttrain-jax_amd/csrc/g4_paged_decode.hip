@@ -8,7 +8,7 @@
 // A (row, head) is one workgroup's work, or, where rows are long or few, pieces of at most `per` chunks of 32
 // slots: `per` follows from the sum of all rows' chunks, so that ragged rows, few long ones and many short
 // ones fill the chip alike. The lengths stand on the device, so each workgroup finds its piece from them
-// itself. A (row, head) of one piece is finished by it; the others leave (m, l, o) per piece, which a second
+// itself, or in a large batch from what one workgroup has made of them. A (row, head) of one piece is finished by it; the others leave (m, l, o) per piece, which a second
 // launch joins in the pieces' order.
 //
 // Bound by HBM where there is enough to read: 16 rows x 2 heads of 1024 .. 32768 keys of 256 dims, 553 MB in bf16 in

@@ -440,10 +440,11 @@ def forward_gemma4_text(
     With a ``PagedKVCache`` (bf16 models) each row holds its real tokens one after the other, whatever
     their ``position_ids``, which only turn the rotary embedding. A prefill takes an empty cache and
     left-padded rows (a mask of zeros, then ones; others are refused, but under capture, where the
-    host cannot look); a masked token of an append is not stored and its row attends to nothing. Sliding layers count their window in tokens that the row holds.
-    ``write_pos`` then only asks for a step without host-side values, whose token ids and positions
-    are int32 on the device; such a step adds to the input cache's ``held`` in place. In a cache
-    without ``held`` an append's place is its ``position_ids``."""
+    host cannot look); a masked token of an append is not stored and its row attends to nothing.
+    Sliding layers count their window in tokens that the row holds. ``write_pos`` then only asks for
+    a step without host-side values, whose token ids and positions are int32 on the device; such a
+    step adds to the input cache's ``held`` in place. In a cache without ``held`` an append's place is
+    its ``position_ids``. An append that may find a row full is refused."""
 
     if lora is not None:
         raise NotImplementedError("LoRA adapters are not supported by the native rollout path")

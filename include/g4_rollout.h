@@ -324,12 +324,13 @@ int g4_paged_append(const G4PagedAppendArgs* args, void* stream);
  * whose scores are all -inf, gives zeros. What the other slots hold, NaN included, does not matter.
  * f32 scores, softmax and sums; the unnormalised probabilities (times the value's scale) are rounded
  * to bf16 as the operand of the value product, the result once to bf16. The same call gives the
- * same bits. Where a row can have more than 640 or 1024 positions (by the number of (row, head) pairs),
- * the rows may be cut into pieces that a second launch joins. The table's max_pages * page_size, or a window
- * of more than 609 or 993 positions in a wider table, decides that, not the lengths, which are on the
- * device. Those calls need g4_paged_decode_workspace_size() bytes of scratch (16-byte aligned; no
- * state is kept in it, so calls ordered on one stream may share it; calls at the same time may not). At most 2^27 positions per row, 2^35 over all (row, head) pairs of a call, and just under 2^23
- * such pairs.
+ * same bits. Where a row can have more than 640 or 1024 positions (by the number of (row, head)
+ * pairs), the rows may be cut into pieces that a second launch joins; the table's max_pages *
+ * page_size, or a window of more than 609 or 993 positions in a wider table, decides that, not the
+ * lengths, which are on the device. Those calls need g4_paged_decode_workspace_size() bytes of
+ * scratch (16-byte aligned; no state is kept in it, so calls ordered on one stream may share it;
+ * calls at the same time may not). At most 2^27 positions per row, 2^35 over all (row, head) pairs
+ * of a call, and just under 2^23 such pairs.
  */
 typedef struct G4PagedDecodeArgs {
   G4PagedCache cache;
