@@ -8,8 +8,8 @@
 // A (row, head) is one workgroup's work, or, where rows are long or few, pieces of at most `per` chunks of 32
 // slots: `per` follows from the sum of all rows' chunks, so that ragged rows, few long ones and many short
 // ones fill the chip alike. The lengths stand on the device, so each workgroup finds its piece from them
-// itself, or in a large batch from what one workgroup has made of them. A (row, head) of one piece is finished by it; the others leave (m, l, o) per piece, which a second
-// launch joins in the pieces' order.
+// itself, or in a large batch from what one workgroup has made of them before. A (row, head) of one piece is
+// finished by it; the others leave (m, l, o) per piece, which a last launch joins in the pieces' order.
 //
 // Bound by HBM where there is enough to read: 16 rows x 2 heads of 1024 .. 32768 keys of 256 dims, 553 MB in bf16 in
 // 87.8 us (6.3 TB/s; a plain non-temporal read reaches 7.1), 277 MB in e4m3 in 45.6 us (6.1), and 3 - 4 us more for the
@@ -629,8 +629,8 @@ size_t lds_bytes(int R) {
 }
 
 // Whether the rows are cut into pieces: where a row can have more chunks than one workgroup is as fast with. Finding
-// the pieces and joining them takes about 4 us up to 512 rows, their plan beyond 2 - 4 us more. us per call at 256 dims
-// from twelve caches in turn, whole / split, bf16 and e4m3:
+// the pieces and joining them takes about 4 us up to 512 rows, the plan of 1024 4 us more, of 4096 8. us per call at 256
+// dims from twelve caches in turn, whole / split, bf16 and e4m3:
 //     pairs   512 keys               1024 keys               2048 keys
 //       2     9.7/9.2   7.8/8.9      15.2/9.4   11.4/8.9     26.2/10.7  17.8/9.5
 //      16     12.8/10.6 8.7/10.1     21.9/11.2  14.1/9.6     39.9/13.6  23.3/11.1
