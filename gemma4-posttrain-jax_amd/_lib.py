@@ -73,6 +73,14 @@ class G4PrefillArgs(ctypes.Structure):
     ]
 
 
+class G4PackedPrefillArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", c_int32), ("kv_heads", c_int32), ("group", c_int32), ("head_dim", c_int32), ("window", c_int32),
+        ("k_stride", c_int32), ("starts", c_void_p), ("q", c_void_p), ("k", c_void_p), ("vt", c_void_p),
+        ("out", c_void_p),
+    ]
+
+
 # Every symbol include/g4_rollout.h declares, with its ctypes prototype.
 class G4SampleArgs(ctypes.Structure):
     _fields_ = [
@@ -168,6 +176,8 @@ PROTOTYPES = {
     "g4_decode_attention": (c_int32, [POINTER(G4DecodeArgs), c_void_p]),
     "g4_decode_attention_noalloc": (c_int32, [POINTER(G4DecodeArgs), c_void_p]),
     "g4_prefill_attention": (c_int32, [POINTER(G4PrefillArgs), c_void_p]),
+    "g4_packed_prefill_attention": (c_int32, [POINTER(G4PackedPrefillArgs), c_void_p]),
+    "g4_packed_starts": (c_int32, [c_int32, c_void_p, c_int32, c_void_p, c_void_p]),
     "g4_paged_append": (c_int32, [POINTER(G4PagedAppendArgs), c_void_p]),
     "g4_paged_decode_workspace_size": (c_size_t, [POINTER(G4PagedDecodeArgs)]),
     "g4_paged_decode_attention": (c_int32, [POINTER(G4PagedDecodeArgs), c_void_p]),
@@ -257,6 +267,6 @@ def ring_slot_positions(last_written: int, window_capacity: int) -> list[int]:
 
 __all__ = [
     "G4AppendArgs", "G4DecodeArgs", "G4PrefillArgs", "G4LinearArgs", "G4PrologueArgs", "G4DecodePrep", "G4PagedCache",
-    "G4PagedAppendArgs", "G4PagedDecodeArgs", "G4PagedReadArgs", "G4Error", "PROTOTYPES", "LIB_PATH", "lib", "check", "init_device",
+    "G4PagedAppendArgs", "G4PagedDecodeArgs", "G4PagedReadArgs", "G4PackedPrefillArgs", "G4Error", "PROTOTYPES", "LIB_PATH", "lib", "check", "init_device",
     "kv_source_layers", "ring_slot_positions", "c_uint8",
 ]

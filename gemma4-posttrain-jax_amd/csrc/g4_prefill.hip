@@ -10,6 +10,7 @@
 // The reference rounds probabilities after an f32 softmax over the full row; to reproduce that
 // rounding the kernel makes two passes over the key range: pass 1 finds each row's max and
 // sum, pass 2 recomputes the scores and forms exact bf16 probabilities for the value product.
+#include "g4_attn_tiles.h"
 #include "g4_common.h"
 #include "g4_internal.h"
 

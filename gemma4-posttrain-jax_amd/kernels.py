@@ -324,11 +324,76 @@ def prefill_attention(
     return out
 
 
-# --- paged cache ------------------------------------------------------------------------------------------
-
-
 _BF16, _E4M3, _E8M0, _I32, _F32 = (torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.int32,
                                    torch.float32)  # a module's name is the cheaper one to look up
+
+
+def _device_of(tensors) -> int:
+    """The index of the device that all operands are on, which has to be the current one: the call goes to its
+    stream. (``get_device`` is -1 on the host.)"""
+
+    dev = torch._C._cuda_getDevice() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"an operand is on {t.device}, where the cache's {tensors[0].device} has to be the current "
+                             f"device and hold them all")
+    if dev < 0:
+        raise ValueError("kernel operands must be device tensors")
+    return dev
+
+
+# --- packed prompts ---------------------------------------------------------------------------------------
+
+
+def packed_starts(cu_seqlens: torch.Tensor, tokens: int) -> torch.Tensor:
+    """g4_packed_starts: the first token of each token's sequence, int32 ``[tokens]``, from the sequences' bounds
+    ``cu_seqlens`` (int32 ``[N + 1]``, from 0 on, not falling); -1 for a token behind the last sequence."""
+
+    if cu_seqlens.dtype is not _I32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or not cu_seqlens.is_contiguous():
+        raise ValueError("cu_seqlens must be a contiguous int32 [N + 1] tensor")
+    if tokens <= 0:
+        raise ValueError(f"tokens must be positive, got {tokens}")
+    dev = _device_of((cu_seqlens,))
+    starts = cu_seqlens.new_empty(tokens)
+    _lib.check(_lib.lib().g4_packed_starts(cu_seqlens.numel() - 1, cu_seqlens.data_ptr(), tokens, starts.data_ptr(),
+                                           torch._C._cuda_getCurrentRawStream(dev)), "g4_packed_starts")
+    return starts
+
+
+def packed_prefill_attention(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, starts: torch.Tensor, *,
+                             window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """g4_packed_prefill_attention: causal attention of prompts that stand one behind the other without pads. q ``[T,
+    Hkv, R, D]`` bf16, k ``key_shape(1, Hkv, Sp, D)`` and vt ``[1, Hkv, Sp / 8, D, 8]`` (a ``kv_append`` of the T tokens as one
+    row; Sp >= T, multiple of 64), ``starts`` int32 ``[T]`` of ``packed_starts``; with ``window`` > 0 the last
+    ``window`` tokens. Returns ``[T, Hkv, R, D]``, zeros for tokens of no sequence."""
+
+    if q.dim() != 4 or q.dtype is not _BF16 or not q.is_contiguous():
+        raise ValueError("q must be a contiguous bfloat16 [T, Hkv, R, D] tensor")
+    T, H, R, D = q.shape
+    if k.dim() != 7 or vt.dim() != 5:
+        raise ValueError(f"k {tuple(k.shape)} / vt {tuple(vt.shape)} are not a layer's layouts")
+    Sp = k.shape[2] * 32
+    if k.shape != key_shape(1, H, Sp, D) or vt.shape != (1, H, Sp // 8, D, 8) or Sp < T:
+        raise ValueError(f"k {tuple(k.shape)} / vt {tuple(vt.shape)} do not match q {tuple(q.shape)}")
+    if k.dtype is not _BF16 or vt.dtype is not _BF16 or not (k.is_contiguous() and vt.is_contiguous()):
+        raise ValueError("k / vt must be contiguous and bfloat16")
+    if starts.dtype is not _I32 or starts.shape != (T,) or not starts.is_contiguous():
+        raise ValueError(f"starts must be a contiguous int32 [{T}] tensor")
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    if out is not None and (out.shape != q.shape or out.dtype is not _BF16 or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous bfloat16 [T, Hkv, R, D] tensor")
+    dev = _device_of((q, k, vt, starts, out))
+    if out is None:
+        out = torch.empty_like(q)
+    a = _lib.G4PackedPrefillArgs(T, H, R, D, window, Sp, starts.data_ptr(), q.data_ptr(), k.data_ptr(), vt.data_ptr(),
+                                 out.data_ptr())
+    _lib.check(_lib.lib().g4_packed_prefill_attention(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)),
+               "g4_packed_prefill_attention")
+    return out
+
+
+# --- paged cache ------------------------------------------------------------------------------------------
 
 
 def _paged_cache(layer: PagedLayerCache) -> _lib.G4PagedCache:
@@ -359,20 +424,6 @@ def _paged_cache(layer: PagedLayerCache) -> _lib.G4PagedCache:
         raise ValueError(f"e4m3 pages need contiguous float8_e8m0fnu scales of shape {scales}")
     return _lib.G4PagedCache(_lib.G4_PAGES_E4M3, P, H, D, page, key.data_ptr(), value.data_ptr(), key_scale.data_ptr(),
                              value_scale.data_ptr())
-
-
-def _device_of(tensors) -> int:
-    """The index of the device that all operands are on, which has to be the current one: the call goes to its
-    stream. (``get_device`` is -1 on the host.)"""
-
-    dev = torch._C._cuda_getDevice() if tensors[0].is_cuda else -1
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"an operand is on {t.device}, where the cache's {tensors[0].device} has to be the current "
-                             f"device and hold them all")
-    if dev < 0:
-        raise ValueError("kernel operands must be device tensors")
-    return dev
 
 
 def _page_rows(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> tuple[int, int, int]:

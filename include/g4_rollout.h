@@ -247,6 +247,36 @@ typedef struct G4PrefillArgs {
 int g4_prefill_attention(const G4PrefillArgs* args, void* stream);
 
 /*
+ * Causal attention of packed prompts: `tokens` tokens, sequences of any lengths one behind the other without pads
+ * (model.py:320-335, 496-499 per sequence; the reference pads to one length). Query t attends key j iff
+ * starts[t] <= j <= t and (window == 0 or j > t - window): starts[t] is the first token of t's sequence
+ * (g4_packed_starts forms it from the sequences' bounds; every layer of a batch uses it). A token with starts[t] < 0
+ * or > t belongs to no sequence: its rows are zeros. bf16, f32 scores, softmax and sums; the unnormalised
+ * probabilities are rounded to bf16 as the operand of the value product, the result once to bf16 (g4_prefill_attention
+ * also rounds the scores, as the reference does). What a row does not see, NaN included, does not reach it; a row
+ * whose scores are all -inf gives zeros. The same call gives the same bits. No workspace.
+ */
+typedef struct G4PackedPrefillArgs {
+  int32_t tokens;         /* T */
+  int32_t kv_heads;
+  int32_t group;          /* R, 1 .. 64 */
+  int32_t head_dim;       /* 64, 128, 256 or 512 */
+  int32_t window;         /* 0 = every earlier token of the sequence */
+  int32_t k_stride;       /* slots of k / vt: >= T, a multiple of 64; k_stride * head_dim * 2 < 2^32 */
+  const int32_t* starts;  /* device [T] */
+  const void* q;          /* [T, Hkv, R, D]; q, k, vt and out 16-byte aligned */
+  const void* k;          /* [1, Hkv, k_stride/32, D/32, 2, 16, 32]: the key layout above, token t in slot t */
+  const void* vt;         /* [1, Hkv, k_stride/8, D, 8] */
+  void* out;              /* [T, Hkv, R, D] */
+} G4PackedPrefillArgs;
+
+int g4_packed_prefill_attention(const G4PackedPrefillArgs* args, void* stream);
+
+/* starts[t] for t < tokens: cu_seqlens[i] of the sequence i with cu_seqlens[i] <= t < cu_seqlens[i + 1], -1 for none.
+ * cu_seqlens: device, sequences + 1 values that do not fall. */
+int g4_packed_starts(int32_t sequences, const int32_t* cu_seqlens, int32_t tokens, int32_t* starts, void* stream);
+
+/*
  * One layer's KV cache in pages, for rows that take memory as they grow and may share it (the
  * completions of one prompt). No reference counterpart: its caches are one dense array per layer.
  * A page holds page_size consecutive positions of a row, all kv heads:

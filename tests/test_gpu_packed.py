@@ -1,0 +1,160 @@
+"""Attention of packed prompts on the GPU against 64 bits: sequences of every length about the tiles' edges, windows,
+groups, tokens of no sequence, and values that a row must not see."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from gemma4_posttrain_jax_amd import kernels
+from gemma4_posttrain_jax_amd.kvcache import group_keys, group_values, slot_stride_for
+from packed_util import packed_reference
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(lens, tail, H, R, D, seed, device, scale=2.0):
+    g = torch.Generator().manual_seed(seed)
+    T = sum(lens) + tail
+    q = (torch.randn(T, H, R, D, generator=g) * scale / math.sqrt(D)).to(torch.bfloat16)
+    k = torch.randn(T, H, D, generator=g).to(torch.bfloat16)
+    v = torch.randn(T, H, D, generator=g).to(torch.bfloat16)
+    return q, k, v
+
+
+def _laid_out(k, v, device, fill=0.0):
+    T, H, D = k.shape
+    Sp = slot_stride_for(T)
+    kk = torch.full((1, H, Sp, D), fill, dtype=torch.bfloat16)
+    vv = torch.full((1, H, Sp, D), fill, dtype=torch.bfloat16)
+    kk[0, :, :T], vv[0, :, :T] = k.transpose(0, 1), v.transpose(0, 1)
+    return group_keys(kk).to(device), group_values(vv).to(device)
+
+
+def _run(q, k, v, lens, window, device, fill=0.0, **kw):
+    cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32, device=device)
+    starts = kernels.packed_starts(cu, q.shape[0])
+    kk, vv = _laid_out(k, v, device, fill)
+    return kernels.packed_prefill_attention(q.to(device), kk, vv, starts, window=window, **kw)
+
+
+def _check(got, q, k, v, lens, window):
+    want, bound = packed_reference(q, k, v, lens, window)
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= bound).all()), f"off by {float((err - bound).max())} at {int((err - bound).argmax())}"
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("lens,tail", [([1], 0), ([33, 0, 1, 65, 2], 3), ([130, 31, 32, 97], 0)])
+def test_lengths_and_windows(D, window, lens, tail, device):
+    q, k, v = _inputs(lens, tail, 2, 4, D, 1, device)
+    _check(_run(q, k, v, lens, window, device), q, k, v, lens, window)
+
+
+@pytest.mark.parametrize("R", [1, 2, 3, 5, 8, 16, 17])
+def test_groups(R, device):
+    lens = [70, 3, 41]
+    q, k, v = _inputs(lens, 0, 1, R, 128, 2, device)
+    _check(_run(q, k, v, lens, 0, device), q, k, v, lens, 0)
+
+
+@pytest.mark.parametrize("D,window", [(256, 0), (256, 512), (128, 0), (512, 0), (64, 100)])
+def test_long_prompts(D, window, device):
+    lens = [1, 1500, 700]
+    q, k, v = _inputs(lens, 11, 1, 2, D, 3, device)
+    _check(_run(q, k, v, lens, window, device), q, k, v, lens, window)
+
+
+@pytest.mark.parametrize("D", [64, 256, 512])
+def test_many_short_prompts(D, device):
+    g = torch.Generator().manual_seed(4)
+    lens = torch.randint(0, 9, (300,), generator=g).tolist()
+    q, k, v = _inputs(lens, 0, 2, 4, D, 5, device)
+    _check(_run(q, k, v, lens, 0, device), q, k, v, lens, 0)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_what_a_row_does_not_see_does_not_reach_it(D, device):
+    """NaN and infinities behind the last token, in another prompt, before the window and behind a token."""
+
+    lens, window, tail = [37, 90, 50], 32, 4
+    q, k, v = _inputs(lens, tail, 2, 4, D, 6, device)
+    clean_k, clean_v = k.clone(), v.clone()
+    for t, x in ((5, math.nan), (60, math.inf), (100, -math.inf), (36, math.nan), (178, math.nan)):
+        v[t, :, ::3] = x
+        k[t, :, ::5] = x if t != 60 else math.nan
+    got = _run(q, k, v, lens, window, device, fill=math.nan).cpu()
+    want, bound = packed_reference(q, clean_k, clean_v, lens, window)
+    start = 0
+    for n in lens:
+        for t in range(start, start + n):
+            seen = range(max(start, t - window + 1), t + 1)
+            if not any(j in seen for j in (5, 60, 100, 36, 178)):
+                assert bool(((got[t].double() - want[t]).abs() <= bound[t]).all()), t
+            elif 5 in seen or 36 in seen:
+                assert bool(got[t].isnan().all()), t  # the scores are NaN
+        start += n
+    assert bool((got[start:] == 0).all())
+
+
+@pytest.mark.parametrize("D", [64, 256, 512])
+def test_a_seen_infinity_and_its_neighbours(D, device):
+    """An infinite value reaches the rows that see it, in its dims, and no other."""
+
+    lens = [45, 45]
+    q, k, v = _inputs(lens, 0, 1, 2, D, 7, device)
+    v[20, 0, 3] = math.inf
+    got = _run(q, k, v, lens, 0, device).cpu().double()
+    v[20, 0, 3] = 0.0
+    want, bound = packed_reference(q, k, v, lens, 0)
+    hit = torch.zeros_like(want, dtype=torch.bool)
+    hit[20:45, :, :, 3] = True
+    assert bool((got[hit] == math.inf).all())
+    assert bool(((got - want).abs() <= bound)[~hit].all())
+
+
+def test_scores_far_apart(device):
+    """Maxima that rise along a row by more than the slack, and scores beyond e^88 of each other."""
+
+    lens = [300]
+    q, k, v = _inputs(lens, 0, 1, 4, 128, 8, device, scale=40.0)
+    k = (k.float() * torch.linspace(0.1, 3.0, 300)[:, None, None]).to(torch.bfloat16)
+    _check(_run(q, k, v, lens, 0, device), q, k, v, lens, 0)
+
+
+def test_the_same_call_gives_the_same_bits_and_takes_an_out(device):
+    lens = [100, 200, 3]
+    q, k, v = _inputs(lens, 0, 2, 4, 256, 9, device)
+    first = _run(q, k, v, lens, 0, device)
+    out = torch.full_like(first, math.nan)
+    assert _run(q, k, v, lens, 0, device, out=out) is out
+    assert torch.equal(out.view(torch.int16), first.view(torch.int16))
+
+
+@pytest.mark.parametrize("bounds,tokens,want", [
+    ([0, 3, 3, 5], 7, [0, 0, 0, 3, 3, -1, -1]),
+    ([0, 0, 0], 2, [-1, -1]),
+    ([0, 4], 2, [0, 0]),
+    ([2, 4], 5, [-1, -1, 2, 2, -1]),
+])
+def test_starts(bounds, tokens, want, device):
+    cu = torch.tensor(bounds, dtype=torch.int32, device=device)
+    assert kernels.packed_starts(cu, tokens).tolist() == want
+
+
+def test_starts_that_are_none(device):
+    """A start behind its token or below 0 is no sequence: zeros, whatever the other rows are."""
+
+    q, k, v = _inputs([64], 0, 1, 1, 128, 10, device)
+    starts = torch.zeros(64, dtype=torch.int32, device=device)
+    starts[10], starts[20], starts[63] = 11, -2 ** 31, 2 ** 31 - 1
+    kk, vv = _laid_out(k, v, device)
+    got = kernels.packed_prefill_attention(q.to(device), kk, vv, starts).cpu().double()
+    want, bound = packed_reference(q, k, v, [64], 0)
+    none = torch.zeros(64, dtype=torch.bool)
+    none[[10, 20, 63]] = True
+    assert bool((got[none] == 0).all())
+    assert bool(((got - want).abs() <= bound)[~none].all())
