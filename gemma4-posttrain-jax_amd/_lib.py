@@ -73,6 +73,38 @@ class G4PrefillArgs(ctypes.Structure):
     ]
 
 
+class G4PageTable(ctypes.Structure):
+    _fields_ = [("rows", c_int32), ("max_pages", c_int32), ("stride", c_int64), ("entries", c_void_p)]
+
+
+class G4PagedReserveArgs(ctypes.Structure):
+    _fields_ = [
+        ("num_pages", c_int32), ("page_size", c_int32), ("table", G4PageTable), ("lengths", c_void_p),
+        ("refs", c_void_p), ("shortage", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class G4PagedForkArgs(ctypes.Structure):
+    _fields_ = [
+        ("layers", c_void_p), ("n_layers", c_int32), ("table", G4PageTable), ("out", G4PageTable),
+        ("parents", c_void_p), ("lengths", c_void_p), ("refs", c_void_p), ("shortage", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class G4PagedFreeArgs(ctypes.Structure):
+    _fields_ = [
+        ("num_pages", c_int32), ("page_size", c_int32), ("table", G4PageTable), ("keep", c_void_p), ("refs", c_void_p),
+    ]
+
+
+class G4PagedCompactArgs(ctypes.Structure):
+    _fields_ = [
+        ("layers", c_void_p), ("n_layers", c_int32), ("table", G4PageTable), ("refs", c_void_p), ("live", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 class G4PackedPrefillArgs(ctypes.Structure):
     _fields_ = [
         ("tokens", c_int32), ("kv_heads", c_int32), ("group", c_int32), ("head_dim", c_int32), ("window", c_int32),
@@ -182,6 +214,14 @@ PROTOTYPES = {
     "g4_paged_decode_workspace_size": (c_size_t, [POINTER(G4PagedDecodeArgs)]),
     "g4_paged_decode_attention": (c_int32, [POINTER(G4PagedDecodeArgs), c_void_p]),
     "g4_paged_read": (c_int32, [POINTER(G4PagedReadArgs), c_void_p]),
+    "g4_paged_reserve_workspace_size": (c_size_t, [POINTER(G4PagedReserveArgs)]),
+    "g4_paged_reserve": (c_int32, [POINTER(G4PagedReserveArgs), c_void_p]),
+    "g4_paged_fork_workspace_size": (c_size_t, [POINTER(G4PagedForkArgs)]),
+    "g4_paged_fork": (c_int32, [POINTER(G4PagedForkArgs), c_void_p]),
+    "g4_paged_copy": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
+    "g4_paged_free": (c_int32, [POINTER(G4PagedFreeArgs), c_void_p]),
+    "g4_paged_compact_workspace_size": (c_size_t, [POINTER(G4PagedCompactArgs)]),
+    "g4_paged_compact": (c_int32, [POINTER(G4PagedCompactArgs), c_void_p]),
     "g4_kv_source_layers": (c_int32, [c_int32, c_int32, POINTER(c_int32), POINTER(c_int32)]),
     "g4_ring_slot_positions": (c_int32, [c_int32, c_int32, POINTER(c_int32)]),
     "g4_sample_tokens": (c_int32, [POINTER(G4SampleArgs), c_void_p]),
@@ -267,6 +307,7 @@ def ring_slot_positions(last_written: int, window_capacity: int) -> list[int]:
 
 __all__ = [
     "G4AppendArgs", "G4DecodeArgs", "G4PrefillArgs", "G4LinearArgs", "G4PrologueArgs", "G4DecodePrep", "G4PagedCache",
-    "G4PagedAppendArgs", "G4PagedDecodeArgs", "G4PagedReadArgs", "G4PackedPrefillArgs", "G4Error", "PROTOTYPES", "LIB_PATH", "lib", "check", "init_device",
+    "G4PagedAppendArgs", "G4PagedDecodeArgs", "G4PagedReadArgs", "G4PackedPrefillArgs",
+    "G4PageTable", "G4PagedReserveArgs", "G4PagedForkArgs", "G4PagedFreeArgs", "G4PagedCompactArgs", "G4Error", "PROTOTYPES", "LIB_PATH", "lib", "check", "init_device",
     "kv_source_layers", "ring_slot_positions", "c_uint8",
 ]

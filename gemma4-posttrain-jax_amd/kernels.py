@@ -426,8 +426,8 @@ def _paged_cache(layer: PagedLayerCache) -> _lib.G4PagedCache:
                              value_scale.data_ptr())
 
 
-def _page_rows(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> tuple[int, int, int]:
-    """(B, entries per row, stride) of a page table, ``rows`` being the int32 [B] tensor ``name``."""
+def _table_rows(page_table: torch.Tensor) -> tuple[int, int, int]:
+    """(B, entries per row, stride) of a page table."""
 
     shape = page_table.shape
     if page_table.dtype is not _I32 or len(shape) != 2 or 0 in shape:
@@ -438,6 +438,13 @@ def _page_rows(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> tuple
         stride = M
     if (M > 1 and inner != 1) or stride < M:
         raise ValueError("page_table rows must be contiguous and apart")
+    return B, M, stride
+
+
+def _page_rows(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> tuple[int, int, int]:
+    """(B, entries per row, stride) of a page table, ``rows`` being the int32 [B] tensor ``name``."""
+
+    B, M, stride = _table_rows(page_table)
     if rows.dtype is not _I32 or rows.shape != (B,) or not rows.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 [{B}] tensor")
     return B, M, stride
@@ -575,6 +582,133 @@ def paged_read(layer: PagedLayerCache, *, page_table: torch.Tensor, lengths: tor
                              k.data_ptr(), v.data_ptr())
     _lib.check(_lib.lib().g4_paged_read(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_read")
     return k, v
+
+
+# --- a pool of pages --------------------------------------------------------------------------------------
+
+
+def _pool_layers(layers):
+    """The C array of a pool's layers, which share its tables."""
+
+    layers = tuple(layers)
+    if not layers:
+        raise ValueError("layers must not be empty")
+    caches = (_lib.G4PagedCache * len(layers))(*map(_paged_cache, layers))
+    for c in caches:
+        if c.num_pages != caches[0].num_pages or c.page_size != caches[0].page_size:
+            raise ValueError(f"layers of {c.num_pages} pages of {c.page_size} positions and of {caches[0].num_pages} of "
+                             f"{caches[0].page_size} share no tables")
+    return layers, caches
+
+
+def _pool_table(page_table: torch.Tensor, name: str, rows: torch.Tensor) -> _lib.G4PageTable:
+    """The C view of a table with one element of ``rows`` (named ``name``) per row."""
+
+    B, M, stride = _page_rows(page_table, name, rows)
+    return _lib.G4PageTable(B, M, stride, page_table.data_ptr())
+
+
+def _refs(refs: torch.Tensor, pages: int | None = None) -> int:
+    if refs.dtype is not _I32 or refs.dim() != 1 or not refs.numel() or not refs.is_contiguous():
+        raise ValueError("refs must be a contiguous, non-empty int32 [P] tensor")
+    if pages is not None and refs.numel() != pages:
+        raise ValueError(f"refs has {refs.numel()} pages, the layers {pages}")
+    return refs.numel()
+
+
+def _indexes(t: torch.Tensor, name: str) -> int:
+    if t.dtype is not _I32 or t.dim() != 1 or not t.numel() or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous, non-empty int32 vector")
+    return t.numel()
+
+
+def _with_workspace(a, size, like: torch.Tensor):
+    need = size(ctypes.byref(a))
+    ws = like.new_empty(need, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    return ws
+
+
+def paged_reserve(refs: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *, page_size: int) -> torch.Tensor:
+    """g4_paged_reserve: fresh pages for the entries of ``page_table [B, M]`` that positions below ``lengths[b]`` need and
+    that hold none, in place, with ``refs [P]`` (all int32). Row by row, the lowest free pages (``refs`` 0) first; returns the
+    number of entries that got none, an int32 ``[1]`` on the device."""
+
+    pages = _refs(refs)
+    table = _pool_table(page_table, "lengths", lengths)
+    dev = _device_of((refs, page_table, lengths))
+    short = refs.new_empty(1)
+    a = _lib.G4PagedReserveArgs(pages, page_size, table, lengths.data_ptr(), refs.data_ptr(), short.data_ptr(), None, 0)
+    lib = _lib.lib()
+    ws = _with_workspace(a, lib.g4_paged_reserve_workspace_size, refs)  # noqa: F841 (held until the launch)
+    _lib.check(lib.g4_paged_reserve(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_reserve")
+    return short
+
+
+def paged_fork(layers, refs: torch.Tensor, page_table: torch.Tensor, parents: torch.Tensor, lengths: torch.Tensor, *,
+               out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """g4_paged_fork: rows that begin as copies of others. Row i of the returned table ``[n, M]`` (``out``, which may be wider or
+    narrower) shares the pages that row ``parents[i]`` (int32 ``[n]``) of ``page_table [B, M]`` fills with its ``lengths[parents[i]]``
+    positions, ``refs`` counting them; the last, partly filled page is a fresh one with its contents copied in all
+    ``layers``. The parents' rows stay (``paged_free`` lets them go). Returns ``(table, shortage)``, the shortage as in
+    ``paged_reserve``."""
+
+    layers, caches = _pool_layers(layers)
+    _refs(refs, caches[0].num_pages)
+    table = _pool_table(page_table, "lengths", lengths)
+    n = _indexes(parents, "parents")
+    dev = _device_of((refs, page_table, parents, lengths, out, *(t for x in layers for t in x)))
+    if out is None:
+        out = refs.new_empty((n, table.max_pages))
+    children = _pool_table(out, "parents", parents)
+    short = refs.new_empty(1)
+    a = _lib.G4PagedForkArgs(ctypes.addressof(caches), len(caches), table, children, parents.data_ptr(), lengths.data_ptr(),
+                             refs.data_ptr(), short.data_ptr(), None, 0)
+    lib = _lib.lib()
+    ws = _with_workspace(a, lib.g4_paged_fork_workspace_size, refs)  # noqa: F841
+    _lib.check(lib.g4_paged_fork(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_fork")
+    return out, short
+
+
+def paged_copy(layers, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """g4_paged_copy: pages ``src[i]`` to ``dst[i]`` (int32 ``[n]``) in all ``layers``. Pairs with a page outside the pool are
+    left out; no page may be the target of two pairs, or of one and the source of another."""
+
+    layers, caches = _pool_layers(layers)
+    n = _indexes(src, "src")
+    if _indexes(dst, "dst") != n:
+        raise ValueError(f"{n} sources and {dst.numel()} targets")
+    dev = _device_of((src, dst, *(t for x in layers for t in x)))
+    _lib.check(_lib.lib().g4_paged_copy(ctypes.addressof(caches), len(caches), n, src.data_ptr(), dst.data_ptr(),
+                                        torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_copy")
+
+
+def paged_free(refs: torch.Tensor, page_table: torch.Tensor, keep: torch.Tensor, *, page_size: int) -> None:
+    """g4_paged_free: row b keeps the pages of its first ``keep[b]`` positions (int32 ``[B]``; 0: none) and lets go of the others,
+    in place: entries -1, ``refs`` one less."""
+
+    pages = _refs(refs)
+    table = _pool_table(page_table, "keep", keep)
+    dev = _device_of((refs, page_table, keep))
+    a = _lib.G4PagedFreeArgs(pages, page_size, table, keep.data_ptr(), refs.data_ptr())
+    _lib.check(_lib.lib().g4_paged_free(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_free")
+
+
+def paged_compact(layers, refs: torch.Tensor, page_table: torch.Tensor) -> torch.Tensor:
+    """g4_paged_compact: the pages in use to the front of the pool, in all ``layers``, with ``refs`` and the entries of
+    ``page_table [B, M]``, which has to hold every entry that ``refs`` counts. Returns their number, an int32 ``[1]`` on the device."""
+
+    layers, caches = _pool_layers(layers)
+    _refs(refs, caches[0].num_pages)
+    B, M, stride = _table_rows(page_table)
+    dev = _device_of((refs, page_table, *(t for x in layers for t in x)))
+    live = refs.new_empty(1)
+    a = _lib.G4PagedCompactArgs(ctypes.addressof(caches), len(caches), _lib.G4PageTable(B, M, stride, page_table.data_ptr()),
+                                refs.data_ptr(), live.data_ptr(), None, 0)
+    lib = _lib.lib()
+    ws = _with_workspace(a, lib.g4_paged_compact_workspace_size, refs)  # noqa: F841
+    _lib.check(lib.g4_paged_compact(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_paged_compact")
+    return live
 
 
 # --- fused decoder-layer glue ------------------------------------------------------------------------

@@ -403,6 +403,101 @@ typedef struct G4PagedReadArgs {
 int g4_paged_read(const G4PagedReadArgs* args, void* stream);
 
 /*
+ * A pool of pages. refs [num_pages] (device) counts the table entries that hold a page: 0 (or less) is a free page. A page
+ * table's rows hold pages as in G4PagedAppendArgs; an entry outside [0, num_pages) holds none. These calls take, share,
+ * copy, give back and move pages on the device, in the stream's order; calls that change the same refs, tables
+ * or pages must be ordered. They allocate nothing and keep no state; workspaces are plain scratch, 16-byte aligned, of
+ * g4_paged_*_workspace_size() bytes.
+ * Fresh pages are handed out in one order: the i-th entry that takes one, row by row, gets the i-th lowest free page, with
+ * refs 1. Where there are too few, the last entries get -1, and *shortage (device int32) is how many; else it is 0.
+ */
+typedef struct G4PageTable {
+  int32_t rows;
+  int32_t max_pages;  /* entries of a row */
+  int64_t stride;     /* elements between rows, >= max_pages */
+  int32_t* entries;   /* device */
+} G4PageTable;
+
+/* Fresh pages for the entries below ceil(lengths[b] / page_size) of every row b that hold none (at most max_pages of
+ * them; lengths[b] <= 0: none). */
+typedef struct G4PagedReserveArgs {
+  int32_t num_pages;
+  int32_t page_size;
+  G4PageTable table;
+  const int32_t* lengths;  /* device [rows] positions that a row shall hold */
+  int32_t* refs;           /* device [num_pages] */
+  int32_t* shortage;       /* device [1] */
+  void* workspace;
+  size_t workspace_bytes;
+} G4PagedReserveArgs;
+
+size_t g4_paged_reserve_workspace_size(const G4PagedReserveArgs* args);
+int g4_paged_reserve(const G4PagedReserveArgs* args, void* stream);
+
+/*
+ * Row i of `out` (all of it is written) becomes a child of row parents[i] of `table`, which holds lengths[parents[i]]
+ * positions: the pages that these fill are shared (refs + 1), the last, partly filled one is a fresh page into which
+ * the 32-slot chunks that hold positions are copied, in every layer; entries behind it are -1. A parent's entry that holds
+ * no page gives -1. parents[i] outside [0, table.rows) gives an empty row. Several children of one parent are the use;
+ * parents' rows stay as they are (g4_paged_free lets them go). `out` must not overlap `table`. Layers share the tables, so
+ * num_pages and page_size; heads, head dims and formats may differ.
+ */
+typedef struct G4PagedForkArgs {
+  const G4PagedCache* layers;  /* host [n_layers] */
+  int32_t n_layers;
+  G4PageTable table;           /* only read */
+  G4PageTable out;
+  const int32_t* parents;      /* device [out.rows] */
+  const int32_t* lengths;      /* device [table.rows] */
+  int32_t* refs;
+  int32_t* shortage;           /* device [1] */
+  void* workspace;
+  size_t workspace_bytes;
+} G4PagedForkArgs;
+
+size_t g4_paged_fork_workspace_size(const G4PagedForkArgs* args);
+int g4_paged_fork(const G4PagedForkArgs* args, void* stream);
+
+/*
+ * Whole pages src[i] -> dst[i] in every layer. A pair with a page outside [0, num_pages), or of one page twice, is left
+ * out. No page may be the target of two pairs, nor the source of one and the target of another: what it would then
+ * hold is not defined. refs and tables stay the caller's.
+ */
+int g4_paged_copy(const G4PagedCache* layers, int32_t n_layers, int32_t pairs, const int32_t* src, const int32_t* dst,
+                  void* stream);
+
+/* Lets go of the entries at and beyond ceil(keep[b] / page_size) of every row b: they become -1 and the pages' refs fall by
+ * one each. keep[b] <= 0: the whole row; more than a row holds: nothing. */
+typedef struct G4PagedFreeArgs {
+  int32_t num_pages;
+  int32_t page_size;
+  G4PageTable table;
+  const int32_t* keep;  /* device [rows] positions that a row keeps */
+  int32_t* refs;
+} G4PagedFreeArgs;
+
+int g4_paged_free(const G4PagedFreeArgs* args, void* stream);
+
+/*
+ * Moves the pages in use to the front of the pool: with n of them, *live = n, and the i-th that lies at n or behind
+ * goes to the i-th free page below n, in every layer, with its refs; the table's entries follow. `table` has to hold every
+ * entry that refs counts (several tables of one pool: as rows of one). Afterwards pages n .. num_pages - 1 are free; what
+ * they hold stays.
+ */
+typedef struct G4PagedCompactArgs {
+  const G4PagedCache* layers;
+  int32_t n_layers;
+  G4PageTable table;
+  int32_t* refs;
+  int32_t* live;  /* device [1] */
+  void* workspace;
+  size_t workspace_bytes;
+} G4PagedCompactArgs;
+
+size_t g4_paged_compact_workspace_size(const G4PagedCompactArgs* args);
+int g4_paged_compact(const G4PagedCompactArgs* args, void* stream);
+
+/*
  * Host-side: KV-sharing map (model.py:153-168). layer_types[i] is 0 (sliding) or 1 (full);
  * out[i] = index of the layer whose K/V layer i uses (itself when not shared).
  */
