@@ -131,6 +131,17 @@ class G4SampleTopKArgs(ctypes.Structure):
     ]
 
 
+class G4VerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int32), ("batch", c_int32), ("drafts", c_int32), ("vocab", c_int32), ("logits", c_void_p),
+        ("batch_stride", c_int64), ("row_stride", c_int64), ("draft_logits", c_void_p),
+        ("draft_batch_stride", c_int64), ("draft_row_stride", c_int64), ("draft_tokens", c_void_p),
+        ("draft_lengths", c_void_p), ("uniforms", c_void_p), ("noise", c_void_p), ("noise_stride", c_int64),
+        ("temperature", c_float), ("token_out", c_void_p), ("count_out", c_void_p), ("logp_out", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 class G4RolloutStepArgs(ctypes.Structure):
     _fields_ = [
         ("batch", c_int32), ("max_new", c_int32), ("step", c_int32), ("pad_id", c_int32), ("n_eos", c_int32),
@@ -226,6 +237,8 @@ PROTOTYPES = {
     "g4_ring_slot_positions": (c_int32, [c_int32, c_int32, POINTER(c_int32)]),
     "g4_sample_tokens": (c_int32, [POINTER(G4SampleArgs), c_void_p]),
     "g4_sample_top_k": (c_int32, [POINTER(G4SampleTopKArgs), c_void_p]),
+    "g4_verify_draft_workspace_size": (c_size_t, [POINTER(G4VerifyArgs)]),
+    "g4_verify_draft": (c_int32, [POINTER(G4VerifyArgs), c_void_p]),
     "g4_softcap_bf16": (c_int32, [c_int64, c_void_p, c_float, c_void_p, c_void_p]),
     "g4_lm_head_sample_workspace_size": (c_size_t, [POINTER(G4LmHeadSampleArgs)]),
     "g4_lm_head_sample": (c_int32, [POINTER(G4LmHeadSampleArgs), c_void_p]),
@@ -308,6 +321,6 @@ def ring_slot_positions(last_written: int, window_capacity: int) -> list[int]:
 __all__ = [
     "G4AppendArgs", "G4DecodeArgs", "G4PrefillArgs", "G4LinearArgs", "G4PrologueArgs", "G4DecodePrep", "G4PagedCache",
     "G4PagedAppendArgs", "G4PagedDecodeArgs", "G4PagedReadArgs", "G4PackedPrefillArgs",
-    "G4PageTable", "G4PagedReserveArgs", "G4PagedForkArgs", "G4PagedFreeArgs", "G4PagedCompactArgs", "G4Error", "PROTOTYPES", "LIB_PATH", "lib", "check", "init_device",
+    "G4PageTable", "G4PagedReserveArgs", "G4PagedForkArgs", "G4PagedFreeArgs", "G4PagedCompactArgs", "G4VerifyArgs", "G4Error", "PROTOTYPES", "LIB_PATH", "lib", "check", "init_device",
     "kv_source_layers", "ring_slot_positions", "c_uint8",
 ]

@@ -895,6 +895,63 @@ def rollout_step(step: int, sampled: torch.Tensor, logp: torch.Tensor, active: t
     _lib.check(_lib.lib().g4_rollout_step(ctypes.byref(a), _stream()), "g4_rollout_step")
 
 
+def _logit_rows(t: torch.Tensor, name: str, shape: tuple) -> tuple[int, int]:
+    """(batch, row) strides of logits ``[B, S, V]`` with contiguous rows; a dim of one element has any stride."""
+
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)} != {shape}")
+    B, S, V = shape
+    batch, row, inner = t.stride()
+    row = row if S > 1 else V
+    batch = batch if B > 1 else S * row
+    if (V > 1 and inner != 1) or row < V or batch < V:
+        raise ValueError(f"{name}: strides {t.stride()} of rows that are not contiguous or overlap")
+    return batch, row
+
+
+def verify_draft(logits: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor | None,
+                 noise: torch.Tensor | None, *, temperature: float, draft_logits: torch.Tensor | None = None,
+                 draft_lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """g4_verify_draft: speculative sampling's verification. ``logits [B, K + 1, V]`` (bf16 or f32, soft-capped) are the
+    target's at the K drafted tokens' positions and behind the last, ``draft_tokens [B, K]`` int32, ``draft_logits
+    [B, K, V]`` (logits' dtype) those they were drawn from, None for drafts that were not drawn (looked up); ``draft_lengths [B]``
+    int32: rows with fewer drafts. Draft s is accepted while ``uniforms[b, s] * q(x) < p(x)``; the next token is ``argmax w /
+    -log(noise[b])`` over the weights left (both f32 in [0, 1), ``[B, K]`` and ``[B, V]``). temperature <= 0: greedy, uniforms and noise not
+    read (None). Returns ``(tokens [B, K + 1], count [B], logp [B, K + 1])``: the accepted drafts, the next token, then
+    -1; the number accepted; log-probabilities under the unscaled logits, 0 behind the last token."""
+
+    if logits.dim() != 3 or logits.shape[1] < 2 or 0 in logits.shape:
+        raise ValueError(f"logits must be a non-empty [B, K + 1, V] tensor, K >= 1, got {tuple(logits.shape)}")
+    B, K, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    code = _code(logits)
+    batch, row = _logit_rows(logits, "logits", (B, K + 1, V))
+    draft_batch = draft_row = 0
+    if draft_logits is not None:
+        if draft_logits.dtype != logits.dtype:
+            raise TypeError(f"draft_logits are {draft_logits.dtype}, logits {logits.dtype}")
+        draft_batch, draft_row = _logit_rows(draft_logits, "draft_logits", (B, K, V))
+    for name, t, dtype, shape in (("draft_tokens", draft_tokens, _I32, (B, K)), ("draft_lengths", draft_lengths, _I32, (B,)),
+                                  ("uniforms", uniforms, _F32, (B, K))):
+        if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)} tensor")
+    noise_stride = 0
+    if noise is not None:
+        if noise.dtype is not _F32 or noise.shape != (B, V) or (V > 1 and noise.stride(1) != 1):
+            raise ValueError(f"noise must be a float32 [{B}, {V}] tensor with unit inner stride")
+        noise_stride = noise.stride(0) if B > 1 else V
+    dev = _device_of((logits, draft_tokens, uniforms, noise, draft_logits, draft_lengths))
+    tokens, logp = draft_tokens.new_empty((B, K + 1)), logits.new_empty((B, K + 1), dtype=_F32)
+    count = draft_tokens.new_empty(B)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    a = _lib.G4VerifyArgs(code, B, K, V, logits.data_ptr(), batch, row, ptr(draft_logits), draft_batch, draft_row,
+                          draft_tokens.data_ptr(), ptr(draft_lengths), ptr(uniforms), ptr(noise), noise_stride,
+                          float(temperature), tokens.data_ptr(), count.data_ptr(), logp.data_ptr(), None, 0)
+    lib = _lib.lib()
+    ws = _with_workspace(a, lib.g4_verify_draft_workspace_size, logits)  # noqa: F841 (held until the launch)
+    _lib.check(lib.g4_verify_draft(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)), "g4_verify_draft")
+    return tokens, count, logp
+
+
 def softcap(x: torch.Tensor, cap: float, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """g4_softcap_bf16: ``bf16(tanh(x / cap) * cap)`` elementwise over a contiguous bf16 tensor (the
     f32 division, tanh and multiply of forward_lm_head's soft-cap); ``out`` may be ``x``."""

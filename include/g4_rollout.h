@@ -574,6 +574,47 @@ typedef struct G4SampleTopKArgs {
 int g4_sample_top_k(const G4SampleTopKArgs* args, void* stream);
 
 /*
+ * g4_verify_draft: of each row's K drafted tokens, how many the target accepts, and the token that follows, from given random
+ * numbers (speculative sampling; no reference counterpart: its decode step takes one token). With p_s and q_s the
+ * softmax of logits[b, s] / temperature and draft_logits[b, s] / temperature over the vocabulary and x_s = draft_tokens[b, s]:
+ *   draft s (s < n = draft_lengths[b], K if NULL) is accepted iff all before it are and uniforms[b, s] * q_s(x_s) < p_s(x_s);
+ *   draft_logits NULL: the drafts were not drawn, q_s(x_s) = 1 (and q_s is 0 elsewhere)
+ *   count = accepted drafts; the weights of the next token are w = max(p_count - q_count, 0) if count < n (p_count where no
+ *   weight is left), else p_count; it is argmax_v w_v / -log(noise[b, v]), ties to the lowest id; noise in [0, 1)
+ *   temperature <= 0: draft s is accepted iff it is the first largest logit's id, and the next token is that id of row count
+ * token_out[b] = the accepted drafts, the next token, then -1; count_out[b] = count; logp_out = the tokens'
+ * log-probabilities under the unscaled logits (f32, 0 behind the last). The logits are soft-capped already. Draft ids outside
+ * the vocabulary are never accepted. Weights that are no numbers are not drawn; with no weight the token is 0.
+ * f32 statistics; workspace of g4_verify_draft_workspace_size() bytes, 16-byte aligned, no state kept in it.
+ */
+typedef struct G4VerifyArgs {
+  int32_t dtype;                  /* of logits and draft_logits: G4_DTYPE_* */
+  int32_t batch;
+  int32_t drafts;                 /* K, 1 .. 63 */
+  int32_t vocab;
+  const void* logits;             /* (b, s): + b * batch_stride + s * row_stride, K + 1 rows of vocab */
+  int64_t batch_stride;
+  int64_t row_stride;
+  const void* draft_logits;       /* K rows of vocab, or NULL */
+  int64_t draft_batch_stride;
+  int64_t draft_row_stride;
+  const int32_t* draft_tokens;    /* device [batch, K] */
+  const int32_t* draft_lengths;   /* device [batch] (clamped to 0 .. K) or NULL */
+  const float* uniforms;          /* device [batch, K]; not read at temperature <= 0 */
+  const float* noise;             /* row b: + b * noise_stride, vocab values; not read at temperature <= 0 */
+  int64_t noise_stride;
+  float temperature;
+  int32_t* token_out;             /* device [batch, K + 1] */
+  int32_t* count_out;             /* device [batch] */
+  float* logp_out;                /* device [batch, K + 1] */
+  void* workspace;
+  size_t workspace_bytes;
+} G4VerifyArgs;
+
+size_t g4_verify_draft_workspace_size(const G4VerifyArgs* args);
+int g4_verify_draft(const G4VerifyArgs* args, void* stream);
+
+/*
  * g4_softcap_bf16: out[i] = cast_bf16(tanh(x[i] / cap) * cap) over n bf16 values, the division,
  * tanh and multiply in f32 -- the soft-cap of forward_lm_head (model.py:676-680) as the samplers
  * apply it. cap finite and > 0; x and out 16-byte aligned (out may alias x).
