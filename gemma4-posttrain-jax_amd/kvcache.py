@@ -239,6 +239,16 @@ class PagedKVCache(NamedTuple):
                              f"{length - self.pad} were processed")
 
 
+def page_counts(capacity: int, window: int, page_size: int) -> tuple[int, int]:
+    """Pages of a row of ``capacity`` positions, and those that a sliding layer's ring takes of them: as many as ``window``
+    positions touch at most."""
+
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    width = (capacity + page_size - 1) // page_size
+    return width, min(width, (window + page_size - 2) // page_size + 1)
+
+
 def init_paged_kv_cache(config: Gemma4TextConfig, batch_size: int, capacity: int, spec: PagedSpec = PagedSpec(),
                         device="cuda") -> PagedKVCache:
     """``init_kv_cache`` in pages: every row gets the pages of ``capacity`` positions on global layers and those
@@ -247,10 +257,7 @@ def init_paged_kv_cache(config: Gemma4TextConfig, batch_size: int, capacity: int
     if batch_size <= 0 or capacity <= 0:
         raise ValueError(f"batch_size and capacity must be positive, got {batch_size} and {capacity}")
     ps = spec.page_size
-    if ps not in PAGE_SIZES:
-        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {ps}")
-    width = (capacity + ps - 1) // ps
-    cycle = min(width, (config.sliding_window + ps - 2) // ps + 1)  # pages that a window touches at most
+    width, cycle = page_counts(capacity, config.sliding_window, ps)
     layers = []
     for i in range(config.num_hidden_layers):
         if is_kv_shared(config, i):
@@ -289,5 +296,5 @@ def init_kv_cache(config: Gemma4TextConfig, batch_size: int, capacity: int, dtyp
 
 
 __all__ = ["LayerKVCache", "KVCache", "PagedLayerCache", "PagedKVCache", "PagedSpec", "PAGE_SIZES", "new_paged_layer",
-           "paged_key_shape", "init_kv_cache", "init_paged_kv_cache", "new_layer_cache", "slot_stride_for", "key_shape",
+           "page_counts", "paged_key_shape", "init_kv_cache", "init_paged_kv_cache", "new_layer_cache", "slot_stride_for", "key_shape",
            "group_keys", "ungroup_keys", "group_values", "ungroup_values", "FULL", "SLIDING"]

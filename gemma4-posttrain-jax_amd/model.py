@@ -95,6 +95,15 @@ class Gemma4TextParams(NamedTuple):
     final_norm: RMSNormParams
 
 
+class PackedPrompts(NamedTuple):
+    """How ``forward_gemma4_text``'s one row of T tokens divides into prompts, each of which fills a row of the cache."""
+
+    starts: torch.Tensor  # [T] int32, the first token of each token's prompt (kernels.packed_starts)
+    rows: torch.Tensor  # [T] the cache row of each token's prompt
+    lengths: torch.Tensor  # [N] int32 tokens per prompt
+    longest: int
+
+
 class Gemma4Output(NamedTuple):
     logits: torch.Tensor  # [B, S', V]
     hidden: torch.Tensor  # [B, S, M]
@@ -409,6 +418,7 @@ def forward_gemma4_text(
     remat_layers: bool = False,
     lora=None,
     write_pos: torch.Tensor | None = None,
+    packed: PackedPrompts | None = None,
 ) -> tuple[torch.Tensor, KVCache | PagedKVCache | None]:
     """model.py:571-673: hidden after the final norm and the updated cache.
 
@@ -444,7 +454,11 @@ def forward_gemma4_text(
     Sliding layers count their window in tokens that the row holds. ``write_pos`` then only asks for
     a step without host-side values, whose token ids and positions are int32 on the device; such a
     step adds to the input cache's ``held`` in place. In a cache without ``held`` an append's place is
-    its ``position_ids``. An append that may find a row full is refused."""
+    its ``position_ids``. An append that may find a row full is refused.
+
+    ``packed`` (prefill into an empty ``PagedKVCache``): ``input_ids [1, T]`` are prompts of different
+    lengths one behind the other, without pads, which attend to themselves
+    (``kernels.packed_prefill_attention``) and fill one cache row each."""
 
     if lora is not None:
         raise NotImplementedError("LoRA adapters are not supported by the native rollout path")
@@ -459,7 +473,16 @@ def forward_gemma4_text(
     paged = isinstance(kv_cache, PagedKVCache)
     if paged and params.embed_tokens.dtype != torch.bfloat16:
         raise ValueError(f"a paged cache needs a bfloat16 model, got {params.embed_tokens.dtype}")
-    if paged:
+    if packed is not None:
+        if not paged or cache_mode != "prefill" or kv_cache.length != 0:
+            raise ValueError('packed prompts need an empty paged cache and cache_mode="prefill"')
+        if B != 1 or packed.starts.shape != (S,) or packed.rows.shape != (S,):
+            raise ValueError(f"packed prompts are one row of T tokens with starts and rows [T], got [{B}, {S}], "
+                             f"{tuple(packed.starts.shape)} and {tuple(packed.rows.shape)}")
+        if packed.lengths.shape != (kv_cache.batch,):
+            raise ValueError(f"{packed.lengths.shape[0]} prompts for a cache of {kv_cache.batch} rows")
+        pad = 0
+    elif paged:
         if attention_mask.dim() != 2 or any(m not in (1, n) for m, n in zip(attention_mask.shape, (B, S))):
             raise ValueError(f"attention_mask {tuple(attention_mask.shape)} does not match [{B}, {S}] tokens")
         attention_mask = attention_mask.expand(B, S)
@@ -503,13 +526,22 @@ def forward_gemma4_text(
         raise ValueError(f'cache_mode="append" requires one token, got {S}')
     length = int(kv_cache.length)
     capacity = kv_cache.capacity if paged else kv_cache.key_mask.shape[1]
-    if S > capacity:
-        raise ValueError(f"{S} tokens do not fit a cache of {capacity} positions")
+    longest = S if packed is None else packed.longest
+    if longest > capacity:
+        raise ValueError(f"{longest} tokens do not fit a cache of {capacity} positions")
     if write_pos is not None and cache_mode != "append":
         raise ValueError("write_pos is only used in append mode")
     if paged:
         tables = {SLIDING: kv_cache.window_table, FULL: kv_cache.page_table}
-        if cache_mode == "prefill":  # token s of a row with n real tokens stands at position s - (S - n)
+        keep = config.sliding_window
+        if packed is not None:  # every token its own row of the append
+            held, keep = packed.lengths, 0
+            tables = {t: table.index_select(0, packed.rows) for t, table in tables.items()}
+            place = torch.arange(S, dtype=torch.int32, device=dev) - packed.starts
+            # a sliding layer stores what the last window holds
+            gone = place < held.index_select(0, packed.rows) - config.sliding_window
+            slots = {FULL: place, SLIDING: place.masked_fill(gone, -1)}
+        elif cache_mode == "prefill":  # token s of a row with n real tokens stands at position s - (S - n)
             held = attention_mask.sum(dim=-1, dtype=torch.int32)
             slot = held - S
         else:
@@ -522,6 +554,8 @@ def forward_gemma4_text(
                 end = held = held + real
             lengths = end * real
             slot = lengths - 1
+        if packed is None:
+            slots = {FULL: slot, SLIDING: slot}
     elif write_pos is not None:
         key_mask = kv_cache.key_mask
         if not fused_prologue:
@@ -572,9 +606,17 @@ def forward_gemma4_text(
                     prompt_kv[i] = (chunk.key, chunk.value_t)
                 else:
                     flags |= flags_q
-                kernels.paged_append(layer_cache, k, v, page_table=tables[lt], write_pos=slot, keep=window, flags=flags,
-                                     k_norm_weight=qk_norms[1], q=q if flags & flags_q else None, q_out=q_out, **prep_q)
-            if cache_mode == "prefill":
+                if packed is not None:
+                    k, v = k.transpose(0, 1), v.transpose(0, 1)
+                    prep_q.update(rope_cos=cos.transpose(0, 1), rope_sin=sin.transpose(0, 1))
+                kernels.paged_append(layer_cache, k, v, page_table=tables[lt], write_pos=slots[lt],
+                                     keep=keep if window else 0, flags=flags, k_norm_weight=qk_norms[1],
+                                     q=q if flags & flags_q else None, q_out=q_out, **prep_q)
+            if packed is not None:
+                attn = kernels.packed_prefill_attention(q_out[0], *prompt_kv[src], packed.starts, window=window)[None]
+                if src not in sources[i + 1:]:
+                    del prompt_kv[src]
+            elif cache_mode == "prefill":
                 attn = kernels.prefill_attention(q_out, *prompt_kv[src], attention_mask.contiguous(), window=window)
                 if src not in sources[i + 1:]:
                     del prompt_kv[src]
@@ -673,7 +715,7 @@ def forward_gemma4_text(
     if scratch_cache:
         return hidden, None
     if paged:
-        return hidden, kv_cache._replace(length=length + S, held=held, pad=pad)
+        return hidden, kv_cache._replace(length=length + longest, held=held, pad=pad)
     return hidden, KVCache(tuple(new_layers), key_mask, length + S)
 
 
@@ -736,7 +778,7 @@ def forward_gemma4_lm(
 
 
 __all__ = [
-    "RMSNormParams", "AttentionParams", "MLPParams", "PerLayerInputParams", "DecoderLayerParams",
+    "PackedPrompts", "RMSNormParams", "AttentionParams", "MLPParams", "PerLayerInputParams", "DecoderLayerParams",
     "Gemma4TextParams", "Gemma4Output", "Gemma4TextConfig", "KVCache", "LayerKVCache", "init_kv_cache",
     "forward_gemma4_text", "forward_gemma4_lm", "forward_lm_head", "checked_softcap", "params_from_numpy", "pack_weights",
     "rms_norm", "layer_head_dim", "layer_kv_heads", "layer_has_v_proj", "layer_intermediate_size",

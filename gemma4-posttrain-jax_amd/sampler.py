@@ -18,9 +18,18 @@ from typing import Any, NamedTuple, Protocol
 import torch
 
 from . import _lib, kernels
-from .config import Gemma4TextConfig
-from .kvcache import KVCache, PagedKVCache, PagedSpec, init_kv_cache, init_paged_kv_cache
-from .model import Gemma4Output, Gemma4TextParams, _proj, checked_softcap, forward_gemma4_lm, forward_gemma4_text
+from .config import FULL, SLIDING, Gemma4TextConfig, is_kv_shared, layer_head_dim, layer_kv_heads
+from .kvcache import KVCache, PagedKVCache, PagedSpec, init_kv_cache, init_paged_kv_cache, new_paged_layer, page_counts
+from .model import (
+    Gemma4Output,
+    Gemma4TextParams,
+    PackedPrompts,
+    _proj,
+    checked_softcap,
+    forward_gemma4_lm,
+    forward_gemma4_text,
+    forward_lm_head,
+)
 
 
 class SamplerConfig(NamedTuple):
@@ -98,6 +107,82 @@ def prefill(
     return forward_gemma4_lm(params, prompt_ids, _position_ids(prompt_mask), config=config,
                              attention_mask=prompt_mask.to(torch.bool), kv_cache=cache, cache_mode="prefill",
                              logits_to_keep=1, lora=lora)
+
+
+def prefill_group(
+    params: Gemma4TextParams,
+    config: Gemma4TextConfig,
+    prompt_ids: torch.Tensor,
+    prompt_mask: torch.Tensor,
+    *,
+    completions: int,
+    max_new_tokens: int,
+    paged: PagedSpec = PagedSpec(),
+    mesh=None,
+    lora=None,
+) -> Gemma4Output:
+    """``prefill`` for ``completions`` rows per prompt (bf16 models): each of the N prompts is encoded once, without its
+    pads, and its cache handed to ``completions`` rows in a row (row ``i * completions + j`` is the j-th of prompt i).
+    Their global layers share the pages that the prompt fills and get pages of their own for its last, partly filled
+    one and for ``max_new_tokens`` tokens; a sliding layer's rings are copied. Returns the logits ``[N *
+    completions, 1, V]``, the packed prompts' hidden states ``[1, T, M]`` and the cache."""
+
+    _no_mesh(mesh)
+    if prompt_ids.dim() != 2 or tuple(prompt_mask.shape) != tuple(prompt_ids.shape):
+        raise ValueError(
+            f"prompt ids/mask must have the same [B, P] shape, got {tuple(prompt_ids.shape)}/{tuple(prompt_mask.shape)}")
+    if max_new_tokens < 0 or completions <= 0:
+        raise ValueError(f"max_new_tokens {max_new_tokens} must be non-negative, completions {completions} positive")
+    if params.embed_tokens.dtype != torch.bfloat16:
+        raise ValueError(f"a paged cache needs a bfloat16 model, got {params.embed_tokens.dtype}")
+    dev, mask = prompt_ids.device, prompt_mask.to(torch.bool)
+    lengths = mask.sum(dim=-1, dtype=torch.int32)
+    host = lengths.tolist()
+    if not host or min(host) == 0:
+        raise ValueError("every prompt needs a token")
+    N, G, ps = len(host), completions, paged.page_size
+    capacity = max(host) + max_new_tokens
+    width, cycle = page_counts(capacity, config.sliding_window, ps)
+    # what the rows hold in the end, and while the prompts' own last pages are still theirs
+    pages = {FULL: sum(n // ps + G * (-(-(n + max_new_tokens) // ps) - n // ps) + 1 for n in host), SLIDING: N * G * cycle}
+    layers = [None if is_kv_shared(config, i) else
+              new_paged_layer(pages[config.layer_types[i]], layer_kv_heads(config, i), layer_head_dim(config, i), ps,
+                              e4m3=paged.e4m3, device=dev) for i in range(config.num_hidden_layers)]
+    of = {t: [x for i, x in enumerate(layers) if x is not None and config.layer_types[i] == t] for t in (FULL, SLIDING)}
+    refs = torch.zeros(pages[FULL], dtype=torch.int32, device=dev)
+    table = torch.full((N, width), -1, dtype=torch.int32, device=dev)
+    kernels.paged_reserve(refs, table, lengths, page_size=ps)
+    entry = torch.arange(width, dtype=torch.int32, device=dev) % cycle
+    rings = torch.arange(N * G, dtype=torch.int32, device=dev)[:, None] * cycle + entry  # a prompt's: its first row's
+
+    cu = torch.cat([lengths.new_zeros(1), lengths.cumsum(0, dtype=torch.int32)])
+    ids = prompt_ids[mask]
+    prompts = torch.arange(N, dtype=torch.int32, device=dev)
+    starts = kernels.packed_starts(cu, ids.numel())
+    places = torch.arange(ids.numel(), dtype=torch.int32, device=dev) - starts
+    packed = PackedPrompts(starts, prompts.repeat_interleave(lengths, output_size=ids.numel()), lengths, max(host))
+    hidden, cache = forward_gemma4_text(params, ids[None], places[None], config=config, lora=lora, packed=packed,
+                                        kv_cache=PagedKVCache(tuple(layers), table, rings[::G].contiguous(), 0))
+    logits = forward_lm_head(params.embed_tokens, hidden[0].index_select(0, cu[1:] - 1)[:, None],
+                             config.final_logit_softcapping)
+
+    parents = prompts.repeat_interleave(G)
+    held = lengths.index_select(0, parents)
+    if of[FULL]:
+        forked, _ = kernels.paged_fork(of[FULL], refs, table, parents, lengths)
+        kernels.paged_free(refs, table, torch.zeros_like(lengths), page_size=ps)
+        kernels.paged_reserve(refs, forked, held + max_new_tokens, page_size=ps)
+    else:  # (its width is the cache's capacity)
+        forked = table.index_select(0, parents)
+    if of[SLIDING] and G > 1:
+        # the ring's places in the order of the row's pages: those of the last window and of the first row's none
+        at = torch.arange(width, dtype=torch.int32, device=dev)
+        live = (at < ((held + ps - 1) // ps)[:, None]) & (at >= ((held - config.sliding_window).clamp(min=0) // ps)[:, None])
+        live &= (torch.arange(N * G, device=dev) % G != 0)[:, None]
+        own = rings.masked_fill(~live, -1)
+        kernels.paged_copy(of[SLIDING], rings[::G].repeat_interleave(G, dim=0).reshape(-1), own.reshape(-1))
+    cache = cache._replace(page_table=forked, window_table=rings, held=held)
+    return Gemma4Output(logits.repeat_interleave(G, dim=0), hidden, cache)
 
 
 def decode_step(
@@ -365,10 +450,13 @@ def generate(
     mesh=None,
     lora=None,
     paged: PagedSpec | None = None,
+    completions: int | None = None,
 ) -> RolloutBatch:
     """sampler.py:204-322: prefill, then up to ``max_new_tokens`` sample + append steps, stopping
     once every row has emitted an EOS id. Inactive rows emit pad with logp 0; the decode on the
-    final step is skipped, so the cache never overflows. ``paged``: the cache in pages (``prefill``)."""
+    final step is skipped, so the cache never overflows. ``paged``: the cache in pages (``prefill``).
+    ``completions`` (with ``paged``): that many rows per prompt, next to each other, which share its encoding and its
+    pages (``prefill_group``); the batch returned has the prompts repeated."""
 
     _no_mesh(mesh)
     sc = sampler_config
@@ -385,8 +473,15 @@ def generate(
     checked_softcap(config.final_logit_softcapping)
 
     prompt_mask = prompt_mask.to(torch.bool)
-    out = prefill(params, config, prompt_ids, prompt_mask, max_new_tokens=sc.max_new_tokens, mesh=mesh, lora=lora,
-                  paged=paged)
+    if completions is not None:
+        if paged is None:
+            raise ValueError("completions of one prompt share its pages: give a PagedSpec")
+        out = prefill_group(params, config, prompt_ids, prompt_mask, completions=completions,
+                            max_new_tokens=sc.max_new_tokens, paged=paged, mesh=mesh, lora=lora)
+        prompt_ids, prompt_mask = (t.repeat_interleave(completions, dim=0) for t in (prompt_ids, prompt_mask))
+    else:
+        out = prefill(params, config, prompt_ids, prompt_mask, max_new_tokens=sc.max_new_tokens, mesh=mesh, lora=lora,
+                      paged=paged)
     dev = prompt_ids.device
     B, N = prompt_ids.shape[0], sc.max_new_tokens
     key_state = key_tensor(key, dev, sc.seed)  # the loop's key, split once per step on the device
@@ -465,9 +560,10 @@ class NativeRollout:
     """sampler.py:325-352 (``PureJaxRollout``): host-side parameter holder around ``generate``."""
 
     def __init__(self, params: Gemma4TextParams, model_config: Gemma4TextConfig, sampler_config: SamplerConfig,
-                 mesh=None, paged: PagedSpec | None = None) -> None:
+                 mesh=None, paged: PagedSpec | None = None, completions: int | None = None) -> None:
         _no_mesh(mesh)
         self.paged = paged
+        self.completions = completions
         self.params = params
         self.model_config = model_config
         self.sampler_config = sampler_config
@@ -478,7 +574,7 @@ class NativeRollout:
 
     def generate(self, prompt_ids: torch.Tensor, prompt_mask: torch.Tensor, *, key=None) -> RolloutBatch:
         return generate(self.params, self.model_config, prompt_ids, prompt_mask, sampler_config=self.sampler_config,
-                        key=key, mesh=self.mesh, paged=self.paged)
+                        key=key, mesh=self.mesh, paged=self.paged, completions=self.completions)
 
 
 PureJaxRollout = NativeRollout  # the reference's class name, for drop-in callers
