@@ -27,42 +27,44 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kSlack = 8.0f;
 
-template <int D, int NB_, int NW_>
+template <int D, int NB_, int NW_, int SLOTS_>
 struct Shape {
-  static constexpr int NB = NB_, NW = NW_;
+  static constexpr int NB = NB_, NW = NW_, SLOTS = SLOTS_;  // chunks of each of K and V^T in LDS
   static constexpr int KS = D / 32;
   static constexpr int T = D / 16;                  // 1 KiB operand tiles of a chunk's K and of its V^T
-  static constexpr int SLOTS = D == 512 ? 2 : 4;    // chunks of each in LDS
   static constexpr int CHUNK = T * 1024;
   static constexpr int TW = T / NW;                 // tiles that a wave fetches of each
   static constexpr int ROWS = NW * NB * 16;         // query rows of a workgroup
   static_assert(T % NW == 0, "the waves share the tiles evenly");
+  static_assert(ROWS * D * 2 <= 2 * SLOTS * CHUNK, "the result goes out through the rings");
 };
 
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v = min(v, __shfl_xor(v, m, 64));
-  return v;
+// Over the 16 columns of an MFMA tile, whose values every row of 16 lanes holds.
+template <typename F>
+__device__ __forceinline__ int columns_reduce(int v, F op) {
+  v = op(v, __builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, true));  // row_ror:8
+  v = op(v, __builtin_amdgcn_update_dpp(v, v, 0x124, 0xf, 0xf, true));  // row_ror:4
+  v = op(v, __builtin_amdgcn_update_dpp(v, v, 0x4e, 0xf, 0xf, true));   // quad_perm:[2,3,0,1]
+  v = op(v, __builtin_amdgcn_update_dpp(v, v, 0xb1, 0xf, 0xf, true));   // quad_perm:[1,0,3,2]
+  return __builtin_amdgcn_readfirstlane(v);
 }
-__device__ __forceinline__ int wave_max(int v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v = max(v, __shfl_xor(v, m, 64));
-  return v;
-}
-__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// The keys [lo, hi] of the wave's rows: this lane's, and over all rows of the wave that have any.
-template <int NB>
+// The wave's rows: row i of column block cb (i = lane % 16) sees the keys [x, y] at LDS address bounds + 8 (16 cb + i).
+// They are read where a chunk is not seen by all rows, and take no registers over the others.
 struct Rows {
-  int lo[NB], hi[NB];
+  uint32_t bounds;
   int first, last;            // the keys that some row sees lie in [first, last]
-  int all_from, all_to;       // every row sees [all_from, all_to]
+  int all_from, all_to;       // every row that sees any sees [all_from, all_to]
   __device__ __forceinline__ bool any(int c) const { return (c << 5) + 31 >= first && (c << 5) <= last; }
   __device__ __forceinline__ bool full(int c) const { return (c << 5) >= all_from && (c << 5) + 31 <= all_to; }
-  // bit e <-> key 32 c + 8 grp + e
-  __device__ __forceinline__ uint32_t bits(int c, int grp, int cb) const {
-    const int k = (c << 5) + 8 * grp;
-    const int from = min(max(lo[cb] - k, 0), 8), to = min(max(hi[cb] - k + 1, 0), 8);  // elements [from, to)
+  __device__ __forceinline__ int2 keys(int cb, int col) const {
+    int2 v;  // (in assembly: the compiler would wait for the DMAs in flight into other LDS)
+    __asm__ volatile("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(v) : "v"(bounds + 8u * (uint32_t)(16 * cb + col)));
+    return v;
+  }
+  // bit e <-> key k + e
+  __device__ static __forceinline__ uint32_t bits(int2 keys, int k) {
+    const int from = min(max(keys.x - k, 0), 8), to = min(max(keys.y - k + 1, 0), 8);  // elements [from, to)
     return (0xffu << from) & ((1u << to) - 1u);
   }
 };
@@ -70,19 +72,22 @@ struct Rows {
 // Softmax of one chunk's scores: `p` as the value product's operand, the row statistics brought forward.
 template <int NB, int VT>
 struct Softmax {
-  float m[NB], ml[NB], l[NB];  // row maximum in use, the same times log2(e), this lane's share of the sum
+  float m[NB], l[NB];  // row maximum in use, this lane's share of the sum
 
   __device__ __forceinline__ void init() {
 #pragma unroll
-    for (int cb = 0; cb < NB; ++cb) m[cb] = kNegInf, ml[cb] = 0.f, l[cb] = 0.f;
+    for (int cb = 0; cb < NB; ++cb) m[cb] = kNegInf, l[cb] = 0.f;
   }
+  // what an exponent subtracts (before the first key, with scores of -inf alone, nothing)
+  __device__ __forceinline__ float base(int cb) const { return m[cb] == kNegInf ? 0.f : m[cb] * kLog2e; }
 
-  __device__ __forceinline__ void chunk(const Rows<NB>& rows, int c, int grp, floatx4 (&acc)[NB][2], bf16x8 (&pop)[NB],
+  __device__ __forceinline__ void chunk(const Rows& rows, int c, int lane, floatx4 (&acc)[NB][2], bf16x8 (&pop)[NB],
                                         floatx4 (&oacc)[NB][VT]) {
     if (!rows.full(c)) {
+      __asm__ volatile("" : "+s"(c));  // hidden: else its place relative to every row advances in registers
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb) {
-        const uint32_t bits = rows.bits(c, grp, cb);
+        const uint32_t bits = Rows::bits(rows.keys(cb, lane & 15), (c << 5) + 8 * (lane >> 4));
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[cb][e >> 2][e & 3] = bits >> e & 1u ? acc[cb][e >> 2][e & 3] : kNegInf;
       }
@@ -103,7 +108,6 @@ struct Softmax {
         // (before the first key m = -inf: nothing to scale yet)
         const float scale = next > m[cb] ? __builtin_amdgcn_exp2f((m[cb] - next) * kLog2e) : 1.f;
         m[cb] = next;
-        ml[cb] = next == kNegInf ? 0.f : next * kLog2e;
         l[cb] *= scale;
 #pragma unroll
         for (int i = 0; i < VT; ++i) oacc[cb][i] *= scale;
@@ -111,10 +115,11 @@ struct Softmax {
     }
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) {
+      const float ml = base(cb);
       float p[8], sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(fmaf(acc[cb][e >> 2][e & 3], kLog2e, -ml[cb]));
+        p[e] = __builtin_amdgcn_exp2f(fmaf(acc[cb][e >> 2][e & 3], kLog2e, -ml));
         sum += p[e];
       }
       l[cb] += sum;
@@ -123,105 +128,118 @@ struct Softmax {
   }
 };
 
-// The values of one column block again, chunk by chunk from memory, with the final row maximum: a chunk whose values
-// are not all finite key by key, so that a row takes only those that it sees. For waves that met such values; speed
-// does not matter.
-template <int D, int NB>
-__device__ __forceinline__ void careful_values(const Rows<NB>& rows, int cb, float ml, const bf16x8 (&qop)[D / 32],
-                                               __amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv,
-                                               floatx4 (&oacc)[D / 16]) {
-  constexpr int KS = D / 32, VT = D / 16;
+// 16 dims of one column block's values again, chunk by chunk from memory, with the final row maximum: a chunk whose
+// values are not all finite key by key, so that a row takes only those that it sees. For waves that met such values: few
+// registers and little code matter here, speed does not (the scores are formed anew for every 16 dims).
+template <int D>
+__device__ __forceinline__ floatx4 careful_values(const Rows& rows, int cb, float ml, const uint16_t* q,
+                                                  __amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv, int i) {
+  constexpr int KS = D / 32;
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const uint32_t k_lane = (uint32_t)(col * 64 + grp * 16), v_lane = vt_operand_bytes(grp, col, D);
-#pragma unroll
-  for (int i = 0; i < VT; ++i) oacc[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int c = rows.first >> 5; c << 5 <= rows.last; ++c) {
     floatx4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 1
+    for (int s = 0; s < KS; ++s) {
+      const bf16x8 qs = as_bf16x8(q ? load16(q + 32 * s + 8 * grp) : u32x4{0u, 0u, 0u, 0u});
 #pragma unroll
-    for (int t = 0; t < 2 * KS; ++t) {
-      const u32x4 k = buffer_load16(rk, k_lane, (uint32_t)c * (uint32_t)(64 * D) + (uint32_t)(2 * (t % KS) + t / KS) * 1024u);
-      acc[t / KS] = mfma16x16x32(as_bf16x8(k), qop[t % KS], acc[t / KS]);
+      for (int bb = 0; bb < 2; ++bb)
+        acc[bb] = mfma16x16x32(as_bf16x8(buffer_load16(rk, k_lane, (uint32_t)c * (uint32_t)(64 * D) + (uint32_t)(2 * s + bb) * 1024u)),
+                               qs, acc[bb]);
     }
     uint32_t seen = 0;  // bit k <-> key 32 c + k
 #pragma unroll
-    for (int g = 0; g < 4; ++g) seen |= rows.bits(c, g, cb) << (8 * g);
+    for (int g = 0; g < 4; ++g) seen |= Rows::bits(rows.keys(cb, col), (c << 5) + 8 * g) << (8 * g);
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       p[e] = seen >> (8 * grp + e) & 1u ? __builtin_amdgcn_exp2f(fmaf(acc[e >> 2][e & 3], kLog2e, -ml)) : 0.f;
     const u32x4 pop = pack8(p);
+    const u32x4 v = buffer_load16(rv, v_lane, (uint32_t)c * (uint32_t)(64 * D) + 256u * i);
+    bool odd = false;
 #pragma unroll
-    for (int i = 0; i < VT; ++i) {
-      const u32x4 v = buffer_load16(rv, v_lane, (uint32_t)c * (uint32_t)(64 * D) + 256u * i);
-      bool odd = false;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) odd |= (v[q] & 0x7f80u) == 0x7f80u || (v[q] & 0x7f800000u) == 0x7f800000u;
-      if (!__any(odd)) {
-        oacc[i] = mfma16x16x32(as_bf16x8(v), as_bf16x8(pop), oacc[i]);
-        continue;
-      }
+    for (int q = 0; q < 4; ++q) odd |= (v[q] & 0x7f80u) == 0x7f80u || (v[q] & 0x7f800000u) == 0x7f800000u;
+    if (!__any(odd)) {
+      o = mfma16x16x32(as_bf16x8(v), as_bf16x8(pop), o);
+      continue;
+    }
 #pragma unroll 1
-      for (int k = 0; k < 32; ++k) {  // this key alone
-        u32x4 keep;
+    for (int k = 0; k < 32; ++k) {  // this key alone
+      u32x4 keep;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) keep[q] = k >> 3 == grp && (k & 7) >> 1 == q ? (k & 1 ? 0xffff0000u : 0xffffu) : 0u;
-        const floatx4 sum = mfma16x16x32(as_bf16x8(v & keep), as_bf16x8(pop & keep), oacc[i]);
-        if (seen >> k & 1u) oacc[i] = sum;
-      }
+      for (int q = 0; q < 4; ++q) keep[q] = k >> 3 == grp && (k & 7) >> 1 == q ? (k & 1 ? 0xffff0000u : 0xffffu) : 0u;
+      const floatx4 sum = mfma16x16x32(as_bf16x8(v & keep), as_bf16x8(pop & keep), o);
+      if (seen >> k & 1u) o = sum;
     }
   }
+  return o;
+}
+
+// Which block of rows and head workgroup i takes. Workgroups are dealt to the 8 XCDs round robin: runs of kRun consecutive
+// blocks of a head, which read the same keys, go to one XCD and its L2, the latest tokens' first (whose keys are the most).
+constexpr int kXcds = 8, kRun = 4;
+__device__ __forceinline__ void place_block(int i, int n_blk, int H, int& blk, int& h) {
+  const int even = n_blk * H / (kXcds * kRun) * (kXcds * kRun);  // as many as fill whole turns of runs
+  int u = i;
+  if (i < even) {
+    const int x = i % kXcds, j = i / kXcds;
+    u = ((j / kRun) * kXcds + x) * kRun + j % kRun;
+  }
+  // u in the order (run of blocks, head, block of the run); the last run may be short
+  const int run = u / (kRun * H), rest = u - run * kRun * H, len = min(kRun, n_blk - run * kRun);
+  h = rest / len;
+  blk = n_blk - 1 - (run * kRun + rest - h * len);
 }
 
 // Waves of the two halves of a workgroup (those that share a SIMD) are half a step apart, as in
 // prefill_bf16_lds_kernel: one runs the MFMAs (the values of chunk c - 1, then the scores of chunk c), at raised
 // priority, while the other runs the softmax of a chunk. Chunks of which a wave sees nothing it skips.
-template <int D, int NB, int NW>
-__global__ __launch_bounds__(NW * 64) void packed_prefill_kernel(G4PackedPrefillArgs a) {
-  using S = Shape<D, NB, NW>;
-  constexpr int KS = S::KS, VT = S::T, SLOTS = S::SLOTS;
+template <int D, int NB, int NW, int SLOTS>
+__global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPrefillArgs a) {
+  using S = Shape<D, NB, NW, SLOTS>;
+  constexpr int KS = S::KS, VT = S::T;
   // read with inline-assembly LDS reads only: the compiler adds no waits of its own for the DMAs in flight
   __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * SLOTS][S::CHUNK];
-  __shared__ int2 spans[NW];
+  __shared__ int2 spans[NW], bounds[NW * NB * 16];
 
   const int R = a.group, H = a.kv_heads, T = a.tokens;
   const int n_blk = (int)(gridDim.x / (unsigned)H);
-  // the latest tokens first, whose keys are the most
-  const int blk = n_blk - 1 - (int)(blockIdx.x / (unsigned)H), h = (int)(blockIdx.x % (unsigned)H);
+  int blk, h;
+  place_block((int)blockIdx.x, n_blk, H, blk, h);
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row0 = blk * S::ROWS + w * (NB * 16);
 
-  Rows<NB> rows;
-  bool row_ok[NB], has_keys[NB];
+  Rows rows{lds_addr(&bounds[w * NB * 16]), 0x7fffffff, -1, 0, 0x7fffffff};
   bf16x8 qop[NB][KS];
-  rows.first = 0x7fffffff, rows.last = -1, rows.all_from = 0, rows.all_to = 0x7fffffff;
 #pragma unroll
   for (int cb = 0; cb < NB; ++cb) {
+    // rows behind the last token read the last row and are not stored
     const int row = row0 + cb * 16 + col, t = row / R;
-    row_ok[cb] = t < T;
-    const int start = row_ok[cb] ? a.starts[t] : -1;
-    has_keys[cb] = start >= 0 && start <= t;
-    rows.lo[cb] = has_keys[cb] ? max(start, a.window > 0 ? t - a.window + 1 : 0) : 0;
-    rows.hi[cb] = has_keys[cb] ? t : -1;
-    if (has_keys[cb]) {
-      rows.first = min(rows.first, rows.lo[cb]);
-      rows.last = max(rows.last, rows.hi[cb]);
-      rows.all_from = max(rows.all_from, rows.lo[cb]);
-      rows.all_to = min(rows.all_to, rows.hi[cb]);
-    }
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (((int64_t)t * H + h) * R + (row - t * R)) * D;
+    const int64_t at = (int64_t)min(row, T * R - 1);  // flat over (t, r) of a head
+    const int tq = min(t, T - 1);
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (at + ((int64_t)tq * (H - 1) + h) * R) * D;
+    const int start = a.starts[tq];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      u32x4 v = {0u, 0u, 0u, 0u};
-      if (has_keys[cb]) v = load16(q + 32 * s + 8 * grp);
-      qop[cb][s] = as_bf16x8(v);
+    for (int s = 0; s < KS; ++s) qop[cb][s] = as_bf16x8(load16(q + 32 * s + 8 * grp));
+    const bool has_keys = t < T && start >= 0 && start <= t;
+    const int lo = has_keys ? max(start, a.window > 0 ? t - a.window + 1 : 0) : 0, hi = has_keys ? t : -1;
+    if (grp == 0) bounds[(w * NB + cb) * 16 + col] = make_int2(lo, hi);
+    if (has_keys) {
+      rows.first = min(rows.first, lo);
+      rows.last = max(rows.last, hi);
+      rows.all_from = max(rows.all_from, lo);
+      rows.all_to = min(rows.all_to, hi);
     }
   }
-  rows.first = __builtin_amdgcn_readfirstlane(wave_min(rows.first));
-  rows.last = __builtin_amdgcn_readfirstlane(wave_max(rows.last));
-  rows.all_from = __builtin_amdgcn_readfirstlane(wave_max(rows.all_from));
-  rows.all_to = __builtin_amdgcn_readfirstlane(wave_min(rows.all_to));
+  const auto least = [](int x, int y) { return min(x, y); };
+  const auto most = [](int x, int y) { return max(x, y); };
+  rows.first = columns_reduce(rows.first, least);
+  rows.last = columns_reduce(rows.last, most);
+  rows.all_from = columns_reduce(rows.all_from, most);
+  rows.all_to = columns_reduce(rows.all_to, least);
   // the q operands have landed here, not inside the loop, where their wait would drain the DMAs in flight
 #pragma unroll
   for (int cb = 0; cb < NB; ++cb)
@@ -296,51 +314,73 @@ __global__ __launch_bounds__(NW * 64) void packed_prefill_kernel(G4PackedPrefill
       if (c + SLOTS - 1 <= c_end) issue_k(c + SLOTS - 1, (i + SLOTS - 1) & (SLOTS - 1));
       if (c + SLOTS - 2 <= c_end) issue_v(c + SLOTS - 2, SLOTS + ((i + SLOTS - 2) & (SLOTS - 1)));
       const bool before = c > c_begin && rows.any(c - 1), now = rows.any(c);
-      if (!lead && before) soft.chunk(rows, c - 1, grp, acc, pop, oacc);
+      if (!lead && before) soft.chunk(rows, c - 1, lane, acc, pop, oacc);
       __builtin_amdgcn_s_setprio(1);
       if (before) pf_pv<VT, NB, 4>(ring0 + (uint32_t)((SLOTS + ((i - 1) & (SLOTS - 1))) * S::CHUNK), pop, oacc);
       if (now) pf_qk<VT, KS, NB, 4>(ring0 + (uint32_t)((i & (SLOTS - 1)) * S::CHUNK), qop, acc);
       __builtin_amdgcn_s_setprio(0);
-      if (lead && now) soft.chunk(rows, c, grp, acc, pop, oacc);
+      if (lead && now) soft.chunk(rows, c, lane, acc, pop, oacc);
     }
     wait_vmcnt<0>();
     wg_barrier();
     if (rows.any(c_end)) {
-      if (!lead) soft.chunk(rows, c_end, grp, acc, pop, oacc);
+      if (!lead) soft.chunk(rows, c_end, lane, acc, pop, oacc);
       pf_pv<VT, NB, 4>(ring0 + (uint32_t)((SLOTS + ((c_end - c_begin) & (SLOTS - 1))) * S::CHUNK), pop, oacc);
     }
   }
 
-  const auto store = [&](int cb, const floatx4 (&o)[VT]) {
-    const float l = column_sum(soft.l[cb]);
-    const float inv = has_keys[cb] && l != 0.f ? 1.0f / l : 0.f;
-    if (!row_ok[cb]) return;
-    const int row = row0 + cb * 16 + col, t = row / R;
-    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (((int64_t)t * H + h) * R + (row - t * R)) * D;
-#pragma unroll
-    for (int i = 0; i < VT; ++i) {
-      const floatx4 x = inv == 0.f ? floatx4{0.f, 0.f, 0.f, 0.f} : o[i] * inv;
-      *reinterpret_cast<uint2*>(out + 16 * i + 4 * grp) = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-    }
-  };
+  // The result through LDS (the rings are done with), where the lanes' 4-dim pieces become whole rows: 16 bytes a lane,
+  // a row's 16-byte units turned by its number so that neither side meets a bank twice. The rows' places are computed afresh (the
+  // lane is hidden from the compiler), not kept in registers since the q loads.
+  constexpr int UNITS = D / 8, RPI = 64 / UNITS;  // 16-byte units of a row, rows per store instruction
+  wg_barrier();
+  unsigned char* mine = &ring[0][0] + w * (NB * 16 * D * 2);
+  int lane_o = lane;
+  __asm__ volatile("" : "+v"(lane_o));
 #pragma unroll
   for (int cb = 0; cb < NB; ++cb) {
-    float sum = 0.f;  // not finite where an accumulator is not: 0 x is 0 or NaN
+    const float l = column_sum(soft.l[cb]);
+    const int row = row0 + cb * 16 + (lane_o & 15), t = row / R;
+    const bool none = rows.keys(cb, lane_o & 15).y < 0 || l == 0.f;
+    const float inv = none ? 0.f : 1.0f / l;
+    const auto store = [&](int i, floatx4 x) {
+      x = none ? floatx4{0.f, 0.f, 0.f, 0.f} : x * inv;
+      const int r = lane_o & 15, unit = (2 * i + (lane_o >> 5)) ^ (r & (UNITS - 1));
+      *reinterpret_cast<uint2*>(mine + (cb * 16 + r) * (D * 2) + unit * 16 + (lane_o >> 4 & 1) * 8) =
+          make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+    };
+    float sum = 0.f;  // not 0 where an accumulator is not finite: 0 x is 0 or NaN
 #pragma unroll
     for (int i = 0; i < VT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum = fmaf(oacc[cb][i][e], 0.f, sum);
-    if (__any(!(sum == 0.f))) careful_values<D, NB>(rows, cb, soft.ml[cb], qop[cb], rk, rv, oacc[cb]);
-    store(cb, oacc[cb]);
+    if (__any(!(sum == 0.f))) {
+      const uint16_t* q = t < T ? reinterpret_cast<const uint16_t*>(a.q) + (((int64_t)t * H + h) * R + (row - t * R)) * D : nullptr;
+#pragma unroll 1
+      for (int i = 0; i < VT; ++i) store(i, careful_values<D>(rows, cb, soft.base(cb), q, rk, rv, i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < VT; ++i) store(i, oacc[cb][i]);
+    }
+    __builtin_amdgcn_wave_barrier();  // (a wave's rows are its own: its LDS operations keep their order)
+#pragma unroll
+    for (int i = 0; i < 16 / RPI; ++i) {
+      const int r = i * RPI + lane_o / UNITS, unit = lane_o % UNITS;
+      const int to = __shfl(t, r, 64), g = row0 + cb * 16 + r;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(mine + (cb * 16 + r) * (D * 2) + (unit ^ (r & (UNITS - 1))) * 16);
+      if (to < T)
+        __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(a.out) +
+                                                                 (((int64_t)to * H + h) * R + (g - to * R)) * D + unit * 8));
+    }
   }
 }
 
 template <int D>
 int launch_packed(const G4PackedPrefillArgs& a, hipStream_t st) {
-  using S = Shape<D, D == 512 ? 1 : 2, D == 64 ? 4 : 8>;
+  using S = Shape<D, D == 512 ? 1 : 2, D == 512 ? 8 : 4, 2>;
   const int64_t blocks = ((int64_t)a.tokens * a.group + S::ROWS - 1) / S::ROWS * a.kv_heads;
   if (blocks * S::NW * 64 > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "g4_packed_prefill_attention: too many tokens");
-  hipLaunchKernelGGL((packed_prefill_kernel<D, S::NB, S::NW>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a);
+  hipLaunchKernelGGL((packed_prefill_kernel<D, S::NB, S::NW, S::SLOTS>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a);
   return check_launch("g4_packed_prefill_attention");
 }
 
