@@ -6,8 +6,9 @@
 // but for near ties.
 //
 // Bound by reading the logits: K + 1 target and K draft rows of the vocabulary once, for their maxima and sums of
-// exponentials (statistics per chunk of a row), then of two rows per b and the noise for the race. Which rows these are
-// every workgroup of the second launch finds from the statistics by itself.
+// exponentials (a first launch, statistics per chunk of a row), then of two rows per b and the noise for the race (a
+// third). Which rows these are a launch between finds from the statistics; it also clears the counter by which the last of
+// a b's workgroups in the race, which writes the token, is found.
 #include "g4_common.h"
 #include "g4_internal.h"
 
@@ -28,25 +29,34 @@ struct Stats {  // of a chunk of a row, or of a row
   float unit;  // sum exp(x - m)
   int idx;     // kGreedy: the first column of the largest
 };
-struct Decision {
-  int count;        // accepted drafts
-  float m, unit;    // of the row that the last token is drawn from
-  int token;        // kGreedy: the token
+struct Decision {  // of one b
+  int count;           // accepted drafts
+  int32_t away;        // rejected without a drafter's logits: the draft's id, which has no weight; else -1
+  int32_t residual;    // whether the drafter's row counts
+  float unit;          // of the target's row: sum exp(x - m)
+  float pm, pz, qm, qz;  // largest logit and sum exp((x - m) / temperature) of both rows
 };
 struct VerifyWorkspace {
-  Stats* stats;      // [batch][rows][splits], the K + 1 target rows first
-  uint64_t* race;    // [batch][splits][2] the best of the residual weights and of p
-  Decision* made;    // [batch]
+  Stats* stats;       // [batch][rows][splits], the K + 1 target rows first
+  Decision* made;     // [batch]
+  uint64_t* best;     // [batch][splits of the race] the workgroups' best
+  uint32_t* arrived;  // [batch * kApart] workgroups that have brought theirs, a cache line each
 };
+constexpr int kApart = 32;  // (counters that share lines: the race of 64 rows 51 us instead of 27)
 
-int chunk_of(const G4VerifyArgs& a) {
+// Logits per workgroup: in the first launch 2^13 where that makes 2048 workgroups or more, else 2^12 (one row of 9 x 262144
+// is 576 of them); in the race 2^12. us per call, first launch / race in vectors of 8 per thread: 64 rows of 9 x 262144
+// 105 (8 / 4), 98 (4 / 2), 101 (8 / 2), 102 (4 / 4), 100 (4 / 1); one row 13.3 (2 / 1), 13.0 (2 / 2), 15.0 (1 / 1).
+constexpr int kLong = 4, kShort = 2;  // vectors of 8 per thread
+constexpr int kRace = 2;              // in the race
+int vecs_of(const G4VerifyArgs& a) {
   const int64_t rows = (int64_t)a.batch * (a.drafts + 1 + (a.draft_logits ? a.drafts : 0));
-  return rows * a.vocab >= 2048LL * 16384 ? 16384 : 4096;
+  return rows * a.vocab >= 2048LL * kLong * 8 * kThreads ? kLong : kShort;
 }
-int splits_of(const G4VerifyArgs& a) { return (int)(((int64_t)a.vocab + chunk_of(a) - 1) / chunk_of(a)); }
+int splits_of(const G4VerifyArgs& a, int vecs) { return (int)(((int64_t)a.vocab + vecs * 8 * kThreads - 1) / (vecs * 8 * kThreads)); }
 
 size_t carve(VerifyWorkspace& w, void* base, const G4VerifyArgs& a) {
-  const int64_t splits = splits_of(a);
+  const int64_t splits = splits_of(a, vecs_of(a));
   size_t at = 0;
   const auto take = [&](int64_t bytes) {
     void* p = base ? static_cast<char*>(base) + at : nullptr;
@@ -54,28 +64,31 @@ size_t carve(VerifyWorkspace& w, void* base, const G4VerifyArgs& a) {
     return p;
   };
   w.stats = static_cast<Stats*>(take(a.batch * (2LL * a.drafts + 1) * splits * (int64_t)sizeof(Stats)));
-  w.race = static_cast<uint64_t*>(take(a.batch * splits * 16));
   w.made = static_cast<Decision*>(take(a.batch * (int64_t)sizeof(Decision)));
+  w.best = static_cast<uint64_t*>(take(a.batch * (int64_t)splits_of(a, kRace) * 8));
+  w.arrived = static_cast<uint32_t*>(take(a.batch * 4LL * kApart));
   return at;
 }
 
 // --- logits ----------------------------------------------------------------------------------------------------
 
-template <typename T>
-struct Unaligned {
-  T v;
-} __attribute__((packed, aligned(2)));
+typedef u32x4 u32x4_anywhere __attribute__((aligned(2)));
 
 // 8 logits from p on, of which `n` are there (others -inf). Rows stand at any element: such loads need no alignment.
-template <bool BF16>
+// NT: past the caches (the first launch where it is long: 98 -> 94 us; short ones lose up to 1 us by it).
+template <bool BF16, bool NT = false>
 __device__ __forceinline__ void load8(const void* row, int64_t i, int n, float (&x)[8]) {
+  const auto load = [](const void* p) {
+    const u32x4_anywhere* q = static_cast<const u32x4_anywhere*>(p);
+    return NT ? __builtin_nontemporal_load(q) : *q;
+  };
   if (n >= 8) {
     if constexpr (BF16) {
-      unpack8(reinterpret_cast<const Unaligned<u32x4>*>(static_cast<const uint16_t*>(row) + i)->v, x);
+      unpack8(load(static_cast<const uint16_t*>(row) + i), x);
     } else {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const u32x4 v = reinterpret_cast<const Unaligned<u32x4>*>(static_cast<const float*>(row) + i + 4 * j)->v;
+        const u32x4 v = load(static_cast<const float*>(row) + i + 4 * j);
 #pragma unroll
         for (int q = 0; q < 4; ++q) x[4 * j + q] = __uint_as_float(v[q]);
       }
@@ -112,32 +125,49 @@ struct Heat {
   }
 };
 
-template <int MODE>
-__device__ __forceinline__ void join(Stats& s, const Stats& o, float c) {
-  if (MODE == kGreedy && (o.m > s.m || (o.m == s.m && o.idx < s.idx))) s.idx = o.idx;
-  const float top = fmaxf(s.m, o.m), m = fmaxf(top, kF32Min);  // (m finite where there is no logit but -inf)
-  const float a = s.m - m, b = o.m - m;
-  if (MODE != kGreedy) s.heat = s.heat * __builtin_amdgcn_exp2f(a * c) + o.heat * __builtin_amdgcn_exp2f(b * c);
-  if (MODE != kUnit) s.unit = s.unit * __builtin_amdgcn_exp2f(a * kLog2e) + o.unit * __builtin_amdgcn_exp2f(b * kLog2e);
-  s.m = top;
-}
+// exp2(x c - m c) with one fma per x, for |m| below 1e30 (else m c may pass f32): the rounding of m c, alike for every x of a
+// sum, is made up for once, by `rest`.
+struct Below {
+  float c, mc, rest;
+  __device__ __forceinline__ Below(float m, float c_) : c(c_), mc(m * c_), rest(__builtin_amdgcn_exp2f(-fmaf(m, c_, -mc))) {}
+  __device__ __forceinline__ float exp(float x) const { return __builtin_amdgcn_exp2f(fmaf(x, c, -mc)); }
+};
 
+// A wave's statistics from its lanes', in every lane. (m is finite in the differences where there is no logit but -inf.)
 template <int MODE>
 __device__ __forceinline__ Stats wave_join(Stats s, float c) {
+  const float top = wave_max(s.m), d = s.m - fmaxf(top, kF32Min);
+  if (MODE == kGreedy) {
+    int idx = s.m == top ? s.idx : kNoColumn;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    Stats o;
-    o.m = __shfl_xor(s.m, d, 64);
-    o.heat = MODE != kGreedy ? __shfl_xor(s.heat, d, 64) : 0.f;
-    o.unit = MODE != kUnit ? __shfl_xor(s.unit, d, 64) : 0.f;
-    o.idx = MODE == kGreedy ? __shfl_xor(s.idx, d, 64) : 0;
-    join<MODE>(s, o, c);
+    for (int i = 32; i; i >>= 1) idx = min(idx, __shfl_xor(idx, i, 64));
+    s.idx = idx;
   }
-  if (MODE == kUnit) s.unit = s.heat;
+  if (MODE != kGreedy) s.heat = wave_sum(s.heat * __builtin_amdgcn_exp2f(d * c));
+  if (MODE != kUnit) s.unit = wave_sum(s.unit * __builtin_amdgcn_exp2f(d * kLog2e));
+  s.m = top;
   return s;
 }
 
 // --- first launch: a chunk's statistics ------------------------------------------------------------------------------
+
+template <int VECS>
+__device__ __forceinline__ float sum_exp(const float (&x)[VECS][8], float m, float c) {
+  float sum = 0.f;
+  if (fabsf(m) < 1e30f) {
+    const Below below(m, c);
+#pragma unroll
+    for (int v = 0; v < VECS; ++v)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += below.exp(x[v][e]);
+    return sum * below.rest;
+  }
+#pragma unroll
+  for (int v = 0; v < VECS; ++v)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += __builtin_amdgcn_exp2f((x[v][e] - m) * c);
+  return sum;
+}
 
 template <bool BF16, int MODE, int VECS>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(G4VerifyArgs a, VerifyWorkspace w, int rows, int splits) {
@@ -154,7 +184,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(G4VerifyArgs a, 
 #pragma unroll
   for (int v = 0; v < VECS; ++v) {
     const int64_t i = i0 + v * (kThreads * 8);
-    load8<BF16>(row, i, (int)min((int64_t)8, a.vocab - i), x[v]);
+    load8<BF16, VECS == kLong>(row, i, (int)min((int64_t)8, a.vocab - i), x[v]);
   }
   Stats s{-__builtin_inff(), 0.f, 0.f, kNoColumn};
 #pragma unroll
@@ -165,42 +195,42 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(G4VerifyArgs a, 
       s.m = fmaxf(s.m, x[v][e]);
     }
   const float m = fmaxf(s.m, kF32Min);
-#pragma unroll
-  for (int v = 0; v < VECS; ++v)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float t = x[v][e] - m;
-      if (MODE != kGreedy) s.heat += __builtin_amdgcn_exp2f(t * c);
-      if (MODE != kUnit) s.unit += __builtin_amdgcn_exp2f(t * kLog2e);
-    }
+  if (MODE != kGreedy) s.heat = sum_exp<VECS>(x, m, c);
+  if (MODE != kUnit && !draft) s.unit = sum_exp<VECS>(x, m, kLog2e);  // (the log-probabilities are the target's)
   s = wave_join<MODE>(s, c);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-#pragma unroll
-    for (int i = 1; i < kWaves; ++i) join<MODE>(s, part[i], c);
+  if (threadIdx.x < 64) {
+    static_assert(kWaves == 4, "lanes 0 .. 3 hold the waves'");
+    s = wave_join<MODE>(threadIdx.x < kWaves ? part[threadIdx.x] : Stats{-__builtin_inff(), 0.f, 0.f, kNoColumn}, c);
     if (MODE == kUnit) s.unit = s.heat;
-    w.stats[((int64_t)b * rows + r) * splits + split] = s;
+    if (threadIdx.x == 0) w.stats[((int64_t)b * rows + r) * splits + split] = s;
   }
 }
 
 // --- which drafts are accepted ------------------------------------------------------------------------------------------
 
-// The rows' statistics from their chunks' (by all waves, rows in turns; a wave's lanes take the chunks).
+// The rows' statistics from their chunks' (the waves take rows in turns, a wave's lanes the chunks).
 template <int MODE>
 __device__ __forceinline__ void join_rows(const G4VerifyArgs& a, const VerifyWorkspace& w, int b, int rows, int splits, int n,
                                           Stats* out) {
   const int lane = threadIdx.x & 63;
   const float c = kLog2e / a.temperature;
-  for (int r = threadIdx.x >> 6; r < rows; r += kWaves) {
-    if (r > a.drafts ? r - a.drafts - 1 >= n : r > n) continue;
-    Stats s{-__builtin_inff(), 0.f, 0.f, kNoColumn};
-    for (int i = lane; i < splits; i += 64) {
-      const Stats o = w.stats[((int64_t)b * rows + r) * splits + i];
-      join<MODE>(s, o, c);
+  const Stats none{-__builtin_inff(), 0.f, 0.f, kNoColumn};
+  const auto reached = [&](int r) { return r < rows && (r > a.drafts ? r - a.drafts - 1 < n : r <= n); };
+  const auto load = [&](int r, int i) { return reached(r) && i < splits ? w.stats[((int64_t)b * rows + r) * splits + i] : none; };
+  int r = threadIdx.x >> 6;
+  Stats s = load(r, lane);
+  for (; r < rows; r += kWaves) {
+    const Stats next = load(r + kWaves, lane);
+    Stats all = wave_join<MODE>(s, c);
+    for (int i = 64; i < splits; i += 64) {  // (joined pairwise: lane 0 the ones before)
+      const Stats more = wave_join<MODE>(load(r, i + lane), c);
+      all = wave_join<MODE>(lane == 0 ? all : lane == 1 ? more : none, c);
     }
-    s = wave_join<MODE>(s, c);
-    if (lane == 0) out[r] = s;
+    if (MODE == kUnit) all.unit = all.heat;
+    if (lane == 0 && reached(r)) out[r] = all;
+    s = next;
   }
   __syncthreads();
 }
@@ -208,26 +238,44 @@ __device__ __forceinline__ void join_rows(const G4VerifyArgs& a, const VerifyWor
 // The log-probability of column i of a row under the unscaled logits.
 __device__ __forceinline__ float log_prob(float x, const Stats& s) { return (x - s.m) - logf(s.unit); }
 
+// What deciding a draft takes from memory but the statistics (lane s: draft s), asked for before they are joined.
+struct Draft {
+  int id;
+  float x, y, u;  // target's and drafter's logit, the random number
+  bool there;     // an id of the vocabulary
+};
+template <bool BF16, int MODE>
+__device__ __forceinline__ Draft load_draft(const G4VerifyArgs& a, int b, int n) {
+  const int s = threadIdx.x & 63;
+  Draft d{0, 0.f, 0.f, 0.f, false};
+  if (s >= n) return d;
+  d.id = a.draft_tokens[(int64_t)b * a.drafts + s];
+  if constexpr (MODE != kGreedy) d.u = a.uniforms[(int64_t)b * a.drafts + s];
+  d.there = (uint32_t)d.id < (uint32_t)a.vocab;
+  if (!d.there) return d;
+  d.x = logit<BF16>(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, s), d.id);
+  if (MODE != kGreedy && a.draft_logits)
+    d.y = logit<BF16>(row_at<BF16>(a.draft_logits, a.draft_batch_stride, a.draft_row_stride, b, s), d.id);
+  return d;
+}
+
 // How many drafts are accepted (by the first wave; lane s decides draft s).
 template <bool BF16, int MODE>
-__device__ __forceinline__ int accepted(const G4VerifyArgs& a, int b, int n, const Stats* st) {
+__device__ __forceinline__ int accepted(const G4VerifyArgs& a, const Heat& heat, int n, const Draft& d, const Stats* st) {
   const int s = threadIdx.x & 63;
   bool good = false;
   if (s < n) {
-    const int d = a.draft_tokens[(int64_t)b * a.drafts + s];
     if constexpr (MODE == kGreedy) {
-      good = d == st[s].idx;
-    } else if ((uint32_t)d < (uint32_t)a.vocab) {
-      const double c = 1.0 / (double)a.temperature;
-      const float x = logit<BF16>(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, s), d);
-      const double p = exp(((double)x - st[s].m) * c) / (double)st[s].heat;
-      double q = 1.0;
+      good = d.id == st[s].idx;
+    } else if (d.there) {
+      const float p = heat.exp(d.x - st[s].m);
+      // u q < p, both sides times both sums (in 64 bits: neither overflows)
       if (a.draft_logits) {
         const Stats& t = st[a.drafts + 1 + s];
-        const float y = logit<BF16>(row_at<BF16>(a.draft_logits, a.draft_batch_stride, a.draft_row_stride, b, s), d);
-        q = exp(((double)y - t.m) * c) / (double)t.heat;
+        good = (double)d.u * heat.exp(d.y - t.m) * st[s].heat < (double)p * t.heat;
+      } else {
+        good = (double)d.u * st[s].heat < (double)p;
       }
-      good = (double)a.uniforms[(int64_t)b * a.drafts + s] * q < p;
     }
   }
   const uint64_t all = __ballot(good);
@@ -235,27 +283,52 @@ __device__ __forceinline__ int accepted(const G4VerifyArgs& a, int b, int n, con
 }
 
 // The accepted tokens with their log-probabilities, and what stands behind the last token (by the first wave).
-template <bool BF16>
-__device__ __forceinline__ void write_accepted(const G4VerifyArgs& a, int b, int count, const Stats* st) {
+__device__ __forceinline__ void write_accepted(const G4VerifyArgs& a, int b, int count, const Draft& d, const Stats* st) {
   const int s = threadIdx.x & 63;
   if (s == 0) a.count_out[b] = count;
   if (s > a.drafts || s == count) return;
   const int64_t at = (int64_t)b * (a.drafts + 1) + s;
-  if (s > count) {
-    a.token_out[at] = -1;
-    a.logp_out[at] = 0.f;
-    return;
-  }
-  const int d = a.draft_tokens[(int64_t)b * a.drafts + s];
-  a.token_out[at] = d;
-  a.logp_out[at] = log_prob(logit<BF16>(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, s), d), st[s]);
+  a.token_out[at] = s < count ? d.id : -1;
+  a.logp_out[at] = s < count ? log_prob(d.x, st[s]) : 0.f;
+}
+template <bool BF16>
+__device__ __forceinline__ void write_token(const G4VerifyArgs& a, int b, int count, int token, float m, float unit) {
+  const int64_t at = (int64_t)b * (a.drafts + 1) + count;
+  a.token_out[at] = token;
+  a.logp_out[at] = log_prob(logit<BF16>(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, count), token), Stats{m, 0.f, unit, 0});
 }
 
-// --- second launch: the race, a chunk per workgroup ----------------------------------------------------------------------
+// --- second launch: the decision, one workgroup per b -----------------------------------------------------------------------
+// (Made by every workgroup of the race for itself it costs these 6 us at 64 rows, and one row no less than the launch, 3 us.)
 
-// 1 / -log(u), the factor of a weight in the race: 0 for u = 0, and finite for u = 1.
+template <bool BF16, int MODE>
+__global__ __launch_bounds__(kThreads) void verify_decide_kernel(G4VerifyArgs a, VerifyWorkspace w, Heat heat, int rows, int splits) {
+  __shared__ Stats st[2 * kMaxDrafts + 1];
+  const int b = blockIdx.x;
+  const int n = drafts_of(a, b);
+  const Draft draft = load_draft<BF16, MODE>(a, b, threadIdx.x < 64 ? n : 0);
+  join_rows<MODE>(a, w, b, rows, splits, n, st);
+  if (threadIdx.x >= 64) return;
+  const int count = accepted<BF16, MODE>(a, heat, n, draft, st);
+  write_accepted(a, b, count, draft, st);
+  const int id = __shfl(draft.id, count < 63 ? count : 63, 64);
+  if (threadIdx.x != 0) return;
+  if constexpr (MODE == kGreedy) {
+    // (a row of nothing but -inf and NaN has no largest)
+    write_token<BF16>(a, b, count, st[count].idx != kNoColumn ? st[count].idx : 0, st[count].m, st[count].unit);
+  } else {
+    const bool rejected = count < n, residual = rejected && a.draft_logits;
+    const Stats &p = st[count], &q = st[residual ? a.drafts + 1 + count : count];
+    w.made[b] = Decision{count, rejected && !residual ? id : -1, residual, p.unit, p.m, p.heat, q.m, q.heat};
+    w.arrived[(int64_t)b * kApart] = 0;
+  }
+}
+
+// --- third launch: the race, a chunk per workgroup ----------------------------------------------------------------------
+
+// 1 / -log(u), the factor of a weight in the race; 0 for u = 0 and outside [0, 1).
 __device__ __forceinline__ float pace(float u) {
-  return u >= kF32Tiny ? __builtin_amdgcn_rcpf(fmaxf(-log_pos_normal(u), 0x1p-25f)) : 0.f;
+  return u >= kF32Tiny && u < 1.f ? __builtin_amdgcn_rcpf(-log_pos_normal(u)) : 0.f;
 }
 
 // A score and its column in one word that grows with the score and falls with the column; 0 for no score above 0.
@@ -272,131 +345,145 @@ __device__ __forceinline__ uint64_t wave_top(uint64_t v) {
   return v;
 }
 
-template <bool BF16, int MODE, int VECS>
-__global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, VerifyWorkspace w, int rows, int splits) {
-  __shared__ Stats st[2 * kMaxDrafts + 1];
-  __shared__ int decided;
-  __shared__ uint64_t best[kWaves][2];
+// A row's probabilities, roughly and well: the rough ones are within 1e-5 of the others.
+struct Row {
+  const void* at;
+  float m, inv;
+  Below rough;
+  __device__ __forceinline__ Row(const void* p, float m_, float z, float c) : at(p), m(m_), inv(1.0f / z), rough(m_, c) {
+    rough.rest *= inv;
+  }
+  __device__ __forceinline__ float well(const Heat& heat, float x) const { return heat.exp(x - m) * inv; }
+};
+
+// The race is decided by scores within a few f32 ulps, which take some 50 instructions each. Rough ones take 15 and give
+// each score's bounds; an element whose upper bound is below the workgroup's largest lower one is out: one per
+// workgroup remains, or a few. (64 rows of 262144: 55 -> 29 us.)
+template <bool BF16, int VECS>
+__global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, VerifyWorkspace w, Heat heat, int splits) {
+  __shared__ uint64_t best_of[kWaves];
+  __shared__ float bars[kWaves];
+  __shared__ bool last;
   const int split = blockIdx.x % splits, b = blockIdx.x / splits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t i0 = (int64_t)split * (VECS * kThreads * 8) + threadIdx.x * 8;
-  // the noise is asked for before the decision
+  const Decision d = w.made[b];
   float u[VECS][8];
 #pragma unroll
   for (int v = 0; v < VECS; ++v) {
     const int64_t i = i0 + v * (kThreads * 8);
     load8<false>(a.noise + b * a.noise_stride, i, (int)min((int64_t)8, a.vocab - i), u[v]);
   }
-  const int n = drafts_of(a, b);
-  join_rows<MODE>(a, w, b, rows, splits, n, st);
-  if (wave == 0) {
-    const int count = accepted<BF16, MODE>(a, b, n, st);
-    if (lane == 0) decided = count;
-    if (split == 0) {
-      write_accepted<BF16>(a, b, count, st);
-      if (lane == 0) w.made[b] = Decision{count, st[count].m, st[count].unit, 0};
-    }
-  }
-  __syncthreads();
-  const int count = decided;
-  const bool rejected = count < n;
-  const void* prow = row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, count);
-  const void* qrow = rejected && a.draft_logits
-                         ? row_at<BF16>(a.draft_logits, a.draft_batch_stride, a.draft_row_stride, b, count) : nullptr;
-  const int64_t away = rejected && !qrow ? a.draft_tokens[(int64_t)b * a.drafts + count] : -1;
-  const Stats ps = st[count], qs = st[qrow ? a.drafts + 1 + count : count];
-  const float pz = 1.0f / ps.heat, qz = 1.0f / qs.heat;
-  const double c = 1.4426950408889634074 / (double)a.temperature;
-  const Heat heat{(float)c, (float)(c - (double)(float)c)};
-  uint64_t top = 0, top_p = 0;
+  const bool residual = d.residual;
+  const int64_t away = d.away;
+  const Row p(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, d.count), d.pm, d.pz, heat.hi);
+  const Row q(residual ? row_at<BF16>(a.draft_logits, a.draft_batch_stride, a.draft_row_stride, b, d.count) : nullptr, d.qm, d.qz,
+              heat.hi);
+  float x[VECS][8], y[VECS][8];
 #pragma unroll
   for (int v = 0; v < VECS; ++v) {
     const int64_t i = i0 + v * (kThreads * 8);
-    const int there = (int)min((int64_t)8, a.vocab - i);
-    float x[8], y[8];
-    load8<BF16>(prow, i, there, x);
-    if (qrow) load8<BF16>(qrow, i, there, y);
+    load8<BF16>(p.at, i, (int)min((int64_t)8, a.vocab - i), x[v]);
+    if (residual) load8<BF16>(q.at, i, (int)min((int64_t)8, a.vocab - i), y[v]);
+  }
+  // ln 2 times the scores' bounds (the pace by log2): the rough probabilities are within 1e-5, and q <= p where r >= 0
+  const bool tame = fabsf(p.m) < 1e30f && fabsf(q.m) < 1e30f;  // else none (Below)
+  float high[VECS][8], bar = 0.f;
+#pragma unroll
+  for (int v = 0; v < VECS; ++v)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (e >= there) continue;
-      const float p = heat.exp(x[e] - ps.m) * pz, g = pace(u[v][e]);
-      float r = p;
-      if (qrow) r = fmaxf(p - heat.exp(y[e] - qs.m) * qz, 0.f);
-      else if (i + e == away) r = 0.f;
-      const uint64_t k = entry(r * g, i + e), kp = entry(p * g, i + e);
-      top = k > top ? k : top;
-      top_p = kp > top_p ? kp : top_p;
+      const float pr = p.rough.exp(x[v][e]) * p.rough.rest;
+      float r = pr;
+      if (residual) r = fmaf(-q.rough.exp(y[v][e]), q.rough.rest, pr);
+      else if (i0 + v * (kThreads * 8) + e == away) r = 0.f;
+      const float g = u[v][e] < 1.f ? -__builtin_amdgcn_rcpf(__builtin_amdgcn_logf(u[v][e])) : 0.f;
+      high[v][e] = fmaf(pr, 4e-5f, r) * g;
+      bar = fmaxf(bar, fmaf(pr, -4e-5f, r) * g);
     }
+  bar = wave_max(bar);
+  if (lane == 0) bars[wave] = bar;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) bar = fmaxf(bar, bars[i]);
+  bar *= 0.9999f;
+  uint32_t mask = 0;  // this lane's elements that may win
+#pragma unroll
+  for (int v = 0; v < VECS; ++v)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mask |= high[v][e] >= bar || !tame ? 1u << (v * 8 + e) : 0u;
+  uint64_t top = 0;
+  while (mask) {
+    const int j = __builtin_ctz(mask);
+    mask &= mask - 1;
+    const int64_t i = i0 + (j >> 3) * (kThreads * 8) + (j & 7);
+    if (i >= a.vocab) continue;
+    const float pw = p.well(heat, logit<BF16>(p.at, i));
+    float r = pw;
+    if (residual) r = fmaxf(pw - q.well(heat, logit<BF16>(q.at, i)), 0.f);
+    else if (i == away) r = 0.f;
+    const uint64_t k = entry(r * pace(a.noise[b * a.noise_stride + i]), i);
+    top = k > top ? k : top;
   }
   top = wave_top(top);
-  top_p = wave_top(top_p);
-  if (lane == 0) best[wave][0] = top, best[wave][1] = top_p;
+  if (lane == 0) best_of[wave] = top;
   __syncthreads();
-  if (threadIdx.x < 2) {
-    uint64_t k = 0;
+  if (threadIdx.x == 0) {
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) k = best[i][threadIdx.x] > k ? best[i][threadIdx.x] : k;
-    w.race[((int64_t)b * splits + split) * 2 + threadIdx.x] = k;
+    for (int i = 1; i < kWaves; ++i) top = best_of[i] > top ? best_of[i] : top;
+    // The best is in memory, where every XCD sees it, once the store has returned; only then is the arrival counted. (With
+    // fences instead, each workgroup writes its L2 back: 85 us in all.)
+    __hip_atomic_store(w.best + blockIdx.x, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    last = __hip_atomic_fetch_add(w.arrived + (int64_t)b * kApart, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)splits - 1;
   }
-}
-
-// --- last launch: the token ------------------------------------------------------------------------------------------------
-
-template <bool BF16, int MODE>
-__global__ __launch_bounds__(MODE == kGreedy ? kThreads : 64) void verify_token_kernel(G4VerifyArgs a, VerifyWorkspace w, int rows,
-                                                                                      int splits) {
-  __shared__ Stats st[MODE == kGreedy ? kMaxDrafts + 1 : 1];
-  const int b = blockIdx.x, lane = threadIdx.x & 63;
-  Decision d;
-  if constexpr (MODE == kGreedy) {
-    const int n = drafts_of(a, b);
-    join_rows<MODE>(a, w, b, rows, splits, n, st);
-    if (threadIdx.x >= 64) return;
-    d.count = accepted<BF16, MODE>(a, b, n, st);
-    write_accepted<BF16>(a, b, d.count, st);
-    d.m = st[d.count].m, d.unit = st[d.count].unit;
-    d.token = st[d.count].idx != kNoColumn ? st[d.count].idx : 0;  // (a row of nothing but -inf and NaN)
-  } else {
-    d = w.made[b];
-    uint64_t k = 0, kp = 0;
-    for (int i = lane; i < splits; i += 64) {
-      const uint64_t o = w.race[((int64_t)b * splits + i) * 2], op = w.race[((int64_t)b * splits + i) * 2 + 1];
-      k = o > k ? o : k;
-      kp = op > kp ? op : kp;
+  __syncthreads();
+  if (!last) return;
+  top = 0;
+  for (int i = lane; i < splits; i += 64) {  // (every wave all of them)
+    const uint64_t k = __hip_atomic_load(w.best + (int64_t)b * splits + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    top = k > top ? k : top;
+  }
+  top = wave_top(top);
+  if (top == 0) {  // (uniform) no weight is left, p = q but for rounding: from p, by this workgroup alone
+    for (int64_t i = threadIdx.x; i < a.vocab; i += kThreads) {
+      const uint64_t k = entry(p.well(heat, logit<BF16>(p.at, i)) * pace(a.noise[b * a.noise_stride + i]), i);
+      top = k > top ? k : top;
     }
-    k = wave_top(k);
-    kp = wave_top(kp);
-    if (!k) k = kp;  // no weight is left: p = q but for rounding
-    d.token = k ? (int)(0xffffffffu - (uint32_t)k) : 0;
+    top = wave_top(top);
+    __syncthreads();
+    if (lane == 0) best_of[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) top = best_of[i] > top ? best_of[i] : top;
   }
-  if (lane != 0) return;
-  const int64_t at = (int64_t)b * (a.drafts + 1) + d.count;
-  const float x = logit<BF16>(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, d.count), d.token);
-  a.token_out[at] = d.token;
-  a.logp_out[at] = log_prob(x, Stats{d.m, 0.f, d.unit, 0});
+  if (threadIdx.x == 0) write_token<BF16>(a, b, d.count, top ? (int)(0xffffffffu - (uint32_t)top) : 0, d.pm, d.unit);
 }
 
 template <bool BF16, int MODE, int VECS>
 int launch_verify(const G4VerifyArgs& a, const VerifyWorkspace& w, hipStream_t st) {
   static const char who[] = "g4_verify_draft";
-  const int splits = splits_of(a), rows = a.drafts + 1 + (MODE != kGreedy && a.draft_logits ? a.drafts : 0);
+  const int splits = splits_of(a, VECS), rows = a.drafts + 1 + (MODE != kGreedy && a.draft_logits ? a.drafts : 0);
   const int64_t blocks = (int64_t)a.batch * rows * splits;
   if (blocks * kThreads > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "%s: too many logits", who);
   hipLaunchKernelGGL((verify_stats_kernel<BF16, MODE, VECS>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, w, rows, splits);
   int rc = check_launch(who);
   if (rc != G4_OK) return rc;
+  const double c = 1.4426950408889634074 / (double)a.temperature;
+  const Heat heat{(float)c, (float)(c - (double)(float)c)};
+  hipLaunchKernelGGL((verify_decide_kernel<BF16, MODE>), dim3((unsigned)a.batch), dim3(kThreads), 0, st, a, w, heat, rows, splits);
+  if ((rc = check_launch(who)) != G4_OK) return rc;
   if constexpr (MODE != kGreedy) {
-    hipLaunchKernelGGL((verify_race_kernel<BF16, MODE, VECS>), dim3((unsigned)((int64_t)a.batch * splits)), dim3(kThreads), 0, st, a, w,
-                       rows, splits);
-    if ((rc = check_launch(who)) != G4_OK) return rc;
+    const int race = splits_of(a, kRace);  // (fewer workgroups than above: rows >= 2)
+    hipLaunchKernelGGL((verify_race_kernel<BF16, kRace>), dim3((unsigned)((int64_t)a.batch * race)), dim3(kThreads), 0, st, a, w, heat,
+                       race);
+    rc = check_launch(who);
   }
-  hipLaunchKernelGGL((verify_token_kernel<BF16, MODE>), dim3((unsigned)a.batch), dim3(MODE == kGreedy ? kThreads : 64), 0, st, a, w,
-                     rows, splits);
-  return check_launch(who);
+  return rc;
 }
 
 template <bool BF16, int MODE>
 int launch_verify(const G4VerifyArgs& a, const VerifyWorkspace& w, hipStream_t st) {
-  return chunk_of(a) == 16384 ? launch_verify<BF16, MODE, 8>(a, w, st) : launch_verify<BF16, MODE, 2>(a, w, st);
+  return vecs_of(a) == kLong ? launch_verify<BF16, MODE, kLong>(a, w, st) : launch_verify<BF16, MODE, kShort>(a, w, st);
 }
 template <bool BF16>
 int launch_verify(const G4VerifyArgs& a, const VerifyWorkspace& w, hipStream_t st) {
