@@ -145,6 +145,17 @@ __device__ __forceinline__ void scan_group(const int32_t* refs, int32_t pages, i
   if (lane == 0) w.counts[g] = count;
 }
 
+// What row b wants, by one wave.
+template <typename Op>
+__device__ __forceinline__ void count_wants(const Op& op, int b, const PoolWorkspace& w, int lane) {
+  const auto row = op.row(b);
+  int n = 0;
+  for (int e0 = 0; e0 < op.last(row); e0 += 64)
+    n += __popcll(__ballot(e0 + lane < op.last(row) && op.wants(row, e0 + lane)));
+  if (lane == 0) w.wants[b] = n;
+}
+
+// Groups of pages in the first `group_blocks` workgroups, rows in the others; a wave each.
 template <typename Op>
 __global__ __launch_bounds__(kThreads) void scan_kernel(Op op, const int32_t* refs, int32_t pages, PoolWorkspace w,
                                                         int group_blocks) {
@@ -156,45 +167,54 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(Op op, const int32_t* re
   }
   if constexpr (!std::is_same_v<Op, int>) {
     const int b = ((int)blockIdx.x - group_blocks) * kWaves + wave;
-    if (b >= op.rows()) return;
-    const auto row = op.row(b);
-    int n = 0;
-    for (int e0 = 0; e0 < op.last(row); e0 += 64)
-      n += __popcll(__ballot(e0 + lane < op.last(row) && op.wants(row, e0 + lane)));
-    if (lane == 0) w.wants[b] = n;
+    if (b < op.rows()) count_wants(op, b, w, lane);
   }
 }
 
-// The free pages by rank, in LDS per workgroup.
+// The free pages by rank, in LDS per workgroup of THREADS.
+template <int THREADS>
 struct FreePages {
   int32_t before[kSpans + 1];  // free pages below a span's first
-  int32_t partial[kThreads];
+  int32_t partial[2][THREADS / 64];
   int spans, per;              // groups per span
 
-  // sum over the workgroup's threads of v below this thread; `total` the whole
+  // The sum of v over the threads below this one; `total` over all. (The caller's next use of `partial` is behind a barrier.)
   __device__ __forceinline__ int exclusive(int v, int& total) {
-    partial[threadIdx.x] = v;
-    __syncthreads();
-#pragma unroll 1
-    for (int d = 1; d < kThreads; d <<= 1) {
-      const int x = (int)threadIdx.x >= d ? partial[threadIdx.x - d] : 0;
-      __syncthreads();
-      partial[threadIdx.x] += x;
-      __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(x, d, 64);
+      x += lane >= d ? y : 0;
     }
-    total = partial[kThreads - 1];
-    const int below = partial[threadIdx.x] - v;
+    if (lane == 63) partial[0][wave] = x;
     __syncthreads();
-    return below;
+    int below = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) {
+      below += i < wave ? partial[0][i] : 0;
+      total += partial[0][i];
+    }
+    __syncthreads();
+    return below + x - v;
+  }
+  // Over all threads.
+  __device__ __forceinline__ void sums(int& u, int& v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) u += __shfl_xor(u, d, 64), v += __shfl_xor(v, d, 64);
+    if ((threadIdx.x & 63) == 0) partial[0][threadIdx.x >> 6] = u, partial[1][threadIdx.x >> 6] = v;
+    __syncthreads();
+    u = v = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) u += partial[0][i], v += partial[1][i];
+    __syncthreads();
   }
 
   __device__ __forceinline__ void load(const PoolWorkspace& w, int64_t groups) {
-    if (threadIdx.x == 0) {
-      per = (int)((groups + kSpans - 1) / kSpans);
-      spans = (int)((groups + per - 1) / per);
-    }
-    __syncthreads();
-    const int each = (spans + kThreads - 1) / kThreads;
+    per = (int)((groups + kSpans - 1) / kSpans);  // (the same in every thread)
+    spans = (int)((groups + per - 1) / per);
+    const int each = (spans + THREADS - 1) / THREADS;
     const int from = min((int)threadIdx.x * each, spans), to = min(from + each, spans);
     int sum = 0;
     for (int s = from; s < to; ++s) {
@@ -257,30 +277,28 @@ struct FreePages {
   }
 };
 
-// The rows' fresh pages, `per` rows per workgroup. shortage: how many entries got none.
-template <typename Op>
-__global__ __launch_bounds__(kThreads) void assign_kernel(Op op, int32_t* refs, int32_t pages, PoolWorkspace w, int per,
-                                                          int32_t* shortage) {
-  __shared__ FreePages free;
-  __shared__ int32_t base[kThreads];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int rows = op.rows(), row0 = blockIdx.x * per;
-  free.load(w, groups_of(pages));
+// The fresh pages of rows row0 .. row0 + per - 1, per <= THREADS. shortage (of all rows): how many entries got none.
+template <int THREADS, typename Op>
+__device__ __forceinline__ void assign_rows(const Op& op, int32_t* refs, int32_t pages, const PoolWorkspace& w, int row0, int per,
+                                            int32_t* shortage) {
+  __shared__ FreePages<THREADS> free;
+  __shared__ int32_t base[THREADS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = op.rows();
   int before = 0, all = 0;
-  for (int i = threadIdx.x; i < (blockIdx.x == 0 ? rows : row0); i += kThreads) {
+  for (int i = threadIdx.x; i < (row0 == 0 ? rows : row0); i += THREADS) {
     const int n = w.wants[i];
     before += i < row0 ? n : 0;
     all += n;
   }
-  int before_all, all_rows;
-  free.exclusive(before, before_all);
-  free.exclusive(all, all_rows);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *shortage = max(0, all_rows - free.total());
-  const int mine = row0 + (int)threadIdx.x;  // per <= kThreads
+  const int mine = row0 + (int)threadIdx.x;
+  const int wanted_here = (int)threadIdx.x < per && mine < rows ? w.wants[mine] : 0;
+  free.load(w, groups_of(pages));
+  free.sums(before, all);
+  if (row0 == 0 && threadIdx.x == 0) *shortage = max(0, all - free.total());
   int total;
-  base[threadIdx.x] = before_all + free.exclusive((int)threadIdx.x < per && mine < rows ? w.wants[mine] : 0, total);
+  base[threadIdx.x] = before + free.exclusive(wanted_here, total);
   __syncthreads();
-  for (int i = wave; i < per && row0 + i < rows; i += kWaves) {
+  for (int i = wave; i < per && row0 + i < rows; i += THREADS / 64) {
     const auto row = op.row(row0 + i);
     int rank = base[i];
     for (int e0 = 0; e0 < op.last(row); e0 += 64) {
@@ -295,10 +313,33 @@ __global__ __launch_bounds__(kThreads) void assign_kernel(Op op, int32_t* refs, 
   }
 }
 
+template <typename Op>
+__global__ __launch_bounds__(kThreads) void assign_kernel(Op op, int32_t* refs, int32_t pages, PoolWorkspace w, int per,
+                                                          int32_t* shortage) {
+  assign_rows<kThreads>(op, refs, pages, w, blockIdx.x * per, per, shortage);
+}
+
+// Both launches in one, of one workgroup, whose waves take the groups and the rows in turns and keep what the launches hand over
+// in LDS: for few rows of a small pool. (One prompt of 701 positions to 4 rows in a pool of 77 pages, fork, free and reserve
+// replayed from a graph: 25.9 -> 21.0 us. 64 rows are four turns of 16 waves, and the two launches as fast.)
+constexpr int kFewRows = 32, kFewPages = 16384, kFewThreads = 1024;
+template <typename Op>
+__global__ __launch_bounds__(kFewThreads) void few_kernel(Op op, int32_t* refs, int32_t pages, int32_t* shortage) {
+  __shared__ uint64_t bits[kFewPages / 64];
+  __shared__ int32_t counts[kFewPages / kGroup], wants[kFewRows];
+  PoolWorkspace w = {};
+  w.bits = bits, w.counts = counts, w.wants = wants;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int b = wave; b < op.rows(); b += kFewThreads / 64) count_wants(op, b, w, lane);
+  for (int g = wave; g < groups_of(pages); g += kFewThreads / 64) scan_group(refs, pages, g, w, lane);
+  __syncthreads();
+  assign_rows<kFewThreads>(op, refs, pages, w, 0, op.rows(), shortage);
+}
+
 // --- copies ----------------------------------------------------------------------------------------------------
 
 constexpr int kMaxLayers = 32;      // per launch (they ride in the kernel's arguments)
-constexpr int kUnitBytes = 16384;   // of keys or values that a workgroup copies at a time
+constexpr int kUnitBytes = 16384;   // of keys or values that a workgroup copies at a time (8 KiB 86, 16 and 32 KiB 67 us below)
 
 struct Layer {
   uint8_t* data[2];   // key, value
@@ -308,62 +349,69 @@ struct Layer {
 };
 struct Copies {
   Layer layers[kMaxLayers];
-  int32_t first[kMaxLayers + 1];  // units per page before a layer, both arrays counted
   int32_t n_layers, num_pages, chunks;  // 32-slot chunks per page and head
 };
 
-// One unit: `per` chunks of one page and array, those of the first `slots` slots.
-__device__ __forceinline__ void copy_unit(const Copies& c, int unit, int32_t from, int32_t to, int slots) {
-  int l = 0;
-  while (l + 1 < c.n_layers && unit >= c.first[l + 1]) ++l;
-  const Layer& layer = c.layers[l];
-  unit -= c.first[l];
-  const int array = unit >= layer.units, j0 = (unit - (array ? layer.units : 0)) * layer.per;
-  const int n = min(layer.per, layer.heads * c.chunks - j0);
-  const int64_t page = (int64_t)layer.heads * c.chunks;  // chunks of a page
-  const int live = (slots + 31) >> 5;
-  const uint8_t* src = layer.data[array] + (from * page + j0) * layer.chunk_bytes;
-  uint8_t* dst = layer.data[array] + (to * page + j0) * layer.chunk_bytes;
-  const int pieces = layer.chunk_bytes / 16, shift = __builtin_ctz(pieces), cshift = __builtin_ctz(c.chunks);
-  const auto on = [&](int piece) {  // in a chunk that holds live slots
-    return ((j0 + (piece >> shift)) & ((1 << cshift) - 1)) < live;
-  };
-  constexpr int kAtOnce = 4;
-  for (int i0 = 0; i0 < n * pieces; i0 += kAtOnce * kThreads) {
-    u32x4 v[kAtOnce];
-    bool go[kAtOnce];
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int piece = i0 + i * kThreads + (int)threadIdx.x;
-      go[i] = piece < n * pieces && on(piece);
-      if (go[i]) v[i] = *reinterpret_cast<const u32x4*>(src + (int64_t)piece * 16);
-    }
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i)
-      if (go[i])
-        __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4*>(dst + (int64_t)(i0 + i * kThreads + (int)threadIdx.x) * 16));
-  }
-  if (layer.scale[array]) {  // 32 bytes per chunk
-    for (int i = threadIdx.x; i < n * 4; i += kThreads) {
-      if (((j0 + i / 4) & (c.chunks - 1)) >= live) continue;
-      const int64_t at = (int64_t)j0 * 32 + i * 8;
-      *reinterpret_cast<uint64_t*>(layer.scale[array] + to * page * 32 + at) =
-          *reinterpret_cast<const uint64_t*>(layer.scale[array] + from * page * 32 + at);
-    }
-  }
-}
+// Where entries of a table go: nothing where map is NULL.
+struct Remap {
+  G4PageTable table;
+  const int32_t* map;
+};
 
-// Pairs of pages (their number on the device where `moved` is given), every layer and array of each: one workgroup
-// per unit, or several units one after the other.
+// Pairs of pages (their number on the device where `moved` is given) in every layer: a workgroup per layer and array (which
+// change fastest), pair and unit of `per` chunks, or several units one after the other. Of a page those chunks that
+// hold its first slots[i] slots, or all. Bound by HBM: 576 e4m3 pages of 32 KiB from 144, 8 layers, in 67 us (5.7 TB/s; a plain copy
+// of as many bytes 5.7, with non-temporal loads 6.4, which here lose what the sources' readers share: 108 us). With the layers
+// slowest instead of fastest 87 us.
 __global__ __launch_bounds__(kThreads) void copy_kernel(Copies c, const int32_t* src, const int32_t* dst, const int32_t* slots,
-                                                        int pairs, const int32_t* moved) {
+                                                        int pairs, const int32_t* moved, Remap remap) {
   if (moved) pairs = *moved;
-  const int per_pair = c.first[c.n_layers];
-  for (int64_t u = blockIdx.x; u < (int64_t)pairs * per_pair; u += gridDim.x) {
-    const int i = (int)(u / per_pair), unit = (int)(u - (int64_t)i * per_pair);
+  if (remap.map) {
+    const G4PageTable& t = remap.table;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)t.rows * t.max_pages;
+         i += (int64_t)gridDim.x * kThreads) {
+      const int b = (int)(i / t.max_pages), e = (int)(i - (int64_t)b * t.max_pages);
+      int32_t& entry = t.entries[b * t.stride + e];
+      const int32_t p = entry;
+      if ((uint32_t)p < (uint32_t)c.num_pages && remap.map[p] != p) entry = remap.map[p];
+    }
+  }
+  const int arrays = 2 * c.n_layers, la = (int)(blockIdx.x % (unsigned)arrays);
+  const Layer& layer = c.layers[la >> 1];
+  const int array = la & 1, units = layer.units, chunks = layer.heads * c.chunks;  // of a page
+  const int shift = __builtin_ctz(layer.chunk_bytes / 16), tid = threadIdx.x;              // 16-byte pieces of a chunk
+  const int64_t page_bytes = (int64_t)chunks * layer.chunk_bytes;
+  uint8_t* const data = layer.data[array];
+  uint8_t* const scale = layer.scale[array];
+  for (int64_t u = blockIdx.x / (unsigned)arrays; u < (int64_t)pairs * units; u += gridDim.x / (unsigned)arrays) {
+    const int i = (int)(u / units), j0 = (int)(u - (int64_t)i * units) * layer.per;
     const int32_t from = src[i], to = dst[i];
     if ((uint32_t)from >= (uint32_t)c.num_pages || (uint32_t)to >= (uint32_t)c.num_pages || from == to) continue;
-    copy_unit(c, unit, from, to, slots ? slots[i] : c.chunks * 32);
+    const int n = min(layer.per, chunks - j0), live = slots ? (slots[i] + 31) >> 5 : c.chunks;
+    const u32x4* const s = reinterpret_cast<const u32x4*>(data + from * page_bytes + (int64_t)j0 * layer.chunk_bytes);
+    u32x4* const d = reinterpret_cast<u32x4*>(data + to * page_bytes + (int64_t)j0 * layer.chunk_bytes);
+    constexpr int kAtOnce = 4;
+    for (int p0 = tid; p0 < n << shift; p0 += kAtOnce * kThreads) {
+      u32x4 v[kAtOnce];
+      bool go[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int p = p0 + k * kThreads;
+        go[k] = p < n << shift && ((j0 + (p >> shift)) & (c.chunks - 1)) < live;
+        if (go[k]) v[k] = s[p];
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (go[k]) __builtin_nontemporal_store(v[k], d + p0 + k * kThreads);
+    }
+    if (scale) {  // 32 bytes per chunk
+      for (int p = tid; p < n * 4; p += kThreads) {
+        if (((j0 + p / 4) & (c.chunks - 1)) >= live) continue;
+        const int64_t at = (int64_t)j0 * 32 + p * 8;
+        *reinterpret_cast<uint64_t*>(scale + (int64_t)to * chunks * 32 + at) =
+            *reinterpret_cast<const uint64_t*>(scale + (int64_t)from * chunks * 32 + at);
+      }
+    }
   }
 }
 
@@ -385,7 +433,7 @@ __global__ __launch_bounds__(kThreads) void free_kernel(G4PageTable t, const int
 
 // Where every page goes: with n pages in use, the i-th in use at n or behind it to the i-th free one below n.
 __global__ __launch_bounds__(kThreads) void move_kernel(int32_t* refs, int32_t pages, PoolWorkspace w, int32_t* live) {
-  __shared__ FreePages free;
+  __shared__ FreePages<kThreads> free;
   const int64_t groups = groups_of(pages);
   free.load(w, groups);
   const int n = pages - free.total();
@@ -402,16 +450,6 @@ __global__ __launch_bounds__(kThreads) void move_kernel(int32_t* refs, int32_t p
       refs[p] = 0;
     }
     w.map[p] = to;
-  }
-}
-
-__global__ __launch_bounds__(kThreads) void remap_kernel(G4PageTable t, const int32_t* map, int32_t num_pages) {
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)t.rows * t.max_pages;
-       i += (int64_t)gridDim.x * kThreads) {
-    const int b = (int)(i / t.max_pages), e = (int)(i - (int64_t)b * t.max_pages);
-    int32_t& entry = t.entries[b * t.stride + e];
-    const int32_t p = entry;
-    if ((uint32_t)p < (uint32_t)num_pages && map[p] != p) entry = map[p];
   }
 }
 
@@ -458,13 +496,15 @@ unsigned blocks_for(int64_t n, int64_t most) { return (unsigned)(n < 1 ? 1 : n >
 
 // `pairs`: their number, or where `moved` is given the most there can be.
 int launch_copies(const G4PagedCache* layers, int32_t n, const int32_t* src, const int32_t* dst, const int32_t* slots,
-                  int64_t pairs, const int32_t* moved, hipStream_t st, const char* who) {
+                  int64_t pairs, const int32_t* moved, Remap remap, hipStream_t st, const char* who) {
   for (int32_t l0 = 0; l0 < n; l0 += kMaxLayers) {
     Copies c = {};
-    c.n_layers = n - l0 < kMaxLayers ? n - l0 : kMaxLayers;
+    const int32_t here = n - l0 < kMaxLayers ? n - l0 : kMaxLayers;
+    c.n_layers = here;
+    int64_t units = 0;
     c.num_pages = layers[0].num_pages;
     c.chunks = layers[0].page_size / 32;
-    for (int32_t l = 0; l < c.n_layers; ++l) {
+    for (int32_t l = 0; l < here; ++l) {
       const G4PagedCache& x = layers[l0 + l];
       Layer& y = c.layers[l];
       y.data[0] = static_cast<uint8_t*>(x.key);
@@ -475,11 +515,12 @@ int launch_copies(const G4PagedCache* layers, int32_t n, const int32_t* src, con
       y.chunk_bytes = 32 * x.head_dim * (x.format == G4_PAGES_E4M3 ? 1 : 2);
       y.per = kUnitBytes / y.chunk_bytes > 0 ? kUnitBytes / y.chunk_bytes : 1;
       y.units = (y.heads * c.chunks + y.per - 1) / y.per;
-      c.first[l + 1] = c.first[l] + 2 * y.units;
+      if (y.units > units) units = y.units;
     }
-    const int64_t units = pairs * c.first[c.n_layers];
-    hipLaunchKernelGGL(copy_kernel, dim3(blocks_for(units, moved ? 4096 : 1 << 24)), dim3(kThreads), 0, st, c, src, dst, slots,
-                       (int)pairs, moved);
+    const int64_t blocks = pairs * units, most = (moved ? 4096 : 1 << 23) / (2 * here) + 1;
+    hipLaunchKernelGGL(copy_kernel, dim3(blocks_for(blocks, most) * 2u * (unsigned)here), dim3(kThreads), 0, st, c, src, dst, slots, (int)pairs,
+                       moved, remap);
+    remap.map = nullptr;  // once
     const int rc = check_launch(who);
     if (rc != G4_OK) return rc;
   }
@@ -489,6 +530,10 @@ int launch_copies(const G4PagedCache* layers, int32_t n, const int32_t* src, con
 template <typename Op>
 int launch_assign(const Op& op, int32_t rows, int32_t pages, int32_t* refs, const PoolWorkspace& w, int32_t* shortage,
                   hipStream_t st, const char* who) {
+  if (rows <= kFewRows && pages <= kFewPages) {
+    hipLaunchKernelGGL(few_kernel<Op>, dim3(1), dim3(kFewThreads), 0, st, op, refs, pages, shortage);
+    return check_launch(who);
+  }
   const int64_t groups = groups_of(pages), group_blocks = (groups + kWaves - 1) / kWaves;
   hipLaunchKernelGGL(scan_kernel<Op>, dim3((unsigned)(group_blocks + (rows + (int64_t)kWaves - 1) / kWaves)), dim3(kThreads), 0, st, op,
                      refs, pages, w, (int)group_blocks);
@@ -512,7 +557,7 @@ extern "C" int g4_paged_copy(const G4PagedCache* layers, int32_t n_layers, int32
   const int rc = check_layers(layers, n_layers, who);
   if (rc != G4_OK) return rc;
   if (pairs <= 0 || !src || !dst) return fail(G4_ERR_INVALID, "%s: %d pairs%s", who, pairs, src && dst ? "" : ", NULL");
-  return launch_copies(layers, n_layers, src, dst, nullptr, pairs, nullptr, reinterpret_cast<hipStream_t>(stream), who);
+  return launch_copies(layers, n_layers, src, dst, nullptr, pairs, nullptr, Remap{}, reinterpret_cast<hipStream_t>(stream), who);
 }
 
 extern "C" size_t g4_paged_reserve_workspace_size(const G4PagedReserveArgs* a) {
@@ -567,7 +612,7 @@ extern "C" int g4_paged_fork(const G4PagedForkArgs* args, void* stream) {
   const Fork op{a.table, a.out, a.parents, a.lengths, a.layers[0].num_pages, ps, w.src, w.dst, w.slots};
   rc = launch_assign(op, a.out.rows, a.layers[0].num_pages, a.refs, w, a.shortage, st, who);
   if (rc != G4_OK) return rc;
-  return launch_copies(a.layers, a.n_layers, w.src, w.dst, w.slots, a.out.rows, nullptr, st, who);
+  return launch_copies(a.layers, a.n_layers, w.src, w.dst, w.slots, a.out.rows, nullptr, Remap{}, st, who);
 }
 
 extern "C" int g4_paged_free(const G4PagedFreeArgs* args, void* stream) {
@@ -612,8 +657,5 @@ extern "C" int g4_paged_compact(const G4PagedCompactArgs* args, void* stream) {
   hipLaunchKernelGGL(move_kernel, dim3(blocks_for((pages + (int64_t)kThreads - 1) / kThreads, 256)), dim3(kThreads), 0, st, a.refs,
                      pages, w, a.live);
   if ((rc = check_launch(who)) != G4_OK) return rc;
-  const int64_t n = (int64_t)a.table.rows * a.table.max_pages;
-  hipLaunchKernelGGL(remap_kernel, dim3(blocks_for((n + kThreads - 1) / kThreads, 1 << 16)), dim3(kThreads), 0, st, a.table, w.map, pages);
-  if ((rc = check_launch(who)) != G4_OK) return rc;
-  return launch_copies(a.layers, a.n_layers, w.src, w.dst, nullptr, pages / 2, w.moved, st, who);
+  return launch_copies(a.layers, a.n_layers, w.src, w.dst, nullptr, pages / 2, w.moved, Remap{a.table, w.map}, st, who);
 }
