@@ -49,6 +49,17 @@ __device__ __forceinline__ int columns_reduce(int v, F op) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
+// row / R of rows below 2^31: floor(row m / 2^s) with m = ceil(2^s / R), s = 31 + ceil(log2 R) (exact, since row (m R - 2^s) < 2^s).
+struct Group {
+  uint32_t m;
+  int s;
+  explicit Group(int R) : s(31) {
+    while (1 << (s - 31) < R) ++s;
+    m = (uint32_t)(((1ull << s) + R - 1) / R);
+  }
+  __device__ __forceinline__ int token(int row) const { return (int)((uint64_t)(uint32_t)row * m >> s); }
+};
+
 // The wave's rows: row i of column block cb (i = lane % 16) sees the keys [x, y] at LDS address bounds + 8 (16 cb + i).
 // They are read where a chunk is not seen by all rows, and take no registers over the others.
 struct Rows {
@@ -84,10 +95,11 @@ struct Softmax {
   __device__ __forceinline__ void chunk(const Rows& rows, int c, int lane, floatx4 (&acc)[NB][2], bf16x8 (&pop)[NB],
                                         floatx4 (&oacc)[NB][VT]) {
     if (!rows.full(c)) {
-      __asm__ volatile("" : "+s"(c));  // hidden: else its place relative to every row advances in registers
+      int k = c << 5;
+      __asm__ volatile("" : "+s"(k));  // hidden: else its place relative to every row advances in registers
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb) {
-        const uint32_t bits = Rows::bits(rows.keys(cb, lane & 15), (c << 5) + 8 * (lane >> 4));
+        const uint32_t bits = Rows::bits(rows.keys(cb, lane & 15), k + 8 * (lane >> 4));
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[cb][e >> 2][e & 3] = bits >> e & 1u ? acc[cb][e >> 2][e & 3] : kNegInf;
       }
@@ -102,6 +114,7 @@ struct Softmax {
       rise |= top[cb] > m[cb] + kSlack;
     }
     if (__any(rise)) {  // (uniform)
+      const bool fresh = c << 5 <= rows.first;  // the wave's first chunk: the accumulators are 0
 #pragma unroll
       for (int cb = 0; cb < NB; ++cb) {
         const float next = fmaxf(m[cb], column_max(top[cb]));
@@ -109,8 +122,10 @@ struct Softmax {
         const float scale = next > m[cb] ? __builtin_amdgcn_exp2f((m[cb] - next) * kLog2e) : 1.f;
         m[cb] = next;
         l[cb] *= scale;
+        if (!fresh) {
 #pragma unroll
-        for (int i = 0; i < VT; ++i) oacc[cb][i] *= scale;
+          for (int i = 0; i < VT; ++i) oacc[cb][i] *= scale;
+        }
       }
     }
 #pragma unroll
@@ -197,7 +212,7 @@ __device__ __forceinline__ void place_block(int i, int n_blk, int H, int& blk, i
 // prefill_bf16_lds_kernel: one runs the MFMAs (the values of chunk c - 1, then the scores of chunk c), at raised
 // priority, while the other runs the softmax of a chunk. Chunks of which a wave sees nothing it skips.
 template <int D, int NB, int NW, int SLOTS>
-__global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPrefillArgs a) {
+__global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPrefillArgs a, Group group) {
   using S = Shape<D, NB, NW, SLOTS>;
   constexpr int KS = S::KS, VT = S::T;
   // read with inline-assembly LDS reads only: the compiler adds no waits of its own for the DMAs in flight
@@ -217,7 +232,7 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPref
 #pragma unroll
   for (int cb = 0; cb < NB; ++cb) {
     // rows behind the last token read the last row and are not stored
-    const int row = row0 + cb * 16 + col, t = row / R;
+    const int row = row0 + cb * 16 + col, t = group.token(row);
     const int64_t at = (int64_t)min(row, T * R - 1);  // flat over (t, r) of a head
     const int tq = min(t, T - 1);
     const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (at + ((int64_t)tq * (H - 1) + h) * R) * D;
@@ -340,27 +355,30 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPref
 #pragma unroll
   for (int cb = 0; cb < NB; ++cb) {
     const float l = column_sum(soft.l[cb]);
-    const int row = row0 + cb * 16 + (lane_o & 15), t = row / R;
+    const int row = row0 + cb * 16 + (lane_o & 15), t = group.token(row);
     const bool none = rows.keys(cb, lane_o & 15).y < 0 || l == 0.f;
     const float inv = none ? 0.f : 1.0f / l;
-    const auto store = [&](int i, floatx4 x) {
+    const auto pack = [&](floatx4 x) {
       x = none ? floatx4{0.f, 0.f, 0.f, 0.f} : x * inv;
-      const int r = lane_o & 15, unit = (2 * i + (lane_o >> 5)) ^ (r & (UNITS - 1));
-      *reinterpret_cast<uint2*>(mine + (cb * 16 + r) * (D * 2) + unit * 16 + (lane_o >> 4 & 1) * 8) =
-          make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
+      return make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
     };
-    float sum = 0.f;  // not 0 where an accumulator is not finite: 0 x is 0 or NaN
+    const auto store = [&](int i, uint2 x) {
+      const int r = lane_o & 15, unit = (2 * i + (lane_o >> 5)) ^ (r & (UNITS - 1));
+      *reinterpret_cast<uint2*>(mine + (cb * 16 + r) * (D * 2) + unit * 16 + (lane_o >> 4 & 1) * 8) = x;
+    };
+    float sum = 0.f;  // not 0 where an element is not finite: 0 x is 0 or NaN
 #pragma unroll
-    for (int i = 0; i < VT; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum = fmaf(oacc[cb][i][e], 0.f, sum);
+    for (int i = 0; i < VT; ++i) {
+      const uint2 x = pack(oacc[cb][i]);
+      const bf16x2_t zero = {0, 0};
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x.x), zero, sum, false);
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x.y), zero, sum, false);
+      store(i, x);
+    }
     if (__any(!(sum == 0.f))) {
       const uint16_t* q = t < T ? reinterpret_cast<const uint16_t*>(a.q) + (((int64_t)t * H + h) * R + (row - t * R)) * D : nullptr;
 #pragma unroll 1
-      for (int i = 0; i < VT; ++i) store(i, careful_values<D>(rows, cb, soft.base(cb), q, rk, rv, i));
-    } else {
-#pragma unroll
-      for (int i = 0; i < VT; ++i) store(i, oacc[cb][i]);
+      for (int i = 0; i < VT; ++i) store(i, pack(careful_values<D>(rows, cb, soft.base(cb), q, rk, rv, i)));
     }
     __builtin_amdgcn_wave_barrier();  // (a wave's rows are its own: its LDS operations keep their order)
 #pragma unroll
@@ -380,7 +398,8 @@ int launch_packed(const G4PackedPrefillArgs& a, hipStream_t st) {
   using S = Shape<D, D == 512 ? 1 : 2, D == 512 ? 8 : 4, 2>;
   const int64_t blocks = ((int64_t)a.tokens * a.group + S::ROWS - 1) / S::ROWS * a.kv_heads;
   if (blocks * S::NW * 64 > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "g4_packed_prefill_attention: too many tokens");
-  hipLaunchKernelGGL((packed_prefill_kernel<D, S::NB, S::NW, S::SLOTS>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a);
+  hipLaunchKernelGGL((packed_prefill_kernel<D, S::NB, S::NW, S::SLOTS>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a,
+                     Group(a.group));
   return check_launch("g4_packed_prefill_attention");
 }
 
