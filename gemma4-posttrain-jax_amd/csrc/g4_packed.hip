@@ -27,16 +27,20 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kSlack = 8.0f;
 
-template <int D, int NB_, int NW_, int SLOTS_>
+// A workgroup's work: NB blocks of 16 query rows by each of NW waves. Head dims up to 256: four waves of two blocks (at 256
+// 248 registers), two workgroups on a CU, each of which fills the other's barriers, softmax and loads; K and V^T take two
+// chunks of LDS each, 64 KiB at 256. (8 x 4096 tokens of 2 x 4 heads of 256: 506 us; one workgroup of eight waves with
+// four chunks of each 586, of one block per wave 589.) Head dim 512, whose K and V^T take 128 KiB: eight waves of one block.
+template <int D>
 struct Shape {
-  static constexpr int NB = NB_, NW = NW_, SLOTS = SLOTS_;  // chunks of each of K and V^T in LDS
+  static constexpr int NB = D == 512 ? 1 : 2, NW = D == 512 ? 8 : 4;
   static constexpr int KS = D / 32;
   static constexpr int T = D / 16;                  // 1 KiB operand tiles of a chunk's K and of its V^T
   static constexpr int CHUNK = T * 1024;
   static constexpr int TW = T / NW;                 // tiles that a wave fetches of each
   static constexpr int ROWS = NW * NB * 16;         // query rows of a workgroup
   static_assert(T % NW == 0, "the waves share the tiles evenly");
-  static_assert(ROWS * D * 2 <= 2 * SLOTS * CHUNK, "the result goes out through the rings");
+  static_assert(ROWS * D * 2 <= 4 * CHUNK, "the result goes out through the rings");
 };
 
 // Over the 16 columns of an MFMA tile, whose values every row of 16 lanes holds.
@@ -193,7 +197,10 @@ __device__ __forceinline__ floatx4 careful_values(const Rows& rows, int cb, floa
 }
 
 // Which block of rows and head workgroup i takes. Workgroups are dealt to the 8 XCDs round robin: runs of kRun consecutive
-// blocks of a head, which read the same keys, go to one XCD and its L2, the latest tokens' first (whose keys are the most).
+// blocks of a head, which read the same keys, go to one XCD and its L2, the latest tokens' first, whose keys are the most
+// (256 prompts of 32 .. 480 tokens, window 512: 3 % over single blocks; runs of 16 lose 10 % on 3 prompts of up to 8191).
+// Blocks in the order of their keys, found by each workgroup from the starts, took 5 % off several long prompts and put
+// 9 (one of 8000) to 50 % (160 of 100) on others.
 constexpr int kXcds = 8, kRun = 4;
 __device__ __forceinline__ void place_block(int i, int n_blk, int H, int& blk, int& h) {
   const int even = n_blk * H / (kXcds * kRun) * (kXcds * kRun);  // as many as fill whole turns of runs
@@ -208,15 +215,18 @@ __device__ __forceinline__ void place_block(int i, int n_blk, int H, int& blk, i
   blk = n_blk - 1 - (run * kRun + rest - h * len);
 }
 
-// Waves of the two halves of a workgroup (those that share a SIMD) are half a step apart, as in
-// prefill_bf16_lds_kernel: one runs the MFMAs (the values of chunk c - 1, then the scores of chunk c), at raised
-// priority, while the other runs the softmax of a chunk. Chunks of which a wave sees nothing it skips.
-template <int D, int NB, int NW, int SLOTS>
-__global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPrefillArgs a, Group group) {
-  using S = Shape<D, NB, NW, SLOTS>;
-  constexpr int KS = S::KS, VT = S::T;
-  // read with inline-assembly LDS reads only: the compiler adds no waits of its own for the DMAs in flight
-  __shared__ __attribute__((aligned(1024))) unsigned char ring[2 * SLOTS][S::CHUNK];
+// A step per chunk c: behind its barrier, which every wave's share of K(c) and V(c - 1) has landed before, K(c + 1) and V(c) are
+// asked for; then the values of chunk c - 1, the scores of chunk c and their softmax. Of a workgroup that has the CU alone (head
+// dim 512) the waves of the second half, which share the SIMDs with those of the first, take the softmax of chunk c - 1
+// first: one runs MFMAs while the other runs vector work (8 x 4096 tokens of 8 heads 1098 us, 1112 without). Chunks of which a
+// wave sees nothing it skips.
+template <int D>
+__global__ __launch_bounds__(Shape<D>::NW * 64, 2) void packed_prefill_kernel(G4PackedPrefillArgs a, Group group) {
+  using S = Shape<D>;
+  constexpr int NB = S::NB, NW = S::NW, KS = S::KS, VT = S::T;
+  // K in slots 0 and 1, V^T in 2 and 3, chunk c in slot (c - c_begin) % 2 of its ring; read with inline-assembly LDS reads only:
+  // the compiler adds no waits of its own for the DMAs in flight
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[4][S::CHUNK];
   __shared__ int2 spans[NW], bounds[NW * NB * 16];
 
   const int R = a.group, H = a.kv_heads, T = a.tokens;
@@ -229,18 +239,27 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPref
 
   Rows rows{lds_addr(&bounds[w * NB * 16]), 0x7fffffff, -1, 0, 0x7fffffff};
   bf16x8 qop[NB][KS];
+  int token[NB], start[NB];
 #pragma unroll
   for (int cb = 0; cb < NB; ++cb) {
-    // rows behind the last token read the last row and are not stored
-    const int row = row0 + cb * 16 + col, t = group.token(row);
-    const int64_t at = (int64_t)min(row, T * R - 1);  // flat over (t, r) of a head
-    const int tq = min(t, T - 1);
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (at + ((int64_t)tq * (H - 1) + h) * R) * D;
-    const int start = a.starts[tq];
+    token[cb] = group.token(row0 + cb * 16 + col);
+    start[cb] = a.starts[min(token[cb], T - 1)];
+  }
+  __builtin_amdgcn_sched_barrier(0);  // the starts are asked for, and so arrive, before q
+#pragma unroll
+  for (int cb = 0; cb < NB; ++cb) {
+    // rows behind the last token read the last row and are not stored; flat over (t, r) of a head
+    const int64_t at = (int64_t)min(row0 + cb * 16 + col, T * R - 1);
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (at + ((int64_t)min(token[cb], T - 1) * (H - 1) + h) * R) * D;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qop[cb][s] = as_bf16x8(load16(q + 32 * s + 8 * grp));
-    const bool has_keys = t < T && start >= 0 && start <= t;
-    const int lo = has_keys ? max(start, a.window > 0 ? t - a.window + 1 : 0) : 0, hi = has_keys ? t : -1;
+  }
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int cb = 0; cb < NB; ++cb) {
+    const int t = token[cb];
+    const bool has_keys = t < T && start[cb] >= 0 && start[cb] <= t;
+    const int lo = has_keys ? max(start[cb], a.window > 0 ? t - a.window + 1 : 0) : 0, hi = has_keys ? t : -1;
     if (grp == 0) bounds[(w * NB + cb) * 16 + col] = make_int2(lo, hi);
     if (has_keys) {
       rows.first = min(rows.first, lo);
@@ -255,17 +274,8 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPref
   rows.last = columns_reduce(rows.last, most);
   rows.all_from = columns_reduce(rows.all_from, most);
   rows.all_to = columns_reduce(rows.all_to, least);
-  // the q operands have landed here, not inside the loop, where their wait would drain the DMAs in flight
-#pragma unroll
-  for (int cb = 0; cb < NB; ++cb)
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      u32x4 v = __builtin_bit_cast(u32x4, qop[cb][s]);
-      __asm__ volatile("" : "+v"(v));
-      qop[cb][s] = as_bf16x8(v);
-    }
   if (lane == 0) spans[w] = make_int2(rows.first, rows.last);
-  __syncthreads();
+  wg_barrier();  // (q is still on its way)
   int first = 0x7fffffff, last = -1;
 #pragma unroll
   for (int i = 0; i < NW; ++i) first = min(first, spans[i].x), last = max(last, spans[i].y);
@@ -303,44 +313,36 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPref
     for (int i = 0; i < VT; ++i) oacc[cb][i] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   if (c_begin <= c_end) {  // (uniform over the workgroup)
-    const bool lead = w < NW / 2;
-    // chunk j sits in slot (j - c_begin) % SLOTS of both rings (V^T behind K); K(c) and V(c - 1) are read in step c
-    // only, whose barrier queues K(c + SLOTS - 1) and V(c + SLOTS - 2) into the slots that step c - 1 finished reading
-    auto wait_step = [&](int c) {
-      constexpr int n = S::TW;
-      if (SLOTS == 2) wait_vmcnt<0>();
-      else if (c + 2 <= c_end) wait_vmcnt<4 * n>();
-      else if (c + 1 <= c_end) wait_vmcnt<3 * n>();
-      else wait_vmcnt<n>();
-      wg_barrier();
-    };
+    const bool late = NW == 8 && w >= NW / 2;
     floatx4 acc[NB][2];
     bf16x8 pop[NB];
     issue_k(c_begin, 0);
-    if constexpr (SLOTS == 4) {
-      if (c_begin + 1 <= c_end) issue_k(c_begin + 1, 1);
-      issue_v(c_begin, SLOTS);
-      if (c_begin + 2 <= c_end) issue_k(c_begin + 2, 2);
-      if (c_begin + 1 <= c_end) issue_v(c_begin + 1, SLOTS + 1);
-    }
+    // the q operands have landed here, not inside the loop, where their wait would drain the DMAs in flight
+#pragma unroll
+    for (int cb = 0; cb < NB; ++cb)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        u32x4 v = __builtin_bit_cast(u32x4, qop[cb][s]);
+        __asm__ volatile("" : "+v"(v));
+        qop[cb][s] = as_bf16x8(v);
+      }
 #pragma unroll 1
     for (int c = c_begin, i = 0; c <= c_end; ++c, ++i) {
-      wait_step(c);
-      if (c + SLOTS - 1 <= c_end) issue_k(c + SLOTS - 1, (i + SLOTS - 1) & (SLOTS - 1));
-      if (c + SLOTS - 2 <= c_end) issue_v(c + SLOTS - 2, SLOTS + ((i + SLOTS - 2) & (SLOTS - 1)));
+      wait_vmcnt<0>();
+      wg_barrier();
+      if (c + 1 <= c_end) issue_k(c + 1, (i + 1) & 1);
+      issue_v(c, 2 + (i & 1));
       const bool before = c > c_begin && rows.any(c - 1), now = rows.any(c);
-      if (!lead && before) soft.chunk(rows, c - 1, lane, acc, pop, oacc);
-      __builtin_amdgcn_s_setprio(1);
-      if (before) pf_pv<VT, NB, 4>(ring0 + (uint32_t)((SLOTS + ((i - 1) & (SLOTS - 1))) * S::CHUNK), pop, oacc);
-      if (now) pf_qk<VT, KS, NB, 4>(ring0 + (uint32_t)((i & (SLOTS - 1)) * S::CHUNK), qop, acc);
-      __builtin_amdgcn_s_setprio(0);
-      if (lead && now) soft.chunk(rows, c, lane, acc, pop, oacc);
+      if (late && before) soft.chunk(rows, c - 1, lane, acc, pop, oacc);
+      if (before) pf_pv<VT, NB, 4>(ring0 + (uint32_t)((2 + ((i - 1) & 1)) * S::CHUNK), pop, oacc);
+      if (now) pf_qk<VT, KS, NB, 4>(ring0 + (uint32_t)((i & 1) * S::CHUNK), qop, acc);
+      if (!late && now) soft.chunk(rows, c, lane, acc, pop, oacc);
     }
     wait_vmcnt<0>();
     wg_barrier();
     if (rows.any(c_end)) {
-      if (!lead) soft.chunk(rows, c_end, lane, acc, pop, oacc);
-      pf_pv<VT, NB, 4>(ring0 + (uint32_t)((SLOTS + ((c_end - c_begin) & (SLOTS - 1))) * S::CHUNK), pop, oacc);
+      if (late) soft.chunk(rows, c_end, lane, acc, pop, oacc);
+      pf_pv<VT, NB, 4>(ring0 + (uint32_t)((2 + ((c_end - c_begin) & 1)) * S::CHUNK), pop, oacc);
     }
   }
 
@@ -395,11 +397,10 @@ __global__ __launch_bounds__(NW * 64, 2) void packed_prefill_kernel(G4PackedPref
 
 template <int D>
 int launch_packed(const G4PackedPrefillArgs& a, hipStream_t st) {
-  using S = Shape<D, D == 512 ? 1 : 2, D == 512 ? 8 : 4, 2>;
+  using S = Shape<D>;
   const int64_t blocks = ((int64_t)a.tokens * a.group + S::ROWS - 1) / S::ROWS * a.kv_heads;
   if (blocks * S::NW * 64 > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "g4_packed_prefill_attention: too many tokens");
-  hipLaunchKernelGGL((packed_prefill_kernel<D, S::NB, S::NW, S::SLOTS>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a,
-                     Group(a.group));
+  hipLaunchKernelGGL(packed_prefill_kernel<D>, dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a, Group(a.group));
   return check_launch("g4_packed_prefill_attention");
 }
 
