@@ -108,8 +108,8 @@ class G4PagedCompactArgs(ctypes.Structure):
 class G4PackedPrefillArgs(ctypes.Structure):
     _fields_ = [
         ("tokens", c_int32), ("kv_heads", c_int32), ("group", c_int32), ("head_dim", c_int32), ("window", c_int32),
-        ("k_stride", c_int32), ("starts", c_void_p), ("q", c_void_p), ("k", c_void_p), ("vt", c_void_p),
-        ("out", c_void_p),
+        ("k_stride", c_int32), ("longest", c_int32), ("starts", c_void_p), ("q", c_void_p), ("k", c_void_p),
+        ("vt", c_void_p), ("out", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
     ]
 
 
@@ -219,6 +219,7 @@ PROTOTYPES = {
     "g4_decode_attention": (c_int32, [POINTER(G4DecodeArgs), c_void_p]),
     "g4_decode_attention_noalloc": (c_int32, [POINTER(G4DecodeArgs), c_void_p]),
     "g4_prefill_attention": (c_int32, [POINTER(G4PrefillArgs), c_void_p]),
+    "g4_packed_prefill_workspace_size": (c_size_t, [POINTER(G4PackedPrefillArgs)]),
     "g4_packed_prefill_attention": (c_int32, [POINTER(G4PackedPrefillArgs), c_void_p]),
     "g4_packed_starts": (c_int32, [c_int32, c_void_p, c_int32, c_void_p, c_void_p]),
     "g4_paged_append": (c_int32, [POINTER(G4PagedAppendArgs), c_void_p]),

@@ -16,6 +16,8 @@
 // NaN and infinities in keys that a row does not see must not reach it: a masked score is replaced, not multiplied, but a
 // masked p = 0 times a NaN value is NaN. A wave whose accumulators are not all finite forms them again from
 // memory, key by key where a chunk holds such values (`careful_values`), which costs other calls one look at the accumulators.
+#include <algorithm>
+
 #include "g4_attn_tiles.h"
 #include "g4_common.h"
 #include "g4_internal.h"
@@ -32,8 +34,10 @@ constexpr float kSlack = 8.0f;
 // chunks of LDS each, 64 KiB at 256. (8 x 4096 tokens of 2 x 4 heads of 256: 506 us; one workgroup of eight waves with
 // four chunks of each 586, of one block per wave 589.) Head dim 512, whose K and V^T take 128 KiB: eight waves of one block.
 template <int D>
+constexpr int kWaves = D == 512 ? 8 : 4;
+template <int D, int NB_>
 struct Shape {
-  static constexpr int NB = D == 512 ? 1 : 2, NW = D == 512 ? 8 : 4;
+  static constexpr int NB = NB_, NW = kWaves<D>;
   static constexpr int KS = D / 32;
   static constexpr int T = D / 16;                  // 1 KiB operand tiles of a chunk's K and of its V^T
   static constexpr int CHUNK = T * 1024;
@@ -215,24 +219,39 @@ __device__ __forceinline__ void place_block(int i, int n_blk, int H, int& blk, i
   blk = n_blk - 1 - (run * kRun + rest - h * len);
 }
 
+// Where few blocks would leave CUs idle for long, a block's chunks are taken in pieces, a workgroup each, whose sums a second
+// launch joins; a block that has chunks for one piece only writes its result itself.
+constexpr int kMostPieces = 16;
+struct Piece {
+  float m, l;   // row maximum in use, sum
+  int pieces;   // of the row's block (in piece 0's; 1: nothing to join)
+  int pad;
+};
+struct Pieces {
+  float* o;      // [most][H][padded rows][D], not divided by the sums
+  Piece* stats;  // [most][H][padded rows]
+  int most, chunks;  // pieces of a block at most; chunks of each, the last's maybe more
+};
+
 // A step per chunk c: behind its barrier, which every wave's share of K(c) and V(c - 1) has landed before, K(c + 1) and V(c) are
 // asked for; then the values of chunk c - 1, the scores of chunk c and their softmax. Of a workgroup that has the CU alone (head
 // dim 512) the waves of the second half, which share the SIMDs with those of the first, take the softmax of chunk c - 1
 // first: one runs MFMAs while the other runs vector work (8 x 4096 tokens of 8 heads 1098 us, 1112 without). Chunks of which a
 // wave sees nothing it skips.
-template <int D>
-__global__ __launch_bounds__(Shape<D>::NW * 64, 2) void packed_prefill_kernel(G4PackedPrefillArgs a, Group group) {
-  using S = Shape<D>;
-  constexpr int NB = S::NB, NW = S::NW, KS = S::KS, VT = S::T;
+template <int D, int NB, bool CUT>
+__global__ __launch_bounds__(kWaves<D> * 64, 2) void packed_prefill_kernel(G4PackedPrefillArgs a, Group group, Pieces pieces) {
+  using S = Shape<D, NB>;
+  constexpr int NW = S::NW, KS = S::KS, VT = S::T;
   // K in slots 0 and 1, V^T in 2 and 3, chunk c in slot (c - c_begin) % 2 of its ring; read with inline-assembly LDS reads only:
   // the compiler adds no waits of its own for the DMAs in flight
   __shared__ __attribute__((aligned(1024))) unsigned char ring[4][S::CHUNK];
   __shared__ int2 spans[NW], bounds[NW * NB * 16];
 
   const int R = a.group, H = a.kv_heads, T = a.tokens;
-  const int n_blk = (int)(gridDim.x / (unsigned)H);
+  const int n_blk = (int)(gridDim.x / (unsigned)(CUT ? H * pieces.most : H));
+  const int piece = CUT ? (int)(blockIdx.x / (unsigned)(n_blk * H)) : 0;
   int blk, h;
-  place_block((int)blockIdx.x, n_blk, H, blk, h);
+  place_block((int)blockIdx.x - piece * n_blk * H, n_blk, H, blk, h);
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row0 = blk * S::ROWS + w * (NB * 16);
@@ -280,7 +299,16 @@ __global__ __launch_bounds__(Shape<D>::NW * 64, 2) void packed_prefill_kernel(G4
 #pragma unroll
   for (int i = 0; i < NW; ++i) first = min(first, spans[i].x), last = max(last, spans[i].y);
   // chunks c_begin .. c_end (none: c_begin > c_end); keys < T <= k_stride
-  const int c_begin = __builtin_amdgcn_readfirstlane(first) >> 5, c_end = __builtin_amdgcn_readfirstlane(last) >> 5;
+  int c_begin = __builtin_amdgcn_readfirstlane(first) >> 5, c_end = __builtin_amdgcn_readfirstlane(last) >> 5;
+  int n_pieces = 1;
+  if constexpr (CUT) {
+    n_pieces = c_begin > c_end ? 1 : min((c_end - c_begin) / pieces.chunks + 1, pieces.most);
+    if (piece >= n_pieces) return;  // (the whole workgroup)
+    c_begin += piece * pieces.chunks;
+    if (piece < n_pieces - 1) c_end = c_begin + pieces.chunks - 1;  // (the last takes what is left)
+    rows.first = max(rows.first, c_begin << 5);
+    rows.last = min(rows.last, (c_end << 5) + 31);
+  }
 
   const int64_t plane = (int64_t)h * a.k_stride * D;
   const __amdgpu_buffer_rsrc_t rk = make_rsrc(reinterpret_cast<const uint16_t*>(a.k) + plane, (uint32_t)a.k_stride * D * 2u);
@@ -346,6 +374,31 @@ __global__ __launch_bounds__(Shape<D>::NW * 64, 2) void packed_prefill_kernel(G4
     }
   }
 
+  if (CUT && n_pieces > 1) {  // what this piece's keys give, for the join
+    const int64_t base = ((int64_t)piece * H + h) * ((int64_t)n_blk * S::ROWS) + row0;
+#pragma unroll
+    for (int cb = 0; cb < NB; ++cb) {
+      float l = column_sum(soft.l[cb]);
+      if (rows.keys(cb, col).y < 0) l = 0.f;  // (chunks that all other rows see whole were not masked)
+      const int64_t row = base + cb * 16 + col;
+      if (grp == 0) pieces.stats[row] = Piece{soft.m[cb], l, n_pieces, 0};
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < VT; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = fmaf(oacc[cb][i][e], 0.f, sum);
+        *reinterpret_cast<floatx4*>(pieces.o + row * D + 16 * i + 4 * grp) = oacc[cb][i];
+      }
+      if (__any(!(sum == 0.f))) {
+        const int g = min(row0 + cb * 16 + col, T * R - 1), t = group.token(g);
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (((int64_t)t * H + h) * R + (g - t * R)) * D;
+#pragma unroll 1
+        for (int i = 0; i < VT; ++i)
+          *reinterpret_cast<floatx4*>(pieces.o + row * D + 16 * i + 4 * grp) = careful_values<D>(rows, cb, soft.base(cb), q, rk, rv, i);
+      }
+    }
+    return;
+  }
   // The result through LDS (the rings are done with), where the lanes' 4-dim pieces become whole rows: 16 bytes a lane,
   // a row's 16-byte units turned by its number so that neither side meets a bank twice. The rows' places are computed afresh (the
   // lane is hidden from the compiler), not kept in registers since the q loads.
@@ -358,6 +411,7 @@ __global__ __launch_bounds__(Shape<D>::NW * 64, 2) void packed_prefill_kernel(G4
   for (int cb = 0; cb < NB; ++cb) {
     const float l = column_sum(soft.l[cb]);
     const int row = row0 + cb * 16 + (lane_o & 15), t = group.token(row);
+    if (CUT && lane_o < 16) pieces.stats[(int64_t)h * ((int64_t)n_blk * S::ROWS) + row] = Piece{0.f, 0.f, 1, 0};  // nothing to join
     const bool none = rows.keys(cb, lane_o & 15).y < 0 || l == 0.f;
     const float inv = none ? 0.f : 1.0f / l;
     const auto pack = [&](floatx4 x) {
@@ -395,13 +449,124 @@ __global__ __launch_bounds__(Shape<D>::NW * 64, 2) void packed_prefill_kernel(G4
   }
 }
 
+// A row's result from its pieces', one wave per row: each piece's sums weigh exp(its maximum - the largest).
 template <int D>
-int launch_packed(const G4PackedPrefillArgs& a, hipStream_t st) {
-  using S = Shape<D>;
-  const int64_t blocks = ((int64_t)a.tokens * a.group + S::ROWS - 1) / S::ROWS * a.kv_heads;
-  if (blocks * S::NW * 64 > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "g4_packed_prefill_attention: too many tokens");
-  hipLaunchKernelGGL(packed_prefill_kernel<D>, dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a, Group(a.group));
-  return check_launch("g4_packed_prefill_attention");
+__global__ __launch_bounds__(256) void packed_join_kernel(G4PackedPrefillArgs a, Group group, Pieces pieces, int64_t padded) {
+  constexpr int PER = D / 64;
+  const int lane = threadIdx.x & 63, H = a.kv_heads, R = a.group;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (int64_t)a.tokens * R;
+  if (i >= rows * H) return;
+  const int h = (int)(i / rows), row = (int)(i - h * rows);
+  const int n = __builtin_amdgcn_readfirstlane(pieces.stats[h * padded + row].pieces);  // (one row per wave)
+  if (n <= 1) return;
+  Piece p{kNegInf, 0.f, 0, 0};
+  if (lane < n) p = pieces.stats[((int64_t)lane * H + h) * padded + row];
+  const bool none = p.l == 0.f;  // (a row of no sequence, no key of the row here, or scores of -inf alone)
+  const float top = wave_max(none ? kNegInf : p.m);
+  const float weight = none ? 0.f : __builtin_amdgcn_exp2f((p.m - top) * kLog2e);
+  const float l = wave_sum(none ? 0.f : weight * p.l);
+  const bool some = __any(!none);
+  float o[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o[e] = 0.f;
+#pragma unroll 1
+  for (int s = 0; s < n; s += 4) {  // four loads in flight
+    float x[4][PER];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      __builtin_memcpy(x[j], __builtin_assume_aligned(pieces.o + (((int64_t)min(s + j, n - 1) * H + h) * padded + row) * D + lane * PER,
+                                                      PER * 4), PER * 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (s + j >= n) break;
+      const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), s + j));
+#pragma unroll
+      for (int e = 0; e < PER; ++e) o[e] = fmaf(w, x[j][e], o[e]);
+    }
+  }
+  const float inv = some ? 1.0f / l : 0.f;
+  const int t = group.token(row);
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (((int64_t)t * H + h) * R + (row - t * R)) * D + lane * PER;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) o[e] = some ? o[e] * inv : 0.f;
+  if constexpr (PER == 1) {
+    *out = (uint16_t)f32_to_bf16_bits(o[0]);
+  } else {
+    uint32_t x[PER / 2];
+#pragma unroll
+    for (int e = 0; e < PER / 2; ++e) x[e] = pack_bf16x2(o[2 * e], o[2 * e + 1]);
+    __builtin_memcpy(__builtin_assume_aligned(out, PER * 2), x, PER * 2);
+  }
+}
+
+// How a call is laid out. A wave takes one column block where the blocks of two would not fill the CUs more than once: more,
+// smaller workgroups then end sooner (one prompt of 500 tokens, 2 x 4 heads of 256: 16 us, 23 with two; of 8000 265 and 299; 160
+// prompts of 60 .. 140 tokens, more blocks than that, 40 and 36).
+// Pieces: only where whole blocks leave CUs free and the longest sequence has 768 tokens (one of 600, 4 x 4 heads of 128: 15.6
+// us in pieces, 13.4 whole; of 1000, 2 x 4 of 256, 23 and 28) that a window does not cut (4000 with window 512: 53 and 26).
+// As many as the CUs take at once, of 8 chunks or more: each piece's sums cost a pass through memory (one prompt of 2000, 2
+// x 4 heads of 256: whole 50, in 2 pieces 41, in 4 46 us; 1 head: whole 48, 8 pieces 20). Where the pieces stay long, of 32
+// chunks or more, twice that, as the blocks with the most keys come first and the rest fill up behind them (one of 8000, 1
+// x 2 heads of 128: whole 128, 2 pieces 81, 4 66; one of 4000, 8 heads of 512: whole 198, 2 pieces 163).
+struct Plan {
+  int nb, most, chunks;    // column blocks per wave; pieces of a block at most (1: whole blocks), chunks of one
+  int64_t blocks, padded;  // workgroups without pieces; rows per head, the last block's filled up
+};
+Plan plan_of(const G4PackedPrefillArgs& a) {
+  const int D = a.head_dim, nw = D == 512 ? kWaves<512> : kWaves<64>;
+  const int64_t rows = (int64_t)a.tokens * a.group, resident = D == 512 ? 256 : 512;
+  const auto per_head = [&](int nb) { return (rows + nw * nb * 16 - 1) / (nw * nb * 16); };
+  Plan p{};
+  p.nb = D == 512 || per_head(2) * a.kv_heads <= resident ? 1 : 2;
+  p.blocks = per_head(p.nb) * a.kv_heads;
+  p.padded = per_head(p.nb) * nw * p.nb * 16;
+  p.most = 1;
+  const int64_t longest = a.longest > 0 && a.longest < a.tokens ? a.longest : a.tokens, chunks = (longest + 31) / 32;
+  if (p.nb == 1 && p.blocks < resident && chunks >= 24 && !(a.window > 0 && a.window < longest)) {
+    const int64_t most = std::min<int64_t>(kMostPieces, std::max(std::min(resident / p.blocks, chunks / 8),
+                                                                std::min(2 * resident / p.blocks, chunks / 32)));
+    if (most > 1) {
+      p.chunks = (int)((chunks + most - 1) / most);
+      p.most = (int)((chunks + p.chunks - 1) / p.chunks);
+    }
+  }
+  return p;
+}
+
+size_t carve(Pieces& p, void* base, const G4PackedPrefillArgs& a, const Plan& plan) {
+  const int64_t rows = (int64_t)plan.most * a.kv_heads * plan.padded;
+  p.most = plan.most;
+  p.chunks = plan.chunks;
+  p.o = static_cast<float*>(base);
+  p.stats = reinterpret_cast<Piece*>(p.o + rows * a.head_dim);
+  return plan.most > 1 ? (size_t)rows * (a.head_dim * 4 + sizeof(Piece)) : 0;
+}
+
+template <int D, int NB>
+int launch_packed(const G4PackedPrefillArgs& a, const Plan& plan, const Pieces& pieces, hipStream_t st) {
+  static const char who[] = "g4_packed_prefill_attention";
+  using S = Shape<D, NB>;
+  const int64_t blocks = plan.blocks * plan.most;
+  if (blocks * S::NW * 64 > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  const Group group(a.group);
+  if (plan.most == 1) {
+    hipLaunchKernelGGL((packed_prefill_kernel<D, NB, false>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a, group, pieces);
+    return check_launch(who);
+  }
+  if constexpr (NB == 1) {
+    hipLaunchKernelGGL((packed_prefill_kernel<D, 1, true>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a, group, pieces);
+    const int rc = check_launch(who);
+    if (rc != G4_OK) return rc;
+    const int64_t rows = (int64_t)a.tokens * a.group * a.kv_heads;
+    hipLaunchKernelGGL(packed_join_kernel<D>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, group, pieces, plan.padded);
+  }
+  return check_launch(who);
+}
+template <int D>
+int launch_packed(const G4PackedPrefillArgs& a, const Plan& plan, const Pieces& pieces, hipStream_t st) {
+  if constexpr (D != 512)
+    if (plan.nb == 2) return launch_packed<D, 2>(a, plan, pieces, st);
+  return launch_packed<D, 1>(a, plan, pieces, st);
 }
 
 // starts[t]: the first token of t's sequence, -1 behind the last sequence. One thread per token, a binary search.
@@ -435,9 +600,9 @@ extern "C" int g4_packed_prefill_attention(const G4PackedPrefillArgs* args, void
   static const char who[] = "g4_packed_prefill_attention";
   if (!args) return fail(G4_ERR_INVALID, "%s: args is NULL", who);
   const G4PackedPrefillArgs& a = *args;
-  if (a.tokens <= 0 || a.kv_heads <= 0 || a.group <= 0 || a.window < 0)
-    return fail(G4_ERR_INVALID, "%s: tokens %d, kv_heads %d, group %d must be positive, window %d not negative", who, a.tokens,
-                a.kv_heads, a.group, a.window);
+  if (a.tokens <= 0 || a.kv_heads <= 0 || a.group <= 0 || a.window < 0 || a.longest < 0)
+    return fail(G4_ERR_INVALID, "%s: tokens %d, kv_heads %d, group %d must be positive, window %d, longest %d not negative", who,
+                a.tokens, a.kv_heads, a.group, a.window, a.longest);
   if (a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256 && a.head_dim != 512)
     return fail(G4_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128, 256 or 512)", who, a.head_dim);
   if (a.group > 64) return fail(G4_ERR_UNSUPPORTED, "%s: group %d (at most 64)", who, a.group);
@@ -449,11 +614,24 @@ extern "C" int g4_packed_prefill_attention(const G4PackedPrefillArgs* args, void
   // a head's keys are addressed by 32-bit byte offsets, rows by 32-bit indexes
   if ((int64_t)a.k_stride * a.head_dim * 2 > 0xffffffffLL || (int64_t)a.tokens * a.group > 0x7fffffffLL - 1024)
     return fail(G4_ERR_UNSUPPORTED, "%s: too many tokens (%d of %d x %d rows of %d)", who, a.tokens, a.kv_heads, a.group, a.head_dim);
+  const Plan plan = plan_of(a);
+  Pieces pieces;
+  const size_t need = carve(pieces, a.workspace, a, plan);
+  if (need && (!a.workspace || a.workspace_bytes < need))
+    return fail(G4_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, a.workspace ? a.workspace_bytes : 0, need);
+  if (need && (uintptr_t)a.workspace % 16) return fail(G4_ERR_INVALID, "%s: workspace must be 16-byte aligned", who);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   switch (a.head_dim) {
-    case 64: return launch_packed<64>(a, st);
-    case 128: return launch_packed<128>(a, st);
-    case 256: return launch_packed<256>(a, st);
-    default: return launch_packed<512>(a, st);
+    case 64: return launch_packed<64>(a, plan, pieces, st);
+    case 128: return launch_packed<128>(a, plan, pieces, st);
+    case 256: return launch_packed<256>(a, plan, pieces, st);
+    default: return launch_packed<512>(a, plan, pieces, st);
   }
+}
+
+extern "C" size_t g4_packed_prefill_workspace_size(const G4PackedPrefillArgs* args) {
+  using namespace g4;
+  if (!args || args->tokens <= 0 || args->kv_heads <= 0 || args->group <= 0 || args->head_dim <= 0) return 0;
+  Pieces pieces;
+  return carve(pieces, nullptr, *args, plan_of(*args));
 }

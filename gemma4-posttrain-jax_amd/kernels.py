@@ -361,11 +361,12 @@ def packed_starts(cu_seqlens: torch.Tensor, tokens: int) -> torch.Tensor:
 
 
 def packed_prefill_attention(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, starts: torch.Tensor, *,
-                             window: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+                             window: int = 0, longest: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
     """g4_packed_prefill_attention: causal attention of prompts that stand one behind the other without pads. q ``[T,
     Hkv, R, D]`` bf16, k ``key_shape(1, Hkv, Sp, D)`` and vt ``[1, Hkv, Sp / 8, D, 8]`` (a ``kv_append`` of the T tokens as one
     row; Sp >= T, multiple of 64), ``starts`` int32 ``[T]`` of ``packed_starts``; with ``window`` > 0 the last
-    ``window`` tokens. Returns ``[T, Hkv, R, D]``, zeros for tokens of no sequence."""
+    ``window`` tokens. ``longest``, the longest sequence's tokens where the caller knows them, only chooses how the work
+    is split. Returns ``[T, Hkv, R, D]``, zeros for tokens of no sequence."""
 
     if q.dim() != 4 or q.dtype is not _BF16 or not q.is_contiguous():
         raise ValueError("q must be a contiguous bfloat16 [T, Hkv, R, D] tensor")
@@ -381,15 +382,21 @@ def packed_prefill_attention(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor,
         raise ValueError(f"starts must be a contiguous int32 [{T}] tensor")
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
+    if longest < 0:
+        raise ValueError(f"longest must not be negative, got {longest}")
     if out is not None and (out.shape != q.shape or out.dtype is not _BF16 or not out.is_contiguous()):
         raise ValueError("out must be a contiguous bfloat16 [T, Hkv, R, D] tensor")
     dev = _device_of((q, k, vt, starts, out))
     if out is None:
         out = torch.empty_like(q)
-    a = _lib.G4PackedPrefillArgs(T, H, R, D, window, Sp, starts.data_ptr(), q.data_ptr(), k.data_ptr(), vt.data_ptr(),
-                                 out.data_ptr())
-    _lib.check(_lib.lib().g4_packed_prefill_attention(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev)),
-               "g4_packed_prefill_attention")
+    a = _lib.G4PackedPrefillArgs(T, H, R, D, window, Sp, longest, starts.data_ptr(), q.data_ptr(), k.data_ptr(),
+                                 vt.data_ptr(), out.data_ptr(), None, 0)
+    lib, ref = _lib.lib(), ctypes.byref(a)
+    need = lib.g4_packed_prefill_workspace_size(ref)
+    if need:
+        ws = q.new_empty(need, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
+    _lib.check(lib.g4_packed_prefill_attention(ref, torch._C._cuda_getCurrentRawStream(dev)), "g4_packed_prefill_attention")
     return out
 
 

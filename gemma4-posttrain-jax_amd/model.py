@@ -613,7 +613,8 @@ def forward_gemma4_text(
                                      keep=keep if window else 0, flags=flags, k_norm_weight=qk_norms[1],
                                      q=q if flags & flags_q else None, q_out=q_out, **prep_q)
             if packed is not None:
-                attn = kernels.packed_prefill_attention(q_out[0], *prompt_kv[src], packed.starts, window=window)[None]
+                attn = kernels.packed_prefill_attention(q_out[0], *prompt_kv[src], packed.starts, window=window,
+                                                        longest=packed.longest)[None]
                 if src not in sources[i + 1:]:
                     del prompt_kv[src]
             elif cache_mode == "prefill":

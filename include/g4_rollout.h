@@ -254,7 +254,9 @@ int g4_prefill_attention(const G4PrefillArgs* args, void* stream);
  * or > t belongs to no sequence: its rows are zeros. bf16, f32 scores, softmax and sums; the unnormalised
  * probabilities are rounded to bf16 as the operand of the value product, the result once to bf16 (g4_prefill_attention
  * also rounds the scores, as the reference does). What a row does not see, NaN included, does not reach it; a row
- * whose scores are all -inf gives zeros. The same call gives the same bits. No workspace.
+ * whose scores are all -inf gives zeros. The same call gives the same bits. Few rows with many keys each are taken in
+ * pieces of the keys that a second launch joins: such calls need g4_packed_prefill_workspace_size() bytes of scratch
+ * (16-byte aligned, no state is kept in it). The sizes decide that, `longest` among them.
  */
 typedef struct G4PackedPrefillArgs {
   int32_t tokens;         /* T */
@@ -263,13 +265,17 @@ typedef struct G4PackedPrefillArgs {
   int32_t head_dim;       /* 64, 128, 256 or 512 */
   int32_t window;         /* 0 = every earlier token of the sequence */
   int32_t k_stride;       /* slots of k / vt: >= T, a multiple of 64; k_stride * head_dim * 2 < 2^32 */
+  int32_t longest;        /* tokens of the longest sequence, 0 = not known (T); a wrong value costs time only */
   const int32_t* starts;  /* device [T] */
   const void* q;          /* [T, Hkv, R, D]; q, k, vt and out 16-byte aligned */
   const void* k;          /* [1, Hkv, k_stride/32, D/32, 2, 16, 32]: the key layout above, token t in slot t */
   const void* vt;         /* [1, Hkv, k_stride/8, D, 8] */
   void* out;              /* [T, Hkv, R, D] */
+  void* workspace;
+  size_t workspace_bytes;
 } G4PackedPrefillArgs;
 
+size_t g4_packed_prefill_workspace_size(const G4PackedPrefillArgs* args);
 int g4_packed_prefill_attention(const G4PackedPrefillArgs* args, void* stream);
 
 /* starts[t] for t < tokens: cu_seqlens[i] of the sequence i with cu_seqlens[i] <= t < cu_seqlens[i + 1], -1 for none.

@@ -43,8 +43,9 @@ def test_the_rows_hold_their_prompt(kwargs, G, pads, S, steps, e4m3, device, mon
     lens = [S - p for p in pads]
     attend, calls = kernels.packed_prefill_attention, []
 
-    def checked(q, k, vt, starts, *, window):
-        out = attend(q, k, vt, starts, window=window)
+    def checked(q, k, vt, starts, *, window, longest):
+        assert longest == max(lens)
+        out = attend(q, k, vt, starts, window=window, longest=longest)
         T = q.shape[0]
         layer = new_layer_cache(1, q.shape[1], q.shape[3], T, False, BF16, device)._replace(key=k, value_t=vt)
         kk, vv = (t[0].cpu() for t in layer.reference_layout())

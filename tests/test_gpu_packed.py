@@ -3,12 +3,13 @@ groups, tokens of no sequence, and values that a row must not see."""
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
-from gemma4_posttrain_jax_amd import kernels
+from gemma4_posttrain_jax_amd import _lib, kernels
 from gemma4_posttrain_jax_amd.kvcache import group_keys, group_values, slot_stride_for
 from packed_util import packed_reference
 
@@ -158,3 +159,130 @@ def test_starts_that_are_none(device):
     none[[10, 20, 63]] = True
     assert bool((got[none] == 0).all())
     assert bool(((got - want).abs() <= bound)[~none].all())
+
+
+# --- few rows with many keys: pieces of the keys, joined --------------------------------------------------------------
+
+
+def _pieces(q, window=0, longest=0):
+    T, H, R, D = q.shape
+    a = _lib.G4PackedPrefillArgs(tokens=T, kv_heads=H, group=R, head_dim=D, window=window, longest=longest)
+    return _lib.lib().g4_packed_prefill_workspace_size(ctypes.byref(a))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("lens,tail,R,longest", [([1100], 0, 2, 0), ([900], 5, 8, 900), ([1, 800, 0, 31, 400, 33], 2, 3, 800),
+                                                 ([2500], 0, 1, 2500)])
+def test_keys_in_pieces(D, lens, tail, R, longest, device):
+    q, k, v = _inputs(lens, tail, 1, R, D, 11, device)
+    assert _pieces(q, 0, longest) > 0
+    got = _run(q, k, v, lens, 0, device, fill=math.nan, longest=longest)
+    _check(got, q, k, v, lens, 0)
+    again = _run(q, k, v, lens, 0, device, fill=math.nan, longest=longest)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("longest", [0, 1, 100, 770, 1000, 5000])
+def test_a_wrong_longest_costs_time_only(longest, device):
+    lens = [30, 1500, 7]
+    q, k, v = _inputs(lens, 3, 2, 2, 64, 12, device)
+    _check(_run(q, k, v, lens, 0, device, longest=longest), q, k, v, lens, 0)
+    _check(_run(q, k, v, lens, 900, device, longest=longest), q, k, v, lens, 900)
+
+
+@pytest.mark.parametrize("D,R", [(64, 2), (512, 1)])
+def test_pieces_of_many_sizes_of_score(D, R, device):
+    """Scores that rise or fall by hundreds along the keys: a piece's maximum is far below or above the others'."""
+
+    T = 1200
+    for sign in (1, -1):
+        q, k, v = _inputs([T], 0, 1, R, D, 13, device)
+        q[..., 0] = 1.0
+        k[..., 0] = (sign * torch.arange(T) / 4).to(torch.bfloat16)[:, None]
+        assert _pieces(q) > 0
+        _check(_run(q, k, v, [T], 0, device), q, k, v, [T], 0)
+
+
+def test_pieces_with_values_that_are_not_finite(device):
+    """A NaN or infinite value reaches the tokens behind it and no other; scores of -inf in whole pieces are as none."""
+
+    T, D = 1300, 64
+    q, k, v = _inputs([T], 0, 1, 2, D, 14, device)
+    assert _pieces(q) > 0
+    want, bound = packed_reference(q, k, v, [T], 0)
+    v[700, 0, 5], v[900, 0, 6] = math.nan, math.inf
+    got = _run(q, k, v, [T], 0, device).cpu().double()
+    assert bool(got[700:, ..., 5].isnan().all()) and bool((got[900:, ..., 6] == math.inf).all())
+    want[700:, ..., 5], want[900:, ..., 6] = 0, 0
+    got[700:, ..., 5], got[900:, ..., 6] = 0, 0
+    assert bool(((got - want).abs() <= bound).all())
+    q, k, v = _inputs([T], 0, 1, 2, D, 14, device)
+    q[..., 0] = 1.0
+    k[:800, :, 0] = -math.inf
+    got = _run(q, k, v, [T], 0, device)
+    assert bool((got[:800] == 0).all())
+    want, bound = packed_reference(q[800:], k[800:], v[800:], [T - 800], 0)
+    assert bool(((got[800:].cpu().double() - want).abs() <= bound).all())
+
+
+def test_pieces_in_a_graph_with_eager_calls_between(device):
+    lens = [1000, 300]
+    (q, k, v), (q2, k2, v2) = (_inputs(lens, 0, 1, 4, 256, s, device) for s in (15, 16))
+    a, b = _run(q, k, v, lens, 0, device), _run(q2, k2, v2, lens, 0, device)
+    starts = kernels.packed_starts(torch.tensor([0, 1000, 1300], dtype=torch.int32, device=device), 1300)
+    qd, (kk, vv) = q.to(device), _laid_out(k, v, device)
+    assert _pieces(q) > 0
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        kernels.packed_prefill_attention(qd, kk, vv, starts)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kernels.packed_prefill_attention(qd, kk, vv, starts)
+    new = (q2.to(device), *_laid_out(k2, v2, device))
+    old = (q.to(device), *_laid_out(k, v, device))
+    for replay in range(4):
+        for to, x in zip((qd, kk, vv), new if replay % 2 else old):
+            to.copy_(x)
+        graph.replay()
+        assert torch.equal(_run(q, k, v, lens, 0, device), a)
+        torch.cuda.synchronize()
+        assert torch.equal(out, b if replay % 2 else a)
+
+
+# --- many rows: two column blocks per wave -----------------------------------------------------------------------------
+
+
+MANY = [33, 0, 1, 130, 65, 2, 250, 31, 45]  # 557 tokens of 8 x 16 heads: 560 workgroups of 128 rows
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 40])
+def test_many_rows(D, window, device):
+    q, k, v = _inputs(MANY, 3, 8, 16, D, 21, device)
+    got = _run(q, k, v, MANY, window, device, fill=math.nan)
+    _check(got, q, k, v, MANY, window)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_rows_with_values_that_are_not_finite(D, device):
+    q, k, v = _inputs(MANY, 3, 8, 16, D, 22, device)
+    want, bound = packed_reference(q, k, v, MANY, 0)
+    v[180, 3, 5], v[400, 2, 6] = math.nan, math.inf  # in the 130 and the 250 tokens
+    got = _run(q, k, v, MANY, 0, device).cpu().double()
+    ends = [sum(MANY[:i + 1]) for i in range(len(MANY))]
+    for at, h, d in ((180, 3, 5), (400, 2, 6)):
+        end = next(e for e in ends if e > at)
+        assert not bool(got[at:end, h, :, d].isfinite().any())
+        got[at:end, h, :, d] = want[at:end, h, :, d] = 0
+    assert bool(((got - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("tokens", [511, 512, 513])
+def test_about_the_change_of_blocks(tokens, device):
+    """8 heads of 16: 512 workgroups of two blocks per wave at 512 tokens, one block per wave up to there."""
+
+    lens = [300, tokens - 300]
+    q, k, v = _inputs(lens, 0, 8, 16, 64, 23, device)
+    _check(_run(q, k, v, lens, 0, device), q, k, v, lens, 0)

@@ -59,9 +59,21 @@ def _packed(**kw):
     (dict(tokens=1 << 23, k_stride=1 << 23), "too many"),  # a head's keys of 2^32 bytes
     (dict(tokens=1 << 25, k_stride=1 << 25, head_dim=64, group=64), "too many"),  # 2^31 rows
     (dict(tokens=1 << 21, k_stride=1 << 21, kv_heads=1 << 13), "too many"),  # a grid of 2^32 threads
+    (dict(longest=-1), "longest"),
 ])
 def test_packed_attention_refuses(override, match):
     _refused("g4_packed_prefill_attention", _packed(**override), match)
+
+
+def test_packed_attention_refuses_a_short_workspace():
+    few = dict(tokens=1000, k_stride=1024, head_dim=64, kv_heads=1)
+    need = _lib.lib().g4_packed_prefill_workspace_size(*_packed(**few))
+    assert need > 0 and _lib.lib().g4_packed_prefill_workspace_size(None) == 0
+    for same in (dict(longest=100), dict(window=512), dict(tokens=700), dict(kv_heads=64)):
+        assert _lib.lib().g4_packed_prefill_workspace_size(*_packed(**{**few, **same})) == 0
+    for override in (dict(), dict(workspace=AT), dict(workspace=AT, workspace_bytes=need - 1), dict(workspace_bytes=need)):
+        _refused("g4_packed_prefill_attention", _packed(**few, **override), "workspace", (_lib.G4_ERR_WORKSPACE,))
+    _refused("g4_packed_prefill_attention", _packed(**few, workspace=AT + 4, workspace_bytes=need), "aligned")
 
 
 @pytest.mark.parametrize("args,match", [((0, AT, 5, AT), "0 sequences"), ((2, None, 5, AT), "NULL"), ((2, AT, 0, AT), "0 tokens"),
