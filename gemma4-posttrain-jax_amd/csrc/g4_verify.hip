@@ -3,9 +3,10 @@
 // inference from transformers via speculative decoding", ICML 2023): draft s is accepted while u_s q_s(x_s) < p_s(x_s); at the
 // first rejection the token is drawn from max(p - q, 0), after all drafts from p. The draw is the race of exponentials,
 // argmax_v w_v / -log(noise_v), which needs no normalisation and no running sum, so that f32 decides it as well as 64 bits
-// but for near ties.
+// but for near ties (p - q, too, is that of f32 probabilities: where all of it is below 1e-6 of p, its rounding decides).
 //
-// Bound by reading the logits: K + 1 target and K draft rows of the vocabulary once, for their maxima and sums of
+// Bound by reading the logits (64 rows of 9 x 262144 in bf16, 369 MB with the noise, 75 us: 4.9 TB/s) and, while it does, by
+// vector instructions: K + 1 target and K draft rows of the vocabulary once, for their largest logits and sums of
 // exponentials (a first launch, statistics per chunk of a row), then of two rows per b and the noise for the race (a
 // third). Which rows these are a launch between finds from the statistics; it also clears the counter by which the last of
 // a b's workgroups in the race, which writes the token, is found.
@@ -24,7 +25,7 @@ constexpr int kNoColumn = 0x7fffffff;
 enum Mode { kGreedy, kUnit, kHeat };  // temperature <= 0, 1, other
 
 struct Stats {  // of a chunk of a row, or of a row
-  float m;     // largest logit
+  float m;     // largest logit, or one at most kSlack below it (kGreedy: the largest)
   float heat;  // sum exp((x - m) / temperature)
   float unit;  // sum exp(x - m)
   int idx;     // kGreedy: the first column of the largest
@@ -34,7 +35,7 @@ struct Decision {  // of one b
   int32_t away;        // rejected without a drafter's logits: the draft's id, which has no weight; else -1
   int32_t residual;    // whether the drafter's row counts
   float unit;          // of the target's row: sum exp(x - m)
-  float pm, pz, qm, qz;  // largest logit and sum exp((x - m) / temperature) of both rows
+  float pm, pz, qm, qz;  // m and sum exp((x - m) / temperature) of both rows
 };
 struct VerifyWorkspace {
   Stats* stats;       // [batch][rows][splits], the K + 1 target rows first
@@ -44,11 +45,12 @@ struct VerifyWorkspace {
 };
 constexpr int kApart = 32;  // (counters that share lines: the race of 64 rows 51 us instead of 27)
 
-// Logits per workgroup: in the first launch 2^13 where that makes 2048 workgroups or more, else 2^12 (one row of 9 x 262144
-// is 576 of them); in the race 2^12. us per call, first launch / race in vectors of 8 per thread: 64 rows of 9 x 262144
-// 105 (8 / 4), 98 (4 / 2), 101 (8 / 2), 102 (4 / 4), 100 (4 / 1); one row 13.3 (2 / 1), 13.0 (2 / 2), 15.0 (1 / 1).
-constexpr int kLong = 4, kShort = 2;  // vectors of 8 per thread
-constexpr int kRace = 2;              // in the race
+// Logits per workgroup: in the first launch 2^14 where that makes 2048 workgroups or more, else 2^12 (one row of 9 x 262144
+// is 576 of them); in the race 2^12. A thread takes the 2^14 in two steps, all loads ahead of both. us per call, 64 rows of 9 x
+// 262144: first launch one step of 4 vectors of 8 per thread 81, two of 4 77, four of 4 79, two of 2 80; the race with 2
+// vectors 74.8, 1 77.7, 4 75.8. One row 13.3 (first launch 2 vectors, race 1), 12.8 (2 and 2), 15.0 (1 and 1).
+constexpr int kStep = 4, kSteps = 2, kLong = kStep * kSteps, kShort = 2;  // vectors of 8 per thread
+constexpr int kRace = 2;                                                  // in the race
 int vecs_of(const G4VerifyArgs& a) {
   const int64_t rows = (int64_t)a.batch * (a.drafts + 1 + (a.draft_logits ? a.drafts : 0));
   return rows * a.vocab >= 2048LL * kLong * 8 * kThreads ? kLong : kShort;
@@ -74,25 +76,34 @@ size_t carve(VerifyWorkspace& w, void* base, const G4VerifyArgs& a) {
 
 typedef u32x4 u32x4_anywhere __attribute__((aligned(2)));
 
-// 8 logits from p on, of which `n` are there (others -inf). Rows stand at any element: such loads need no alignment.
+// 8 logits as they stand in memory. Rows stand at any element: such loads need no alignment.
 // NT: past the caches (the first launch where it is long: 98 -> 94 us; short ones lose up to 1 us by it).
-template <bool BF16, bool NT = false>
-__device__ __forceinline__ void load8(const void* row, int64_t i, int n, float (&x)[8]) {
-  const auto load = [](const void* p) {
-    const u32x4_anywhere* q = static_cast<const u32x4_anywhere*>(p);
-    return NT ? __builtin_nontemporal_load(q) : *q;
-  };
-  if (n >= 8) {
+template <bool BF16>
+struct Eight {
+  u32x4 raw[BF16 ? 1 : 2];
+  template <bool NT = false>
+  __device__ __forceinline__ void load(const void* row, int64_t i) {
+    const u32x4_anywhere* p = reinterpret_cast<const u32x4_anywhere*>(static_cast<const char*>(row) + i * (BF16 ? 2 : 4));
+#pragma unroll
+    for (int j = 0; j < (BF16 ? 1 : 2); ++j) raw[j] = NT ? __builtin_nontemporal_load(p + j) : p[j];
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
     if constexpr (BF16) {
-      unpack8(load(static_cast<const uint16_t*>(row) + i), x);
+      unpack8(raw[0], x);
     } else {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const u32x4 v = load(static_cast<const float*>(row) + i + 4 * j);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) x[4 * j + q] = __uint_as_float(v[q]);
-      }
+      for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(raw[e >> 2][e & 3]);
     }
+  }
+};
+
+// The logits from i on, of which `n` are there (others -inf).
+template <bool BF16>
+__device__ __forceinline__ void load8(const void* row, int64_t i, int n, float (&x)[8]) {
+  if (n >= 8) {
+    Eight<BF16> v;
+    v.load(row, i);
+    v.values(x);
     return;
   }
 #pragma unroll
@@ -113,7 +124,7 @@ __device__ __forceinline__ int drafts_of(const G4VerifyArgs& a, int b) {
   return a.draft_lengths ? min(max(a.draft_lengths[b], 0), a.drafts) : a.drafts;
 }
 
-// exp(t c) for t <= 0 with c = 1 / temperature, c log2(e) held in two parts: the rounding of a large t c log2(e) would
+// exp(t c) for t c <= kSlack with c = 1 / temperature, c log2(e) held in two parts: the rounding of a large t c log2(e) would
 // be the result's largest error.
 struct Heat {
   float hi, lo;  // log2(e) / temperature
@@ -169,7 +180,54 @@ __device__ __forceinline__ float sum_exp(const float (&x)[VECS][8], float m, flo
   return sum;
 }
 
-template <bool BF16, int MODE, int VECS>
+// Of three floats that are no signalling NaN (fmaxf makes sure of that by an instruction each).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  __asm__("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
+// A thread's statistics, VECS vectors at a time. The vector work is as long as the loads: instructions count (81 -> 94 us with
+// fmaxf, the loads behind a bounds check each and the reduction over the workgroup after every 4 vectors). The largest logit that exponents refer to follows lazily: it stays while no
+// logit passes it by more than `slack` (exponents of at most kSlack), but for kGreedy, which asks for the largest itself.
+constexpr float kSlack = 8.f;
+template <int MODE, int VECS>
+struct Running {
+  Stats s{-__builtin_inff(), 0.f, 0.f, kNoColumn};
+  float m = kF32Min;  // s.m, finite where there is no logit but -inf
+  float c, slack;     // log2(e) / temperature
+  __device__ __forceinline__ Running(float temperature)
+      : c(kLog2e / temperature), slack(MODE == kGreedy ? 0.f : MODE == kHeat ? kSlack * fminf(temperature, 1.f) : kSlack) {}
+
+  __device__ __forceinline__ void take(const float (&x)[VECS][8], int64_t i, bool draft) {
+    float top = s.m;
+#pragma unroll
+    for (int v = 0; v < VECS; ++v)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        if (MODE == kGreedy) {
+#pragma unroll
+          for (int f = e; f < e + 2; ++f) {
+            if (x[v][f] > top) s.idx = (int)i + v * (kThreads * 8) + f;
+            top = fmaxf(top, x[v][f]);
+          }
+        } else {
+          top = max3(top, x[v][e], x[v][e + 1]);
+        }
+      }
+    if (top > s.m + slack) {
+      const float next = fmaxf(top, kF32Min);
+      if (MODE != kGreedy) s.heat *= __builtin_amdgcn_exp2f((m - next) * c);
+      if (MODE != kUnit) s.unit *= __builtin_amdgcn_exp2f((m - next) * kLog2e);
+      s.m = top;
+      m = next;
+    }
+    if (MODE != kGreedy) s.heat += sum_exp<VECS>(x, m, c);
+    if (MODE != kUnit && !draft) s.unit += sum_exp<VECS>(x, m, kLog2e);  // (the log-probabilities are the target's)
+  }
+};
+
+template <bool BF16, int MODE, int VECS, int TIMES>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(G4VerifyArgs a, VerifyWorkspace w, int rows, int splits) {
   __shared__ Stats part[kWaves];
   const int split = blockIdx.x % splits, br = blockIdx.x / splits, b = br / rows, r = br - b * rows;
@@ -178,31 +236,39 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(G4VerifyArgs a, 
   if (draft ? r - a.drafts - 1 >= n : r > n) return;  // (uniform) no draft reaches this row
   const void* row = draft ? row_at<BF16>(a.draft_logits, a.draft_batch_stride, a.draft_row_stride, b, r - a.drafts - 1)
                           : row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, r);
-  const float c = kLog2e / a.temperature;
-  const int64_t i0 = (int64_t)split * (VECS * kThreads * 8) + threadIdx.x * 8;
+  constexpr int STEP = kThreads * 8;
+  const int64_t from = (int64_t)split * (TIMES * VECS * STEP), i0 = from + threadIdx.x * 8;
+  Running<MODE, VECS> run(a.temperature);
   float x[VECS][8];
+  if (from + TIMES * VECS * STEP <= a.vocab) {  // (uniform) all there: all loads ahead of the work
+    Eight<BF16> raw[TIMES][VECS];
 #pragma unroll
-  for (int v = 0; v < VECS; ++v) {
-    const int64_t i = i0 + v * (kThreads * 8);
-    load8<BF16, VECS == kLong>(row, i, (int)min((int64_t)8, a.vocab - i), x[v]);
-  }
-  Stats s{-__builtin_inff(), 0.f, 0.f, kNoColumn};
+    for (int t = 0; t < TIMES; ++t)
 #pragma unroll
-  for (int v = 0; v < VECS; ++v)
+      for (int v = 0; v < VECS; ++v) raw[t][v].template load<(TIMES > 1)>(row, i0 + (t * VECS + v) * STEP);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (MODE == kGreedy && x[v][e] > s.m) s.idx = (int)(i0 + v * (kThreads * 8)) + e;
-      s.m = fmaxf(s.m, x[v][e]);
+    for (int t = 0; t < TIMES; ++t) {
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) raw[t][v].values(x[v]);
+      run.take(x, i0 + t * VECS * STEP, draft);
     }
-  const float m = fmaxf(s.m, kF32Min);
-  if (MODE != kGreedy) s.heat = sum_exp<VECS>(x, m, c);
-  if (MODE != kUnit && !draft) s.unit = sum_exp<VECS>(x, m, kLog2e);  // (the log-probabilities are the target's)
-  s = wave_join<MODE>(s, c);
+  } else {
+#pragma unroll 1
+    for (int t = 0; t < TIMES; ++t) {
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) {
+        const int64_t i = i0 + (t * VECS + v) * STEP;
+        load8<BF16>(row, i, (int)min((int64_t)8, a.vocab - i), x[v]);
+      }
+      run.take(x, i0 + t * VECS * STEP, draft);
+    }
+  }
+  Stats s = wave_join<MODE>(run.s, run.c);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x < 64) {
     static_assert(kWaves == 4, "lanes 0 .. 3 hold the waves'");
-    s = wave_join<MODE>(threadIdx.x < kWaves ? part[threadIdx.x] : Stats{-__builtin_inff(), 0.f, 0.f, kNoColumn}, c);
+    s = wave_join<MODE>(threadIdx.x < kWaves ? part[threadIdx.x] : Stats{-__builtin_inff(), 0.f, 0.f, kNoColumn}, run.c);
     if (MODE == kUnit) s.unit = s.heat;
     if (threadIdx.x == 0) w.stats[((int64_t)b * rows + r) * splits + split] = s;
   }
@@ -261,20 +327,20 @@ __device__ __forceinline__ Draft load_draft(const G4VerifyArgs& a, int b, int n)
 
 // How many drafts are accepted (by the first wave; lane s decides draft s).
 template <bool BF16, int MODE>
-__device__ __forceinline__ int accepted(const G4VerifyArgs& a, const Heat& heat, int n, const Draft& d, const Stats* st) {
+__device__ __forceinline__ int accepted(const G4VerifyArgs& a, int n, const Draft& d, const Stats* st) {
   const int s = threadIdx.x & 63;
   bool good = false;
   if (s < n) {
     if constexpr (MODE == kGreedy) {
       good = d.id == st[s].idx;
     } else if (d.there) {
-      const float p = heat.exp(d.x - st[s].m);
-      // u q < p, both sides times both sums (in 64 bits: neither overflows)
+      // u q < p, both sides times both sums, in 64 bits: neither over- nor underflows where the draft is unlikely
+      const double c = 1.0 / (double)a.temperature, p = exp(((double)d.x - st[s].m) * c);
       if (a.draft_logits) {
         const Stats& t = st[a.drafts + 1 + s];
-        good = (double)d.u * heat.exp(d.y - t.m) * st[s].heat < (double)p * t.heat;
+        good = d.u * exp(((double)d.y - t.m) * c) * st[s].heat < p * t.heat;
       } else {
-        good = (double)d.u * st[s].heat < (double)p;
+        good = (double)d.u * st[s].heat < p;
       }
     }
   }
@@ -302,14 +368,14 @@ __device__ __forceinline__ void write_token(const G4VerifyArgs& a, int b, int co
 // (Made by every workgroup of the race for itself it costs these 6 us at 64 rows, and one row no less than the launch, 3 us.)
 
 template <bool BF16, int MODE>
-__global__ __launch_bounds__(kThreads) void verify_decide_kernel(G4VerifyArgs a, VerifyWorkspace w, Heat heat, int rows, int splits) {
+__global__ __launch_bounds__(kThreads) void verify_decide_kernel(G4VerifyArgs a, VerifyWorkspace w, int rows, int splits) {
   __shared__ Stats st[2 * kMaxDrafts + 1];
   const int b = blockIdx.x;
   const int n = drafts_of(a, b);
   const Draft draft = load_draft<BF16, MODE>(a, b, threadIdx.x < 64 ? n : 0);
   join_rows<MODE>(a, w, b, rows, splits, n, st);
   if (threadIdx.x >= 64) return;
-  const int count = accepted<BF16, MODE>(a, heat, n, draft, st);
+  const int count = accepted<BF16, MODE>(a, n, draft, st);
   write_accepted(a, b, count, draft, st);
   const int id = __shfl(draft.id, count < 63 ? count : 63, 64);
   if (threadIdx.x != 0) return;
@@ -366,24 +432,43 @@ __global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, V
   __shared__ bool last;
   const int split = blockIdx.x % splits, b = blockIdx.x / splits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t i0 = (int64_t)split * (VECS * kThreads * 8) + threadIdx.x * 8;
-  const Decision d = w.made[b];
-  float u[VECS][8];
+  constexpr int STEP = kThreads * 8;
+  const float* noise = a.noise + b * a.noise_stride;
+  const bool whole = (int64_t)(split + 1) * (VECS * STEP) <= a.vocab;  // (uniform) else a chunk that ends inside: load8
+  Eight<false> us[VECS];
+  if (whole) {
 #pragma unroll
-  for (int v = 0; v < VECS; ++v) {
-    const int64_t i = i0 + v * (kThreads * 8);
-    load8<false>(a.noise + b * a.noise_stride, i, (int)min((int64_t)8, a.vocab - i), u[v]);
+    for (int v = 0; v < VECS; ++v) us[v].load(noise, i0 + v * STEP);
   }
+  const Decision d = w.made[b];
   const bool residual = d.residual;
   const int64_t away = d.away;
   const Row p(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, d.count), d.pm, d.pz, heat.hi);
   const Row q(residual ? row_at<BF16>(a.draft_logits, a.draft_batch_stride, a.draft_row_stride, b, d.count) : nullptr, d.qm, d.qz,
               heat.hi);
-  float x[VECS][8], y[VECS][8];
+  float u[VECS][8], x[VECS][8], y[VECS][8];
+  if (whole) {
+    Eight<BF16> xs[VECS], ys[VECS];
 #pragma unroll
-  for (int v = 0; v < VECS; ++v) {
-    const int64_t i = i0 + v * (kThreads * 8);
-    load8<BF16>(p.at, i, (int)min((int64_t)8, a.vocab - i), x[v]);
-    if (residual) load8<BF16>(q.at, i, (int)min((int64_t)8, a.vocab - i), y[v]);
+    for (int v = 0; v < VECS; ++v) {
+      xs[v].load(p.at, i0 + v * STEP);
+      if (residual) ys[v].load(q.at, i0 + v * STEP);
+    }
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      us[v].values(u[v]);
+      xs[v].values(x[v]);
+      if (residual) ys[v].values(y[v]);
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+      const int64_t i = i0 + v * STEP;
+      const int n = (int)min((int64_t)8, a.vocab - i);
+      load8<false>(noise, i, n, u[v]);
+      load8<BF16>(p.at, i, n, x[v]);
+      if (residual) load8<BF16>(q.at, i, n, y[v]);
+    }
   }
   // ln 2 times the scores' bounds (the pace by log2): the rough probabilities are within 1e-5, and q <= p where r >= 0
   const bool tame = fabsf(p.m) < 1e30f && fabsf(q.m) < 1e30f;  // else none (Below)
@@ -395,7 +480,7 @@ __global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, V
       const float pr = p.rough.exp(x[v][e]) * p.rough.rest;
       float r = pr;
       if (residual) r = fmaf(-q.rough.exp(y[v][e]), q.rough.rest, pr);
-      else if (i0 + v * (kThreads * 8) + e == away) r = 0.f;
+      else if (i0 + v * STEP + e == away) r = 0.f;
       const float g = u[v][e] < 1.f ? -__builtin_amdgcn_rcpf(__builtin_amdgcn_logf(u[v][e])) : 0.f;
       high[v][e] = fmaf(pr, 4e-5f, r) * g;
       bar = fmaxf(bar, fmaf(pr, -4e-5f, r) * g);
@@ -415,13 +500,13 @@ __global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, V
   while (mask) {
     const int j = __builtin_ctz(mask);
     mask &= mask - 1;
-    const int64_t i = i0 + (j >> 3) * (kThreads * 8) + (j & 7);
+    const int64_t i = i0 + (j >> 3) * STEP + (j & 7);
     if (i >= a.vocab) continue;
     const float pw = p.well(heat, logit<BF16>(p.at, i));
     float r = pw;
     if (residual) r = fmaxf(pw - q.well(heat, logit<BF16>(q.at, i)), 0.f);
     else if (i == away) r = 0.f;
-    const uint64_t k = entry(r * pace(a.noise[b * a.noise_stride + i]), i);
+    const uint64_t k = entry(r * pace(noise[i]), i);
     top = k > top ? k : top;
   }
   top = wave_top(top);
@@ -446,7 +531,7 @@ __global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, V
   top = wave_top(top);
   if (top == 0) {  // (uniform) no weight is left, p = q but for rounding: from p, by this workgroup alone
     for (int64_t i = threadIdx.x; i < a.vocab; i += kThreads) {
-      const uint64_t k = entry(p.well(heat, logit<BF16>(p.at, i)) * pace(a.noise[b * a.noise_stride + i]), i);
+      const uint64_t k = entry(p.well(heat, logit<BF16>(p.at, i)) * pace(noise[i]), i);
       top = k > top ? k : top;
     }
     top = wave_top(top);
@@ -459,18 +544,18 @@ __global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, V
   if (threadIdx.x == 0) write_token<BF16>(a, b, d.count, top ? (int)(0xffffffffu - (uint32_t)top) : 0, d.pm, d.unit);
 }
 
-template <bool BF16, int MODE, int VECS>
+template <bool BF16, int MODE, int VECS, int TIMES>
 int launch_verify(const G4VerifyArgs& a, const VerifyWorkspace& w, hipStream_t st) {
   static const char who[] = "g4_verify_draft";
-  const int splits = splits_of(a, VECS), rows = a.drafts + 1 + (MODE != kGreedy && a.draft_logits ? a.drafts : 0);
+  const int splits = splits_of(a, VECS * TIMES), rows = a.drafts + 1 + (MODE != kGreedy && a.draft_logits ? a.drafts : 0);
   const int64_t blocks = (int64_t)a.batch * rows * splits;
   if (blocks * kThreads > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "%s: too many logits", who);
-  hipLaunchKernelGGL((verify_stats_kernel<BF16, MODE, VECS>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, w, rows, splits);
+  hipLaunchKernelGGL((verify_stats_kernel<BF16, MODE, VECS, TIMES>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, w, rows, splits);
   int rc = check_launch(who);
   if (rc != G4_OK) return rc;
   const double c = 1.4426950408889634074 / (double)a.temperature;
   const Heat heat{(float)c, (float)(c - (double)(float)c)};
-  hipLaunchKernelGGL((verify_decide_kernel<BF16, MODE>), dim3((unsigned)a.batch), dim3(kThreads), 0, st, a, w, heat, rows, splits);
+  hipLaunchKernelGGL((verify_decide_kernel<BF16, MODE>), dim3((unsigned)a.batch), dim3(kThreads), 0, st, a, w, rows, splits);
   if ((rc = check_launch(who)) != G4_OK) return rc;
   if constexpr (MODE != kGreedy) {
     const int race = splits_of(a, kRace);  // (fewer workgroups than above: rows >= 2)
@@ -483,7 +568,7 @@ int launch_verify(const G4VerifyArgs& a, const VerifyWorkspace& w, hipStream_t s
 
 template <bool BF16, int MODE>
 int launch_verify(const G4VerifyArgs& a, const VerifyWorkspace& w, hipStream_t st) {
-  return vecs_of(a) == kLong ? launch_verify<BF16, MODE, kLong>(a, w, st) : launch_verify<BF16, MODE, kShort>(a, w, st);
+  return vecs_of(a) == kLong ? launch_verify<BF16, MODE, kStep, kSteps>(a, w, st) : launch_verify<BF16, MODE, kShort, 1>(a, w, st);
 }
 template <bool BF16>
 int launch_verify(const G4VerifyArgs& a, const VerifyWorkspace& w, hipStream_t st) {

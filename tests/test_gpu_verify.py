@@ -221,3 +221,112 @@ def test_the_same_call_gives_the_same_bits(device):
     first = kernels.verify_draft(*args, temperature=0.9, draft_logits=q.to(device))
     again = kernels.verify_draft(*args, temperature=0.9, draft_logits=q.to(device))
     assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
+# --- many logits: two steps per thread -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [0.0, 0.05, 1.0, 1.3])
+def test_many_logits(dtype, temperature, device):
+    """2^25 logits and more; the levels of a row's stretches of 2048 columns rise and fall, by less and by more than what a running
+    maximum may lag, and some stretches are masked."""
+
+    B, K, V = 58, 7, 40001
+    logits, drafts, u, noise, q = _inputs(B, K, V, dtype, 31, True)
+    assert logits.numel() + q.numel() >= 2 ** 25
+    level = torch.tensor([0, 3, 6, 9, -4, 40, 7, 60, -math.inf, 0, 2, 61, 5, -30, -math.inf, 4, 62, 1, 66, 0.5])
+    for b in range(0, B, 3):
+        shift = level.roll(b).repeat_interleave(2048)[:V]
+        logits[b] += shift.to(dtype)
+        q[b] += shift.to(dtype)
+    logits[1, :, :20000] = -math.inf
+    got = kernels.verify_draft(logits.to(device), drafts.to(device), u.to(device), noise.to(device), temperature=temperature,
+                               draft_logits=q.to(device))
+    want = verified(logits, drafts, u, noise, temperature, q)
+    if temperature == 0.05:
+        _near_ties(got[0].cpu(), want, logits, q, noise, temperature)
+    _check(got, want)
+
+
+def _near_ties(tokens, want, logits, q, noise, temperature):
+    """Where the next token differs, takes the operator's into ``want`` if the race is a tie for f32 probabilities. Each is off by
+    eps = u (120 + 2 |x - max| / T) of itself: a sum of up to 100 levels, exp and the product within 2 u each, and the
+    exponent's rounding. The drafts here are not drawn at this temperature, so that rows are rejected whose p and q both
+    are one token's but for 2^-24: all that p - q has is below its error eps (p + q)."""
+
+    wt, wc, wl = want
+    for b in (tokens != wt).any(dim=-1).nonzero()[:, 0].tolist():
+        i = int(wc[b])
+        got = int(tokens[b, i])
+        x, y = logits[b, i].double(), q[b, min(i, q.shape[1] - 1)].double()
+        p = torch.softmax(x / temperature, dim=-1)
+        z = torch.softmax(y / temperature, dim=-1) if i < q.shape[1] else torch.zeros_like(p)
+        eps = [2.0 ** -24 * (120 + 2 * (t.max() - t).clamp(max=1e4) / temperature) for t in (x, y)]
+        pace = torch.where(noise[b] > 0, 1 / -torch.log(noise[b].double()), torch.zeros(()).double()) * (1 + 2.0 ** -20)
+        w, error = torch.clamp(p - z, min=0.0), eps[0] * p + eps[1] * z
+        assert float((w + error)[got] * pace[got]) >= float(((w - error) * pace).max())
+        wt[b, i], wl[b, i] = got, torch.log_softmax(x, dim=-1)[got]
+
+
+def test_unlikely_drafts(device):
+    """Drafts whose probabilities are far below f32's range are accepted by their ratio."""
+
+    B, K, V = 4, 1, 300
+    logits, q = torch.zeros(B, K + 1, V), torch.zeros(B, K, V)
+    logits[:, 0, 7], q[:, 0, 7] = 40.0, 40.0
+    logits[:, 0, 9], q[:, 0, 9] = torch.tensor([-80.0, -81.0, -80.0, -80.0]), torch.tensor([-80.25, -80.0, -79.875, -80.0])
+    drafts, u = torch.full((B, K), 9, dtype=torch.int32), torch.tensor([[0.9], [0.9], [0.25], [0.4]])
+    noise = torch.rand(B, V, generator=torch.Generator().manual_seed(3))
+    got = kernels.verify_draft(logits.to(device), drafts.to(device), u.to(device), noise.to(device), temperature=0.5,
+                               draft_logits=q.to(device))
+    assert got[1].tolist() == [1, 0, 1, 1]  # p / q = e^.5, e^-2, e^-.25, 1
+
+
+def test_many_logits_replayed_in_a_graph(device):
+    """Replays with new inputs between eager calls of other sizes give what eager calls give."""
+
+    B, K, V = 4, 3, 5000
+    sets = [[None if t is None else t.to(device) for t in _inputs(B, K, V, torch.bfloat16, s, True)] for s in (41, 42, 43)]
+    other = [t.to(device) for t in _inputs(9, 5, 3001, torch.bfloat16, 44, True)]
+
+    def run(logits, drafts, u, noise, q):
+        return kernels.verify_draft(logits, drafts, u, noise, temperature=0.9, draft_logits=q)
+
+    want = [[t.clone() for t in run(*s)] for s in sets]
+    theirs = [t.clone() for t in run(*other)]
+    static = [t.clone() for t in sets[0]]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(*static)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*static)
+    for i in (1, 2, 0, 1):
+        for to, x in zip(static, sets[i]):
+            to.copy_(x)
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(run(*other), theirs))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want[i]))
+
+
+def test_two_streams_at_once(device):
+    """Calls that overlap on two streams have workspaces of their own."""
+
+    sets = [[t.to(device) for t in _inputs(6, 3, 20000, torch.bfloat16, s, True)] for s in (45, 46)]
+    run = lambda s: kernels.verify_draft(s[0], s[1], s[2], s[3], temperature=0.8, draft_logits=s[4])  # noqa: E731
+    want = [[t.clone() for t in run(s)] for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(out, want[i]))
