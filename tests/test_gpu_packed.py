@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from gemma4_posttrain_jax_amd import _lib, kernels
-from gemma4_posttrain_jax_amd.kvcache import group_keys, group_values, slot_stride_for
+from gemma4_posttrain_jax_amd.kvcache import group_keys, group_values, key_shape, slot_stride_for
 from packed_util import packed_reference
 
 pytestmark = pytest.mark.gpu
@@ -286,3 +286,57 @@ def test_about_the_change_of_blocks(tokens, device):
     lens = [300, tokens - 300]
     q, k, v = _inputs(lens, 0, 8, 16, 64, 23, device)
     _check(_run(q, k, v, lens, 0, device), q, k, v, lens, 0)
+
+
+# --- far offsets, other streams ----------------------------------------------------------------------------------------
+
+
+def test_heads_past_4_gib(device):
+    """Keys and values of 2 GiB a head: the fourth head's lie past 2^32 bytes, as does what the call must not reach."""
+
+    H, D, T, Sp = 4, 512, 150, 1 << 21
+    lens = [40, 110]
+    q, k, v = _inputs(lens, 0, H, 2, D, 41, device)
+    kk = torch.empty(key_shape(1, H, Sp, D), dtype=torch.bfloat16, device=device)
+    vv = torch.empty((1, H, Sp // 8, D, 8), dtype=torch.bfloat16, device=device)
+    ks, vs = _laid_out(k, v, device, math.nan)
+    kk[:, :, :ks.shape[2]], vv[:, :, :vs.shape[2]] = ks, vs
+    starts = kernels.packed_starts(torch.tensor([0, 40, 150], dtype=torch.int32, device=device), T)
+    _check(kernels.packed_prefill_attention(q.to(device), kk, vv, starts), q, k, v, lens, 0)
+
+
+def test_rows_past_4_gib(device):
+    """66000 tokens of 2 x 64 heads of 256: queries and results of 4.3 GB; the last sequences against 64 bits."""
+
+    H, R, D, T = 2, 64, 256, 66000
+    lens = [600] * 109 + [500, 90, 10]
+    assert sum(lens) == T
+    g = torch.Generator(device=device).manual_seed(42)
+    q = torch.empty((T, H, R, D), dtype=torch.bfloat16, device=device).normal_(0, 0.1, generator=g)
+    k, v = (torch.empty((T, H, D), dtype=torch.bfloat16, device=device).normal_(0, 1, generator=g) for _ in range(2))
+    kk, vv = _laid_out(k.cpu(), v.cpu(), device)
+    cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32, device=device)
+    out = kernels.packed_prefill_attention(q, kk, vv, kernels.packed_starts(cu, T), window=64)
+    for a, n in ((0, 600), (T - 100, 90), (T - 10, 10)):
+        _check(out[a:a + n], q[a:a + n].cpu(), k[a:a + n].cpu(), v[a:a + n].cpu(), [n], 64)
+
+
+def test_calls_on_two_streams(device):
+    """Calls in pieces that overlap on two streams have workspaces of their own."""
+
+    lens = [1200]
+    calls = []
+    for seed in (43, 44):
+        q, k, v = _inputs(lens, 0, 1, 4, 128, seed, device)
+        calls.append((q.to(device), *_laid_out(k, v, device)))
+    starts = kernels.packed_starts(torch.tensor([0, 1200], dtype=torch.int32, device=device), 1200)
+    assert _pieces(calls[0][0]) > 0
+    want = [kernels.packed_prefill_attention(*c, starts) for c in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(kernels.packed_prefill_attention(*calls[i], starts))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])

@@ -218,3 +218,120 @@ def test_copy_past_4_gib(device):
     kernels.paged_copy([layer], _i32([3, 2098], device), _i32([2099, 1], device))
     assert bool((layer.key[2099] == 1.5).all()) and bool((layer.value[1] == 2.5).all())
     assert bool((layer.key[1] == 0).all()) and bool((layer.value[2099] == 0).all())
+
+
+@pytest.mark.parametrize("rows", [1, 31, 32, 33])
+@pytest.mark.parametrize("P", [1, 255, 16384, 16385])
+def test_about_the_change_to_one_launch(P, rows, device):
+    """Up to 32 rows of up to 16384 pages go by one launch."""
+
+    refs, table = _pool(P, rows, 7, P // 2, 20 + rows)
+    lengths = [(37 * b) % 300 for b in range(rows)]
+    r, t = _i32(refs, device), _i32(table, device)
+    short = kernels.paged_reserve(r, t, _i32(lengths, device), page_size=32)
+    assert short.tolist() == [plain.reserve(refs, table, lengths, 32)] and r.tolist() == refs and t.tolist() == table
+    layer = _layer(P, 1, 64, 32, True, 21, device)
+    old = type(layer)(*(None if x is None else x.clone() for x in layer))
+    parents = [(5 * b) % (rows + 1) for b in range(rows)]  # one of them outside, several of one row
+    children, short = kernels.paged_fork([layer], r, t, _i32(parents, device), _i32(lengths, device))
+    want, moves, lacking = plain.fork(refs, table, parents, lengths, 32, 7)
+    assert children.tolist() == want and short.tolist() == [lacking] and r.tolist() == refs
+    _same(layer, plain.moved(old, moves, 32))
+
+
+def _step(layers, refs, table, parents, lengths, none, target):
+    """A serving step: children in place of their parents, pages for what they will hold, the pool compacted."""
+
+    children, short = kernels.paged_fork(layers, refs, table, parents, lengths)
+    kernels.paged_free(refs, table, none, page_size=32)
+    lacking = kernels.paged_reserve(refs, children, target, page_size=32)
+    live = kernels.paged_compact(layers, refs, children)
+    return children, short, lacking, live
+
+
+@pytest.mark.parametrize("rows,P", [(6, 120), (50, 700)])
+def test_replays_between_eager_calls(rows, P, device):
+    """The five calls captured into a graph, replayed on new tables with eager calls of another pool between."""
+
+    width, layers = 6, [_layer(P, 1, 64, 32, False, 30, device), _layer(P, 2, 128, 32, True, 31, device)]
+    other = [_layer(90, 1, 64, 32, False, 32, device)]
+    first = [[None if t is None else t.clone() for t in x] for x in layers + other]
+
+    def restore(xs, was):
+        for x, old in zip(xs, was):
+            for t, o in zip(x, old):
+                if t is not None:
+                    t.copy_(o)
+
+    def inputs(seed, P, rows):
+        refs, table = _pool(P, rows, width, P // 2, seed)
+        g = torch.Generator().manual_seed(seed)
+        parents = torch.randint(0, rows, (rows,), generator=g).tolist()
+        lengths = torch.randint(0, 32 * width, (rows,), generator=g).tolist()
+        return [_i32(x, device) for x in (refs, table, parents, lengths, [0] * rows, [n + 20 for n in lengths])]
+
+    def outcome(xs, args, out):
+        return [t.clone() for t in (*args[:2], *out)] + [b for x in xs for b in _bytes(x) if b is not None]
+
+    def eager(xs, was, args):
+        restore(xs, was)
+        args = [t.clone() for t in args]
+        return outcome(xs, args, _step(xs, *args))
+
+    sets = [inputs(s, P, rows) for s in (41, 42, 43)]
+    want = [eager(layers, first[:2], s) for s in sets]
+    theirs = inputs(44, 90, 9)
+    want_theirs = eager(other, first[2:], theirs)
+    static = [t.clone() for t in sets[0]]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        _step(layers, *[t.clone() for t in static])
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _step(layers, *static)
+    for i in (1, 2, 0, 1):
+        restore(layers, first[:2])
+        for to, x in zip(static, sets[i]):
+            to.copy_(x)
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(eager(other, first[2:], theirs), want_theirs))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outcome(layers, static, out), want[i]))
+
+
+def test_pools_on_two_streams(device):
+    """Calls of two pools that overlap on two streams."""
+
+    pools = []
+    for seed in (51, 52):
+        refs, table = _pool(3000, 200, 9, 1500, seed)
+        pools.append((_layer(3000, 1, 64, 32, False, seed, device), refs, table))
+    torch.cuda.synchronize()
+    lengths, parents = [(31 * b) % 280 for b in range(200)], [(7 * b) % 200 for b in range(200)]
+    args = [_i32(x, device) for x in (parents, lengths)]
+    got, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    ready = [(_i32(refs, device), _i32(table, device)) for _, refs, table in pools]
+    torch.cuda.synchronize()
+    for (layer, _, _), (r, t), stream in zip(pools, ready, streams):
+        with torch.cuda.stream(stream):
+            got.append((r, *kernels.paged_fork([layer], r, t, *args)))
+    torch.cuda.synchronize()
+    for (_, refs, table), (r, children, short) in zip(pools, got):
+        want, _, lacking = plain.fork(refs, table, parents, lengths, 32, 9)
+        assert children.tolist() == want and short.tolist() == [lacking] and r.tolist() == refs
+
+
+def test_the_same_layer_twice_and_one_page(device):
+    """A layer that is named twice is copied alike; a pool of one page."""
+
+    layer = _layer(1, 1, 64, 32, True, 60, device)
+    r, t = _i32([1], device), _i32([[0]], device)
+    children, short = kernels.paged_fork([layer, layer], r, t, _i32([0, 0], device), _i32([32], device))
+    assert children.tolist() == [[0], [0]] and r.tolist() == [3] and short.tolist() == [0]
+    children, short = kernels.paged_fork([layer], r, t, _i32([0, 0], device), _i32([31], device))
+    assert children.tolist() == [[-1], [-1]] and r.tolist() == [3] and short.tolist() == [2]
+    assert kernels.paged_compact([layer], r, t).tolist() == [1] and t.tolist() == [[0]]
+    kernels.paged_free(r, t, _i32([0], device), page_size=32)
+    assert r.tolist() == [2] and t.tolist() == [[-1]]

@@ -330,3 +330,24 @@ def test_two_streams_at_once(device):
     for i in range(2):
         for out in got[i]:
             assert all(torch.equal(x, y) for x, y in zip(out, want[i]))
+
+
+def test_rows_past_4_gib(device):
+    """Logits and the drafter's of more than 2^32 bytes each: their last rows give what they give alone."""
+
+    B, K, V = 260, 33, 262144
+    logits = torch.empty((B, K + 1, V), dtype=torch.bfloat16, device=device).normal_()
+    q = torch.empty((B, K, V), dtype=torch.bfloat16, device=device).normal_()
+    assert min(logits.numel(), q.numel()) * 2 > 2 ** 32
+    g = torch.Generator(device=device).manual_seed(5)
+    drafts = torch.randint(0, V, (B, K), generator=g, device=device, dtype=torch.int32)
+    drafts[:, 2:] = q[:, 2:].argmax(dim=-1).to(torch.int32)
+    u = torch.rand(B, K, generator=g, device=device) * 0.5
+    noise = torch.rand(B, V, generator=g, device=device)
+    got = kernels.verify_draft(logits, drafts, u, noise, temperature=1.0, draft_logits=q)
+    for rows in (slice(0, 3), slice(B - 3, B)):
+        want = kernels.verify_draft(logits[rows], drafts[rows], u[rows], noise[rows], temperature=1.0, draft_logits=q[rows])
+        assert torch.equal(got[0][rows], want[0]) and torch.equal(got[1][rows], want[1])
+        # another split of the sums: 84 levels' roundings, and those of the logarithm and the difference
+        bound = 2.0 ** -23 * (2 * want[2].abs() + 120)
+        assert bool(((got[2][rows] - want[2]).abs() <= bound).all())
