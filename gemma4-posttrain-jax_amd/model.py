@@ -98,8 +98,8 @@ class Gemma4TextParams(NamedTuple):
 class PackedPrompts(NamedTuple):
     """How ``forward_gemma4_text``'s one row of T tokens divides into prompts, each of which fills a row of the cache."""
 
-    starts: torch.Tensor  # [T] int32, the first token of each token's prompt (kernels.packed_starts)
-    rows: torch.Tensor  # [T] the cache row of each token's prompt
+    starts: torch.Tensor  # [T] int32, the first token of each token's prompt (kernels.packed_starts); -1: of no prompt, not stored
+    rows: torch.Tensor  # [T] the cache row of each token's prompt (of no prompt: any)
     lengths: torch.Tensor  # [N] int32 tokens per prompt
     longest: int
 
@@ -466,6 +466,8 @@ def forward_gemma4_text(
     dev = input_ids.device
     pw = pack_weights(params, config)
     eps = config.rms_norm_eps
+    if packed is not None and attention_mask is not None:
+        raise ValueError("packed prompts have no pads to mask: attention_mask must be None")
     if attention_mask is None:
         attention_mask = torch.ones((B, S), dtype=torch.bool, device=dev)
     attention_mask = attention_mask.to(torch.bool)
@@ -538,6 +540,7 @@ def forward_gemma4_text(
             held, keep = packed.lengths, 0
             tables = {t: table.index_select(0, packed.rows) for t, table in tables.items()}
             place = torch.arange(S, dtype=torch.int32, device=dev) - packed.starts
+            place = place.masked_fill(packed.starts < 0, -1)  # of no prompt
             # a sliding layer stores what the last window holds
             gone = place < held.index_select(0, packed.rows) - config.sliding_window
             slots = {FULL: place, SLIDING: place.masked_fill(gone, -1)}

@@ -124,7 +124,7 @@ def prefill_group(
     """``prefill`` for ``completions`` rows per prompt (bf16 models): each of the N prompts is encoded once, without its
     pads, and its cache handed to ``completions`` rows in a row (row ``i * completions + j`` is the j-th of prompt i).
     Their global layers share the pages that the prompt fills and get pages of their own for its last, partly filled
-    one and for ``max_new_tokens`` tokens; a sliding layer's rings are copied. Returns the logits ``[N *
+    one and for ``max_new_tokens`` tokens (the longest row's last page filled up); a sliding layer's rings are copied. Returns the logits ``[N *
     completions, 1, V]``, the packed prompts' hidden states ``[1, T, M]`` and the cache."""
 
     _no_mesh(mesh)
@@ -143,8 +143,9 @@ def prefill_group(
     N, G, ps = len(host), completions, paged.page_size
     capacity = max(host) + max_new_tokens
     width, cycle = page_counts(capacity, config.sliding_window, ps)
+    room = width * ps - max(host)  # of every row, so that none is full before the longest, whose end the cache refuses to pass
     # what the rows hold in the end, and while the prompts' own last pages are still theirs
-    pages = {FULL: sum(n // ps + G * (-(-(n + max_new_tokens) // ps) - n // ps) + 1 for n in host), SLIDING: N * G * cycle}
+    pages = {FULL: sum(n // ps + G * (-(-(n + room) // ps) - n // ps) + 1 for n in host), SLIDING: N * G * cycle}
     layers = [None if is_kv_shared(config, i) else
               new_paged_layer(pages[config.layer_types[i]], layer_kv_heads(config, i), layer_head_dim(config, i), ps,
                               e4m3=paged.e4m3, device=dev) for i in range(config.num_hidden_layers)]
@@ -171,7 +172,7 @@ def prefill_group(
     if of[FULL]:
         forked, _ = kernels.paged_fork(of[FULL], refs, table, parents, lengths)
         kernels.paged_free(refs, table, torch.zeros_like(lengths), page_size=ps)
-        kernels.paged_reserve(refs, forked, held + max_new_tokens, page_size=ps)
+        kernels.paged_reserve(refs, forked, held + room, page_size=ps)
     else:  # (its width is the cache's capacity)
         forked = table.index_select(0, parents)
     if of[SLIDING] and G > 1:

@@ -10,8 +10,9 @@ import paged_util as P
 import pool_util as plain
 from gemma4_posttrain_jax_amd import config as C
 from gemma4_posttrain_jax_amd import kernels
+from gemma4_posttrain_jax_amd import model as M
 from gemma4_posttrain_jax_amd import sampler as SMP
-from gemma4_posttrain_jax_amd.kvcache import PagedSpec, new_layer_cache, new_paged_layer
+from gemma4_posttrain_jax_amd.kvcache import PagedSpec, init_paged_kv_cache, new_layer_cache, new_paged_layer
 from packed_util import packed_reference
 from test_gpu_paged_run import CFG, CFG512, _params, _prompts
 
@@ -152,6 +153,52 @@ def test_group_refusals(device):
         cache = SMP.decode_step(params, cfg, tok, cache.held, cache).kv_cache
     with pytest.raises(ValueError, match="no place"):
         SMP.decode_step(params, cfg, tok, cache.held, cache)
+
+
+def test_short_rows_have_place_as_long_as_the_longest(device):
+    """100 and 10 tokens, five more asked for, pages of 32: every row has a page for each token up to the 28th, which fills the
+    longest row's last page; the 29th is refused."""
+
+    cfg = C.config_from_hf(CFG)
+    params = _params(cfg, device)
+    ids, mask = _prompts(cfg, [0, 90], 100, device)
+    cache = SMP.prefill_group(params, cfg, ids, mask, completions=2, max_new_tokens=5, paged=PagedSpec(32)).kv_cache
+    tok = torch.zeros(4, dtype=torch.int32, device=device)
+    for _ in range(28):
+        cache = SMP.decode_step(params, cfg, tok, cache.held, cache).kv_cache
+    last = ((cache.held - 1) // 32).long()
+    assert cache.held.tolist() == [128, 128, 38, 38]
+    assert bool((cache.page_table.gather(1, last[:, None]) >= 0).all())
+    full = next(i for i, t in enumerate(cfg.layer_types) if t != C.SLIDING and cache.layers[i] is not None)
+    k, _ = kernels.paged_read(cache.layers[full], page_table=cache.page_table, lengths=cache.held, start=0, count=128)
+    assert all(bool((k[b, :n].float().abs().amax(dim=(1, 2)) > 0).all()) for b, n in enumerate(cache.held.tolist()))
+    with pytest.raises(ValueError, match="no place"):
+        SMP.decode_step(params, cfg, tok, cache.held, cache)
+
+
+def test_packed_tokens_of_no_prompt_are_not_stored(device):
+    cfg = C.config_from_hf(CFG)
+    params = _params(cfg, device)
+    lens, T = [20, 7], 40
+    ids = torch.arange(T, device=device)[None] * 3 % 500
+    cu = torch.tensor([0, 20, 27], dtype=torch.int32, device=device)
+    starts = kernels.packed_starts(cu, T)
+    rows = torch.tensor([0] * 20 + [1] * 7 + [0] * 13, dtype=torch.int32, device=device)
+    places = (torch.arange(T, dtype=torch.int32, device=device) - starts)[None]
+    packed = M.PackedPrompts(starts, rows, cu.diff(), 20)
+    empty = init_paged_kv_cache(cfg, 2, 64, PagedSpec(32), device)
+    _, cache = M.forward_gemma4_text(params, ids, places, config=cfg, kv_cache=empty, packed=packed)
+    assert cache.held.tolist() == lens
+    for i, layer in enumerate(cache.layers):
+        if layer is None:
+            continue
+        table = cache.window_table if cfg.layer_types[i] == C.SLIDING else cache.page_table
+        k, v = kernels.paged_read(layer, page_table=table, lengths=torch.full_like(cache.held, 32), start=0, count=32)
+        for b, n in enumerate(lens):
+            assert bool((k[b, n:] == 0).all()) and bool((v[b, n:] == 0).all()) and bool((k[b, n - 1] != 0).any())
+    with pytest.raises(ValueError, match="attention_mask"):
+        M.forward_gemma4_text(params, ids, places, config=cfg, kv_cache=empty, packed=packed,
+                              attention_mask=torch.ones(1, T, device=device))
 
 
 @pytest.mark.parametrize("e4m3", [False, True])

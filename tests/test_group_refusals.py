@@ -240,6 +240,7 @@ def test_front_end_of_packed_attention():
     _error("starts must", call, q, k, vt, starts.long())
     _error("starts must", call, q, k, vt, starts[:60])
     _error("window", call, q, k, vt, starts, window=-2)
+    _error("longest", call, q, k, vt, starts, longest=-1)
     _error("out must", call, q, k, vt, starts, out=_bf(70, 2, 4, 32))
     _error("cu_seqlens", kernels.packed_starts, starts.long(), 5)
     _error("cu_seqlens", kernels.packed_starts, starts[:1], 5)
