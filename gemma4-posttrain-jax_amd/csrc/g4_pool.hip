@@ -518,8 +518,8 @@ int launch_copies(const G4PagedCache* layers, int32_t n, const int32_t* src, con
       if (y.units > units) units = y.units;
     }
     const int64_t blocks = pairs * units, most = (moved ? 4096 : 1 << 23) / (2 * here) + 1;
-    hipLaunchKernelGGL(copy_kernel, dim3(blocks_for(blocks, most) * 2u * (unsigned)here), dim3(kThreads), 0, st, c, src, dst, slots, (int)pairs,
-                       moved, remap);
+    hipLaunchKernelGGL(copy_kernel, dim3(blocks_for(blocks, most) * 2u * (unsigned)here), dim3(kThreads), 0, st, c, src, dst, slots,
+                       (int)pairs, moved, remap);
     remap.map = nullptr;  // once
     const int rc = check_launch(who);
     if (rc != G4_OK) return rc;

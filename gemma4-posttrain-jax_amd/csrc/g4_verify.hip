@@ -187,9 +187,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// A thread's statistics, VECS vectors at a time. The vector work is as long as the loads: instructions count (81 -> 94 us with
-// fmaxf, the loads behind a bounds check each and the reduction over the workgroup after every 4 vectors). The largest logit that exponents refer to follows lazily: it stays while no
-// logit passes it by more than `slack` (exponents of at most kSlack), but for kGreedy, which asks for the largest itself.
+// A thread's statistics, VECS vectors at a time. The vector work is as long as the loads: instructions count (77 us; 94 with fmaxf,
+// a bounds check around each load and the reduction over the workgroup after every 4 vectors). The largest logit that exponents
+// refer to follows lazily: it stays while no logit passes it by more than `slack` (exponents of at most kSlack), but for
+// kGreedy, which asks for the largest itself.
 constexpr float kSlack = 8.f;
 template <int MODE, int VECS>
 struct Running {
