@@ -7,9 +7,9 @@
 //
 // Bound by reading the logits (64 rows of 9 x 262144 in bf16, 369 MB with the noise, 75 us: 4.9 TB/s) and, while it does, by
 // vector instructions: K + 1 target and K draft rows of the vocabulary once, for their largest logits and sums of
-// exponentials (a first launch, statistics per chunk of a row), then of two rows per b and the noise for the race (a
-// third). Which rows these are a launch between finds from the statistics; it also clears the counter by which the last of
-// a b's workgroups in the race, which writes the token, is found.
+// exponentials (a first launch, statistics per chunk of a row, which also clears the counters by which the last of a b's
+// workgroups in the race, which writes the token, is found), then of two rows per b and the noise for the race (a
+// third). Which rows these are a launch between finds from the statistics, or the race itself.
 #include "g4_common.h"
 #include "g4_internal.h"
 
@@ -235,6 +235,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(G4VerifyArgs a, 
   const bool draft = r > a.drafts;
   const int n = drafts_of(a, b);
   if (draft ? r - a.drafts - 1 >= n : r > n) return;  // (uniform) no draft reaches this row
+  if (MODE != kGreedy && r == 0 && split == 0 && threadIdx.x == 0) w.arrived[(int64_t)b * kApart] = 0;
   const void* row = draft ? row_at<BF16>(a.draft_logits, a.draft_batch_stride, a.draft_row_stride, b, r - a.drafts - 1)
                           : row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, r);
   constexpr int STEP = kThreads * 8;
@@ -365,19 +366,21 @@ __device__ __forceinline__ void write_token(const G4VerifyArgs& a, int b, int co
   a.logp_out[at] = log_prob(logit<BF16>(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, count), token), Stats{m, 0.f, unit, 0});
 }
 
-// --- second launch: the decision, one workgroup per b -----------------------------------------------------------------------
-// (Made by every workgroup of the race for itself it costs these 6 us at 64 rows, and one row no less than the launch, 3 us.)
-
+// The decision on row b by a workgroup, in its LDS; `write`: with the accepted tokens, or greedily all of them, to memory.
+struct Decided {
+  Stats st[2 * kMaxDrafts + 1];
+  Decision made;
+};
 template <bool BF16, int MODE>
-__global__ __launch_bounds__(kThreads) void verify_decide_kernel(G4VerifyArgs a, VerifyWorkspace w, int rows, int splits) {
-  __shared__ Stats st[2 * kMaxDrafts + 1];
-  const int b = blockIdx.x;
+__device__ __forceinline__ void decide(const G4VerifyArgs& a, const VerifyWorkspace& w, int b, int rows, int splits, bool write,
+                                       Decided& out) {
   const int n = drafts_of(a, b);
   const Draft draft = load_draft<BF16, MODE>(a, b, threadIdx.x < 64 ? n : 0);
-  join_rows<MODE>(a, w, b, rows, splits, n, st);
+  const Stats* st = out.st;
+  join_rows<MODE>(a, w, b, rows, splits, n, out.st);
   if (threadIdx.x >= 64) return;
   const int count = accepted<BF16, MODE>(a, n, draft, st);
-  write_accepted(a, b, count, draft, st);
+  if (write) write_accepted(a, b, count, draft, st);
   const int id = __shfl(draft.id, count < 63 ? count : 63, 64);
   if (threadIdx.x != 0) return;
   if constexpr (MODE == kGreedy) {
@@ -386,9 +389,20 @@ __global__ __launch_bounds__(kThreads) void verify_decide_kernel(G4VerifyArgs a,
   } else {
     const bool rejected = count < n, residual = rejected && a.draft_logits;
     const Stats &p = st[count], &q = st[residual ? a.drafts + 1 + count : count];
-    w.made[b] = Decision{count, rejected && !residual ? id : -1, residual, p.unit, p.m, p.heat, q.m, q.heat};
-    w.arrived[(int64_t)b * kApart] = 0;
+    out.made = Decision{count, rejected && !residual ? id : -1, residual, p.unit, p.m, p.heat, q.m, q.heat};
   }
+}
+
+// --- second launch: the decision, one workgroup per b -----------------------------------------------------------------------
+
+// Where the race has few workgroups each decides for itself, and this launch is saved: 1 row of 4 drafts over 262144 logits (64
+// workgroups) 13.0 -> 11.4 us, 16 rows (1024) 31.0 -> 29.6; 32 rows 46.2 -> 47.6, 64 rows 76.8 -> 80.5.
+constexpr int kOwn = 1024;
+template <bool BF16, int MODE>
+__global__ __launch_bounds__(kThreads) void verify_decide_kernel(G4VerifyArgs a, VerifyWorkspace w, int rows, int splits) {
+  __shared__ Decided decided;
+  decide<BF16, MODE>(a, w, blockIdx.x, rows, splits, true, decided);
+  if (MODE != kGreedy && threadIdx.x == 0) w.made[blockIdx.x] = decided.made;
 }
 
 // --- third launch: the race, a chunk per workgroup ----------------------------------------------------------------------
@@ -426,8 +440,9 @@ struct Row {
 // The race is decided by scores within a few f32 ulps, which take some 50 instructions each. Rough ones take 15 and give
 // each score's bounds; an element whose upper bound is below the workgroup's largest lower one is out: one per
 // workgroup remains, or a few. (64 rows of 262144: 55 -> 29 us.)
-template <bool BF16, int VECS>
-__global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, VerifyWorkspace w, Heat heat, int splits) {
+template <bool BF16, int MODE, int VECS, bool OWN>
+__global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, VerifyWorkspace w, Heat heat, int splits, int rows,
+                                                               int stats_splits) {
   __shared__ uint64_t best_of[kWaves];
   __shared__ float bars[kWaves];
   __shared__ bool last;
@@ -441,7 +456,15 @@ __global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, V
 #pragma unroll
     for (int v = 0; v < VECS; ++v) us[v].load(noise, i0 + v * STEP);
   }
-  const Decision d = w.made[b];
+  Decision d;
+  if constexpr (OWN) {
+    __shared__ Decided decided;
+    decide<BF16, MODE>(a, w, b, rows, stats_splits, split == 0, decided);
+    __syncthreads();
+    d = decided.made;
+  } else {
+    d = w.made[b];
+  }
   const bool residual = d.residual;
   const int64_t away = d.away;
   const Row p(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, d.count), d.pm, d.pz, heat.hi);
@@ -556,12 +579,15 @@ int launch_verify(const G4VerifyArgs& a, const VerifyWorkspace& w, hipStream_t s
   if (rc != G4_OK) return rc;
   const double c = 1.4426950408889634074 / (double)a.temperature;
   const Heat heat{(float)c, (float)(c - (double)(float)c)};
-  hipLaunchKernelGGL((verify_decide_kernel<BF16, MODE>), dim3((unsigned)a.batch), dim3(kThreads), 0, st, a, w, rows, splits);
-  if ((rc = check_launch(who)) != G4_OK) return rc;
+  const int race = splits_of(a, kRace);
+  const int64_t racers = (int64_t)a.batch * race;  // (fewer than above: rows >= 2)
+  if (MODE == kGreedy || racers > kOwn) {
+    hipLaunchKernelGGL((verify_decide_kernel<BF16, MODE>), dim3((unsigned)a.batch), dim3(kThreads), 0, st, a, w, rows, splits);
+    if ((rc = check_launch(who)) != G4_OK) return rc;
+  }
   if constexpr (MODE != kGreedy) {
-    const int race = splits_of(a, kRace);  // (fewer workgroups than above: rows >= 2)
-    hipLaunchKernelGGL((verify_race_kernel<BF16, kRace>), dim3((unsigned)((int64_t)a.batch * race)), dim3(kThreads), 0, st, a, w, heat,
-                       race);
+    const auto kernel = racers > kOwn ? verify_race_kernel<BF16, MODE, kRace, false> : verify_race_kernel<BF16, MODE, kRace, true>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)racers), dim3(kThreads), 0, st, a, w, heat, race, rows, splits);
     rc = check_launch(who);
   }
   return rc;

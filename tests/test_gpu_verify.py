@@ -351,3 +351,14 @@ def test_rows_past_4_gib(device):
         # another split of the sums: 84 levels' roundings, and those of the logarithm and the difference
         bound = 2.0 ** -23 * (2 * want[2].abs() + 120)
         assert bool(((got[2][rows] - want[2]).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("B,V", [(1024, 500), (1025, 500), (205, 20000), (205, 20481)])  # 1024, 1025, 1025, 1230 chunks of 4096
+@pytest.mark.parametrize("temperature,draft", [(0.7, True), (1.0, False)])
+def test_about_the_change_of_who_decides(B, V, temperature, draft, device):
+    K = 3
+    logits, drafts, u, noise, q = _inputs(B, K, V, torch.bfloat16, 51, draft)
+    lengths = (torch.arange(B, dtype=torch.int32) * 7 % (K + 1))
+    got = kernels.verify_draft(logits.to(device), drafts.to(device), u.to(device), noise.to(device), temperature=temperature,
+                               draft_logits=None if q is None else q.to(device), draft_lengths=lengths.to(device))
+    _check(got, verified(logits, drafts, u, noise, temperature, q, lengths))
