@@ -499,9 +499,10 @@ __global__ __launch_bounds__(256) void packed_join_kernel(G4PackedPrefillArgs a,
   }
 }
 
-// How a call is laid out. A wave takes one column block where the blocks of two would not fill the CUs more than once: more,
-// smaller workgroups then end sooner (one prompt of 500 tokens, 2 x 4 heads of 256: 16 us, 23 with two; of 8000 265 and 299; 160
-// prompts of 60 .. 140 tokens, more blocks than that, 40 and 36).
+// How a call is laid out. A wave takes one column block where the blocks of two would leave CUs without a workgroup: more, smaller
+// workgroups then end sooner (one prompt of 500 tokens, 2 x 4 heads of 256: 16 us, 23 with two). Between one and two of them per CU
+// those of two columns are all at work at once, which is faster where their keys are about as many (8000 tokens with window 1024: 76
+// us, 94 in twice as many blocks of one; 8 prompts of 1000 52 and 58) and slower where a few have most (one of 8000 300 and 267).
 // Pieces: only where whole blocks leave CUs free and the longest sequence has 768 tokens (one of 600, 4 x 4 heads of 128: 15.6
 // us in pieces, 13.4 whole; of 1000, 2 x 4 of 256, 23 and 28) that a window does not cut (4000 with window 512: 53 and 26).
 // As many as the CUs take at once, of 8 chunks or more: each piece's sums cost a pass through memory (one prompt of 2000, 2
@@ -517,12 +518,13 @@ Plan plan_of(const G4PackedPrefillArgs& a) {
   const int64_t rows = (int64_t)a.tokens * a.group, resident = D == 512 ? 256 : 512;
   const auto per_head = [&](int nb) { return (rows + nw * nb * 16 - 1) / (nw * nb * 16); };
   Plan p{};
-  p.nb = D == 512 || per_head(2) * a.kv_heads <= resident ? 1 : 2;
+  const int64_t longest = a.longest > 0 && a.longest < a.tokens ? a.longest : a.tokens, chunks = (longest + 31) / 32;
+  const bool cut = a.window > 0 && a.window < longest, alike = cut || longest * 4 < a.tokens;
+  p.nb = D == 512 || per_head(2) * a.kv_heads <= (alike ? resident / 2 : resident) ? 1 : 2;
   p.blocks = per_head(p.nb) * a.kv_heads;
   p.padded = per_head(p.nb) * nw * p.nb * 16;
   p.most = 1;
-  const int64_t longest = a.longest > 0 && a.longest < a.tokens ? a.longest : a.tokens, chunks = (longest + 31) / 32;
-  if (p.nb == 1 && p.blocks < resident && chunks >= 24 && !(a.window > 0 && a.window < longest)) {
+  if (p.nb == 1 && p.blocks < resident && chunks >= 24 && !cut) {
     const int64_t most = std::min<int64_t>(kMostPieces, std::max(std::min(resident / p.blocks, chunks / 8),
                                                                 std::min(2 * resident / p.blocks, chunks / 32)));
     if (most > 1) {

@@ -279,13 +279,15 @@ def test_many_rows_with_values_that_are_not_finite(D, device):
     assert bool(((got - want).abs() <= bound).all())
 
 
-@pytest.mark.parametrize("tokens", [511, 512, 513])
-def test_about_the_change_of_blocks(tokens, device):
-    """8 heads of 16: 512 workgroups of two blocks per wave at 512 tokens, one block per wave up to there."""
+@pytest.mark.parametrize("tokens,window,longest", [(511, 0, 0), (512, 0, 0), (513, 0, 0), (255, 40, 0), (256, 40, 0), (257, 40, 0),
+                                                   (257, 0, 50)])
+def test_about_the_change_of_blocks(tokens, window, longest, device):
+    """8 heads of 16: as many workgroups of two blocks per wave as tokens. One block per wave up to 512, up to 256 where a window or
+    the sequences' length make them alike."""
 
-    lens = [300, tokens - 300]
+    lens = [50] * 5 + [tokens - 250] if longest else [tokens - 200, 200]
     q, k, v = _inputs(lens, 0, 8, 16, 64, 23, device)
-    _check(_run(q, k, v, lens, 0, device), q, k, v, lens, 0)
+    _check(_run(q, k, v, lens, window, device, longest=longest), q, k, v, lens, window)
 
 
 # --- far offsets, other streams ----------------------------------------------------------------------------------------
