@@ -201,12 +201,10 @@ __device__ __forceinline__ floatx4 careful_values(const Rows& rows, int cb, floa
 }
 
 // Which block of rows and head workgroup i takes. Workgroups are dealt to the 8 XCDs round robin: runs of kRun consecutive
-// blocks of a head, which read the same keys, go to one XCD and its L2, the latest tokens' first, whose keys are the most
-// (256 prompts of 32 .. 480 tokens, window 512: 3 % over single blocks; runs of 16 lose 10 % on 3 prompts of up to 8191).
-// Blocks in the order of their keys, found by each workgroup from the starts, took 5 % off several long prompts and put
-// 9 (one of 8000) to 50 % (160 of 100) on others.
+// blocks of a head, which read the same keys, go to one XCD and its L2 (256 prompts of 32 .. 480 tokens, window 512: 3 % over
+// single blocks; runs of 16 lose 10 % on 3 prompts of up to 8191). The runs go in `order`, or the latest tokens' first.
 constexpr int kXcds = 8, kRun = 4;
-__device__ __forceinline__ void place_block(int i, int n_blk, int H, int& blk, int& h) {
+__device__ __forceinline__ void place_block(int i, int n_blk, int H, const int32_t* order, int& blk, int& h) {
   const int even = n_blk * H / (kXcds * kRun) * (kXcds * kRun);  // as many as fill whole turns of runs
   int u = i;
   if (i < even) {
@@ -216,7 +214,7 @@ __device__ __forceinline__ void place_block(int i, int n_blk, int H, int& blk, i
   // u in the order (run of blocks, head, block of the run); the last run may be short
   const int run = u / (kRun * H), rest = u - run * kRun * H, len = min(kRun, n_blk - run * kRun);
   h = rest / len;
-  blk = n_blk - 1 - (run * kRun + rest - h * len);
+  blk = n_blk - 1 - ((order && len == kRun ? order[run] : run) * kRun + rest - h * len);
 }
 
 // Where few blocks would leave CUs idle for long, a block's chunks are taken in pieces, a workgroup each, whose sums a second
@@ -231,7 +229,46 @@ struct Pieces {
   float* o;      // [most][H][padded rows][D], not divided by the sums
   Piece* stats;  // [most][H][padded rows]
   int most, chunks;  // pieces of a block at most; chunks of each, the last's maybe more
+  int32_t* order;    // [blocks / kRun] the runs of blocks in the order that they are taken; NULL: the latest first
 };
+
+// The runs of blocks by the chunks of their longest block, most first: the last workgroups to start are short ones (CUs at work for 71 %
+// of the time on 3 prompts of up to 8191 tokens without it; 398 -> 368 us). By bins of 2^shift chunks, within one in any
+// order, which no result depends on. One workgroup, 4 us with its launch. (By single blocks, whose neighbours then lie on other XCDs:
+// 420 us.)
+constexpr int kBins = 1024;
+__global__ __launch_bounds__(kBins) void packed_order_kernel(G4PackedPrefillArgs a, Group group, int n_blk, int rows, int shift,
+                                                             int32_t* order) {
+  __shared__ int bins[kBins], sums[kBins / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, T = a.tokens, runs = n_blk / kRun;
+  const auto bin = [&](int run) {  // a block's chunks: from its first token's first key to its last token
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int b = n_blk - 1 - run * kRun - i, t0 = group.token(b * rows), t1 = min(group.token(b * rows + rows - 1), T - 1);
+      const int start = a.starts[t0], lo = max(start, a.window > 0 ? t0 - a.window + 1 : 0);
+      most = max(most, start < 0 ? 0 : (t1 - lo) >> 5);
+    }
+    return kBins - 1 - min(most >> shift, kBins - 1);
+  };
+  bins[tid] = 0;
+  __syncthreads();
+  for (int run = tid; run < runs; run += kBins) atomicAdd(&bins[bin(run)], 1);
+  __syncthreads();
+  const int mine = bins[tid];
+  int x = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d, 64);
+    x += lane >= d ? y : 0;
+  }
+  if (lane == 63) sums[wave] = x;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) x += sums[i];
+  bins[tid] = x - mine;
+  __syncthreads();
+  for (int run = tid; run < runs; run += kBins) order[atomicAdd(&bins[bin(run)], 1)] = run;
+}
 
 // A step per chunk c: behind its barrier, which every wave's share of K(c) and V(c - 1) has landed before, K(c + 1) and V(c) are
 // asked for; then the values of chunk c - 1, the scores of chunk c and their softmax. Of a workgroup that has the CU alone (head
@@ -251,7 +288,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, 2) void packed_prefill_kernel(G4Pac
   const int n_blk = (int)(gridDim.x / (unsigned)(CUT ? H * pieces.most : H));
   const int piece = CUT ? (int)(blockIdx.x / (unsigned)(n_blk * H)) : 0;
   int blk, h;
-  place_block((int)blockIdx.x - piece * n_blk * H, n_blk, H, blk, h);
+  place_block((int)blockIdx.x - piece * n_blk * H, n_blk, H, CUT ? nullptr : pieces.order, blk, h);
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row0 = blk * S::ROWS + w * (NB * 16);
@@ -509,9 +546,13 @@ __global__ __launch_bounds__(256) void packed_join_kernel(G4PackedPrefillArgs a,
 // x 4 heads of 256: whole 50, in 2 pieces 41, in 4 46 us; 1 head: whole 48, 8 pieces 20). Where the pieces stay long, of 32
 // chunks or more, twice that, as the blocks with the most keys come first and the rest fill up behind them (one of 8000, 1
 // x 2 heads of 128: whole 128, 2 pieces 81, 4 66; one of 4000, 8 heads of 512: whole 198, 2 pieces 163).
+// Sorting: more blocks than are at work at once, whose keys may differ: no window that makes them alike, sequences of 256 tokens
+// and more (8 of 4096, 2 x 4 heads of 256: 504 -> 450 us; 160 of 20 .. 500 70 -> 60; where all are short it is the launch's 4 us:
+// 160 of 60 .. 140 36 -> 39; with window 512 256 prompts of 32 .. 480 175 -> 180).
 struct Plan {
   int nb, most, chunks;    // column blocks per wave; pieces of a block at most (1: whole blocks), chunks of one
   int64_t blocks, padded;  // workgroups without pieces; rows per head, the last block's filled up
+  bool sort;               // the runs of blocks by their chunks
 };
 Plan plan_of(const G4PackedPrefillArgs& a) {
   const int D = a.head_dim, nw = D == 512 ? kWaves<512> : kWaves<64>;
@@ -532,6 +573,7 @@ Plan plan_of(const G4PackedPrefillArgs& a) {
       p.most = (int)((chunks + p.chunks - 1) / p.chunks);
     }
   }
+  p.sort = p.most == 1 && p.blocks > resident && chunks >= 8 && !cut;
   return p;
 }
 
@@ -541,6 +583,8 @@ size_t carve(Pieces& p, void* base, const G4PackedPrefillArgs& a, const Plan& pl
   p.chunks = plan.chunks;
   p.o = static_cast<float*>(base);
   p.stats = reinterpret_cast<Piece*>(p.o + rows * a.head_dim);
+  p.order = plan.sort ? static_cast<int32_t*>(base) : nullptr;
+  if (plan.sort) return (size_t)(plan.blocks / a.kv_heads / kRun) * 4;
   return plan.most > 1 ? (size_t)rows * (a.head_dim * 4 + sizeof(Piece)) : 0;
 }
 
@@ -549,9 +593,16 @@ int launch_packed(const G4PackedPrefillArgs& a, const Plan& plan, const Pieces& 
   static const char who[] = "g4_packed_prefill_attention";
   using S = Shape<D, NB>;
   const int64_t blocks = plan.blocks * plan.most;
-  if (blocks * S::NW * 64 > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "%s: too many tokens", who);
   const Group group(a.group);
   if (plan.most == 1) {
+    if (plan.sort) {
+      int shift = 0;
+      while (a.tokens >> 5 >> shift >= kBins) ++shift;
+      hipLaunchKernelGGL(packed_order_kernel, dim3(1), dim3(kBins), 0, st, a, group, (int)(blocks / a.kv_heads), S::ROWS, shift,
+                         pieces.order);
+      const int rc = check_launch(who);
+      if (rc != G4_OK) return rc;
+    }
     hipLaunchKernelGGL((packed_prefill_kernel<D, NB, false>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a, group, pieces);
     return check_launch(who);
   }
@@ -617,6 +668,8 @@ extern "C" int g4_packed_prefill_attention(const G4PackedPrefillArgs* args, void
   if ((int64_t)a.k_stride * a.head_dim * 2 > 0xffffffffLL || (int64_t)a.tokens * a.group > 0x7fffffffLL - 1024)
     return fail(G4_ERR_UNSUPPORTED, "%s: too many tokens (%d of %d x %d rows of %d)", who, a.tokens, a.kv_heads, a.group, a.head_dim);
   const Plan plan = plan_of(a);
+  if (plan.blocks * plan.most * (a.head_dim == 512 ? kWaves<512> : kWaves<64>) * 64 > 0xffffffffLL)
+    return fail(G4_ERR_UNSUPPORTED, "%s: too many tokens (%d of %d heads)", who, a.tokens, a.kv_heads);
   Pieces pieces;
   const size_t need = carve(pieces, a.workspace, a, plan);
   if (need && (!a.workspace || a.workspace_bytes < need))

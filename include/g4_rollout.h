@@ -255,8 +255,9 @@ int g4_prefill_attention(const G4PrefillArgs* args, void* stream);
  * probabilities are rounded to bf16 as the operand of the value product, the result once to bf16 (g4_prefill_attention
  * also rounds the scores, as the reference does). What a row does not see, NaN included, does not reach it; a row
  * whose scores are all -inf gives zeros. The same call gives the same bits. Few rows with many keys each are taken in
- * pieces of the keys that a second launch joins: such calls need g4_packed_prefill_workspace_size() bytes of scratch
- * (16-byte aligned, no state is kept in it). The sizes decide that, `longest` among them.
+ * pieces of the keys that a second launch joins, and many rows in an order that a launch before finds: such calls need
+ * g4_packed_prefill_workspace_size() bytes of scratch (16-byte aligned, no state is kept in it). The sizes decide that,
+ * `longest` among them.
  */
 typedef struct G4PackedPrefillArgs {
   int32_t tokens;         /* T */

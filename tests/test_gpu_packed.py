@@ -342,3 +342,38 @@ def test_calls_on_two_streams(device):
                 got[i].append(kernels.packed_prefill_attention(*calls[i], starts))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want[i]) for i in range(2) for x in got[i])
+
+
+# --- more blocks than are at work at once: in the order of their keys ----------------------------------------------------
+
+
+@pytest.mark.parametrize("D,H,R", [(64, 2, 16), (256, 8, 4), (512, 3, 8)])
+@pytest.mark.parametrize("lens,tail", [([700, 1, 0, 400, 33, 64, 1000, 3], 45), ([2201], 0)])
+def test_sorted_blocks(D, H, R, lens, tail, device):
+    """Runs of blocks across the sequences' borders and the tokens of none, a short run at the end."""
+
+    q, k, v = _inputs(lens, tail, H, R, D, 61, device)
+    assert 0 < _pieces(q) < 4096 and _pieces(q, 0, 200) == 0
+    got = _run(q, k, v, lens, 0, device, fill=math.nan)
+    _check(got, q, k, v, lens, 0)
+    for longest in (1, 300, 2201):  # whatever the order, the same bits
+        assert torch.equal(_run(q, k, v, lens, 0, device, fill=math.nan, longest=longest), got)
+
+
+def test_sorted_blocks_with_any_starts(device):
+    """starts that no sequences give: tokens of none in the middle, a start behind its token, one far back."""
+
+    T, H, R, D = 1500, 4, 16, 128
+    q, k, v = _inputs([T], 0, H, R, D, 62, device)
+    starts = (torch.arange(T, dtype=torch.int32) // 300) * 300
+    starts[100:230], starts[500], starts[700:705], starts[1400] = -1, 501, 2 ** 31 - 1, 3
+    assert 0 < _pieces(q) < 4096
+    kk, vv = _laid_out(k, v, device)
+    got = kernels.packed_prefill_attention(q.to(device), kk, vv, starts.to(device)).cpu().double()
+    for t in (0, 99, 100, 229, 230, 499, 500, 501, 702, 705, 1399, 1400, 1499):
+        a = int(starts[t])
+        if not 0 <= a <= t:
+            assert bool((got[t] == 0).all())
+            continue
+        want, bound = packed_reference(q[a:t + 1], k[a:t + 1], v[a:t + 1], [t + 1 - a], 0)
+        assert bool(((got[t] - want[-1]).abs() <= bound[-1]).all()), t

@@ -69,8 +69,10 @@ def test_packed_attention_refuses_a_short_workspace():
     few = dict(tokens=1000, k_stride=1024, head_dim=64, kv_heads=1)
     need = _lib.lib().g4_packed_prefill_workspace_size(*_packed(**few))
     assert need > 0 and _lib.lib().g4_packed_prefill_workspace_size(None) == 0
-    for same in (dict(longest=100), dict(window=512), dict(tokens=700), dict(kv_heads=64)):
-        assert _lib.lib().g4_packed_prefill_workspace_size(*_packed(**{**few, **same})) == 0
+    for none in (dict(longest=100), dict(window=512), dict(tokens=700), dict(kv_heads=64, window=500), dict(kv_heads=64, longest=224)):
+        assert _lib.lib().g4_packed_prefill_workspace_size(*_packed(**{**few, **none})) == 0
+    # 2048 workgroups of 128 rows, 32 to a head: the order of 8 runs of them
+    assert _lib.lib().g4_packed_prefill_workspace_size(*_packed(**{**few, "kv_heads": 64})) == 32
     for override in (dict(), dict(workspace=AT), dict(workspace=AT, workspace_bytes=need - 1), dict(workspace_bytes=need)):
         _refused("g4_packed_prefill_attention", _packed(**few, **override), "workspace", (_lib.G4_ERR_WORKSPACE,))
     _refused("g4_packed_prefill_attention", _packed(**few, workspace=AT + 4, workspace_bytes=need), "aligned")
