@@ -31,8 +31,9 @@ constexpr float kSlack = 8.0f;
 
 // A workgroup's work: NB blocks of 16 query rows by each of NW waves. Head dims up to 256: four waves of two blocks (at 256
 // 248 registers), two workgroups on a CU, each of which fills the other's barriers, softmax and loads; K and V^T take two
-// chunks of LDS each, 64 KiB at 256. (8 x 4096 tokens of 2 x 4 heads of 256: 506 us; one workgroup of eight waves with
-// four chunks of each 586, of one block per wave 589.) Head dim 512, whose K and V^T take 128 KiB: eight waves of one block.
+// chunks of LDS each, 64 KiB at 256. (8 x 4096 tokens of 2 x 4 heads of 256, before the blocks were sorted: 506 us; one workgroup
+// of eight waves with four chunks of each 586, of one block per wave 589.) Head dim 512, whose K and V^T take 128 KiB: eight
+// waves of one block.
 template <int D>
 constexpr int kWaves = D == 512 ? 8 : 4;
 template <int D, int NB_>
