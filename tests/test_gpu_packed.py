@@ -377,3 +377,24 @@ def test_sorted_blocks_with_any_starts(device):
             continue
         want, bound = packed_reference(q[a:t + 1], k[a:t + 1], v[a:t + 1], [t + 1 - a], 0)
         assert bool(((got[t] - want[-1]).abs() <= bound[-1]).all()), t
+
+
+def test_sorted_blocks_of_long_sequences(device):
+    """Blocks of more than 1024 chunks, which share bins; sampled tokens against 64 bits."""
+
+    lens, R, D = [7777, 36000, 1], 4, 64
+    q, k, v = _inputs(lens, 0, 1, R, D, 63, device)
+    assert 0 < _pieces(q) < 4096
+    got = _run(q, k, v, lens, 0, device).cpu().double()
+    for t in list(range(0, 43778, 1999)) + [7776, 7777, 43776, 43777]:
+        a = 0 if t < 7777 else 7777 if t < 43777 else 43777
+        x, kk, vv = q[t, 0].double(), k[a:t + 1, 0].double(), v[a:t + 1, 0].double()
+        s = x @ kk.T
+        top = s.amax(dim=-1, keepdim=True)
+        w = torch.softmax(s, dim=-1)
+        # packed_reference's bound for one token
+        ds = (D + 2) * 2.0 ** -24 * (x.abs() @ kk.abs().T) + 4 * 2.0 ** -24 * (1 + s.abs() + top.abs())
+        rel = 2 * ds.amax(dim=-1, keepdim=True) + (2 * len(kk) + 16) * 2.0 ** -24
+        mass = w @ vv.abs()
+        bound = (2.0 ** -8 + rel) * mass * (1 + 2.0 ** -8) + 2.0 ** -8 * (w @ vv).abs() + 1e-37
+        assert bool(((got[t, 0] - w @ vv).abs() <= bound).all()), t
