@@ -335,3 +335,15 @@ def test_the_same_layer_twice_and_one_page(device):
     assert kernels.paged_compact([layer], r, t).tolist() == [1] and t.tolist() == [[0]]
     kernels.paged_free(r, t, _i32([0], device), page_size=32)
     assert r.tolist() == [2] and t.tolist() == [[-1]]
+
+
+@pytest.mark.parametrize("P", [2559, 2560, 2561])
+def test_compact_about_the_change_to_one_launch(P, device):
+    refs, table = _pool(P, 100, 30, P // 2, 71)
+    layer = _layer(P, 1, 64, 32, True, 72, device)
+    old = type(layer)(*(None if x is None else x.clone() for x in layer))
+    r, t = _i32(refs, device), _i32(table, device)
+    live = kernels.paged_compact([layer], r, t)
+    n, moves = plain.compact(refs, table)
+    assert live.tolist() == [n] and r.tolist() == refs and t.tolist() == table
+    _same(layer, plain.moved(old, [(a, b, 32) for a, b in moves], 32))
