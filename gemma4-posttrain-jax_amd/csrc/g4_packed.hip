@@ -29,23 +29,23 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kSlack = 8.0f;
 
-// A workgroup's work: NB blocks of 16 query rows by each of NW waves. Head dims up to 256: four waves of two blocks (at 256
-// 248 registers), two workgroups on a CU, each of which fills the other's barriers, softmax and loads; K and V^T take two
-// chunks of LDS each, 64 KiB at 256. (8 x 4096 tokens of 2 x 4 heads of 256, before the blocks were sorted: 506 us; one workgroup
-// of eight waves with four chunks of each 586, of one block per wave 589.) Head dim 512, whose K and V^T take 128 KiB: eight
-// waves of one block.
-template <int D>
-constexpr int kWaves = D == 512 ? 8 : 4;
-template <int D, int NB_>
+// A workgroup's work: NB blocks of 16 query rows by each of NW waves, 128 rows (BIG) or 64. Head dims up to 256: four waves of two
+// blocks (at 256 248 registers) or one, two workgroups on a CU, each of which fills the other's barriers, softmax and loads; K and
+// V^T take two chunks of LDS each, 64 KiB at 256. (8 x 4096 tokens of 2 x 4 heads of 256, before the blocks were sorted: 506 us; one
+// workgroup of eight waves with four chunks of each 586, of one block per wave 589.) Head dim 512: eight waves of one block alone on
+// the CU, two chunks of each in 128 KiB, or four, two workgroups, one chunk of each (ONE).
+template <int D, bool BIG>
 struct Shape {
-  static constexpr int NB = NB_, NW = kWaves<D>;
+  static constexpr int NB = BIG && D != 512 ? 2 : 1, NW = BIG && D == 512 ? 8 : 4;
+  static constexpr bool ONE = D == 512 && !BIG;
   static constexpr int KS = D / 32;
   static constexpr int T = D / 16;                  // 1 KiB operand tiles of a chunk's K and of its V^T
   static constexpr int CHUNK = T * 1024;
   static constexpr int TW = T / NW;                 // tiles that a wave fetches of each
   static constexpr int ROWS = NW * NB * 16;         // query rows of a workgroup
   static_assert(T % NW == 0, "the waves share the tiles evenly");
-  static_assert(ROWS * D * 2 <= 4 * CHUNK, "the result goes out through the rings");
+  static constexpr int SLOTS = ONE ? 2 : 4;
+  static_assert(ROWS * D * 2 <= SLOTS * CHUNK, "the result goes out through the rings");
 };
 
 // Over the 16 columns of an MFMA tile, whose values every row of 16 lanes holds.
@@ -276,13 +276,14 @@ __global__ __launch_bounds__(kBins) void packed_order_kernel(G4PackedPrefillArgs
 // dim 512) the waves of the second half, which share the SIMDs with those of the first, take the softmax of chunk c - 1
 // first: one runs MFMAs while the other runs vector work (8 x 4096 tokens of 8 heads 1098 us, 1112 without). Chunks of which a
 // wave sees nothing it skips.
-template <int D, int NB, bool CUT>
-__global__ __launch_bounds__(kWaves<D> * 64, 2) void packed_prefill_kernel(G4PackedPrefillArgs a, Group group, Pieces pieces) {
-  using S = Shape<D, NB>;
-  constexpr int NW = S::NW, KS = S::KS, VT = S::T;
-  // K in slots 0 and 1, V^T in 2 and 3, chunk c in slot (c - c_begin) % 2 of its ring; read with inline-assembly LDS reads only:
+template <int D, bool BIG, bool CUT>
+__global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefill_kernel(G4PackedPrefillArgs a, Group group,
+                                                                                         Pieces pieces) {
+  using S = Shape<D, BIG>;
+  constexpr int NB = S::NB, NW = S::NW, KS = S::KS, VT = S::T;
+  // K in slots 0 and 1, V^T in 2 and 3, chunk c in slot (c - c_begin) % 2 of its ring (ONE: K in 0, V^T in 1); read with inline-assembly LDS reads only:
   // the compiler adds no waits of its own for the DMAs in flight
-  __shared__ __attribute__((aligned(1024))) unsigned char ring[4][S::CHUNK];
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[S::SLOTS][S::CHUNK];
   __shared__ int2 spans[NW], bounds[NW * NB * 16];
 
   const int R = a.group, H = a.kv_heads, T = a.tokens;
@@ -392,23 +393,43 @@ __global__ __launch_bounds__(kWaves<D> * 64, 2) void packed_prefill_kernel(G4Pac
         __asm__ volatile("" : "+v"(v));
         qop[cb][s] = as_bf16x8(v);
       }
+    if constexpr (S::ONE) {
 #pragma unroll 1
-    for (int c = c_begin, i = 0; c <= c_end; ++c, ++i) {
+      for (int c = c_begin; c <= c_end; ++c) {
+        const bool now = rows.any(c), more = c < c_end;
+        wait_vmcnt<0>();
+        wg_barrier();  // K(c) is there, V(c - 1) done with
+        issue_v(c, 1);
+        if (now) pf_qk<VT, KS, NB, 4>(ring0, qop, acc);
+        if (more) {
+          wg_barrier();  // K(c) is done with
+          issue_k(c + 1, 0);
+        }
+        if (now) soft.chunk(rows, c, lane, acc, pop, oacc);
+        if (more) wait_vmcnt<S::TW>();
+        else wait_vmcnt<0>();
+        wg_barrier();  // V(c) is there
+        if (now) pf_pv<VT, NB, 4>(ring0 + (uint32_t)S::CHUNK, pop, oacc);
+      }
+    } else {
+#pragma unroll 1
+      for (int c = c_begin, i = 0; c <= c_end; ++c, ++i) {
+        wait_vmcnt<0>();
+        wg_barrier();
+        if (c + 1 <= c_end) issue_k(c + 1, (i + 1) & 1);
+        issue_v(c, 2 + (i & 1));
+        const bool before = c > c_begin && rows.any(c - 1), now = rows.any(c);
+        if (late && before) soft.chunk(rows, c - 1, lane, acc, pop, oacc);
+        if (before) pf_pv<VT, NB, 4>(ring0 + (uint32_t)((2 + ((i - 1) & 1)) * S::CHUNK), pop, oacc);
+        if (now) pf_qk<VT, KS, NB, 4>(ring0 + (uint32_t)((i & 1) * S::CHUNK), qop, acc);
+        if (!late && now) soft.chunk(rows, c, lane, acc, pop, oacc);
+      }
       wait_vmcnt<0>();
       wg_barrier();
-      if (c + 1 <= c_end) issue_k(c + 1, (i + 1) & 1);
-      issue_v(c, 2 + (i & 1));
-      const bool before = c > c_begin && rows.any(c - 1), now = rows.any(c);
-      if (late && before) soft.chunk(rows, c - 1, lane, acc, pop, oacc);
-      if (before) pf_pv<VT, NB, 4>(ring0 + (uint32_t)((2 + ((i - 1) & 1)) * S::CHUNK), pop, oacc);
-      if (now) pf_qk<VT, KS, NB, 4>(ring0 + (uint32_t)((i & 1) * S::CHUNK), qop, acc);
-      if (!late && now) soft.chunk(rows, c, lane, acc, pop, oacc);
-    }
-    wait_vmcnt<0>();
-    wg_barrier();
-    if (rows.any(c_end)) {
-      if (late) soft.chunk(rows, c_end, lane, acc, pop, oacc);
-      pf_pv<VT, NB, 4>(ring0 + (uint32_t)((2 + ((c_end - c_begin) & 1)) * S::CHUNK), pop, oacc);
+      if (rows.any(c_end)) {
+        if (late) soft.chunk(rows, c_end, lane, acc, pop, oacc);
+        pf_pv<VT, NB, 4>(ring0 + (uint32_t)((2 + ((c_end - c_begin) & 1)) * S::CHUNK), pop, oacc);
+      }
     }
   }
 
@@ -537,36 +558,39 @@ __global__ __launch_bounds__(256) void packed_join_kernel(G4PackedPrefillArgs a,
   }
 }
 
-// How a call is laid out. A wave takes one column block where the blocks of two would leave CUs without a workgroup: more, smaller
-// workgroups then end sooner (one prompt of 500 tokens, 2 x 4 heads of 256: 16 us, 23 with two). Between one and two of them per CU
-// those of two columns are all at work at once, which is faster where their keys are about as many (8000 tokens with window 1024: 76
-// us, 94 in twice as many blocks of one; 8 prompts of 1000 52 and 58) and slower where a few have most (one of 8000 300 and 267).
+// How a call is laid out. Blocks of 64 rows where those of 128 would leave CUs without a workgroup: more, smaller workgroups then end
+// sooner (one prompt of 500 tokens, 2 x 4 heads of 256: 16 us, 23 of 128). Between one and two of 128 per CU these are all
+// at work at once, which is faster where their keys are about as many (8000 tokens with window 1024: 76 us, 94 in twice as many of
+// 64; 8 prompts of 1000 52 and 58) and slower where a few have most (one of 8000 300 and 267). Head dim 512, whose blocks of 64 share
+// a CU and those of 128 do not: of 64 up to two of 128 per CU (8 heads: 500 tokens 26 and 32 us, 2 prompts of 1200 and 2000 83 and 94,
+// 13 of up to 2001 189 and 192), beyond that the keys' second way through the L2 costs more (8000 of 2 x 8 heads 963 and 924).
 // Pieces: only where whole blocks leave CUs free and the longest sequence has 768 tokens (one of 600, 4 x 4 heads of 128: 15.6
 // us in pieces, 13.4 whole; of 1000, 2 x 4 of 256, 23 and 28) that a window does not cut (4000 with window 512: 53 and 26).
 // As many as the CUs take at once, of 8 chunks or more: each piece's sums cost a pass through memory (one prompt of 2000, 2
 // x 4 heads of 256: whole 50, in 2 pieces 41, in 4 46 us; 1 head: whole 48, 8 pieces 20). Where the pieces stay long, of 32
 // chunks or more, twice that, as the blocks with the most keys come first and the rest fill up behind them (one of 8000, 1
-// x 2 heads of 128: whole 128, 2 pieces 81, 4 66; one of 4000, 8 heads of 512: whole 198, 2 pieces 163).
+// x 2 heads of 128: whole 128, 2 pieces 81, 4 66; one of 4000, 8 heads of 512: whole 198, 2 pieces 163, in blocks of 128).
 // Sorting: more blocks than are at work at once, whose keys may differ: no window that makes them alike, sequences of 256 tokens
 // and more (8 of 4096, 2 x 4 heads of 256: 504 -> 450 us; 160 of 20 .. 500 70 -> 60; where all are short it is the launch's 4 us:
 // 160 of 60 .. 140 36 -> 39; with window 512 256 prompts of 32 .. 480 175 -> 180).
 struct Plan {
-  int nb, most, chunks;    // column blocks per wave; pieces of a block at most (1: whole blocks), chunks of one
+  bool big;                // Shape's
+  int most, chunks;        // pieces of a block at most (1: whole blocks), chunks of one
   int64_t blocks, padded;  // workgroups without pieces; rows per head, the last block's filled up
   bool sort;               // the runs of blocks by their chunks
 };
 Plan plan_of(const G4PackedPrefillArgs& a) {
-  const int D = a.head_dim, nw = D == 512 ? kWaves<512> : kWaves<64>;
-  const int64_t rows = (int64_t)a.tokens * a.group, resident = D == 512 ? 256 : 512;
-  const auto per_head = [&](int nb) { return (rows + nw * nb * 16 - 1) / (nw * nb * 16); };
+  const int64_t rows = (int64_t)a.tokens * a.group;
+  const auto per_head = [&](bool big) { return (rows + (big ? 127 : 63)) / (big ? 128 : 64); };
   Plan p{};
   const int64_t longest = a.longest > 0 && a.longest < a.tokens ? a.longest : a.tokens, chunks = (longest + 31) / 32;
   const bool cut = a.window > 0 && a.window < longest, alike = cut || longest * 4 < a.tokens;
-  p.nb = D == 512 || per_head(2) * a.kv_heads <= (alike ? resident / 2 : resident) ? 1 : 2;
-  p.blocks = per_head(p.nb) * a.kv_heads;
-  p.padded = per_head(p.nb) * nw * p.nb * 16;
+  p.big = per_head(true) * a.kv_heads > (a.head_dim != 512 && alike ? 256 : 512);
+  const int64_t resident = a.head_dim == 512 && p.big ? 256 : 512;
+  p.blocks = per_head(p.big) * a.kv_heads;
+  p.padded = per_head(p.big) * (p.big ? 128 : 64);
   p.most = 1;
-  if (p.nb == 1 && p.blocks < resident && chunks >= 24 && !cut) {
+  if (!p.big && p.blocks < resident && chunks >= 24 && !cut) {
     const int64_t most = std::min<int64_t>(kMostPieces, std::max(std::min(resident / p.blocks, chunks / 8),
                                                                 std::min(2 * resident / p.blocks, chunks / 32)));
     if (most > 1) {
@@ -589,10 +613,10 @@ size_t carve(Pieces& p, void* base, const G4PackedPrefillArgs& a, const Plan& pl
   return plan.most > 1 ? (size_t)rows * (a.head_dim * 4 + sizeof(Piece)) : 0;
 }
 
-template <int D, int NB>
+template <int D, bool BIG>
 int launch_packed(const G4PackedPrefillArgs& a, const Plan& plan, const Pieces& pieces, hipStream_t st) {
   static const char who[] = "g4_packed_prefill_attention";
-  using S = Shape<D, NB>;
+  using S = Shape<D, BIG>;
   const int64_t blocks = plan.blocks * plan.most;
   const Group group(a.group);
   if (plan.most == 1) {
@@ -604,11 +628,11 @@ int launch_packed(const G4PackedPrefillArgs& a, const Plan& plan, const Pieces& 
       const int rc = check_launch(who);
       if (rc != G4_OK) return rc;
     }
-    hipLaunchKernelGGL((packed_prefill_kernel<D, NB, false>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a, group, pieces);
+    hipLaunchKernelGGL((packed_prefill_kernel<D, BIG, false>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a, group, pieces);
     return check_launch(who);
   }
-  if constexpr (NB == 1) {
-    hipLaunchKernelGGL((packed_prefill_kernel<D, 1, true>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a, group, pieces);
+  if constexpr (!BIG) {
+    hipLaunchKernelGGL((packed_prefill_kernel<D, false, true>), dim3((unsigned)blocks), dim3(S::NW * 64), 0, st, a, group, pieces);
     const int rc = check_launch(who);
     if (rc != G4_OK) return rc;
     const int64_t rows = (int64_t)a.tokens * a.group * a.kv_heads;
@@ -618,9 +642,7 @@ int launch_packed(const G4PackedPrefillArgs& a, const Plan& plan, const Pieces& 
 }
 template <int D>
 int launch_packed(const G4PackedPrefillArgs& a, const Plan& plan, const Pieces& pieces, hipStream_t st) {
-  if constexpr (D != 512)
-    if (plan.nb == 2) return launch_packed<D, 2>(a, plan, pieces, st);
-  return launch_packed<D, 1>(a, plan, pieces, st);
+  return plan.big ? launch_packed<D, true>(a, plan, pieces, st) : launch_packed<D, false>(a, plan, pieces, st);
 }
 
 // starts[t]: the first token of t's sequence, -1 behind the last sequence. One thread per token, a binary search.
@@ -669,7 +691,7 @@ extern "C" int g4_packed_prefill_attention(const G4PackedPrefillArgs* args, void
   if ((int64_t)a.k_stride * a.head_dim * 2 > 0xffffffffLL || (int64_t)a.tokens * a.group > 0x7fffffffLL - 1024)
     return fail(G4_ERR_UNSUPPORTED, "%s: too many tokens (%d of %d x %d rows of %d)", who, a.tokens, a.kv_heads, a.group, a.head_dim);
   const Plan plan = plan_of(a);
-  if (plan.blocks * plan.most * (a.head_dim == 512 ? kWaves<512> : kWaves<64>) * 64 > 0xffffffffLL)
+  if (plan.blocks * plan.most * (a.head_dim == 512 && plan.big ? 512 : 256) > 0xffffffffLL)
     return fail(G4_ERR_UNSUPPORTED, "%s: too many tokens (%d of %d heads)", who, a.tokens, a.kv_heads);
   Pieces pieces;
   const size_t need = carve(pieces, a.workspace, a, plan);

@@ -251,13 +251,13 @@ def test_pieces_in_a_graph_with_eager_calls_between(device):
         assert torch.equal(out, b if replay % 2 else a)
 
 
-# --- many rows: two column blocks per wave -----------------------------------------------------------------------------
+# --- many rows: blocks of 128 -----------------------------------------------------------------------------
 
 
 MANY = [33, 0, 1, 130, 65, 2, 250, 31, 45]  # 557 tokens of 8 x 16 heads: 560 workgroups of 128 rows
 
 
-@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
 @pytest.mark.parametrize("window", [0, 40])
 def test_many_rows(D, window, device):
     q, k, v = _inputs(MANY, 3, 8, 16, D, 21, device)
@@ -265,7 +265,7 @@ def test_many_rows(D, window, device):
     _check(got, q, k, v, MANY, window)
 
 
-@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
 def test_many_rows_with_values_that_are_not_finite(D, device):
     q, k, v = _inputs(MANY, 3, 8, 16, D, 22, device)
     want, bound = packed_reference(q, k, v, MANY, 0)
@@ -347,7 +347,7 @@ def test_calls_on_two_streams(device):
 # --- more blocks than are at work at once: in the order of their keys ----------------------------------------------------
 
 
-@pytest.mark.parametrize("D,H,R", [(64, 2, 16), (256, 8, 4), (512, 3, 8)])
+@pytest.mark.parametrize("D,H,R", [(64, 2, 16), (256, 8, 4), (512, 3, 8), (512, 4, 8)])
 @pytest.mark.parametrize("lens,tail", [([700, 1, 0, 400, 33, 64, 1000, 3], 45), ([2201], 0)])
 def test_sorted_blocks(D, H, R, lens, tail, device):
     """Runs of blocks across the sequences' borders and the tokens of none, a short run at the end."""
