@@ -598,7 +598,7 @@ Plan plan_of(const G4PackedPrefillArgs& a) {
       p.most = (int)((chunks + p.chunks - 1) / p.chunks);
     }
   }
-  p.sort = p.most == 1 && p.blocks > resident && chunks >= 8 && !cut;
+  p.sort = p.most == 1 && p.blocks > resident && p.blocks >= 2 * kRun * (int64_t)a.kv_heads && chunks >= 8 && !cut;
   return p;
 }
 

@@ -398,3 +398,49 @@ def test_sorted_blocks_of_long_sequences(device):
         mass = w @ vv.abs()
         bound = (2.0 ** -8 + rel) * mass * (1 + 2.0 ** -8) + 2.0 ** -8 * (w @ vv).abs() + 1e-37
         assert bool(((got[t, 0] - w @ vv).abs() <= bound).all()), t
+
+
+def test_sorted_blocks_in_a_graph_and_on_streams(device):
+    """Replays with other sequences and calls on two streams, each with an order of its own."""
+
+    T, H, R, D = 2201, 2, 16, 64
+    sets = []
+    for i, lens in enumerate(([2201], [300, 1901], [1100, 1, 1100])):
+        q, k, v = _inputs(lens, 0, H, R, D, 70 + i, device)
+        cu = torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=torch.int32, device=device)
+        sets.append((q.to(device), *_laid_out(k, v, device), kernels.packed_starts(cu, T)))
+    assert 0 < _pieces(sets[0][0]) < 4096
+    want = [kernels.packed_prefill_attention(*s) for s in sets]
+    static = [t.clone() for t in sets[0]]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        kernels.packed_prefill_attention(*static)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = kernels.packed_prefill_attention(*static)
+    for i in (1, 2, 0, 1):
+        for to, x in zip(static, sets[i]):
+            to.copy_(x)
+        graph.replay()
+        assert torch.equal(kernels.packed_prefill_attention(*sets[2 - i]), want[2 - i])
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])
+    streams, got = [torch.cuda.Stream() for _ in sets], [[] for _ in sets]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(kernels.packed_prefill_attention(*sets[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for g, w in zip(got, want) for x in g)
+
+
+def test_many_heads_of_few_blocks(device):
+    """More workgroups than are at work at once, but one or two blocks a head: no order to find."""
+
+    T, H, R, D = 300, 260, 1, 64
+    q, k, v = _inputs([T], 0, H, R, D, 75, device)
+    assert _pieces(q) == 0
+    got = _run(q, k, v, [T], 0, device)
+    _check(got[:, ::37], q[:, ::37], k[:, ::37], v[:, ::37], [T], 0)
