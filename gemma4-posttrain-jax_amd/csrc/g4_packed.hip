@@ -3,7 +3,7 @@
 // scores and the softmax of model.py:320-335, 496-499 per sequence.
 //
 // The query rows of one kv head are the (token, r) pairs in order, T R of them; a workgroup takes the next
-// NW * NB * 16, whatever sequences they belong to, and walks the 32-key chunks from the first key that one of them
+// 128 or 64, whatever sequences they belong to, and walks the 32-key chunks from the first key that one of them
 // sees to its last token. A row's keys are one interval [lo, hi], so that a mask is two comparisons: no list of
 // tiles, and short sequences share a workgroup. Per chunk S^T = K q^T and O^T += V^T P^T by MFMA 16x16x32, the
 // layouts' operand order making the scores' registers the value product's operand.
@@ -274,15 +274,15 @@ __global__ __launch_bounds__(kBins) void packed_order_kernel(G4PackedPrefillArgs
 // A step per chunk c: behind its barrier, which every wave's share of K(c) and V(c - 1) has landed before, K(c + 1) and V(c) are
 // asked for; then the values of chunk c - 1, the scores of chunk c and their softmax. Of a workgroup that has the CU alone (head
 // dim 512) the waves of the second half, which share the SIMDs with those of the first, take the softmax of chunk c - 1
-// first: one runs MFMAs while the other runs vector work (8 x 4096 tokens of 8 heads 1098 us, 1112 without). Chunks of which a
-// wave sees nothing it skips.
+// first: one runs MFMAs while the other runs vector work (8 x 4096 tokens of 8 heads 1098 us, 1112 without). ONE asks for K(c + 1)
+// behind the scores of chunk c and for V(c) behind the values of chunk c - 1. Chunks of which a wave sees nothing it skips.
 template <int D, bool BIG, bool CUT>
 __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefill_kernel(G4PackedPrefillArgs a, Group group,
                                                                                          Pieces pieces) {
   using S = Shape<D, BIG>;
   constexpr int NB = S::NB, NW = S::NW, KS = S::KS, VT = S::T;
-  // K in slots 0 and 1, V^T in 2 and 3, chunk c in slot (c - c_begin) % 2 of its ring (ONE: K in 0, V^T in 1); read with inline-assembly LDS reads only:
-  // the compiler adds no waits of its own for the DMAs in flight
+  // K in slots 0 and 1, V^T in 2 and 3, chunk c in slot (c - c_begin) % 2 of its ring (ONE: K in 0, V^T in 1); read with
+  // inline-assembly LDS reads only: the compiler adds no waits of its own for the DMAs in flight
   __shared__ __attribute__((aligned(1024))) unsigned char ring[S::SLOTS][S::CHUNK];
   __shared__ int2 spans[NW], bounds[NW * NB * 16];
 
@@ -562,8 +562,8 @@ __global__ __launch_bounds__(256) void packed_join_kernel(G4PackedPrefillArgs a,
 // sooner (one prompt of 500 tokens, 2 x 4 heads of 256: 16 us, 23 of 128). Between one and two of 128 per CU these are all
 // at work at once, which is faster where their keys are about as many (8000 tokens with window 1024: 76 us, 94 in twice as many of
 // 64; 8 prompts of 1000 52 and 58) and slower where a few have most (one of 8000 300 and 267). Head dim 512, whose blocks of 64 share
-// a CU and those of 128 do not: of 64 up to two of 128 per CU (8 heads: 500 tokens 26 and 32 us, 2 prompts of 1200 and 2000 83 and 94,
-// 13 of up to 2001 189 and 192), beyond that the keys' second way through the L2 costs more (8000 of 2 x 8 heads 963 and 924).
+// a CU and those of 128 do not: of 64 up to two of 128 per CU (8 heads: 500 tokens 26 and 32 us, 2 prompts of 1200 and 2000 83 and
+// 94), beyond that the keys' second way through the L2 costs more (8000 tokens of 2 x 8 heads 963 and 924).
 // Pieces: only where whole blocks leave CUs free and the longest sequence has 768 tokens (one of 600, 4 x 4 heads of 128: 15.6
 // us in pieces, 13.4 whole; of 1000, 2 x 4 of 256, 23 and 28) that a window does not cut (4000 with window 512: 53 and 26).
 // As many as the CUs take at once, of 8 chunks or more: each piece's sums cost a pass through memory (one prompt of 2000, 2
