@@ -570,9 +570,10 @@ __global__ __launch_bounds__(256) void packed_join_kernel(G4PackedPrefillArgs a,
 // x 4 heads of 256: whole 50, in 2 pieces 41, in 4 46 us; 1 head: whole 48, 8 pieces 20). Where the pieces stay long, of 32
 // chunks or more, twice that, as the blocks with the most keys come first and the rest fill up behind them (one of 8000, 1
 // x 2 heads of 128: whole 128, 2 pieces 81, 4 66; one of 4000, 8 heads of 512: whole 198, 2 pieces 163, in blocks of 128).
-// Sorting: more blocks than are at work at once, whose keys may differ: no window that makes them alike, sequences of 256 tokens
-// and more (8 of 4096, 2 x 4 heads of 256: 504 -> 450 us; 160 of 20 .. 500 70 -> 60; where all are short it is the launch's 4 us:
-// 160 of 60 .. 140 36 -> 39; with window 512 256 prompts of 32 .. 480 175 -> 180).
+// Sorting: more blocks than are at work at once, whose keys may differ (no window that makes them alike), the longest of them long beside
+// the rounds that all take (8 prompts of 4096, 2 x 4 heads of 256: 504 -> 450 us; 30 of 100 .. 900 72 -> 60; 64 of 32 .. 1000 136 -> 129).
+// Else the end weighs little, and the launch and the keys that neighbours no longer share cost more (256 of 32 .. 480 188 -> 190,
+// 512 of them 337 -> 358). Where the longest is not known up to four rounds are sorted.
 struct Plan {
   bool big;                // Shape's
   int most, chunks;        // pieces of a block at most (1: whole blocks), chunks of one
@@ -598,7 +599,8 @@ Plan plan_of(const G4PackedPrefillArgs& a) {
       p.most = (int)((chunks + p.chunks - 1) / p.chunks);
     }
   }
-  p.sort = p.most == 1 && p.blocks > resident && p.blocks >= 2 * kRun * (int64_t)a.kv_heads && chunks >= 8 && !cut;
+  p.sort = p.most == 1 && p.blocks > resident && p.blocks >= 2 * kRun * (int64_t)a.kv_heads && chunks >= 8 && !cut &&
+           (a.longest > 0 ? chunks : std::min<int64_t>(chunks, 24)) * resident >= 6 * p.blocks;
   return p;
 }
 
@@ -709,7 +711,7 @@ extern "C" int g4_packed_prefill_attention(const G4PackedPrefillArgs* args, void
 
 extern "C" size_t g4_packed_prefill_workspace_size(const G4PackedPrefillArgs* args) {
   using namespace g4;
-  if (!args || args->tokens <= 0 || args->kv_heads <= 0 || args->group <= 0 || args->head_dim <= 0) return 0;
+  if (!args || args->tokens <= 0 || args->kv_heads <= 0 || args->group <= 0 || args->group > 64 || args->head_dim <= 0) return 0;
   Pieces pieces;
   return carve(pieces, nullptr, *args, plan_of(*args));
 }
