@@ -201,21 +201,22 @@ __device__ __forceinline__ floatx4 careful_values(const Rows& rows, int cb, floa
   return o;
 }
 
-// Which block of rows and head workgroup i takes. Workgroups are dealt to the 8 XCDs round robin: runs of kRun consecutive
-// blocks of a head, which read the same keys, go to one XCD and its L2 (256 prompts of 32 .. 480 tokens, window 512: 3 % over
-// single blocks; runs of 16 lose 10 % on 3 prompts of up to 8191). The runs go in `order`, or the latest tokens' first.
-constexpr int kXcds = 8, kRun = 4;
+// Which block of rows and head workgroup i takes. Workgroups are dealt to the 8 XCDs round robin: runs of consecutive blocks of a
+// head, which read the same keys, go to one XCD and its L2. Runs of kRun in `order`, or of kLongRun, the latest tokens' first (256
+// prompts of 32 .. 480 tokens, window 512: single blocks 181 us, runs of 4 178, 8 174, 16 174; of 256 each 177, 171, 149, 151).
+constexpr int kXcds = 8, kRun = 4, kLongRun = 8;
 __device__ __forceinline__ void place_block(int i, int n_blk, int H, const int32_t* order, int& blk, int& h) {
-  const int even = n_blk * H / (kXcds * kRun) * (kXcds * kRun);  // as many as fill whole turns of runs
+  const int each = order ? kRun : kLongRun;
+  const int even = n_blk * H / (kXcds * each) * (kXcds * each);  // as many as fill whole turns of runs
   int u = i;
   if (i < even) {
     const int x = i % kXcds, j = i / kXcds;
-    u = ((j / kRun) * kXcds + x) * kRun + j % kRun;
+    u = ((j / each) * kXcds + x) * each + j % each;
   }
   // u in the order (run of blocks, head, block of the run); the last run may be short
-  const int run = u / (kRun * H), rest = u - run * kRun * H, len = min(kRun, n_blk - run * kRun);
+  const int run = u / (each * H), rest = u - run * each * H, len = min(each, n_blk - run * each);
   h = rest / len;
-  blk = n_blk - 1 - ((order && len == kRun ? order[run] : run) * kRun + rest - h * len);
+  blk = n_blk - 1 - ((order && len == each ? order[run] : run) * each + rest - h * len);
 }
 
 // Where few blocks would leave CUs idle for long, a block's chunks are taken in pieces, a workgroup each, whose sums a second
