@@ -69,22 +69,16 @@ struct Group {
   __device__ __forceinline__ int token(int row) const { return (int)((uint64_t)(uint32_t)row * m >> s); }
 };
 
-// The wave's rows: row i of column block cb (i = lane % 16) sees the keys [x, y] at LDS address bounds + 8 (16 cb + i).
-// They are read where a chunk is not seen by all rows, and take no registers over the others.
+// The wave's rows. This lane's row of column block cb (lane % 16) sees the keys [keys[cb].x, keys[cb].y].
 struct Rows {
-  uint32_t bounds;
+  int2 keys[2];
   int first, last;            // the keys that some row sees lie in [first, last]
-  int all_from, all_to;       // every row that sees any sees [all_from, all_to]
+  int all_from[2], all_to[2];  // every row of the column block that sees any sees [all_from, all_to]
   __device__ __forceinline__ bool any(int c) const { return (c << 5) + 31 >= first && (c << 5) <= last; }
-  __device__ __forceinline__ bool full(int c) const { return (c << 5) >= all_from && (c << 5) + 31 <= all_to; }
-  __device__ __forceinline__ int2 keys(int cb, int col) const {
-    int2 v;  // (in assembly: the compiler would wait for the DMAs in flight into other LDS)
-    __asm__ volatile("ds_read_b64 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(v) : "v"(bounds + 8u * (uint32_t)(16 * cb + col)));
-    return v;
-  }
+  __device__ __forceinline__ bool full(int cb, int c) const { return (c << 5) >= all_from[cb] && (c << 5) + 31 <= all_to[cb]; }
   // bit e <-> key k + e
-  __device__ static __forceinline__ uint32_t bits(int2 keys, int k) {
-    const int from = min(max(keys.x - k, 0), 8), to = min(max(keys.y - k + 1, 0), 8);  // elements [from, to)
+  __device__ static __forceinline__ uint32_t bits(int2 seen, int k) {
+    const int from = min(max(seen.x - k, 0), 8), to = min(max(seen.y - k + 1, 0), 8);  // elements [from, to)
     return (0xffu << from) & ((1u << to) - 1u);
   }
 };
@@ -103,14 +97,16 @@ struct Softmax {
 
   __device__ __forceinline__ void chunk(const Rows& rows, int c, int lane, floatx4 (&acc)[NB][2], bf16x8 (&pop)[NB],
                                         floatx4 (&oacc)[NB][VT]) {
-    if (!rows.full(c)) {
+#pragma unroll
+    for (int cb = 0; cb < NB; ++cb) {  // (a wave across a sequence's end masks one of them in every chunk)
+      if (rows.full(cb, c)) continue;
       int k = c << 5;
       __asm__ volatile("" : "+s"(k));  // hidden: else its place relative to every row advances in registers
+      const uint32_t bits = Rows::bits(rows.keys[cb], k + 8 * (lane >> 4));
 #pragma unroll
-      for (int cb = 0; cb < NB; ++cb) {
-        const uint32_t bits = Rows::bits(rows.keys(cb, lane & 15), k + 8 * (lane >> 4));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[cb][e >> 2][e & 3] = bits >> e & 1u ? acc[cb][e >> 2][e & 3] : kNegInf;
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t seen = (uint32_t)__builtin_amdgcn_sbfe((int)bits, e, 1);  // all bits or none
+        acc[cb][e >> 2][e & 3] = __uint_as_float((seen & __float_as_uint(acc[cb][e >> 2][e & 3])) | (~seen & 0xff800000u));
       }
     }
     float top[NB];
@@ -175,7 +171,7 @@ __device__ __forceinline__ floatx4 careful_values(const Rows& rows, int cb, floa
     }
     uint32_t seen = 0;  // bit k <-> key 32 c + k
 #pragma unroll
-    for (int g = 0; g < 4; ++g) seen |= Rows::bits(rows.keys(cb, col), (c << 5) + 8 * g) << (8 * g);
+    for (int g = 0; g < 4; ++g) seen |= Rows::bits(rows.keys[cb], (c << 5) + 8 * g) << (8 * g);
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -285,7 +281,7 @@ __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefi
   // K in slots 0 and 1, V^T in 2 and 3, chunk c in slot (c - c_begin) % 2 of its ring (ONE: K in 0, V^T in 1); read with
   // inline-assembly LDS reads only: the compiler adds no waits of its own for the DMAs in flight
   __shared__ __attribute__((aligned(1024))) unsigned char ring[S::SLOTS][S::CHUNK];
-  __shared__ int2 spans[NW], bounds[NW * NB * 16];
+  __shared__ int2 spans[NW];
 
   const int R = a.group, H = a.kv_heads, T = a.tokens;
   const int n_blk = (int)(gridDim.x / (unsigned)(CUT ? H * pieces.most : H));
@@ -296,7 +292,7 @@ __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefi
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row0 = blk * S::ROWS + w * (NB * 16);
 
-  Rows rows{lds_addr(&bounds[w * NB * 16]), 0x7fffffff, -1, 0, 0x7fffffff};
+  Rows rows{{}, 0x7fffffff, -1, {0, 0}, {0x7fffffff, 0x7fffffff}};
   bf16x8 qop[NB][KS];
   int token[NB], start[NB];
 #pragma unroll
@@ -319,20 +315,23 @@ __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefi
     const int t = token[cb];
     const bool has_keys = t < T && start[cb] >= 0 && start[cb] <= t;
     const int lo = has_keys ? max(start[cb], a.window > 0 ? t - a.window + 1 : 0) : 0, hi = has_keys ? t : -1;
-    if (grp == 0) bounds[(w * NB + cb) * 16 + col] = make_int2(lo, hi);
+    rows.keys[cb] = make_int2(lo, hi);
     if (has_keys) {
       rows.first = min(rows.first, lo);
       rows.last = max(rows.last, hi);
-      rows.all_from = max(rows.all_from, lo);
-      rows.all_to = min(rows.all_to, hi);
+      rows.all_from[cb] = lo;
+      rows.all_to[cb] = hi;
     }
   }
   const auto least = [](int x, int y) { return min(x, y); };
   const auto most = [](int x, int y) { return max(x, y); };
   rows.first = columns_reduce(rows.first, least);
   rows.last = columns_reduce(rows.last, most);
-  rows.all_from = columns_reduce(rows.all_from, most);
-  rows.all_to = columns_reduce(rows.all_to, least);
+#pragma unroll
+  for (int cb = 0; cb < NB; ++cb) {
+    rows.all_from[cb] = columns_reduce(rows.all_from[cb], most);
+    rows.all_to[cb] = columns_reduce(rows.all_to[cb], least);
+  }
   if (lane == 0) spans[w] = make_int2(rows.first, rows.last);
   wg_barrier();  // (q is still on its way)
   int first = 0x7fffffff, last = -1;
@@ -439,7 +438,7 @@ __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefi
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) {
       float l = column_sum(soft.l[cb]);
-      if (rows.keys(cb, col).y < 0) l = 0.f;  // (chunks that all other rows see whole were not masked)
+      if (rows.keys[cb].y < 0) l = 0.f;  // (chunks that all other rows see whole were not masked)
       const int64_t row = base + cb * 16 + col;
       if (grp == 0) pieces.stats[row] = Piece{soft.m[cb], l, n_pieces, 0};
       float sum = 0.f;
@@ -472,7 +471,7 @@ __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefi
     const float l = column_sum(soft.l[cb]);
     const int row = row0 + cb * 16 + (lane_o & 15), t = group.token(row);
     if (CUT && lane_o < 16) pieces.stats[(int64_t)h * ((int64_t)n_blk * S::ROWS) + row] = Piece{0.f, 0.f, 1, 0};  // nothing to join
-    const bool none = rows.keys(cb, lane_o & 15).y < 0 || l == 0.f;
+    const bool none = rows.keys[cb].y < 0 || l == 0.f;
     const float inv = none ? 0.f : 1.0f / l;
     const auto pack = [&](floatx4 x) {
       x = none ? floatx4{0.f, 0.f, 0.f, 0.f} : x * inv;
