@@ -231,7 +231,7 @@ struct Pieces {
 };
 
 // The runs of blocks by the chunks of their longest block, most first: the last workgroups to start are short ones (CUs at work for 71 %
-// of the time on 3 prompts of up to 8191 tokens without it; 398 -> 368 us). By bins of 2^shift chunks, within one in any
+// of the time on 3 prompts of up to 8191 tokens without it, 79 % with; 398 -> 368 us). By bins of 2^shift chunks, within one in any
 // order, which no result depends on. One workgroup, 4 us with its launch. (By single blocks, whose neighbours then lie on other XCDs:
 // 420 us.)
 constexpr int kBins = 1024;
