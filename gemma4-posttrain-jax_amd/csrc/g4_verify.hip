@@ -136,11 +136,13 @@ struct Heat {
   }
 };
 
-// exp2(x c - m c) with one fma per x, for |m| below 1e30 (else m c may pass f32): the rounding of m c, alike for every x of a
-// sum, is made up for once, by `rest`.
+// exp2(x c - m c) with one fma per x, where |m c| is below 2^27 (`tame`): the rounding of m c, alike for every x of a sum, is made up
+// for once, by `rest`. It is at most 4 there, so that both factors are within 2^4 of what they would be without it; of a larger m c
+// it may pass 127, one factor be 0 and the other infinite.
 struct Below {
   float c, mc, rest;
   __device__ __forceinline__ Below(float m, float c_) : c(c_), mc(m * c_), rest(__builtin_amdgcn_exp2f(-fmaf(m, c_, -mc))) {}
+  __device__ __forceinline__ bool tame() const { return fabsf(mc) < 0x1p27f; }
   __device__ __forceinline__ float exp(float x) const { return __builtin_amdgcn_exp2f(fmaf(x, c, -mc)); }
 };
 
@@ -165,8 +167,8 @@ __device__ __forceinline__ Stats wave_join(Stats s, float c) {
 template <int VECS>
 __device__ __forceinline__ float sum_exp(const float (&x)[VECS][8], float m, float c) {
   float sum = 0.f;
-  if (fabsf(m) < 1e30f) {
-    const Below below(m, c);
+  const Below below(m, c);
+  if (below.tame()) {
 #pragma unroll
     for (int v = 0; v < VECS; ++v)
 #pragma unroll
@@ -495,7 +497,7 @@ __global__ __launch_bounds__(kThreads) void verify_race_kernel(G4VerifyArgs a, V
     }
   }
   // ln 2 times the scores' bounds (the pace by log2): the rough probabilities are within 1e-5, and q <= p where r >= 0
-  const bool tame = fabsf(p.m) < 1e30f && fabsf(q.m) < 1e30f;  // else none (Below)
+  const bool tame = p.rough.tame() && q.rough.tame();  // else there are none, and every element may win
   float high[VECS][8], bar = 0.f;
 #pragma unroll
   for (int v = 0; v < VECS; ++v)
