@@ -336,7 +336,7 @@ __device__ __forceinline__ int accepted(const G4VerifyArgs& a, int n, const Draf
   bool good = false;
   if (s < n) {
     if constexpr (MODE == kGreedy) {
-      good = d.id == st[s].idx;
+      good = d.there && d.id == st[s].idx;
     } else if (d.there) {
       // u q < p, both sides times both sums, in 64 bits: neither over- nor underflows where the draft is unlikely
       const double c = 1.0 / (double)a.temperature, p = exp(((double)d.x - st[s].m) * c);
