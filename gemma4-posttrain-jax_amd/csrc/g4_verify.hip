@@ -280,8 +280,20 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(G4VerifyArgs a, 
 
 // --- which drafts are accepted ------------------------------------------------------------------------------------------
 
+// The first column of -inf in a row of nothing but -inf and NaN, by one wave (kNoColumn: none).
+template <bool BF16>
+__device__ __forceinline__ int first_lowest(const void* row, int vocab) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int i = 0; i < vocab; i += 64) {
+    const uint64_t low = __ballot(i + lane < vocab && logit<BF16>(row, i + lane) == -__builtin_inff());
+    if (low) return i + __builtin_ctzll(low);
+  }
+  return kNoColumn;
+}
+
 // The rows' statistics from their chunks' (the waves take rows in turns, a wave's lanes the chunks).
-template <int MODE>
+template <bool BF16, int MODE>
 __device__ __forceinline__ void join_rows(const G4VerifyArgs& a, const VerifyWorkspace& w, int b, int rows, int splits, int n,
                                           Stats* out) {
   const int lane = threadIdx.x & 63;
@@ -299,6 +311,8 @@ __device__ __forceinline__ void join_rows(const G4VerifyArgs& a, const VerifyWor
       all = wave_join<MODE>(lane == 0 ? all : lane == 1 ? more : none, c);
     }
     if (MODE == kUnit) all.unit = all.heat;
+    if (MODE == kGreedy && all.idx == kNoColumn && reached(r))  // (uniform) no logit above -inf
+      all.idx = first_lowest<BF16>(row_at<BF16>(a.logits, a.batch_stride, a.row_stride, b, r), a.vocab);
     if (lane == 0 && reached(r)) out[r] = all;
     s = next;
   }
@@ -379,14 +393,14 @@ __device__ __forceinline__ void decide(const G4VerifyArgs& a, const VerifyWorksp
   const int n = drafts_of(a, b);
   const Draft draft = load_draft<BF16, MODE>(a, b, threadIdx.x < 64 ? n : 0);
   const Stats* st = out.st;
-  join_rows<MODE>(a, w, b, rows, splits, n, out.st);
+  join_rows<BF16, MODE>(a, w, b, rows, splits, n, out.st);
   if (threadIdx.x >= 64) return;
   const int count = accepted<BF16, MODE>(a, n, draft, st);
   if (write) write_accepted(a, b, count, draft, st);
   const int id = __shfl(draft.id, count < 63 ? count : 63, 64);
   if (threadIdx.x != 0) return;
   if constexpr (MODE == kGreedy) {
-    // (a row of nothing but -inf and NaN has no largest)
+    // (a row of nothing but NaN has no largest)
     write_token<BF16>(a, b, count, st[count].idx != kNoColumn ? st[count].idx : 0, st[count].m, st[count].unit);
   } else {
     const bool rejected = count < n, residual = rejected && a.draft_logits;
