@@ -10,6 +10,8 @@
 // exponentials (a first launch, statistics per chunk of a row, which also clears the counters by which the last of a b's
 // workgroups in the race, which writes the token, is found), then of two rows per b and the noise for the race (a
 // third). Which rows these are a launch between finds from the statistics, or the race itself.
+#include <algorithm>
+
 #include "g4_common.h"
 #include "g4_internal.h"
 
@@ -588,15 +590,14 @@ template <bool BF16, int MODE, int VECS, int TIMES>
 int launch_verify(const G4VerifyArgs& a, const VerifyWorkspace& w, hipStream_t st) {
   static const char who[] = "g4_verify_draft";
   const int splits = splits_of(a, VECS * TIMES), rows = a.drafts + 1 + (MODE != kGreedy && a.draft_logits ? a.drafts : 0);
-  const int64_t blocks = (int64_t)a.batch * rows * splits;
-  if (blocks * kThreads > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "%s: too many logits", who);
+  const int race = splits_of(a, kRace);
+  const int64_t blocks = (int64_t)a.batch * rows * splits, racers = (int64_t)a.batch * race;  // (either may be the larger grid)
+  if (std::max(blocks, MODE == kGreedy ? 0 : racers) * kThreads > 0xffffffffLL) return fail(G4_ERR_UNSUPPORTED, "%s: too many logits", who);
   hipLaunchKernelGGL((verify_stats_kernel<BF16, MODE, VECS, TIMES>), dim3((unsigned)blocks), dim3(kThreads), 0, st, a, w, rows, splits);
   int rc = check_launch(who);
   if (rc != G4_OK) return rc;
   const double c = 1.4426950408889634074 / (double)a.temperature;
   const Heat heat{(float)c, (float)(c - (double)(float)c)};
-  const int race = splits_of(a, kRace);
-  const int64_t racers = (int64_t)a.batch * race;  // (fewer than above: rows >= 2)
   if (MODE == kGreedy || racers > kOwn) {
     hipLaunchKernelGGL((verify_decide_kernel<BF16, MODE>), dim3((unsigned)a.batch), dim3(kThreads), 0, st, a, w, rows, splits);
     if ((rc = check_launch(who)) != G4_OK) return rc;
