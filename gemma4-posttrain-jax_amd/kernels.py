@@ -639,7 +639,7 @@ def _with_workspace(a, size, like: torch.Tensor):
 def paged_reserve(refs: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, *, page_size: int) -> torch.Tensor:
     """g4_paged_reserve: fresh pages for the entries of ``page_table [B, M]`` that positions below ``lengths[b]`` need and
     that hold none, in place, with ``refs [P]`` (all int32). Row by row, the lowest free pages (``refs`` 0) first; returns the
-    number of entries that got none, an int32 ``[1]`` on the device."""
+    number of entries that got none and stay as they were, an int32 ``[1]`` on the device."""
 
     pages = _refs(refs)
     table = _pool_table(page_table, "lengths", lengths)

@@ -416,7 +416,8 @@ int g4_paged_read(const G4PagedReadArgs* args, void* stream);
  * or pages must be ordered. They allocate nothing and keep no state; workspaces are plain scratch, 16-byte aligned, of
  * g4_paged_*_workspace_size() bytes.
  * Fresh pages are handed out in one order: the i-th entry that takes one, row by row, gets the i-th lowest free page, with
- * refs 1. Where there are too few, the last entries get -1, and *shortage (device int32) is how many; else it is 0.
+ * refs 1. Where there are too few, the last entries get none, and *shortage (device int32) is how many; else it is 0. Such
+ * an entry holds no page then: a fork writes -1, a reserve leaves it as it was (-1 or another value outside the pool).
  */
 typedef struct G4PageTable {
   int32_t rows;
