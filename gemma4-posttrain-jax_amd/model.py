@@ -537,7 +537,7 @@ def forward_gemma4_text(
         tables = {SLIDING: kv_cache.window_table, FULL: kv_cache.page_table}
         keep = config.sliding_window
         if packed is not None:  # every token its own row of the append
-            held, keep = packed.lengths, 0
+            held, keep = packed.lengths.clone(), 0  # (steps add to held in place)
             tables = {t: table.index_select(0, packed.rows) for t, table in tables.items()}
             place = torch.arange(S, dtype=torch.int32, device=dev) - packed.starts
             place = place.masked_fill(packed.starts < 0, -1)  # of no prompt
