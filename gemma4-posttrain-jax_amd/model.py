@@ -538,12 +538,15 @@ def forward_gemma4_text(
         keep = config.sliding_window
         if packed is not None:  # every token its own row of the append
             held, keep = packed.lengths.clone(), 0  # (steps add to held in place)
-            tables = {t: table.index_select(0, packed.rows) for t, table in tables.items()}
             place = torch.arange(S, dtype=torch.int32, device=dev) - packed.starts
-            place = place.masked_fill(packed.starts < 0, -1)  # of no prompt
+            width, ps = kv_cache.page_table.shape[1], kv_cache.capacity // kv_cache.page_table.shape[1]
+            none = (packed.starts < 0) | (place < 0) | (place >= width * ps)  # of no prompt, or behind the table's end
+            entry = (place // ps).masked_fill(none, 0)
+            # a table of the one page that the token goes to
+            tables = {t: table[packed.rows.long(), entry.long()][:, None] for t, table in tables.items()}
             # a sliding layer stores what the last window holds
-            gone = place < held.index_select(0, packed.rows) - config.sliding_window
-            slots = {FULL: place, SLIDING: place.masked_fill(gone, -1)}
+            gone = none | (place < held.index_select(0, packed.rows) - config.sliding_window)
+            slots = {t: (place % ps).masked_fill(x, -1) for t, x in ((FULL, none), (SLIDING, gone))}
         elif cache_mode == "prefill":  # token s of a row with n real tokens stands at position s - (S - n)
             held = attention_mask.sum(dim=-1, dtype=torch.int32)
             slot = held - S

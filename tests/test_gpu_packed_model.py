@@ -52,3 +52,47 @@ def test_steps_leave_the_prompts_description(device):
     for x, y in zip(first.layers, again.layers):
         if x is not None:
             assert torch.equal(x.key, y.key) and torch.equal(x.value, y.value)
+
+
+@pytest.mark.parametrize("lens,tail,capacity", [([300, 1, 64], 7, 320), ([2500], 0, 4096)])
+def test_a_prompts_tokens_share_its_table(lens, tail, capacity, device, monkeypatch):
+    """The tables that go into the pages' appends hold an entry per token, however long the rows may become; what a row
+    holds is read back through its own table, and a prefill of padded rows stores the same places."""
+
+    cfg = C.config_from_hf(CFG)
+    params = _params(cfg, device)
+    packed, ids, places = _packed(lens, tail, device)
+    append, entries = kernels.paged_append, []
+
+    def spy(layer, k, v, *, page_table, **kw):
+        entries.append(page_table.numel())
+        return append(layer, k, v, page_table=page_table, **kw)
+
+    monkeypatch.setattr(kernels, "paged_append", spy)
+    empty = init_paged_kv_cache(cfg, len(lens), capacity, PagedSpec(32), device)
+    _, cache = M.forward_gemma4_text(params, ids, places, config=cfg, kv_cache=empty, packed=packed)
+    assert entries and max(entries) <= ids.shape[1]
+    monkeypatch.undo()
+    S = max(lens)
+    padded, at = torch.zeros((len(lens), S), dtype=ids.dtype, device=device), 0
+    for b, n in enumerate(lens):
+        padded[b, S - n:] = ids[0, at:at + n]
+        at += n
+    mask = torch.arange(S, device=device)[None] >= S - cache.held[:, None]
+    pos = (mask.cumsum(dim=1) - 1).clamp(min=0).to(torch.int32)
+    other = init_paged_kv_cache(cfg, len(lens), capacity, PagedSpec(32), device)
+    _, dense = M.forward_gemma4_text(params, padded, pos, config=cfg, attention_mask=mask, kv_cache=other)
+    for i, (x, y) in enumerate(zip(cache.layers, dense.layers)):
+        if x is None:
+            continue
+        table = cache.window_table if cfg.layer_types[i] == C.SLIDING else cache.page_table
+        for b, n in enumerate(lens):
+            first = max(0, n - cfg.sliding_window) if cfg.layer_types[i] == C.SLIDING else 0
+            read = [kernels.paged_read(z, page_table=table[b:b + 1].contiguous(), lengths=cache.held[b:b + 1].contiguous(),
+                                       start=first, count=n - first) for z in (x, y)]
+            for got, want in zip(*read):
+                got, want = got.float(), want.float()
+                # places: a token's neighbour is some 1.4 of its size away; the roundings of a few bf16 layers, a few hundredths
+                assert bool(((got - want).norm(dim=-1) <= 0.2 * want.norm(dim=-1) + 1e-3).all()), (i, b)
+        used = (y.key != 0).flatten(1).any(dim=1)
+        assert torch.equal((x.key != 0).flatten(1).any(dim=1), used) and int(used.sum()) >= len(lens)
