@@ -541,11 +541,12 @@ def forward_gemma4_text(
             place = torch.arange(S, dtype=torch.int32, device=dev) - packed.starts
             width, ps = kv_cache.page_table.shape[1], kv_cache.capacity // kv_cache.page_table.shape[1]
             none = (packed.starts < 0) | (place < 0) | (place >= width * ps)  # of no prompt, or behind the table's end
+            rows = packed.rows.long().masked_fill(none, 0)
             entry = (place // ps).masked_fill(none, 0)
             # a table of the one page that the token goes to
-            tables = {t: table[packed.rows.long(), entry.long()][:, None] for t, table in tables.items()}
+            tables = {t: table[rows, entry.long()][:, None] for t, table in tables.items()}
             # a sliding layer stores what the last window holds
-            gone = none | (place < held.index_select(0, packed.rows) - config.sliding_window)
+            gone = none | (place < held.index_select(0, rows) - config.sliding_window)
             slots = {t: (place % ps).masked_fill(x, -1) for t, x in ((FULL, none), (SLIDING, gone))}
         elif cache_mode == "prefill":  # token s of a row with n real tokens stands at position s - (S - n)
             held = attention_mask.sum(dim=-1, dtype=torch.int32)

@@ -96,3 +96,19 @@ def test_a_prompts_tokens_share_its_table(lens, tail, capacity, device, monkeypa
                 assert bool(((got - want).norm(dim=-1) <= 0.2 * want.norm(dim=-1) + 1e-3).all()), (i, b)
         used = (y.key != 0).flatten(1).any(dim=1)
         assert torch.equal((x.key != 0).flatten(1).any(dim=1), used) and int(used.sum()) >= len(lens)
+
+
+@pytest.mark.parametrize("other", [-1, 2, 2 ** 31 - 1])
+def test_the_rows_of_tokens_of_no_prompt_may_be_any(other, device):
+    cfg = C.config_from_hf(CFG)
+    params = _params(cfg, device)
+    packed, ids, places = _packed([33, 4], 9, device)
+    rows = packed.rows.clone()
+    rows[37:] = other
+    caches = []
+    for p in (packed, packed._replace(rows=rows)):
+        empty = init_paged_kv_cache(cfg, 2, 64, PagedSpec(32), device)
+        caches.append(M.forward_gemma4_text(params, ids, places, config=cfg, kv_cache=empty, packed=p)[1])
+    for x, y in zip(*(c.layers for c in caches)):
+        if x is not None:
+            assert torch.equal(x.key, y.key) and torch.equal(x.value, y.value)
