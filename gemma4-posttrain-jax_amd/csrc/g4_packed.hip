@@ -534,7 +534,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(G4PackedPrefillArgs a,
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       __builtin_memcpy(x[j], __builtin_assume_aligned(pieces.o + (((int64_t)min(s + j, n - 1) * H + h) * padded + row) * D + lane * PER,
-                                                      PER * 4), PER * 4);
+                                                      PER * 4 < 16 ? PER * 4 : 16), PER * 4);  // (the workspace: 16 bytes)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (s + j >= n) break;
