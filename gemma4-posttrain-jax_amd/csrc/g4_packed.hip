@@ -84,18 +84,25 @@ struct Rows {
 };
 
 // Softmax of one chunk's scores: `p` as the value product's operand, the row statistics brought forward.
+// p = exp2(s log2(e) - m log2(e)) takes one fma per score, but the rounding of m log2(e) is another for each maximum, and for one of 2^31
+// it is larger than any exponent. Rows whose maximum passes kFar, where it is 2^-14, therefore take their scores less an origin, a
+// maximum of theirs, exactly where it counts. That goes with the mask, which such a wave's blocks then have in every chunk: other waves
+// pay for it in masked chunks only (packed prompts of up to 8191 tokens 373 -> 376 us; 379 with a branch of its own behind the maximum).
+constexpr float kFar = 1024.0f;
 template <int NB, int VT>
 struct Softmax {
-  float m[NB], l[NB];  // row maximum in use, this lane's share of the sum
+  float m[NB], l[NB];  // row maximum in use, less the origin; this lane's share of the sum
+  float origin[NB];
 
   __device__ __forceinline__ void init() {
 #pragma unroll
-    for (int cb = 0; cb < NB; ++cb) m[cb] = kNegInf, l[cb] = 0.f;
+    for (int cb = 0; cb < NB; ++cb) m[cb] = kNegInf, l[cb] = origin[cb] = 0.f;
   }
+  __device__ static __forceinline__ bool is_far(float x) { return fabsf(x) > kFar && fabsf(x) < -kNegInf; }
   // what an exponent subtracts (before the first key, with scores of -inf alone, nothing)
   __device__ __forceinline__ float base(int cb) const { return m[cb] == kNegInf ? 0.f : m[cb] * kLog2e; }
 
-  __device__ __forceinline__ void chunk(const Rows& rows, int c, int lane, floatx4 (&acc)[NB][2], bf16x8 (&pop)[NB],
+  __device__ __forceinline__ void chunk(Rows& rows, int c, int lane, floatx4 (&acc)[NB][2], bf16x8 (&pop)[NB],
                                         floatx4 (&oacc)[NB][VT]) {
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) {  // (a wave across a sequence's end masks one of them in every chunk)
@@ -106,7 +113,7 @@ struct Softmax {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t seen = (uint32_t)__builtin_amdgcn_sbfe((int)bits, e, 1);  // all bits or none
-        acc[cb][e >> 2][e & 3] = __uint_as_float((seen & __float_as_uint(acc[cb][e >> 2][e & 3])) | (~seen & 0xff800000u));
+        acc[cb][e >> 2][e & 3] = __uint_as_float((seen & __float_as_uint(acc[cb][e >> 2][e & 3])) | (~seen & 0xff800000u)) - origin[cb];
       }
     }
     float top[NB];
@@ -132,6 +139,20 @@ struct Softmax {
           for (int i = 0; i < VT; ++i) oacc[cb][i] *= scale;
         }
       }
+      bool beyond = false;
+#pragma unroll
+      for (int cb = 0; cb < NB; ++cb) beyond |= is_far(m[cb]);
+      if (__builtin_expect(__any(beyond), 0)) {  // (what a row has summed up stays: sums of another origin's weigh e^-kFar)
+#pragma unroll
+        for (int cb = 0; cb < NB; ++cb) {
+          const float by = is_far(m[cb]) ? m[cb] : 0.f;
+          origin[cb] += by;
+          m[cb] -= by;
+          acc[cb][0] -= by;
+          acc[cb][1] -= by;
+          rows.all_from[cb] = 0x7fffffff;  // no chunk is full
+        }
+      }
     }
 #pragma unroll
     for (int cb = 0; cb < NB; ++cb) {
@@ -152,7 +173,7 @@ struct Softmax {
 // values are not all finite key by key, so that a row takes only those that it sees. For waves that met such values: few
 // registers and little code matter here, speed does not (the scores are formed anew for every 16 dims).
 template <int D>
-__device__ __forceinline__ floatx4 careful_values(const Rows& rows, int cb, float ml, const uint16_t* q,
+__device__ __forceinline__ floatx4 careful_values(const Rows& rows, int cb, float origin, float ml, const uint16_t* q,
                                                   __amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv, int i) {
   constexpr int KS = D / 32;
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
@@ -175,7 +196,7 @@ __device__ __forceinline__ floatx4 careful_values(const Rows& rows, int cb, floa
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      p[e] = seen >> (8 * grp + e) & 1u ? __builtin_amdgcn_exp2f(fmaf(acc[e >> 2][e & 3], kLog2e, -ml)) : 0.f;
+      p[e] = seen >> (8 * grp + e) & 1u ? __builtin_amdgcn_exp2f(fmaf(acc[e >> 2][e & 3] - origin, kLog2e, -ml)) : 0.f;
     const u32x4 pop = pack8(p);
     const u32x4 v = buffer_load16(rv, v_lane, (uint32_t)c * (uint32_t)(64 * D) + 256u * i);
     bool odd = false;
@@ -219,9 +240,9 @@ __device__ __forceinline__ void place_block(int i, int n_blk, int H, const int32
 // launch joins; a block that has chunks for one piece only writes its result itself.
 constexpr int kMostPieces = 16;
 struct Piece {
-  float m, l;   // row maximum in use, sum
-  int pieces;   // of the row's block (in piece 0's; 1: nothing to join)
-  int pad;
+  float m, l;    // row maximum in use, less the origin; sum
+  int pieces;    // of the row's block (in piece 0's; 1: nothing to join)
+  float origin;
 };
 struct Pieces {
   float* o;      // [most][H][padded rows][D], not divided by the sums
@@ -440,7 +461,7 @@ __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefi
       float l = column_sum(soft.l[cb]);
       if (rows.keys[cb].y < 0) l = 0.f;  // (chunks that all other rows see whole were not masked)
       const int64_t row = base + cb * 16 + col;
-      if (grp == 0) pieces.stats[row] = Piece{soft.m[cb], l, n_pieces, 0};
+      if (grp == 0) pieces.stats[row] = Piece{soft.m[cb], l, n_pieces, soft.origin[cb]};
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < VT; ++i) {
@@ -453,7 +474,7 @@ __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefi
         const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (((int64_t)t * H + h) * R + (g - t * R)) * D;
 #pragma unroll 1
         for (int i = 0; i < VT; ++i)
-          *reinterpret_cast<floatx4*>(pieces.o + row * D + 16 * i + 4 * grp) = careful_values<D>(rows, cb, soft.base(cb), q, rk, rv, i);
+          *reinterpret_cast<floatx4*>(pieces.o + row * D + 16 * i + 4 * grp) = careful_values<D>(rows, cb, soft.origin[cb], soft.base(cb), q, rk, rv, i);
       }
     }
     return;
@@ -470,7 +491,7 @@ __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefi
   for (int cb = 0; cb < NB; ++cb) {
     const float l = column_sum(soft.l[cb]);
     const int row = row0 + cb * 16 + (lane_o & 15), t = group.token(row);
-    if (CUT && lane_o < 16) pieces.stats[(int64_t)h * ((int64_t)n_blk * S::ROWS) + row] = Piece{0.f, 0.f, 1, 0};  // nothing to join
+    if (CUT && lane_o < 16) pieces.stats[(int64_t)h * ((int64_t)n_blk * S::ROWS) + row] = Piece{0.f, 0.f, 1, 0.f};  // nothing to join
     const bool none = rows.keys[cb].y < 0 || l == 0.f;
     const float inv = none ? 0.f : 1.0f / l;
     const auto pack = [&](floatx4 x) {
@@ -493,7 +514,7 @@ __global__ __launch_bounds__((BIG && D == 512 ? 512 : 256), 2) void packed_prefi
     if (__any(!(sum == 0.f))) {
       const uint16_t* q = t < T ? reinterpret_cast<const uint16_t*>(a.q) + (((int64_t)t * H + h) * R + (row - t * R)) * D : nullptr;
 #pragma unroll 1
-      for (int i = 0; i < VT; ++i) store(i, pack(careful_values<D>(rows, cb, soft.base(cb), q, rk, rv, i)));
+      for (int i = 0; i < VT; ++i) store(i, pack(careful_values<D>(rows, cb, soft.origin[cb], soft.base(cb), q, rk, rv, i)));
     }
     __builtin_amdgcn_wave_barrier();  // (a wave's rows are its own: its LDS operations keep their order)
 #pragma unroll
@@ -518,11 +539,12 @@ __global__ __launch_bounds__(256) void packed_join_kernel(G4PackedPrefillArgs a,
   const int h = (int)(i / rows), row = (int)(i - h * rows);
   const int n = __builtin_amdgcn_readfirstlane(pieces.stats[h * padded + row].pieces);  // (one row per wave)
   if (n <= 1) return;
-  Piece p{kNegInf, 0.f, 0, 0};
+  Piece p{kNegInf, 0.f, 0, 0.f};
   if (lane < n) p = pieces.stats[((int64_t)lane * H + h) * padded + row];
   const bool none = p.l == 0.f;  // (a row of no sequence, no key of the row here, or scores of -inf alone)
-  const float top = wave_max(none ? kNegInf : p.m);
-  const float weight = none ? 0.f : __builtin_amdgcn_exp2f((p.m - top) * kLog2e);
+  const float m = p.origin - wave_max(none ? kNegInf : p.origin) + p.m;  // (origins are maxima: one with weight is next to the largest)
+  const float top = wave_max(none ? kNegInf : m);
+  const float weight = none ? 0.f : __builtin_amdgcn_exp2f((m - top) * kLog2e);
   const float l = wave_sum(none ? 0.f : weight * p.l);
   const bool some = __any(!none);
   float o[PER];
