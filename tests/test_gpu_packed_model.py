@@ -8,8 +8,9 @@ import torch
 from gemma4_posttrain_jax_amd import config as C
 from gemma4_posttrain_jax_amd import kernels
 from gemma4_posttrain_jax_amd import model as M
+from gemma4_posttrain_jax_amd import sampler as SMP
 from gemma4_posttrain_jax_amd.kvcache import PagedSpec, init_paged_kv_cache
-from test_gpu_paged_run import CFG, _params
+from test_gpu_paged_run import CFG, CFG512, _params, _prompts
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +113,43 @@ def test_the_rows_of_tokens_of_no_prompt_may_be_any(other, device):
     for x, y in zip(*(c.layers for c in caches)):
         if x is not None:
             assert torch.equal(x.key, y.key) and torch.equal(x.value, y.value)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("kwargs,G,pads,S,steps", [(CFG, 3, [0, 11, 59], 60, 50), (CFG512, 2, [5, 0, 64], 70, 40),
+                                                   (CFG, 1, [0, 3], 33, 34)])
+def test_steps_after_a_group_are_those_of_rows_of_their_own(kwargs, G, pads, S, steps, e4m3, device):
+    """Decode steps over shared, forked and copied pages give the bits that they give over a cache in which every row has pages of
+    its own with the same contents; each row takes other tokens. Beside them the steps after a prefill of the repeated rows."""
+
+    cfg = C.config_from_hf(kwargs)
+    params = _params(cfg, device)
+    ids, mask = _prompts(cfg, pads, S, device)
+    spec = PagedSpec(32, e4m3)
+    cache = SMP.prefill_group(params, cfg, ids, mask, completions=G, max_new_tokens=steps, paged=spec).kv_cache
+    B, held = len(pads) * G, cache.held.tolist()
+    own = init_paged_kv_cache(cfg, B, cache.capacity, spec, device)
+    assert own.capacity == cache.capacity
+    for i, (x, y) in enumerate(zip(cache.layers, own.layers)):
+        if x is None:
+            continue
+        sliding = cfg.layer_types[i] == C.SLIDING
+        src, dst = (cache.window_table, own.window_table) if sliding else (cache.page_table, own.page_table)
+        for b, n in enumerate(held):
+            first = max(0, n - cfg.sliding_window) // 32 if sliding else 0
+            for e in range(first, -(-n // 32)):
+                for t, u in zip(x, y):
+                    if t is not None:
+                        u[int(dst[b, e])] = t[int(src[b, e])]
+    own = own._replace(length=cache.length, held=cache.held.clone())
+    G_rows = lambda t: t.repeat_interleave(G, dim=0)  # noqa: E731
+    dense = SMP.prefill(params, cfg, G_rows(ids), G_rows(mask), max_new_tokens=steps, paged=spec).kv_cache
+    for s in range(steps):
+        tok = (torch.arange(B, dtype=torch.int32, device=device) * 13 + 7 * s) % cfg.vocab_size
+        got, want, near = [SMP.decode_step(params, cfg, tok, c.held.clone(), c) for c in (cache, own, dense)]
+        cache, own, dense = got.kv_cache, want.kv_cache, near.kv_cache
+        assert torch.equal(got.logits, want.logits), s
+        assert got.kv_cache.held.tolist() == [n + s + 1 for n in held]
+        if not e4m3:  # other GEMM shapes and attention roundings of the prompt: a bf16 model's last bits, amplified by a few layers
+            far = (got.logits.float() - near.logits.float()).abs().max()
+            assert float(far) <= 2e-2 * max(1.0, float(near.logits.float().abs().max())), s
