@@ -30,7 +30,7 @@ constexpr float kNegInf = -__builtin_inff();
 constexpr float kSlack = 8.0f;
 
 // A workgroup's work: NB blocks of 16 query rows by each of NW waves, 128 rows (BIG) or 64. Head dims up to 256: four waves of two
-// blocks (at 256 248 registers) or one, two workgroups on a CU, each of which fills the other's barriers, softmax and loads; K and
+// blocks (at 256 250 registers) or one, two workgroups on a CU, each of which fills the other's barriers, softmax and loads; K and
 // V^T take two chunks of LDS each, 64 KiB at 256. (8 x 4096 tokens of 2 x 4 heads of 256, before the blocks were sorted: 506 us; one
 // workgroup of eight waves with four chunks of each 586, of one block per wave 589.) Head dim 512: eight waves of one block alone on
 // the CU, two chunks of each in 128 KiB, or four, two workgroups, one chunk of each (ONE).
@@ -252,7 +252,7 @@ struct Pieces {
 };
 
 // The runs of blocks by the chunks of their longest block, most first: the last workgroups to start are short ones (CUs at work for 71 %
-// of the time on 3 prompts of up to 8191 tokens without it, 79 % with; 398 -> 368 us). By bins of 2^shift chunks, within one in any
+// of the time on 3 prompts of up to 8191 tokens without it, 81 % with; 398 -> 368 us). By bins of 2^shift chunks, within one in any
 // order, which no result depends on. One workgroup, 4 us with its launch. (By single blocks, whose neighbours then lie on other XCDs:
 // 420 us.)
 constexpr int kBins = 1024;
@@ -594,8 +594,11 @@ __global__ __launch_bounds__(256) void packed_join_kernel(G4PackedPrefillArgs a,
 // x 2 heads of 128: whole 128, 2 pieces 81, 4 66; one of 4000, 8 heads of 512: whole 198, 2 pieces 163, in blocks of 128).
 // Sorting: more blocks than are at work at once, whose keys may differ (no window that makes them alike), the longest of them long beside
 // the rounds that all take (8 prompts of 4096, 2 x 4 heads of 256: 504 -> 450 us; 30 of 100 .. 900 72 -> 60; 64 of 32 .. 1000 136 -> 129).
-// Else the end weighs little, and the launch and the keys that neighbours no longer share cost more (256 of 32 .. 480 188 -> 190,
-// 512 of them 337 -> 358). Where the longest is not known up to four rounds are sorted.
+// Else the end weighs little, and the launch and the keys that neighbours no longer share cost more (256 of 32 .. 480 188 -> 190, 512
+// of them 337 -> 358, before runs of 8 blocks went to an XCD: unsorted 173 and 328 since). Where the longest is not known up to four
+// rounds are sorted. "At work at once" is two workgroups per CU, of 128 rows at head dim 512 one, as 256 and 512 hold them, at which nearly
+// all of this was measured. At 64 and 128 more fit (at 128 three of 128 rows, four of 64), which the rules do not count: grids of these
+// are sorted, or left whole, that the CUs would take at once.
 struct Plan {
   bool big;                // Shape's
   int most, chunks;        // pieces of a block at most (1: whole blocks), chunks of one
