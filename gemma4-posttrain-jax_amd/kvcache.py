@@ -208,7 +208,11 @@ class PagedKVCache(NamedTuple):
     cache, or one whose pages the caller fills by ``kernels.paged_append``) leaves the places to the caller: a
     step's token goes to ``position_ids``, and every place below it has to be filled. ``pad`` are the pads that
     all rows of the prefill began with: the longest row holds at most ``length - pad`` tokens, and a step is
-    refused where that is ``capacity``."""
+    refused where that is ``capacity``.
+
+    ``refs`` counts the entries of ``page_table`` that hold each page, where rows share pages (``prefill_group``): what
+    ``kernels.paged_free`` takes to let rows go that have ended, and ``kernels.paged_compact`` with the global layers. The
+    rings are each row's own."""
 
     layers: tuple  # PagedLayerCache | None per layer
     page_table: torch.Tensor  # [B, M] int32, of the global layers
@@ -216,6 +220,7 @@ class PagedKVCache(NamedTuple):
     length: int
     held: torch.Tensor | None = None  # [B] int32
     pad: int = 0
+    refs: torch.Tensor | None = None  # [P] int32, of the global layers' pages
 
     @property
     def batch(self) -> int:

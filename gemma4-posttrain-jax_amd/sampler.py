@@ -125,7 +125,7 @@ def prefill_group(
     pads, and its cache handed to ``completions`` rows in a row (row ``i * completions + j`` is the j-th of prompt i).
     Their global layers share the pages that the prompt fills and get pages of their own for its last, partly filled
     one and for ``max_new_tokens`` tokens (the longest row's last page filled up); a sliding layer's rings are copied. Returns the logits ``[N *
-    completions, 1, V]``, the packed prompts' hidden states ``[1, T, M]`` and the cache."""
+    completions, 1, V]``, the packed prompts' hidden states ``[1, T, M]`` and the cache, whose ``refs`` count the global layers' pages."""
 
     _no_mesh(mesh)
     if prompt_ids.dim() != 2 or tuple(prompt_mask.shape) != tuple(prompt_ids.shape):
@@ -174,7 +174,7 @@ def prefill_group(
         kernels.paged_free(refs, table, torch.zeros_like(lengths), page_size=ps)
         kernels.paged_reserve(refs, forked, held + room, page_size=ps)
     else:  # (its width is the cache's capacity)
-        forked = table.index_select(0, parents)
+        forked, refs = table.index_select(0, parents), None
     if of[SLIDING] and G > 1:
         # the ring's places in the order of the row's pages: those of the last window and of the first row's none
         at = torch.arange(width, dtype=torch.int32, device=dev)
@@ -182,7 +182,7 @@ def prefill_group(
         live &= (torch.arange(N * G, device=dev) % G != 0)[:, None]
         own = rings.masked_fill(~live, -1)
         kernels.paged_copy(of[SLIDING], rings[::G].repeat_interleave(G, dim=0).reshape(-1), own.reshape(-1))
-    cache = cache._replace(page_table=forked, window_table=rings, held=held)
+    cache = cache._replace(page_table=forked, window_table=rings, held=held, refs=refs)
     return Gemma4Output(logits.repeat_interleave(G, dim=0), hidden, cache)
 
 

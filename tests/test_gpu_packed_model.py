@@ -153,3 +153,34 @@ def test_steps_after_a_group_are_those_of_rows_of_their_own(kwargs, G, pads, S, 
         if not e4m3:  # other GEMM shapes and attention roundings of the prompt: a bf16 model's last bits, amplified by a few layers
             far = (got.logits.float() - near.logits.float()).abs().max()
             assert float(far) <= 2e-2 * max(1.0, float(near.logits.float().abs().max())), s
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("kwargs", [CFG, CFG512])
+def test_rows_that_ended_are_freed_and_the_pool_compacted(kwargs, e4m3, device):
+    """By the counts that the cache carries; the rows that go on give the bits that they give without."""
+
+    cfg = C.config_from_hf(kwargs)
+    params = _params(cfg, device)
+    ids, mask = _prompts(cfg, [0, 20, 65], 70, device)
+    G, steps = 3, 30
+    caches = [SMP.prefill_group(params, cfg, ids, mask, completions=G, max_new_tokens=steps, paged=PagedSpec(32, e4m3)).kv_cache
+              for _ in range(2)]
+    count = lambda c: torch.bincount(c.page_table[c.page_table >= 0].long(), minlength=c.refs.numel()).to(torch.int32)  # noqa: E731
+    full = [x for i, x in enumerate(caches[0].layers) if x is not None and cfg.layer_types[i] != C.SLIDING]
+    assert torch.equal(caches[0].refs, count(caches[0])) and int(caches[0].refs.max()) == G
+    ended = [0, 3, 4, 5, 8]
+    going = [b for b in range(9) if b not in ended]
+    for s in range(steps):
+        tok = (torch.arange(9, dtype=torch.int32, device=device) * 11 + s) % cfg.vocab_size
+        got, want = [SMP.decode_step(params, cfg, tok, c.held.clone(), c) for c in caches]
+        caches = [got.kv_cache, want.kv_cache]
+        assert torch.equal(got.logits[going], want.logits[going]), s
+        if s == 10:
+            c = caches[0]
+            keep = torch.full((9,), c.capacity, dtype=torch.int32, device=device)
+            keep[ended] = 0
+            kernels.paged_free(c.refs, c.page_table, keep, page_size=32)
+            live = int(kernels.paged_compact(full, c.refs, c.page_table))
+            assert torch.equal(c.refs, count(c)) and bool((c.refs[:live] > 0).all()) and bool((c.refs[live:] == 0).all())
+            assert live < int((caches[1].refs > 0).sum()) and bool((c.page_table[ended] == -1).all())
